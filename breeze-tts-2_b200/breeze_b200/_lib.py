@@ -21,12 +21,13 @@ LIB_PATH = Path(__file__).resolve().parent / "libbreeze_b200.so"
 BQ_OK = 0
 BQ_ERR_INVALID_ARG, BQ_ERR_SHAPE, BQ_ERR_ALIGN, BQ_ERR_FORMAT = -1, -2, -3, -4
 BQ_ERR_WORKSPACE, BQ_ERR_CUDA, BQ_ERR_DEVICE = -5, -6, -7
-BQ_DEVERR_WAIT_TIMEOUT = 1
+BQ_DEVERR_WAIT_TIMEOUT, BQ_DEVERR_POSITION, BQ_DEVERR_PAGE = 1, 2, 4
 
 W_BF16, W_INT4_TINYGEMM, W_INT4_PLAIN, W_FP8_E4M3, W_INT8 = 0, 1, 2, 3, 4
 EPI_NONE, EPI_SILU_MUL, EPI_ADD_RESIDUAL = 0, 1, 2
 DT_BF16, DT_F16, DT_F32 = 0, 1, 2
 FLAG_PDL, FLAG_SCALE_ROUND_BF16, FLAG_NO_TC, FLAG_RING_KERNEL = 1, 2, 4, 8
+PAGED_FULL = 2
 
 _DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32}
 
@@ -103,6 +104,37 @@ class SampleDesc(ctypes.Structure):
     ]
 
 
+_PAGED_KV_FIELDS = [
+    ("B", ctypes.c_int32), ("HKV", ctypes.c_int32), ("D", ctypes.c_int32), ("page_size", ctypes.c_int32),
+    ("num_pages", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ("k_pages", ctypes.c_void_p), ("k_page_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+    ("k_slot_stride", ctypes.c_int64), ("v_pages", ctypes.c_void_p), ("v_page_stride", ctypes.c_int64),
+    ("v_head_stride", ctypes.c_int64), ("v_slot_stride", ctypes.c_int64), ("page_table", ctypes.c_void_p),
+    ("ld_table", ctypes.c_int64), ("seq_lens", ctypes.c_void_p), ("q_starts", ctypes.c_void_p),
+]
+
+
+class PagedAppendDesc(ctypes.Structure):
+    """bq_paged_append_desc with its bq_paged_kv laid out in line (include/breeze_b200.h)."""
+
+    _fields_ = _PAGED_KV_FIELDS + [
+        ("T", ctypes.c_int32), ("HQ", ctypes.c_int32), ("cs_dtype", ctypes.c_int32), ("rope_rows", ctypes.c_int32),
+        ("eps", ctypes.c_float), ("flags", ctypes.c_uint32), ("qkv", ctypes.c_void_p), ("ldqkv", ctypes.c_int64),
+        ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("ldcs", ctypes.c_int64), ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("ldq", ctypes.c_int64),
+    ]
+
+
+class PagedAttnDesc(ctypes.Structure):
+    """bq_paged_attn_desc with its bq_paged_kv laid out in line (include/breeze_b200.h)."""
+
+    _fields_ = _PAGED_KV_FIELDS + [
+        ("T", ctypes.c_int32), ("HQ", ctypes.c_int32), ("prefix_len", ctypes.c_int32), ("max_q", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("flags", ctypes.c_uint32), ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64), ("lse", ctypes.c_void_p), ("ldl", ctypes.c_int64),
+    ]
+
+
 class ChainOptions(ctypes.Structure):
     """bq_chain_options (include/breeze_b200.h)."""
 
@@ -142,6 +174,10 @@ _SIGS = {
     "bq_embed_rows": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
                                        ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,
                                        ctypes.c_uint32, ctypes.c_void_p]),
+    "bq_paged_append": (ctypes.c_int32, [ctypes.POINTER(PagedAppendDesc), ctypes.c_void_p]),
+    "bq_paged_attention_workspace_bytes": (ctypes.c_int32, [ctypes.POINTER(PagedAttnDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "bq_paged_attention": (ctypes.c_int32, [ctypes.POINTER(PagedAttnDesc), ctypes.c_void_p, ctypes.c_size_t,
+                                            ctypes.c_void_p]),
     "bq_int4_tinygemm_pack": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
                                                ctypes.c_int32, ctypes.c_void_p]),
     "bq_int4_tinygemm_unpack": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,

@@ -8,6 +8,7 @@
 
 #define BQ_DEVERR_WAIT_TIMEOUT_BIT 1u
 #define BQ_DEVERR_POSITION_BIT 2u
+#define BQ_DEVERR_PAGE_BIT 4u
 
 namespace bq {
 

@@ -1,0 +1,22 @@
+// Host-side helpers of the paged KV-cache operators.
+#pragma once
+
+#include "bq_host.h"
+
+namespace bq {
+
+struct PagedKV;
+
+// Checks the cache part of a descriptor with T new rows of HQ query heads.
+int paged_validate(const bq_paged_kv* kv, int T, int HQ);
+// BQ_OK when the current device is the one this library is built for.
+int paged_check_device();
+void paged_fill(PagedKV* out, const bq_paged_kv* kv, int T, int HQ);
+// 16-byte aligned base and row stride (NULL counts as aligned).
+inline bool paged_aligned(const void* p, int64_t ld, int elem) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * elem) % 16 == 0;
+}
+int paged_launch(const void* fn, dim3 grid, dim3 block, uint32_t smem, void** args, uint32_t flags, void* stream,
+                 const char* what);
+
+}  // namespace bq

@@ -52,7 +52,9 @@ extern "C" {
 
 /* Device-side error bits, read with bq_device_status(). */
 #define BQ_DEVERR_WAIT_TIMEOUT 1u /* a bounded device wait gave up */
-#define BQ_DEVERR_POSITION 2u     /* bq_attention_step saw a cache position outside [0, S) */
+#define BQ_DEVERR_POSITION 2u     /* bq_attention_step saw a cache position outside [0, S); a paged
+                                     operator saw a position behind its page table or cos / sin rows */
+#define BQ_DEVERR_PAGE 4u         /* a paged operator needed a page-table entry outside [0, num_pages) */
 
 /* ---- enums --------------------------------------------------------------- */
 /* Weight formats. */
@@ -266,6 +268,104 @@ typedef struct bq_attn_o_desc {
  * kernel leaves at zero; it may be shared with bq_attention_step's. */
 int32_t bq_attention_o_workspace_bytes(const bq_attn_o_desc* desc, size_t* bytes);
 int32_t bq_attention_o_step(const bq_attn_o_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- paged KV cache ------------------------------------------------------ */
+/* A KV cache in pages of page_size positions, and a batch of B sequences of
+ * unequal length that uses it. No counterpart in the reference, whose static
+ * cache has one position for the whole batch (models/fused/kernels.py:505).
+ * Position p of sequence b lives in slot p % page_size of page
+ * page_table[b * ld_table + p / page_size]. seq_lens[b] counts the positions
+ * of sequence b, this call's new tokens included. The new tokens are T rows:
+ * rows q_starts[b] .. q_starts[b + 1] - 1 are the last positions of sequence b
+ * (q_starts NULL: T = B, row b is the one new token of sequence b). Rows from
+ * q_starts[B] on belong to no sequence and are left as they were.
+ * Lengths, rows and table entries are device data, read when the kernel runs:
+ * a captured graph replays with new ones. What they may not be:
+ *   - a length behind the table (seq_lens[b] > max_pages * page_size) or, in
+ *     bq_paged_append, behind the cos / sin rows sets BQ_DEVERR_POSITION; the
+ *     append skips such tokens, the attention reads what the table holds;
+ *   - an entry outside [0, num_pages) where a position needs it sets
+ *     BQ_DEVERR_PAGE; the append skips the token, the attention reads page 0,
+ *     so the outputs of that sequence mean nothing. Entries that no position
+ *     needs may hold anything.
+ * Slots that hold no position may hold anything, NaN included; the positions'
+ * own k and v must be finite. */
+typedef struct bq_paged_kv {
+    int32_t B;             /* sequences, >= 1 */
+    int32_t HKV, D;        /* kv heads, head dim (64 or 128) */
+    int32_t page_size;     /* positions per page: a power of two, 16 .. 1024 */
+    int32_t num_pages;     /* pages in k_pages / v_pages */
+    int32_t max_pages;     /* page-table columns */
+    int32_t dtype;         /* BQ_DT_BF16 or BQ_DT_F16: pages, q / k / v rows, outputs */
+    int32_t reserved;
+    void* k_pages;         /* element strides of a page, a kv head and a slot; the D elements of a */
+    int64_t k_stride[3];   /* slot are contiguous; bases 16-byte aligned, strides multiples of 8   */
+    void* v_pages;
+    int64_t v_stride[3];
+    const int32_t* page_table; /* [B, ld_table] */
+    int64_t ld_table;
+    const int32_t* seq_lens;   /* [B] */
+    const int32_t* q_starts;   /* [B + 1] ascending, or NULL */
+} bq_paged_kv;
+
+/* New tokens into the cache: qkv rows [q heads | k heads | v heads], per-head
+ * RMSNorm of q and k (when q_norm / k_norm are given) and RoPE (rotate_half)
+ * at each token's own position, in fp32, rounded once; k and v into their
+ * pages, q to q_out. Tokens whose position would be negative (an unused batch
+ * slot: seq_lens[b] less than its rows) are skipped: nothing is written for
+ * them. Two tokens must not share a slot (a page listed twice at positions
+ * both written): one of them would be lost. */
+typedef struct bq_paged_append_desc {
+    bq_paged_kv kv;
+    int32_t T, HQ;
+    int32_t cs_dtype;          /* cos / sin: the cache's dtype or BQ_DT_F32 */
+    int32_t rope_rows;         /* rows of cos / sin, one per position */
+    float eps;                 /* RMSNorm epsilon */
+    uint32_t flags;            /* BQ_FLAG_PDL */
+    const void* qkv;           /* [T, ldqkv], 16-byte aligned rows (as all rows here) */
+    int64_t ldqkv;
+    const void* cos;           /* [rope_rows, ldcs] */
+    const void* sin;
+    int64_t ldcs;
+    const void* q_norm;        /* [D] in the cache's dtype, both or neither */
+    const void* k_norm;
+    void* q_out;               /* [T, ldq]: HQ * D elements a row; may be the q columns of qkv itself */
+    int64_t ldq;
+} bq_paged_append_desc;
+
+int32_t bq_paged_append(const bq_paged_append_desc* desc, void* stream);
+
+/* out = softmax(scale * q k^T) v over each sequence's paged cache, the new
+ * tokens included (append them first): row i of the n new rows of sequence b
+ * sees positions [0, seq_lens[b] - n + i + 1), or all seq_lens[b] with
+ * BQ_PAGED_FULL. A row that sees none gets zeros (lse -inf). Query head h reads
+ * kv head h / (HQ / HKV). fp32 softmax statistics and accumulation; lse, when
+ * given, is the natural logarithm of each row's sum of exponentials.
+ * prefix_len > 0: the first prefix_len positions (a multiple of page_size) are
+ * the same pages in every row of the table and are read once for the whole
+ * batch, through row 0; the value is the same. */
+#define BQ_PAGED_FULL 2u
+
+typedef struct bq_paged_attn_desc {
+    bq_paged_kv kv;
+    int32_t T, HQ;
+    int32_t prefix_len;        /* shared positions, 0 = none */
+    int32_t max_q;             /* most new rows of one sequence as far as the caller knows (a hint that
+                                  picks the kernel, not a limit); 0 = T / B rounded up */
+    float scale;
+    uint32_t flags;            /* BQ_FLAG_PDL | BQ_PAGED_FULL */
+    const void* q;             /* [T, ldq]: HQ * D elements a row */
+    int64_t ldq;
+    void* out;                 /* [T, ldo] */
+    int64_t ldo;
+    float* lse;                /* [T, ldl] or NULL */
+    int64_t ldl;
+} bq_paged_attn_desc;
+
+/* The workspace (256-byte aligned) needs no initial value and keeps none
+ * between calls; calls that can run at the same time need one each. */
+int32_t bq_paged_attention_workspace_bytes(const bq_paged_attn_desc* desc, size_t* bytes);
+int32_t bq_paged_attention(const bq_paged_attn_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- fp32 output heads -------------------------------------------------- */
 /* out[M, N] (fp32) = y @ W, W fp32, where y is x or, when gamma is given, the
