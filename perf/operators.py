@@ -17,8 +17,13 @@ has one new token.
 
 import math
 import random
+import sys
+from pathlib import Path
 
 import torch
+
+# where the package lives in this repository
+sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "breeze-tts-2_b200"))
 
 own = False
 
