@@ -94,92 +94,181 @@ int paged_launch(const void* fn, dim3 grid, dim3 block, uint32_t smem, void** ar
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kJoinThreads = 128;
 
-struct PagedAttnParams {
-    PagedKV kv;
-    int32_t causal;
-    float scale;
-    const void* q;
-    int64_t ldq;
-    void* out;
-    int64_t ldo;
-    float* lse;
-    int64_t ldl;
+// What the joining kernel needs of the prefix pass.
+struct PagedPrefixParts {
+    const float* part_o;
+    const float2* part_ml;
+    const float* row_o;
+    const float2* row_ml;
+    int32_t rows, unit, grid;  // ROWS and UNIT of the pass, its CTAs
 };
 
-// One CTA per (row, query head): warps take every fourth cached position, the
-// lanes of a warp the head's dimensions, with a running maximum and sum per
-// warp; the four are joined at the end.
-template <typename E, int D>
-__global__ void __launch_bounds__(kThreads) paged_attention_rows_kernel(const __grid_constant__ PagedAttnParams p) {
+struct PagedJoin {
+    PagedWork own;
+    int32_t own_grid;
+    PagedPrefixParts pre;
+};
+
+// Parts of one output row: either the row buffer (a tile that one CTA held) or
+// the slots of CTAs c0 .. c1.
+struct PagedParts {
+    const float* part_o;
+    const float2* part_ml;
+    const float* row_o;
+    const float2* row_ml;
+    int64_t row;            // index into the row buffers
+    int32_t rows, r, c0, n; // rows per slot, row within the tile, first CTA, parts
+    long long u0, q;        // first unit of the tile; share
+    int32_t rem;
+    __device__ __forceinline__ int64_t at(int i) const {
+        const long long lo = q * (c0 + i) + min(c0 + i, rem);
+        return int64_t(paged_slot(c0 + i, u0, lo)) * rows + r;
+    }
+};
+
+__device__ __forceinline__ PagedParts paged_parts(const PagedShare& sh, long long u0, int units, int rows, int r) {
+    PagedParts t;
+    t.u0 = u0;
+    t.q = sh.q;
+    t.rem = sh.r;
+    t.rows = rows;
+    t.r = r;
+    t.c0 = sh.owner(u0);
+    t.n = sh.owner(u0 + units - 1) - t.c0 + 1;
+    return t;
+}
+
+// Joins the parts of one output row (grid (T, HQ)): out = sum f_i o_i / sum f_i
+// l_i with f_i = 2^(m_i - max m), over the prefix's parts, then the sequence's
+// own, in CTA order. A row whose tile one CTA held, and that has no prefix, is
+// finished already. The statistics of up to 32 parts are read at once, one per
+// lane; the four warps then take every fourth part's output row.
+template <typename E, int D, int ROWS, int UNIT>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedJoin p) {
     constexpr int DPL = D / 32;
-    __shared__ float s_acc[4][D + 2];
+    __shared__ float s_acc[4][D];
     pdl_launch_dependents();
     pdl_wait();
-    const PagedKV& kv = p.kv;
-    const int t = blockIdx.x, h = blockIdx.y, j = h / (kv.HQ / kv.HKV);
+    const PagedWork& w = p.own;
+    const PagedKV& kv = w.kv;
+    const int t = blockIdx.x, h = blockIdx.y, j = h / w.G;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int b = t;
     if (kv.starts) {
         int n = 0;
-        for (int i0 = 0; i0 < kv.B; i0 += kThreads) {
+        for (int i0 = 0; i0 < kv.B; i0 += kJoinThreads) {
             const int i = i0 + int(threadIdx.x);
             n += __syncthreads_count(i < kv.B && kv.starts[i + 1] <= t);
         }
         b = n;
-        if (b >= kv.B) return;
+        if (b >= kv.B) return;  // a row behind the last sequence
     }
-    int begin, count;
-    paged_rows(kv, b, begin, count);
-    if (t < begin || t >= begin + count) return;
-    bool cut, ok = true;
-    const int len = paged_len(kv, b, cut);
-    const int limit = p.causal ? min(len, kv.lens[b] - count + (t - begin) + 1) : len;
-    float qv[DPL], acc[DPL], m = -INFINITY, l = 0.f;
-    const E* q = static_cast<const E*>(p.q) + int64_t(t) * p.ldq + h * D + lane * DPL;
-#pragma unroll
-    for (int e = 0; e < DPL; ++e) {
-        qv[e] = float(q[e]) * p.scale;
-        acc[e] = 0.f;
+    bool cut;
+    const PagedSeq s = paged_seq(w, b, cut);
+    if (t < s.begin || t >= s.begin + s.count) return;
+    const int r = (t - s.begin) * w.G + (h - j * w.G), tile = r / ROWS;
+    const long long base = w.bases[b];
+    const int head_units = int((w.bases[b + 1] - base) / kv.HKV);
+    long long u0 = base + (long long)j * head_units;
+    for (int i = 0; i < tile; ++i) u0 += paged_tile_units<ROWS, UNIT>(w, s, i);
+    const PagedShare sh(w.bases[kv.B], p.own_grid);
+    PagedParts part[2];
+    int np = 1;
+    part[0] = paged_parts(sh, u0, paged_tile_units<ROWS, UNIT>(w, s, tile), ROWS, r - tile * ROWS);
+    part[0].part_o = w.part_o, part[0].part_ml = w.part_ml, part[0].row_o = w.row_o, part[0].row_ml = w.row_ml;
+    part[0].row = int64_t(t) * kv.HQ + h;
+    if (p.pre.grid) {
+        const int rows = (kv.starts ? min(max(kv.starts[kv.B], 0), kv.T) : kv.T) * w.G;
+        const int tiles = (rows + p.pre.rows - 1) / p.pre.rows, units = (w.prefix_len + p.pre.unit - 1) / p.pre.unit;
+        const int pr = t * w.G + (h - j * w.G), pt = pr / p.pre.rows;
+        const PagedShare ps((long long)tiles * units * kv.HKV, p.pre.grid);
+        part[1] = part[0];
+        part[0] = paged_parts(ps, ((long long)j * tiles + pt) * units, units, p.pre.rows, pr - pt * p.pre.rows);
+        part[0].part_o = p.pre.part_o, part[0].part_ml = p.pre.part_ml;
+        part[0].row_o = p.pre.row_o, part[0].row_ml = p.pre.row_ml;
+        part[0].row = part[1].row;
+        np = 2;
+    } else if (part[0].n == 1) {
+        return;
     }
-    for (int s = warp; s < limit; s += 4) {
-        const int64_t page = paged_page(kv, b, s, ok);
-        const E* k = static_cast<const E*>(kv.k) + page * kv.ks_page + j * kv.ks_head + (s & kv.page_mask) * kv.ks_slot;
-        const E* v = static_cast<const E*>(kv.v) + page * kv.vs_page + j * kv.vs_head + (s & kv.page_mask) * kv.vs_slot;
-        float d = 0.f;
+    float M = -INFINITY;
+    for (int k = 0; k < np; ++k)
+        for (int i = lane; i < part[k].n; i += 32)
+            M = fmaxf(M, part[k].n == 1 ? part[k].row_ml[part[k].row].x : part[k].part_ml[part[k].at(i)].x);
 #pragma unroll
-        for (int e = 0; e < DPL; ++e) d = fmaf(qv[e], float(k[lane * DPL + e]), d);
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float u = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc[DPL] = {};
+    for (int k = 0; k < np; ++k) {
+        for (int i0 = 0; i0 < part[k].n; i0 += 32) {
+            const int i = i0 + lane;
+            float f = 0.f, l = 0.f;
+            if (i < part[k].n) {
+                const float2 ml = part[k].n == 1 ? part[k].row_ml[part[k].row] : part[k].part_ml[part[k].at(i)];
+                f = ex2(ml.x - u);
+                l = f * ml.y;
+            }
 #pragma unroll
-        for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        const float nm = fmaxf(m, d), a = __expf(m - nm), w = __expf(d - nm);
-        l = l * a + w;
+            for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            L += l;
+#pragma unroll 4
+            for (int a = warp; a < min(32, part[k].n - i0); a += 4) {
+                const float fa = __shfl_sync(0xffffffffu, f, a);
+                const float* src = (part[k].n == 1 ? part[k].row_o + part[k].row * D : part[k].part_o + part[k].at(i0 + a) * D) + lane * DPL;
 #pragma unroll
-        for (int e = 0; e < DPL; ++e) acc[e] = fmaf(w, float(v[lane * DPL + e]), acc[e] * a);
-        m = nm;
+                for (int e = 0; e < DPL; ++e) acc[e] = fmaf(fa, src[e], acc[e]);
+            }
+        }
     }
 #pragma unroll
     for (int e = 0; e < DPL; ++e) s_acc[warp][lane * DPL + e] = acc[e];
-    if (lane == 0) {
-        s_acc[warp][D] = m;
-        s_acc[warp][D + 1] = l;
-        if (!ok) atomicOr(&g_device_error, BQ_DEVERR_PAGE_BIT);
-        if (cut) atomicOr(&g_device_error, BQ_DEVERR_POSITION_BIT);
-    }
     __syncthreads();
     const int d = threadIdx.x;
-    if (d >= D) return;
-    float mm = -INFINITY, ll = 0.f, aa = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, s_acc[w][D]);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float f = s_acc[w][D + 1] > 0.f ? __expf(s_acc[w][D] - mm) : 0.f;
-        ll += f * s_acc[w][D + 1];
-        aa += f * s_acc[w][d];
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    if (d < D)
+        static_cast<E*>(w.out)[int64_t(t) * w.ldo + h * D + d] = E((s_acc[0][d] + s_acc[1][d] + s_acc[2][d] + s_acc[3][d]) * inv);
+    if (w.lse && d == 0) w.lse[int64_t(t) * w.ldl + h] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+}
+
+template <typename E, int D>
+const void* join_kernel() {
+    return reinterpret_cast<const void*>(&paged_join_kernel<E, D, kNarrowRows, kNarrowUnit>);
+}
+
+// Scratch of a call, in order: first units of the sequences, then per pass the
+// shared tiles' partials, then, with a prefix, both passes' row buffers.
+struct PagedPlan {
+    int grid;
+    size_t bases, own_o, own_ml, pre_o, pre_ml, row_o, row_ml, pre_row_o, pre_row_ml, total;
+};
+
+int plan_paged(const bq_paged_attn_desc* d, PagedPlan* pl) {
+    const DeviceInfo* di = device_info();
+    if (!di) return BQ_ERR_CUDA;
+    pl->grid = 2 * di->sm_count;  // both kernels keep two CTAs on an SM
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) & ~size_t(255);
+        return here;
+    };
+    const size_t slots = size_t(2) * pl->grid * kNarrowRows;
+    pl->bases = take((size_t(d->kv.B) + 1) * 8);
+    pl->own_o = take(slots * d->kv.D * 4);
+    pl->own_ml = take(slots * 8);
+    if (d->prefix_len > 0) {
+        const size_t rows = size_t(d->T) * d->HQ;
+        pl->pre_o = take(slots * d->kv.D * 4);
+        pl->pre_ml = take(slots * 8);
+        pl->row_o = take(rows * d->kv.D * 4);
+        pl->row_ml = take(rows * 8);
+        pl->pre_row_o = take(rows * d->kv.D * 4);
+        pl->pre_row_ml = take(rows * 8);
     }
-    static_cast<E*>(p.out)[int64_t(t) * p.ldo + h * D + d] = E(ll > 0.f ? aa / ll : 0.f);
-    if (p.lse && d == 0) p.lse[int64_t(t) * p.ldl + h] = ll > 0.f ? mm + logf(ll) : -INFINITY;
+    pl->total = at;
+    return BQ_OK;
 }
 
 int validate_attention(const bq_paged_attn_desc* d) {
@@ -211,38 +300,69 @@ extern "C" {
 
 int32_t bq_paged_attention_workspace_bytes(const bq_paged_attn_desc* d, size_t* bytes) {
     if (!bytes) return set_error(BQ_ERR_INVALID_ARG, "bytes is NULL");
-    const int rc = validate_attention(d);
+    int rc = validate_attention(d);
     if (rc) return rc;
-    *bytes = 0;
+    PagedPlan pl;
+    rc = plan_paged(d, &pl);
+    if (rc) return rc;
+    *bytes = d->T ? pl.total : 0;
     return BQ_OK;
 }
 
 int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = validate_attention(d);
     if (rc) return rc;
-    (void)workspace;
-    (void)workspace_bytes;
     if (d->T == 0) return BQ_OK;
     rc = paged_check_device();
     if (rc) return rc;
-    PagedAttnParams p;
+    PagedPlan pl;
+    rc = plan_paged(d, &pl);
+    if (rc) return rc;
+    if (!workspace || workspace_bytes < pl.total)
+        return set_error(BQ_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", workspace_bytes, pl.total);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255) return set_error(BQ_ERR_ALIGN, "workspace must be 256-byte aligned");
+    char* ws = static_cast<char*>(workspace);
+    auto f32 = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
+    auto f32x2 = [&](size_t at) { return reinterpret_cast<float2*>(ws + at); };
+    PagedJoin p;
     std::memset(&p, 0, sizeof(p));
-    paged_fill(&p.kv, &d->kv, d->T, d->HQ);
-    p.causal = (d->flags & BQ_PAGED_FULL) ? 0 : 1;
-    p.scale = d->scale;
-    p.q = d->q;
-    p.ldq = d->ldq;
-    p.out = d->out;
-    p.ldo = d->ldo;
-    p.lse = d->lse;
-    p.ldl = d->ldl;
+    PagedWork& w = p.own;
+    paged_fill(&w.kv, &d->kv, d->T, d->HQ);
+    w.G = d->HQ / d->kv.HKV;
+    w.causal = (d->flags & BQ_PAGED_FULL) ? 0 : 1;
+    w.prefix_len = d->prefix_len;
+    w.scale_log2 = d->scale * 1.4426950408889634f;
+    w.q = d->q;
+    w.ldq = d->ldq;
+    w.out = d->out;
+    w.ldo = d->ldo;
+    w.lse = d->lse;
+    w.ldl = d->ldl;
+    w.bases = reinterpret_cast<long long*>(ws + pl.bases);
+    w.part_o = f32(pl.own_o);
+    w.part_ml = f32x2(pl.own_ml);
+    p.own_grid = pl.grid;
+    if (d->prefix_len > 0) {
+        w.row_o = f32(pl.row_o);
+        w.row_ml = f32x2(pl.row_ml);
+        PagedWork pre = w;
+        pre.prefix_pass = 1;
+        pre.bases = nullptr;
+        pre.part_o = f32(pl.pre_o);
+        pre.part_ml = f32x2(pl.pre_ml);
+        pre.row_o = f32(pl.pre_row_o);
+        pre.row_ml = f32x2(pl.pre_row_ml);
+        rc = paged_launch_narrow(pre, d->kv.dtype, d->kv.D, pl.grid, d->flags, stream);
+        if (rc) return rc;
+        p.pre = PagedPrefixParts{pre.part_o, pre.part_ml, pre.row_o, pre.row_ml, kNarrowRows, kNarrowUnit, pl.grid};
+    }
+    rc = paged_launch_narrow(w, d->kv.dtype, d->kv.D, pl.grid, d->flags, stream);
+    if (rc) return rc;
     const bool bf = d->kv.dtype == BQ_DT_BF16;
-    const void* fn = d->kv.D == 128 ? (bf ? reinterpret_cast<const void*>(&paged_attention_rows_kernel<__nv_bfloat16, 128>)
-                                          : reinterpret_cast<const void*>(&paged_attention_rows_kernel<__half, 128>))
-                                    : (bf ? reinterpret_cast<const void*>(&paged_attention_rows_kernel<__nv_bfloat16, 64>)
-                                          : reinterpret_cast<const void*>(&paged_attention_rows_kernel<__half, 64>));
+    const void* fn = d->kv.D == 128 ? (bf ? join_kernel<__nv_bfloat16, 128>() : join_kernel<__half, 128>())
+                                    : (bf ? join_kernel<__nv_bfloat16, 64>() : join_kernel<__half, 64>());
     void* args[] = {&p};
-    return paged_launch(fn, dim3(d->T, d->HQ), dim3(kThreads), 0, args, d->flags, stream, "paged attention");
+    return paged_launch(fn, dim3(d->T, d->HQ), dim3(kJoinThreads), 0, args, d->flags, stream, "paged attention join");
 }
 
 }  // extern "C"

@@ -57,6 +57,226 @@ __device__ __forceinline__ int paged_page(const PagedKV& kv, int b, int pos, boo
     return good ? page : 0;
 }
 
+// ---------------------------------------------------------------- schedule
+// The attention kernels cut the batch into tiles of ROWS rows -- row r of
+// sequence b and kv head j is query head j * G + r % G of token r / G, so the
+// query heads that share a kv head share a tile -- and each tile's positions
+// into units of UNIT. All units of the batch, in (sequence, kv head, tile,
+// position) order, are dealt to the CTAs in equal contiguous shares: however
+// uneven the lengths, every CTA reads the same number of positions. A tile
+// that ends up in several CTAs leaves one partial (largest score, sum of
+// exponentials, unnormalized output) per CTA; a CTA can only share its first
+// and its last tile, so two partial slots per CTA hold them all, and a second
+// kernel joins them in CTA order (deterministic; no counters, no atomics).
+//
+// With a shared prefix there are two such schedules: the prefix over all rows
+// of the batch at once (one pseudo-sequence), and each sequence's own positions
+// from prefix_len on.
+struct PagedWork {
+    PagedKV kv;
+    int32_t G, causal, prefix_len, prefix_pass;  // prefix_pass: this launch handles [0, prefix_len) for all rows
+    float scale_log2;                            // scale * log2(e): scores are kept in base 2
+    const void* q;
+    int64_t ldq;
+    void* out;
+    int64_t ldo;
+    float* lse;
+    int64_t ldl;
+    long long* bases;  // [B + 1] first unit of every sequence, then their number (written by CTA 0)
+    float* part_o;     // [2 grid][ROWS][D] unnormalized outputs of shared tiles
+    float2* part_ml;   // [2 grid][ROWS] (largest score, sum of exponentials)
+    float* row_o;      // [T][HQ][D] own parts of tiles that one CTA holds, when a prefix part follows
+    float2* row_ml;    // [T][HQ]
+};
+
+struct PagedSeq {
+    int begin, count, rows, len, off;  // first row, new rows, rows * G, positions, position of the first new row
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedWork& p, int b, bool& cut) {
+    PagedSeq s;
+    cut = false;
+    if (p.prefix_pass) {
+        s.begin = 0;
+        s.count = p.kv.starts ? min(max(p.kv.starts[p.kv.B], 0), p.kv.T) : p.kv.T;
+        s.len = p.prefix_len;
+        s.off = 0;
+    } else {
+        paged_rows(p.kv, b, s.begin, s.count);
+        s.len = max(paged_len(p.kv, b, cut), 0);
+        s.off = p.kv.lens[b] - s.count;
+    }
+    s.rows = s.count * p.G;
+    return s;
+}
+
+// Positions that the last row of tile i sees (all that any row of it sees).
+template <int ROWS>
+__device__ __forceinline__ int paged_tile_limit(const PagedWork& p, const PagedSeq& s, int i) {
+    if (p.prefix_pass || !p.causal) return s.len;
+    const int tok = (min(s.rows, (i + 1) * ROWS) - 1) / p.G;
+    return max(0, min(s.len, s.off + tok + 1));
+}
+
+// Units of tile i: at least one, so that rows that see nothing are written too.
+template <int ROWS, int UNIT>
+__device__ __forceinline__ int paged_tile_units(const PagedWork& p, const PagedSeq& s, int i) {
+    const int n = paged_tile_limit<ROWS>(p, s, i) - (p.prefix_pass ? 0 : p.prefix_len);
+    return max(1, (n + UNIT - 1) / UNIT);
+}
+
+template <int ROWS, int UNIT>
+__device__ __forceinline__ int paged_head_units(const PagedWork& p, const PagedSeq& s, int tiles) {
+    int n = 0;
+    for (int i = 0; i < tiles; ++i) n += paged_tile_units<ROWS, UNIT>(p, s, i);
+    return n;
+}
+
+// Share of CTA c: units [c q + min(c, r), ...) with q = U / grid, r = U % grid.
+struct PagedShare {
+    long long q;
+    int r;
+    __device__ __forceinline__ PagedShare(long long U, int grid) {
+        if (U >> 32) {
+            q = U / grid;
+            r = int(U - q * grid);
+        } else {  // one 32-bit division
+            const uint32_t u = uint32_t(U), d = u / uint32_t(grid);
+            q = d;
+            r = int(u - d * uint32_t(grid));
+        }
+    }
+    __device__ __forceinline__ long long lo(int c) const { return q * c + min(c, r); }
+    __device__ __forceinline__ int owner(long long u) const {
+        const long long head = (q + 1) * r;
+        if (u < head) return (head >> 32) ? int(u / (q + 1)) : int(uint32_t(u) / uint32_t(q + 1));
+        return (u >> 32) || (q >> 32) ? r + int((u - head) / q) : r + int(uint32_t(u - head) / uint32_t(q));
+    }
+};
+
+// Partial slot of a shared tile whose first unit is u0, in the CTA whose share begins at lo.
+__device__ __forceinline__ int paged_slot(int cta, long long u0, long long lo) { return 2 * cta + (u0 < lo ? 0 : 1); }
+
+// Place of a CTA's first unit.
+struct PagedCursor {
+    int b, j, i, k;        // sequence, kv head, tile, unit within the tile
+    int tiles, head_units; // of sequence b
+    long long u, hi;       // next unit, end of the share
+};
+
+// All NT threads: finds the share of CTA `cta`. CTA 0 also writes p.bases.
+template <int ROWS, int UNIT, int NT>
+__device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, int grid) {
+    __shared__ long long s_sum[NT / 32];
+    __shared__ long long s_rem;
+    __shared__ int s_b;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int B = p.prefix_pass ? 1 : p.kv.B;
+    const int per = (B + NT - 1) / NT, b0 = min(int(threadIdx.x) * per, B), b1 = min(b0 + per, B);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        bool cut;
+        const PagedSeq s = paged_seq(p, b, cut);
+        if (cut && cta == 0) atomicOr(&g_device_error, BQ_DEVERR_POSITION_BIT);
+        mine += (long long)paged_head_units<ROWS, UNIT>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
+    }
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) s_sum[warp] = incl;
+    if (threadIdx.x == 0) s_b = -1;
+    __syncthreads();
+    long long before = incl - mine, U = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+        if (w < warp) before += s_sum[w];
+        U += s_sum[w];
+    }
+    const PagedShare sh(U, grid);
+    PagedCursor c;
+    c.u = sh.lo(cta);
+    c.hi = sh.lo(cta + 1);
+    const bool has = mine > 0 && c.u < c.hi && c.u >= before && c.u < before + mine;
+    if (has || (cta == 0 && p.bases)) {
+        long long at = before;
+        for (int b = b0; b < b1; ++b) {
+            bool cut;
+            const PagedSeq s = paged_seq(p, b, cut);
+            const long long n =
+                (long long)paged_head_units<ROWS, UNIT>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
+            if (has && c.u >= at && c.u < at + n) {
+                s_b = b;
+                s_rem = c.u - at;
+            }
+            if (cta == 0 && p.bases) p.bases[b] = at;
+            at += n;
+        }
+    }
+    if (cta == 0 && p.bases && threadIdx.x == 0) p.bases[B] = U;
+    __syncthreads();
+    c.b = s_b;
+    c.i = c.j = c.k = c.tiles = c.head_units = 0;
+    if (c.b < 0) {
+        c.hi = c.u;  // nothing for this CTA
+        return c;
+    }
+    bool cut;
+    const PagedSeq s = paged_seq(p, c.b, cut);
+    c.tiles = (s.rows + ROWS - 1) / ROWS;
+    c.head_units = paged_head_units<ROWS, UNIT>(p, s, c.tiles);
+    long long rem = s_rem;
+    c.j = (rem >> 32) ? int(rem / c.head_units) : int(uint32_t(rem) / uint32_t(c.head_units));
+    int left = int(rem - (long long)c.j * c.head_units);
+    for (;; ++c.i) {
+        const int n = paged_tile_units<ROWS, UNIT>(p, s, c.i);
+        if (left < n) break;
+        left -= n;
+    }
+    c.k = left;
+    return c;
+}
+
+// The tile after the cursor's (sequences without rows have none).
+template <int ROWS, int UNIT>
+__device__ __forceinline__ void paged_next(const PagedWork& p, PagedCursor& c) {
+    c.k = 0;
+    if (++c.i < c.tiles) return;
+    c.i = 0;
+    if (++c.j < p.kv.HKV) return;
+    c.j = 0;
+    const int B = p.prefix_pass ? 1 : p.kv.B;
+    for (++c.b; c.b < B; ++c.b) {
+        bool cut;
+        const PagedSeq s = paged_seq(p, c.b, cut);
+        c.tiles = (s.rows + ROWS - 1) / ROWS;
+        if (c.tiles > 0) return;
+    }
+}
+
+// Positions [0, limit) are seen by row r (of sequence s; in the prefix pass, of all rows).
+__device__ __forceinline__ int paged_row_limit(const PagedWork& p, const PagedSeq& s, int r) {
+    const int tok = r / p.G;
+    if (!p.prefix_pass) return p.causal ? max(0, min(s.len, s.off + tok + 1)) : s.len;
+    int b = tok;
+    if (p.kv.starts) {  // the sequence of row tok: starts[b] <= tok < starts[b + 1]
+        int lo = 0, hi = p.kv.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.kv.starts[mid] <= tok) lo = mid; else hi = mid;
+        }
+        b = lo;
+    }
+    int begin, count;
+    paged_rows(p.kv, b, begin, count);
+    bool cut;
+    const int len = max(paged_len(p.kv, b, cut), 0);
+    const int lim = p.causal ? min(len, p.kv.lens[b] - count + (tok - begin) + 1) : len;
+    return max(0, min(lim, p.prefix_len));
+}
+
 // Eight elements of a 16-byte vector <-> fp32.
 template <typename T>
 __device__ __forceinline__ void unpack8(const uint4& r, float (&v)[8]);
@@ -96,5 +316,19 @@ template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
     return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }
+
+
+// Four fp32 values as elements, 8 bytes.
+template <typename T>
+__device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
+    return make_uint2(pack2<T>(a, b), pack2<T>(c, d));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLn2 = 0.6931471805599453f;
 
 }  // namespace bq

@@ -6,6 +6,11 @@
 namespace bq {
 
 struct PagedKV;
+struct PagedWork;
+
+// Tile and unit of the kernel for few rows (bq_paged_narrow.cu) and its warps.
+constexpr int kNarrowRows = 16, kNarrowUnit = 64, kNarrowWarps = 4;
+int paged_launch_narrow(const PagedWork& w, int dtype, int D, int grid, uint32_t flags, void* stream);
 
 // Checks the cache part of a descriptor with T new rows of HQ query heads.
 int paged_validate(const bq_paged_kv* kv, int T, int HQ);
