@@ -27,6 +27,14 @@ int dtype_size(int dt);
 // Raises the kernel's dynamic shared memory limit once per (kernel, device).
 int ensure_smem_attr(const void* fn, uint32_t bytes);
 
+// cuTensorMapEncodeTiled through the runtime (the library does not link libcuda),
+// or nullptr.
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn tensor_map_encoder();
+
 struct Gemv3Plan {
     int rows, mt, upc, tpu, gpk, ug, ksplit;
     int even_k;  // 1: every warp of every K slice owns an even number of k-blocks

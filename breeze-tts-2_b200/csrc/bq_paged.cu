@@ -233,35 +233,52 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 }
 
 template <typename E, int D>
-const void* join_kernel() {
-    return reinterpret_cast<const void*>(&paged_join_kernel<E, D, kNarrowRows, kNarrowUnit>);
+const void* join_kernel(bool wide) {
+    return wide ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, kWideRows, kWideUnit>)
+                : reinterpret_cast<const void*>(&paged_join_kernel<E, D, kNarrowRows, kNarrowUnit>);
 }
+
+// One pass over positions: its kernel and its CTAs.
+struct PagedPass {
+    bool wide;
+    int rows, unit, grid;
+};
 
 // Scratch of a call, in order: first units of the sequences, then per pass the
 // shared tiles' partials, then, with a prefix, both passes' row buffers.
 struct PagedPlan {
-    int grid;
+    PagedPass own, pre;
     size_t bases, own_o, own_ml, pre_o, pre_ml, row_o, row_ml, pre_row_o, pre_row_ml, total;
 };
+
+// rows: rows of one tile as far as is known. Tiles of up to 16 rows take the
+// kernel for few rows, two CTAs per SM; larger ones the 256-row kernel, one per SM.
+PagedPass paged_pass(int64_t rows, int sms) {
+    if (rows <= kNarrowRows) return PagedPass{false, kNarrowRows, kNarrowUnit, 2 * sms};
+    return PagedPass{true, kWideRows, kWideUnit, sms};
+}
 
 int plan_paged(const bq_paged_attn_desc* d, PagedPlan* pl) {
     const DeviceInfo* di = device_info();
     if (!di) return BQ_ERR_CUDA;
-    pl->grid = 2 * di->sm_count;  // both kernels keep two CTAs on an SM
+    const int G = d->HQ / d->kv.HKV;
+    const int64_t most = !d->kv.q_starts ? 1 : d->max_q > 0 ? d->max_q : (int64_t(d->T) + d->kv.B - 1) / d->kv.B;
+    pl->own = paged_pass(most * G, di->sm_count);
+    pl->pre = paged_pass(int64_t(d->T) * G, di->sm_count);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += (bytes + 255) & ~size_t(255);
         return here;
     };
-    const size_t slots = size_t(2) * pl->grid * kNarrowRows;
+    const size_t own = size_t(2) * pl->own.grid * pl->own.rows, pre = size_t(2) * pl->pre.grid * pl->pre.rows;
     pl->bases = take((size_t(d->kv.B) + 1) * 8);
-    pl->own_o = take(slots * d->kv.D * 4);
-    pl->own_ml = take(slots * 8);
+    pl->own_o = take(own * d->kv.D * 4);
+    pl->own_ml = take(own * 8);
     if (d->prefix_len > 0) {
         const size_t rows = size_t(d->T) * d->HQ;
-        pl->pre_o = take(slots * d->kv.D * 4);
-        pl->pre_ml = take(slots * 8);
+        pl->pre_o = take(pre * d->kv.D * 4);
+        pl->pre_ml = take(pre * 8);
         pl->row_o = take(rows * d->kv.D * 4);
         pl->row_ml = take(rows * 8);
         pl->pre_row_o = take(rows * d->kv.D * 4);
@@ -269,6 +286,11 @@ int plan_paged(const bq_paged_attn_desc* d, PagedPlan* pl) {
     }
     pl->total = at;
     return BQ_OK;
+}
+
+int launch_pass(const PagedPass& ps, const PagedWork& w, const bq_paged_attn_desc* d, void* stream) {
+    return ps.wide ? paged_launch_wide(w, &d->kv, ps.grid, d->flags, stream)
+                   : paged_launch_narrow(w, d->kv.dtype, d->kv.D, ps.grid, d->flags, stream);
 }
 
 int validate_attention(const bq_paged_attn_desc* d) {
@@ -341,7 +363,7 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
     w.bases = reinterpret_cast<long long*>(ws + pl.bases);
     w.part_o = f32(pl.own_o);
     w.part_ml = f32x2(pl.own_ml);
-    p.own_grid = pl.grid;
+    p.own_grid = pl.own.grid;
     if (d->prefix_len > 0) {
         w.row_o = f32(pl.row_o);
         w.row_ml = f32x2(pl.row_ml);
@@ -352,15 +374,15 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
         pre.part_ml = f32x2(pl.pre_ml);
         pre.row_o = f32(pl.pre_row_o);
         pre.row_ml = f32x2(pl.pre_row_ml);
-        rc = paged_launch_narrow(pre, d->kv.dtype, d->kv.D, pl.grid, d->flags, stream);
+        rc = launch_pass(pl.pre, pre, d, stream);
         if (rc) return rc;
-        p.pre = PagedPrefixParts{pre.part_o, pre.part_ml, pre.row_o, pre.row_ml, kNarrowRows, kNarrowUnit, pl.grid};
+        p.pre = PagedPrefixParts{pre.part_o, pre.part_ml, pre.row_o, pre.row_ml, pl.pre.rows, pl.pre.unit, pl.pre.grid};
     }
-    rc = paged_launch_narrow(w, d->kv.dtype, d->kv.D, pl.grid, d->flags, stream);
+    rc = launch_pass(pl.own, w, d, stream);
     if (rc) return rc;
     const bool bf = d->kv.dtype == BQ_DT_BF16;
-    const void* fn = d->kv.D == 128 ? (bf ? join_kernel<__nv_bfloat16, 128>() : join_kernel<__half, 128>())
-                                    : (bf ? join_kernel<__nv_bfloat16, 64>() : join_kernel<__half, 64>());
+    const void* fn = d->kv.D == 128 ? (bf ? join_kernel<__nv_bfloat16, 128>(pl.own.wide) : join_kernel<__half, 128>(pl.own.wide))
+                                    : (bf ? join_kernel<__nv_bfloat16, 64>(pl.own.wide) : join_kernel<__half, 64>(pl.own.wide));
     void* args[] = {&p};
     return paged_launch(fn, dim3(d->T, d->HQ), dim3(kJoinThreads), 0, args, d->flags, stream, "paged attention join");
 }

@@ -53,6 +53,7 @@
 
 #include "bq_device.cuh"
 #include "bq_host.h"
+#include "bq_tmem.cuh"
 
 namespace bq {
 namespace {
@@ -96,70 +97,6 @@ __host__ __device__ constexpr int tc_row_bytes(int fmt) {
     return (fmt == BQ_W_INT4_TINYGEMM || fmt == BQ_W_INT4_PLAIN) ? 64 : fmt == BQ_W_BF16 ? 256 : 128;
 }
 
-// ------------------------------------------------------------- tcgen05 / TMEM
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_alloc(uint32_t slot_smem, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_smem), "r"(cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// D[tmem] (+)= A[tmem] . B[smem]^T, one 128 x N x 16 step.
-__device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                       uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// The mbarrier completes one phase once every tcgen05 op issued so far by this thread is done.
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-                 : "memory");
-}
-
-// Shared-memory matrix descriptor of the K-major bf16 activation tile as the
-// tensor map writes it: rows of 64 k (128 B) in 128-byte swizzle atoms of 8
-// rows; a k16 step inside the atom starts 32 B further (the swizzle is applied
-// to the final address); bit 46 is the sm_100 descriptor version.
-__device__ __forceinline__ uint64_t tc_bdesc(uint32_t saddr) {
-    // K-major, 128-byte swizzle: 8-row groups 1024 B apart (stride offset); the
-    // leading offset is unused for swizzled K-major layouts; layout type 2 = 128B
-    return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) |
-           (uint64_t(2) << 61);
-}
-
 // Tiled TMA load of a 2-D box (no multicast), completion on an mbarrier.
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -168,9 +105,6 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
 }
 
 // ------------------------------------------------------------- small helpers
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -211,24 +145,6 @@ __device__ __forceinline__ uint32_t f16x2_to_bf16x2(uint32_t h) {
 constexpr uint32_t kOne2 = 0x3F803F80u;   // bf16 (1, 1)
 constexpr uint32_t kM136x2 = 0xC308C308u; // bf16 (-136, -136)
 constexpr uint32_t kM128x2 = 0xC300C300u; // bf16 (-128, -128)
-
-// Waits for a phase of `bar` with a bound; gives up when another role has
-// already given up (abort flag) or after p.wait_cycles, recording the timeout.
-__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    for (int it = 0;; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 15) == 15) {
-            if (abort && *abort) return false;
-            if (clock64() - t0 > limit) {
-                atomicOr(&g_device_error, BQ_DEVERR_WAIT_TIMEOUT_BIT);
-                if (abort) *abort = 1;
-                return false;
-            }
-        }
-    }
-}
 
 // Weight row of lane r of unit u.
 __device__ __forceinline__ int tc_row(const TcParams& p, int u, int r) {
@@ -655,28 +571,11 @@ const void* tc_kernel_for(int fmt) {
 }  // namespace
 
 namespace {
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(f);
-    });
-    return fn;
-}
-
 // Tensor map of the activation rows: [M][K] bf16 with row stride ldx, boxes of
 // 64 k x n_mma rows (rows past M read as zeros), 128-byte swizzle -- the K-major
 // layout the MMA's B descriptor (tc_bdesc) describes.
 int tc_encode_x(const void* x, int64_t ldx, int M, int K, int n_mma, CUtensorMap* map) {
-    EncodeTiledFn enc = encode_fn();
+    EncodeTiledFn enc = tensor_map_encoder();
     if (!enc) return set_error(BQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     const cuuint64_t dims[2] = {cuuint64_t(K), cuuint64_t(M)};
     const cuuint64_t strides[1] = {cuuint64_t(ldx) * 2};
@@ -694,7 +593,7 @@ int tc_encode_x(const void* x, int64_t ldx, int M, int K, int n_mma, CUtensorMap
 // [N/8][K/128][8 rows][64 B] (64-byte swizzle), fp8 / int8 rows of K bytes and
 // bf16 rows of K elements in 64-element halves (128-byte swizzle).
 int tc_encode_weights(const bq_gemv_desc* d, CUtensorMap* map) {
-    EncodeTiledFn enc = encode_fn();
+    EncodeTiledFn enc = tensor_map_encoder();
     if (!enc) return set_error(BQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     const cuuint32_t brows = d->epilogue == BQ_EPI_SILU_MUL ? 64u : 128u;
     const cuuint32_t es[4] = {1, 1, 1, 1};
