@@ -94,148 +94,186 @@ int paged_launch(const void* fn, dim3 grid, dim3 block, uint32_t smem, void** ar
 
 namespace {
 
-constexpr int kJoinThreads = 128;
+constexpr int kJoinWarps = 8;
 
-// What the joining kernel needs of the prefix pass.
-struct PagedPrefixParts {
-    const float* part_o;
-    const float2* part_ml;
-    const float* row_o;
-    const float2* row_ml;
-    int32_t rows, unit, grid;  // ROWS and UNIT of the pass, its CTAs
-};
-
-struct PagedJoin {
-    PagedWork own;
-    int32_t own_grid;
-    PagedPrefixParts pre;
-};
-
-// Parts of one output row: either the row buffer (a tile that one CTA held) or
-// the slots of CTAs c0 .. c1.
+// One pass's parts, as the joining kernel reads them.
 struct PagedParts {
     const float* part_o;
     const float2* part_ml;
     const float* row_o;
     const float2* row_ml;
-    int64_t row;            // index into the row buffers
-    int32_t rows, r, c0, n; // rows per slot, row within the tile, first CTA, parts
-    long long u0, q;        // first unit of the tile; share
-    int32_t rem;
-    __device__ __forceinline__ int64_t at(int i) const {
-        const long long lo = q * (c0 + i) + min(c0 + i, rem);
-        return int64_t(paged_slot(c0 + i, u0, lo)) * rows + r;
-    }
+    const int2* row_at;
+    int32_t rows, grid;
 };
 
-__device__ __forceinline__ PagedParts paged_parts(const PagedShare& sh, long long u0, int units, int rows, int r) {
-    PagedParts t;
-    t.u0 = u0;
-    t.q = sh.q;
-    t.rem = sh.r;
-    t.rows = rows;
-    t.r = r;
-    t.c0 = sh.owner(u0);
-    t.n = sh.owner(u0 + units - 1) - t.c0 + 1;
-    return t;
+struct PagedJoin {
+    PagedParts pass[2];  // own positions; the shared prefix (grid 0: none)
+    const PagedShared* shared;
+    const int32_t* starts;
+    void* out;
+    int64_t ldo;
+    float* lse;
+    int64_t ldl;
+    int32_t B, T, HQ, G;
+    FastDiv by_G, by_HQ;
+};
+
+// The parts of one output row in one pass.
+struct RowParts {
+    const float* o;
+    const float2* ml;
+    int64_t first, step;  // row of the first part (slot 2 c + 1), and from each CTA's slot 2 c to the next CTA's
+    int64_t head;         // row of slot 2 c of the first CTA
+    int32_t n;
+    __device__ __forceinline__ int64_t at(int i) const { return i == 0 ? first : head + i * step; }
+};
+
+__device__ __forceinline__ RowParts shared_row(const PagedParts& p, int cta, int parts, int r) {
+    RowParts x;
+    x.o = p.part_o;
+    x.ml = p.part_ml;
+    x.head = int64_t(2 * cta) * p.rows + r;
+    x.first = x.head + p.rows;
+    x.step = int64_t(2) * p.rows;
+    x.n = parts;
+    return x;
 }
 
-// Joins the parts of one output row (grid (T, HQ)): out = sum f_i o_i / sum f_i
-// l_i with f_i = 2^(m_i - max m), over the prefix's parts, then the sequence's
-// own, in CTA order. A row whose tile one CTA held, and that has no prefix, is
-// finished already. The statistics of up to 32 parts are read at once, one per
-// lane; the four warps then take every fourth part's output row.
-template <typename E, int D, int ROWS, int UNIT>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedJoin p) {
-    constexpr int DPL = D / 32;
-    __shared__ float s_acc[4][D];
+// Joins output rows: out = sum f_i o_i / sum f_i l_i with f_i = 2^(m_i - max m),
+// over the prefix's parts, then the sequence's own, in CTA order. WPR warps work
+// on a row, each on every WPR-th part: eight for tiles of few rows, which may be
+// spread over all CTAs, one where rows are many. Without a prefix, block (c, y)
+// takes rows of the shared tile that begins in CTA c -- tiles that one CTA held
+// are finished already; with one, blocks take all rows in turn.
+// Bound: latency (a record, the statistics, then all parts' rows in flight).
+template <typename E, int D, int WPR, bool PREFIX>
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __grid_constant__ PagedJoin p) {
+    constexpr int DPL = D / 32, RPB = kJoinWarps / WPR;  // rows per block at a time
+    __shared__ float s_acc[kJoinWarps][D];
     pdl_launch_dependents();
     pdl_wait();
-    const PagedWork& w = p.own;
-    const PagedKV& kv = w.kv;
-    const int t = blockIdx.x, h = blockIdx.y, j = h / w.G;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int b = t;
-    if (kv.starts) {
-        int n = 0;
-        for (int i0 = 0; i0 < kv.B; i0 += kJoinThreads) {
-            const int i = i0 + int(threadIdx.x);
-            n += __syncthreads_count(i < kv.B && kv.starts[i + 1] <= t);
-        }
-        b = n;
-        if (b >= kv.B) return;  // a row behind the last sequence
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WPR;
+    PagedShared sh{};
+    int total, first, stride;
+    if constexpr (PREFIX) {
+        total = p.T * p.HQ;
+        first = blockIdx.x * RPB + warp / WPR;
+        stride = gridDim.x * RPB;
+    } else {
+        sh = p.shared[blockIdx.x];
+        total = sh.parts ? sh.rows : 0;
+        first = blockIdx.y * RPB + warp / WPR;
+        stride = gridDim.y * RPB;
     }
-    bool cut;
-    const PagedSeq s = paged_seq(w, b, cut);
-    if (t < s.begin || t >= s.begin + s.count) return;
-    const int r = (t - s.begin) * w.G + (h - j * w.G), tile = r / ROWS;
-    const long long base = w.bases[b];
-    const int head_units = int((w.bases[b + 1] - base) / kv.HKV);
-    long long u0 = base + (long long)j * head_units;
-    for (int i = 0; i < tile; ++i) u0 += paged_tile_units<ROWS, UNIT>(w, s, i);
-    const PagedShare sh(w.bases[kv.B], p.own_grid);
-    PagedParts part[2];
-    int np = 1;
-    part[0] = paged_parts(sh, u0, paged_tile_units<ROWS, UNIT>(w, s, tile), ROWS, r - tile * ROWS);
-    part[0].part_o = w.part_o, part[0].part_ml = w.part_ml, part[0].row_o = w.row_o, part[0].row_ml = w.row_ml;
-    part[0].row = int64_t(t) * kv.HQ + h;
-    if (p.pre.grid) {
-        const int rows = (kv.starts ? min(max(kv.starts[kv.B], 0), kv.T) : kv.T) * w.G;
-        const int tiles = (rows + p.pre.rows - 1) / p.pre.rows, units = (w.prefix_len + p.pre.unit - 1) / p.pre.unit;
-        const int pr = t * w.G + (h - j * w.G), pt = pr / p.pre.rows;
-        const PagedShare ps((long long)tiles * units * kv.HKV, p.pre.grid);
-        part[1] = part[0];
-        part[0] = paged_parts(ps, ((long long)j * tiles + pt) * units, units, p.pre.rows, pr - pt * p.pre.rows);
-        part[0].part_o = p.pre.part_o, part[0].part_ml = p.pre.part_ml;
-        part[0].row_o = p.pre.row_o, part[0].row_ml = p.pre.row_ml;
-        part[0].row = part[1].row;
-        np = 2;
-    } else if (part[0].n == 1) {
-        return;
+    const int rounds = (total + stride - 1) / stride;  // the same for all warps: they meet at barriers
+    int row_lo = 0, row_hi = p.T;  // rows of sequences
+    if (PREFIX && p.starts) {
+        row_lo = p.starts[0];
+        row_hi = p.starts[p.B];
     }
-    float M = -INFINITY;
-    for (int k = 0; k < np; ++k)
-        for (int i = lane; i < part[k].n; i += 32)
-            M = fmaxf(M, part[k].n == 1 ? part[k].row_ml[part[k].row].x : part[k].part_ml[part[k].at(i)].x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float u = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[DPL] = {};
-    for (int k = 0; k < np; ++k) {
-        for (int i0 = 0; i0 < part[k].n; i0 += 32) {
-            const int i = i0 + lane;
-            float f = 0.f, l = 0.f;
-            if (i < part[k].n) {
-                const float2 ml = part[k].n == 1 ? part[k].row_ml[part[k].row] : part[k].part_ml[part[k].at(i)];
-                f = ex2(ml.x - u);
-                l = f * ml.y;
+    for (int k = 0; k < rounds; ++k) {
+        const int idx = first + k * stride;
+        bool live = idx < total;
+        int t = 0, h = 0;
+        RowParts part[2];
+        part[0].n = part[1].n = 0;
+        if (PREFIX) {
+            if (live) {
+                t = p.by_HQ(idx);
+                h = idx - t * p.HQ;
+                live = t >= row_lo && t < row_hi;
             }
+            if (live) {
 #pragma unroll
-            for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            L += l;
+                for (int a = 0; a < 2; ++a) {  // a = 0: the prefix, which comes first
+                    const PagedParts& ps = p.pass[1 - a];
+                    const int2 at = ps.row_at[idx];
+                    const int n = at.y >> 8;
+                    if (n > 0) {  // clamped: a row that ill-ordered starts left out reads no address outside
+                        const int cta = min(max(at.x, 0), ps.grid - 1);
+                        part[a] = shared_row(ps, cta, min(n, ps.grid - cta), min(at.y & 255, ps.rows - 1));
+                    } else {
+                        part[a].o = ps.row_o;
+                        part[a].ml = ps.row_ml;
+                        part[a].first = idx;
+                        part[a].n = 1;
+                    }
+                }
+            }
+        } else if (live) {
+            const int rr = sh.r0 + idx, tok = p.by_G(rr);
+            t = sh.begin + tok;
+            h = sh.j * p.G + rr - tok * p.G;
+            part[1] = shared_row(p.pass[0], blockIdx.x, sh.parts, idx);
+        }
+        float M = -INFINITY, L = 0.f, acc[DPL] = {};
+        if (live) {
+#pragma unroll
+            for (int a = PREFIX ? 0 : 1; a < 2; ++a)
+                for (int i = lane; i < part[a].n; i += 32) M = fmaxf(M, part[a].ml[part[a].at(i)].x);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float u = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int a = PREFIX ? 0 : 1; a < 2; ++a) {
+            for (int i0 = 0; i0 < part[a].n; i0 += 32) {  // the statistics of 32 parts at once, one per lane
+                const int n = min(32, part[a].n - i0);
+                float f = 0.f, l = 0.f;
+                if (lane < n) {
+                    const float2 ml = part[a].ml[part[a].at(i0 + lane)];
+                    f = ex2(ml.x - u);
+                    l = f * ml.y;
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+                L += l;
 #pragma unroll 4
-            for (int a = warp; a < min(32, part[k].n - i0); a += 4) {
-                const float fa = __shfl_sync(0xffffffffu, f, a);
-                const float* src = (part[k].n == 1 ? part[k].row_o + part[k].row * D : part[k].part_o + part[k].at(i0 + a) * D) + lane * DPL;
-#pragma unroll
-                for (int e = 0; e < DPL; ++e) acc[e] = fmaf(fa, src[e], acc[e]);
+                for (int i = sub; i < n; i += WPR) {
+                    const float fa = __shfl_sync(0xffffffffu, f, i);
+                    const float* src = part[a].o + part[a].at(i0 + i) * D + lane * DPL;
+                    if constexpr (DPL == 4) {
+                        const float4 v = *reinterpret_cast<const float4*>(src);
+                        acc[0] = fmaf(fa, v.x, acc[0]), acc[1] = fmaf(fa, v.y, acc[1]);
+                        acc[2] = fmaf(fa, v.z, acc[2]), acc[3] = fmaf(fa, v.w, acc[3]);
+                    } else {
+                        const float2 v = *reinterpret_cast<const float2*>(src);
+                        acc[0] = fmaf(fa, v.x, acc[0]), acc[1] = fmaf(fa, v.y, acc[1]);
+                    }
+                }
             }
         }
-    }
+        if constexpr (WPR > 1) {
+            __syncthreads();
 #pragma unroll
-    for (int e = 0; e < DPL; ++e) s_acc[warp][lane * DPL + e] = acc[e];
-    __syncthreads();
-    const int d = threadIdx.x;
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    if (d < D)
-        static_cast<E*>(w.out)[int64_t(t) * w.ldo + h * D + d] = E((s_acc[0][d] + s_acc[1][d] + s_acc[2][d] + s_acc[3][d]) * inv);
-    if (w.lse && d == 0) w.lse[int64_t(t) * w.ldl + h] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+            for (int e = 0; e < DPL; ++e) s_acc[warp][lane * DPL + e] = acc[e];
+            __syncthreads();
+            if (sub == 0) {
+#pragma unroll
+                for (int q = 1; q < WPR; ++q)
+#pragma unroll
+                    for (int e = 0; e < DPL; ++e) acc[e] += s_acc[warp + q][lane * DPL + e];
+            }
+        }
+        if (live && sub == 0) {
+            const float inv = L > 0.f ? 1.f / L : 0.f;
+            E* dst = static_cast<E*>(p.out) + int64_t(t) * p.ldo + h * D + lane * DPL;
+            if constexpr (DPL == 4)
+                *reinterpret_cast<uint2*>(dst) = pack4<E>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+            else
+                *reinterpret_cast<uint32_t*>(dst) = pack2<E>(acc[0] * inv, acc[1] * inv);
+            if (p.lse && lane == 0) p.lse[int64_t(t) * p.ldl + h] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+        }
+    }
 }
 
 template <typename E, int D>
-const void* join_kernel(bool wide) {
-    return wide ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, kWideRows, kWideUnit>)
-                : reinterpret_cast<const void*>(&paged_join_kernel<E, D, kNarrowRows, kNarrowUnit>);
+const void* join_kernel(bool prefix, bool many) {
+    if (prefix)
+        return many ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1, true>)
+                    : reinterpret_cast<const void*>(&paged_join_kernel<E, D, kJoinWarps, true>);
+    return many ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1, false>)
+                : reinterpret_cast<const void*>(&paged_join_kernel<E, D, kJoinWarps, false>);
 }
 
 // One pass over positions: its kernel and its CTAs.
@@ -244,11 +282,16 @@ struct PagedPass {
     int rows, unit, grid;
 };
 
-// Scratch of a call, in order: first units of the sequences, then per pass the
-// shared tiles' partials, then, with a prefix, both passes' row buffers.
+// Scratch of one pass: the shared tiles' partials and records, then, with a
+// prefix, the row buffers.
+struct PagedScratch {
+    size_t part_o, part_ml, shared, row_o, row_ml, row_at;
+};
 struct PagedPlan {
-    PagedPass own, pre;
-    size_t bases, own_o, own_ml, pre_o, pre_ml, row_o, row_ml, pre_row_o, pre_row_ml, total;
+    PagedPass pass[2];  // own positions, the prefix
+    PagedScratch at[2];
+    int64_t tile_rows;  // rows of one own tile as far as is known
+    size_t total;
 };
 
 // rows: rows of one tile as far as is known. Tiles of up to 16 rows take the
@@ -262,27 +305,28 @@ int plan_paged(const bq_paged_attn_desc* d, PagedPlan* pl) {
     const DeviceInfo* di = device_info();
     if (!di) return BQ_ERR_CUDA;
     const int G = d->HQ / d->kv.HKV;
+    *pl = PagedPlan{};
     const int64_t most = !d->kv.q_starts ? 1 : d->max_q > 0 ? d->max_q : (int64_t(d->T) + d->kv.B - 1) / d->kv.B;
-    pl->own = paged_pass(most * G, di->sm_count);
-    pl->pre = paged_pass(int64_t(d->T) * G, di->sm_count);
+    pl->tile_rows = most * G;
+    pl->pass[0] = paged_pass(most * G, di->sm_count);
+    pl->pass[1] = paged_pass(int64_t(d->T) * G, di->sm_count);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += (bytes + 255) & ~size_t(255);
         return here;
     };
-    const size_t own = size_t(2) * pl->own.grid * pl->own.rows, pre = size_t(2) * pl->pre.grid * pl->pre.rows;
-    pl->bases = take((size_t(d->kv.B) + 1) * 8);
-    pl->own_o = take(own * d->kv.D * 4);
-    pl->own_ml = take(own * 8);
-    if (d->prefix_len > 0) {
-        const size_t rows = size_t(d->T) * d->HQ;
-        pl->pre_o = take(pre * d->kv.D * 4);
-        pl->pre_ml = take(pre * 8);
-        pl->row_o = take(rows * d->kv.D * 4);
-        pl->row_ml = take(rows * 8);
-        pl->pre_row_o = take(rows * d->kv.D * 4);
-        pl->pre_row_ml = take(rows * 8);
+    for (int i = 0; i < (d->prefix_len > 0 ? 2 : 1); ++i) {
+        const size_t slots = size_t(2) * pl->pass[i].grid * pl->pass[i].rows, rows = size_t(d->T) * d->HQ;
+        PagedScratch& s = pl->at[i];
+        s.part_o = take(slots * d->kv.D * 4);
+        s.part_ml = take(slots * 8);
+        s.shared = take(size_t(pl->pass[i].grid) * sizeof(PagedShared));
+        if (d->prefix_len > 0) {
+            s.row_o = take(rows * d->kv.D * 4);
+            s.row_ml = take(rows * 8);
+            s.row_at = take(rows * 8);
+        }
     }
     pl->total = at;
     return BQ_OK;
@@ -344,13 +388,11 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
         return set_error(BQ_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", workspace_bytes, pl.total);
     if (reinterpret_cast<uintptr_t>(workspace) & 255) return set_error(BQ_ERR_ALIGN, "workspace must be 256-byte aligned");
     char* ws = static_cast<char*>(workspace);
-    auto f32 = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
-    auto f32x2 = [&](size_t at) { return reinterpret_cast<float2*>(ws + at); };
-    PagedJoin p;
-    std::memset(&p, 0, sizeof(p));
-    PagedWork& w = p.own;
+    PagedWork w;
+    std::memset(&w, 0, sizeof(w));
     paged_fill(&w.kv, &d->kv, d->T, d->HQ);
     w.G = d->HQ / d->kv.HKV;
+    w.by_G.set(uint32_t(w.G));
     w.causal = (d->flags & BQ_PAGED_FULL) ? 0 : 1;
     w.prefix_len = d->prefix_len;
     w.scale_log2 = d->scale * 1.4426950408889634f;
@@ -360,31 +402,47 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
     w.ldo = d->ldo;
     w.lse = d->lse;
     w.ldl = d->ldl;
-    w.bases = reinterpret_cast<long long*>(ws + pl.bases);
-    w.part_o = f32(pl.own_o);
-    w.part_ml = f32x2(pl.own_ml);
-    p.own_grid = pl.own.grid;
-    if (d->prefix_len > 0) {
-        w.row_o = f32(pl.row_o);
-        w.row_ml = f32x2(pl.row_ml);
-        PagedWork pre = w;
-        pre.prefix_pass = 1;
-        pre.bases = nullptr;
-        pre.part_o = f32(pl.pre_o);
-        pre.part_ml = f32x2(pl.pre_ml);
-        pre.row_o = f32(pl.pre_row_o);
-        pre.row_ml = f32x2(pl.pre_row_ml);
-        rc = launch_pass(pl.pre, pre, d, stream);
+    PagedJoin p;
+    std::memset(&p, 0, sizeof(p));
+    const bool prefix = d->prefix_len > 0;
+    for (int i = prefix ? 1 : 0; i >= 0; --i) {  // the prefix first
+        const PagedScratch& s = pl.at[i];
+        w.prefix_pass = i;
+        w.part_o = reinterpret_cast<float*>(ws + s.part_o);
+        w.part_ml = reinterpret_cast<float2*>(ws + s.part_ml);
+        w.shared = reinterpret_cast<PagedShared*>(ws + s.shared);
+        if (prefix) {
+            w.row_o = reinterpret_cast<float*>(ws + s.row_o);
+            w.row_ml = reinterpret_cast<float2*>(ws + s.row_ml);
+            w.row_at = reinterpret_cast<int2*>(ws + s.row_at);
+        }
+        rc = launch_pass(pl.pass[i], w, d, stream);
         if (rc) return rc;
-        p.pre = PagedPrefixParts{pre.part_o, pre.part_ml, pre.row_o, pre.row_ml, pl.pre.rows, pl.pre.unit, pl.pre.grid};
+        p.pass[i] = PagedParts{w.part_o, w.part_ml, w.row_o, w.row_ml, w.row_at, pl.pass[i].rows, pl.pass[i].grid};
     }
-    rc = launch_pass(pl.own, w, d, stream);
-    if (rc) return rc;
+    p.shared = w.shared;
+    p.starts = w.kv.starts;
+    p.out = w.out;
+    p.ldo = w.ldo;
+    p.lse = w.lse;
+    p.ldl = w.ldl;
+    p.B = w.kv.B;
+    p.T = d->T;
+    p.HQ = d->HQ;
+    p.G = w.G;
+    p.by_G = w.by_G;
+    p.by_HQ.set(uint32_t(d->HQ));
+    // warps per row: see paged_join_kernel; with a prefix 1024 rows give every SM a row per warp
+    const int64_t rows = int64_t(d->T) * d->HQ;
+    const bool many = prefix ? rows >= 1024 : pl.pass[0].wide;
+    const int rpb = many ? kJoinWarps : 1;
+    const dim3 grid = prefix ? dim3(unsigned(std::min<int64_t>((rows + rpb - 1) / rpb, 1 << 20)))
+                             : dim3(pl.pass[0].grid, unsigned(std::min<int64_t>(pl.pass[0].rows, pl.tile_rows) + rpb - 1) / rpb);
     const bool bf = d->kv.dtype == BQ_DT_BF16;
-    const void* fn = d->kv.D == 128 ? (bf ? join_kernel<__nv_bfloat16, 128>(pl.own.wide) : join_kernel<__half, 128>(pl.own.wide))
-                                    : (bf ? join_kernel<__nv_bfloat16, 64>(pl.own.wide) : join_kernel<__half, 64>(pl.own.wide));
+    const void* fn = d->kv.D == 128 ? (bf ? join_kernel<__nv_bfloat16, 128>(prefix, many) : join_kernel<__half, 128>(prefix, many))
+                                    : (bf ? join_kernel<__nv_bfloat16, 64>(prefix, many) : join_kernel<__half, 64>(prefix, many));
     void* args[] = {&p};
-    return paged_launch(fn, dim3(d->T, d->HQ), dim3(kJoinThreads), 0, args, d->flags, stream, "paged attention join");
+    return paged_launch(fn, grid, dim3(32 * kJoinWarps), 0, args, d->flags, stream, "paged attention join");
 }
 
 }  // extern "C"

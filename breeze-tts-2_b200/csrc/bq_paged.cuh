@@ -57,6 +57,21 @@ __device__ __forceinline__ int paged_page(const PagedKV& kv, int b, int pos, boo
     return good ? page : 0;
 }
 
+// Division of 0 <= n < 2^31 by a constant of the launch: the round-up multiplier
+// of Granlund and Montgomery ("Division by invariant integers using
+// multiplication"), so that walking tiles and rows costs no integer division.
+struct FastDiv {
+    uint32_t mul, shift;
+    __host__ void set(uint32_t d) {
+        shift = 0;
+        while ((uint64_t(1) << shift) < d) ++shift;
+        mul = uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int operator()(int n) const {
+        return int((__umulhi(mul, uint32_t(n)) + uint32_t(n)) >> shift);
+    }
+};
+
 // ---------------------------------------------------------------- schedule
 // The attention kernels cut the batch into tiles of ROWS rows -- row r of
 // sequence b and kv head j is query head j * G + r % G of token r / G, so the
@@ -72,9 +87,14 @@ __device__ __forceinline__ int paged_page(const PagedKV& kv, int b, int pos, boo
 // With a shared prefix there are two such schedules: the prefix over all rows
 // of the batch at once (one pseudo-sequence), and each sequence's own positions
 // from prefix_len on.
+struct PagedShared {
+    int32_t parts, rows, r0, begin, j;  // CTAs that hold it (0: none), its rows, first row, first token of the sequence, kv head
+};
+
 struct PagedWork {
     PagedKV kv;
     int32_t G, causal, prefix_len, prefix_pass;  // prefix_pass: this launch handles [0, prefix_len) for all rows
+    FastDiv by_G;
     float scale_log2;                            // scale * log2(e): scores are kept in base 2
     const void* q;
     int64_t ldq;
@@ -82,12 +102,18 @@ struct PagedWork {
     int64_t ldo;
     float* lse;
     int64_t ldl;
-    long long* bases;  // [B + 1] first unit of every sequence, then their number (written by CTA 0)
     float* part_o;     // [2 grid][ROWS][D] unnormalized outputs of shared tiles
     float2* part_ml;   // [2 grid][ROWS] (largest score, sum of exponentials)
-    float* row_o;      // [T][HQ][D] own parts of tiles that one CTA holds, when a prefix part follows
+    PagedShared* shared;  // [grid] the shared tile that begins in each CTA
+    // with a prefix every row is joined from both passes' parts:
+    float* row_o;      // [T][HQ][D] parts of tiles that one CTA holds
     float2* row_ml;    // [T][HQ]
+    int2* row_at;      // [T][HQ] where the row's parts are (paged_row_at)
 };
+
+// Where a row's parts of one pass are: x = CTA of the first, y = parts << 8 | row
+// within the tile; no parts: in the row buffers.
+__device__ __forceinline__ int2 paged_row_at(int cta, int parts, int row) { return make_int2(cta, parts << 8 | row); }
 
 struct PagedSeq {
     int begin, count, rows, len, off;  // first row, new rows, rows * G, positions, position of the first new row
@@ -114,7 +140,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedWork& p, int b, bool& c
 template <int ROWS>
 __device__ __forceinline__ int paged_tile_limit(const PagedWork& p, const PagedSeq& s, int i) {
     if (p.prefix_pass || !p.causal) return s.len;
-    const int tok = (min(s.rows, (i + 1) * ROWS) - 1) / p.G;
+    const int tok = p.by_G(min(s.rows, (i + 1) * ROWS) - 1);
     return max(0, min(s.len, s.off + tok + 1));
 }
 
@@ -136,6 +162,7 @@ __device__ __forceinline__ int paged_head_units(const PagedWork& p, const PagedS
 struct PagedShare {
     long long q;
     int r;
+    PagedShare() = default;
     __device__ __forceinline__ PagedShare(long long U, int grid) {
         if (U >> 32) {
             q = U / grid;
@@ -154,17 +181,15 @@ struct PagedShare {
     }
 };
 
-// Partial slot of a shared tile whose first unit is u0, in the CTA whose share begins at lo.
-__device__ __forceinline__ int paged_slot(int cta, long long u0, long long lo) { return 2 * cta + (u0 < lo ? 0 : 1); }
-
 // Place of a CTA's first unit.
 struct PagedCursor {
     int b, j, i, k;        // sequence, kv head, tile, unit within the tile
     int tiles, head_units; // of sequence b
     long long u, hi;       // next unit, end of the share
+    PagedShare share;
 };
 
-// All NT threads: finds the share of CTA `cta`. CTA 0 also writes p.bases.
+// All NT threads: finds the share of CTA `cta`.
 template <int ROWS, int UNIT, int NT>
 __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, int grid) {
     __shared__ long long s_sum[NT / 32];
@@ -195,27 +220,24 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
         if (w < warp) before += s_sum[w];
         U += s_sum[w];
     }
-    const PagedShare sh(U, grid);
     PagedCursor c;
-    c.u = sh.lo(cta);
-    c.hi = sh.lo(cta + 1);
-    const bool has = mine > 0 && c.u < c.hi && c.u >= before && c.u < before + mine;
-    if (has || (cta == 0 && p.bases)) {
+    c.share = PagedShare(U, grid);
+    c.u = c.share.lo(cta);
+    c.hi = c.share.lo(cta + 1);
+    if (mine > 0 && c.u < c.hi && c.u >= before && c.u < before + mine) {
         long long at = before;
         for (int b = b0; b < b1; ++b) {
             bool cut;
             const PagedSeq s = paged_seq(p, b, cut);
             const long long n =
                 (long long)paged_head_units<ROWS, UNIT>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
-            if (has && c.u >= at && c.u < at + n) {
+            if (c.u >= at && c.u < at + n) {
                 s_b = b;
                 s_rem = c.u - at;
             }
-            if (cta == 0 && p.bases) p.bases[b] = at;
             at += n;
         }
     }
-    if (cta == 0 && p.bases && threadIdx.x == 0) p.bases[B] = U;
     __syncthreads();
     c.b = s_b;
     c.i = c.j = c.k = c.tiles = c.head_units = 0;
@@ -258,7 +280,7 @@ __device__ __forceinline__ void paged_next(const PagedWork& p, PagedCursor& c) {
 
 // Positions [0, limit) are seen by row r (of sequence s; in the prefix pass, of all rows).
 __device__ __forceinline__ int paged_row_limit(const PagedWork& p, const PagedSeq& s, int r) {
-    const int tok = r / p.G;
+    const int tok = p.by_G(r);
     if (!p.prefix_pass) return p.causal ? max(0, min(s.len, s.off + tok + 1)) : s.len;
     int b = tok;
     if (p.kv.starts) {  // the sequence of row tok: starts[b] <= tok < starts[b + 1]

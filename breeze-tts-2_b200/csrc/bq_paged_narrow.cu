@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
     pdl_launch_dependents();
     pdl_wait();
     PagedCursor c = paged_find<ROWS, UNIT, kThreads>(p, blockIdx.x, gridDim.x);
-    const long long lo = c.u;
+    bool shares = false;  // the last tile goes on in the next CTA
     const int kv_lo = p.prefix_pass ? 0 : p.prefix_len;
     const uint32_t ring = sb + warp * SM::kRing;
 
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
 
         // query tile: row r0 + r is head j G + (r0 + r) % G of token (r0 + r) / G
         for (int idx = threadIdx.x; idx < ROWS * CH; idx += kThreads) {
-            const int r = idx / CH, ch = idx - r * CH, rr = r0 + min(r, nrows - 1), tok = rr / p.G;
+            const int r = idx / CH, ch = idx - r * CH, rr = r0 + min(r, nrows - 1), tok = p.by_G(rr);
             const E* src = static_cast<const E*>(p.q) + int64_t(s.begin + tok) * p.ldq + (c.j * p.G + rr - tok * p.G) * D + ch * 8;
             cp_async16_zfill(sb + SM::kQ + r * (D * 2) + ((ch ^ (r & 7)) << 4), src, r < nrows);
         }
@@ -236,7 +236,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
         }
         __syncthreads();
         const bool whole = c.k == 0 && nu == units;
-        const int slot = paged_slot(blockIdx.x, c.u - c.k, lo);
+        const int slot = 2 * blockIdx.x + (c.k == 0 ? 1 : 0);
+        const int parts = whole || c.k ? 0 : c.share.owner(c.u + units - 1) - int(blockIdx.x) + 1;
+        if (parts) {
+            shares = true;
+            if (threadIdx.x == 0) p.shared[blockIdx.x] = PagedShared{parts, nrows, r0, s.begin, c.j};
+        }
         for (int idx = threadIdx.x; idx < nrows * (D / 4); idx += kThreads) {
             const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
             float mm = -INFINITY, ll = 0.f;
@@ -251,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
                 ll = fmaf(f, s_ml[w][r].y, ll);
                 a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
             }
-            const int rr = r0 + r, tok = rr / p.G, head = c.j * p.G + rr - tok * p.G;
+            const int rr = r0 + r, tok = p.by_G(rr), head = c.j * p.G + rr - tok * p.G;
             const int64_t row = s.begin + tok;
             if (whole && !p.row_o) {
                 const float inv = ll > 0.f ? 1.f / ll : 0.f;
@@ -261,13 +266,17 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
             } else {
                 const int64_t at = whole ? row * kv.HQ + head : int64_t(slot) * ROWS + r;
                 *reinterpret_cast<float4*>((whole ? p.row_o : p.part_o) + at * D + d) = a;
-                if (d == 0) (whole ? p.row_ml : p.part_ml)[at] = make_float2(mm, ll);
+                if (d == 0) {
+                    (whole ? p.row_ml : p.part_ml)[at] = make_float2(mm, ll);
+                    if (p.row_at && c.k == 0) p.row_at[row * kv.HQ + head] = paged_row_at(blockIdx.x, parts, r);
+                }
             }
         }
         __syncthreads();  // the rings are free again
         c.u += nu;
         paged_next<ROWS, UNIT>(p, c);
     }
+    if (!shares && threadIdx.x == 0) p.shared[blockIdx.x].parts = 0;
 }
 
 }  // namespace

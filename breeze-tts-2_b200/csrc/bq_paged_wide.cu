@@ -159,7 +159,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
     tc_fence_after();
     pdl_launch_dependents();
     const uint32_t tmem = s_tmem;  // scores / probabilities of half h at columns 128 h, outputs at 256 + 128 h
-    const long long lo = c.u;
     const int sequences = w.prefix_pass ? 1 : kv.B;
 
     if (warp < 8) {
@@ -168,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
         const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
         const uint32_t t_s = lanes + 128 * h, t_o = lanes + 256 + 128 * h;
         int seg = 0, ph_s = 0, it = 0;  // tiles of this half done, score phases, ring stages passed
-        bool ok = true;
+        bool ok = true, shares = false;  // shares: the last tile goes on in the next CTA
         for (; ok && c.u < c.hi && c.b < sequences;) {
             const WideTile t(w, c);
             const int hrows = t.nrows - 128 * h;  // valid rows of this half
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     const int r = idx / CH, ch = idx - r * CH;
                     uint4 v = make_uint4(0, 0, 0, 0);
                     if (r < hrows) {
-                        const int rr = t.r0 + 128 * h + r, tok = rr / w.G;
+                        const int rr = t.r0 + 128 * h + r, tok = w.by_G(rr);
                         v = *reinterpret_cast<const uint4*>(static_cast<const E*>(w.q) + int64_t(t.s.begin + tok) * w.ldq +
                                                             (c.j * w.G + rr - tok * w.G) * D + ch * 8);
                     }
@@ -268,12 +267,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 if (!ok) break;
                 ++seg;
                 tc_fence_after();
+                const bool whole = c.k == 0 && t.nu == t.units, final = whole && !w.row_o;
+                const int parts = whole || c.k ? 0 : c.share.owner(c.u + t.units - 1) - int(blockIdx.x) + 1;
+                if (parts) {
+                    shares = true;
+                    if (threadIdx.x == 0) w.shared[blockIdx.x] = PagedShared{parts, t.nrows, t.r0, t.s.begin, c.j};
+                }
                 if (!idle) {
-                    const bool whole = c.k == 0 && t.nu == t.units, final = whole && !w.row_o;
-                    const int tok = myrow / w.G, head = c.j * w.G + myrow - tok * w.G;
+                    const int tok = w.by_G(myrow), head = c.j * w.G + myrow - tok * w.G;
                     const int64_t orow = t.s.begin + tok;
                     const int64_t at = whole ? orow * kv.HQ + head
-                                             : int64_t(paged_slot(blockIdx.x, c.u - c.k, lo)) * kRows + 128 * h + row;
+                                             : int64_t(2 * blockIdx.x + (c.k == 0 ? 1 : 0)) * kRows + 128 * h + row;
                     const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
                     for (int q = 0; q < D / 16; ++q) {
@@ -297,10 +301,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                         }
                     }
                     if (row < hrows) {
-                        if (!final)
+                        if (!final) {
                             (whole ? w.row_ml : w.part_ml)[at] = make_float2(mref, l);
-                        else if (w.lse)
+                            if (w.row_at && c.k == 0)
+                                w.row_at[orow * kv.HQ + head] = paged_row_at(blockIdx.x, parts, 128 * h + row);
+                        } else if (w.lse) {
                             w.lse[orow * w.ldl + head] = l > 0.f ? (mref + log2f(l)) * kLn2 : -INFINITY;
+                        }
                     }
                 }
                 __syncwarp();
@@ -311,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             c.u += t.nu;
             paged_next<kRows, kUnit>(w, c);
         }
+        if (threadIdx.x == 0 && !shares) w.shared[blockIdx.x].parts = 0;
     } else if (warp == 8) {
         // ------------------------------------------------------------ k / v loads
         int it = 0;

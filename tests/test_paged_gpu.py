@@ -349,18 +349,18 @@ def test_append_flags_what_does_not_fit():
     cases = [("page", _lib.BQ_DEVERR_PAGE), ("table", _lib.BQ_DEVERR_POSITION), ("rope", _lib.BQ_DEVERR_POSITION)]
     for what, bit in cases:
         c = pc.batch([40, 20], None, 2, 1, 64, 16, BF, seed=1, spare_cols=0)
-        qkv = torch.randn(2, 4 * 64).to(BF)
+        qkv = torch.randn(2, 4 * 64, generator=torch.Generator().manual_seed(12)).to(BF)
         cos, sin = rope(30 if what == "rope" else 64, 64, BF)
         if what == "page":
             c["table"][0, 2] = -3
         if what == "table":
             c["lens"][0] = 49
         d = pc.to(c, DEV)
-        out = torch.full((2, 128), 3.0, dtype=BF, device=DEV)
+        out = torch.full((2, 128), 300.0, dtype=BF, device=DEV)  # no q is that large
         _api().paged_append(qkv.to(DEV), cos.to(DEV), sin.to(DEV), d["k"], d["v"], d["table"], d["lens"], out=out)
         torch.cuda.synchronize()
         assert _status() == bit
-        assert (out[0] == 3.0).all() and not (out[1] == 3.0).any()
+        assert (out[0] == 300.0).all() and not (out[1] == 300.0).any()
         k = d["k"].cpu()
         changed = (k.view(torch.int16) != c["k"].view(torch.int16)).any(-1).any(1).nonzero().tolist()
         assert changed == [[int(c["table"][1, 1]), 3]]
