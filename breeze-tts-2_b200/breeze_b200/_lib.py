@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -135,6 +136,19 @@ class PagedAttnDesc(ctypes.Structure):
     ]
 
 
+_PACK_CODES = {ctypes.c_int32: "i", ctypes.c_uint32: "I", ctypes.c_float: "f", ctypes.c_int64: "q", ctypes.c_void_p: "Q"}
+
+
+def packer(desc: type[ctypes.Structure]):
+    """A function of the descriptor's field values (NULL pointers as 0) that
+    returns its bytes. An argument of type c_void_p takes them as they are; a
+    third of the time that filling a Structure takes."""
+    s = struct.Struct("<" + "".join(_PACK_CODES[t] for _, t in desc._fields_))
+    if s.size != ctypes.sizeof(desc):
+        raise TypeError(f"{desc.__name__} has padding")
+    return s.pack
+
+
 class ChainOptions(ctypes.Structure):
     """bq_chain_options (include/breeze_b200.h)."""
 
@@ -174,10 +188,9 @@ _SIGS = {
     "bq_embed_rows": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
                                        ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,
                                        ctypes.c_uint32, ctypes.c_void_p]),
-    "bq_paged_append": (ctypes.c_int32, [ctypes.POINTER(PagedAppendDesc), ctypes.c_void_p]),
-    "bq_paged_attention_workspace_bytes": (ctypes.c_int32, [ctypes.POINTER(PagedAttnDesc), ctypes.POINTER(ctypes.c_size_t)]),
-    "bq_paged_attention": (ctypes.c_int32, [ctypes.POINTER(PagedAttnDesc), ctypes.c_void_p, ctypes.c_size_t,
-                                            ctypes.c_void_p]),
+    "bq_paged_append": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
+    "bq_paged_attention_workspace_bytes": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "bq_paged_attention": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "bq_int4_tinygemm_pack": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
                                                ctypes.c_int32, ctypes.c_void_p]),
     "bq_int4_tinygemm_unpack": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,

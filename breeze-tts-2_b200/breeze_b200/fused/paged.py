@@ -43,50 +43,64 @@ import torch
 
 from .. import _lib
 
-_I32 = torch.int32
+_I32, _F32 = torch.int32, torch.float32
+_pack_append = _lib.packer(_lib.PagedAppendDesc)
+_pack_attn = _lib.packer(_lib.PagedAttnDesc)
+_WORKSPACE: dict = {}  # bytes by shape; a decode loop asks once
 
 
-def _check(cond: bool, message: str) -> None:
-    if not cond:
-        raise ValueError(message)
-
-
-def _cache_fields(rows: int, dtype: torch.dtype, dev: torch.device, k_pages, v_pages, page_table, seq_lens, q_starts):
-    """The leading fields of both descriptors, after the checks both calls share."""
-    for t in (k_pages, v_pages, page_table, seq_lens, q_starts):
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
-    if dev.type != "cuda":
-        raise RuntimeError("breeze_b200 kernels need CUDA tensors (there is no CPU path)")
-    _check(dtype in (torch.bfloat16, torch.float16), f"paged caches are bf16 or fp16 (got {dtype})")
-    _check(k_pages.dtype == dtype and v_pages.dtype == dtype, "rows and pages must have one dtype")
-    shape = k_pages.shape
-    _check(len(shape) == 4 and v_pages.shape == shape, "k_pages and v_pages must be (pages, HKV, page size, D)")
-    ks, vs = k_pages.stride(), v_pages.stride()
-    _check(ks[3] == 1 and vs[3] == 1, "the last dimension of the pages must be contiguous")
-    _check(page_table.dtype == _I32 and page_table.dim() == 2 and page_table.stride(1) == 1,
-           "page_table must be int32 (B, columns) with contiguous rows")
-    batch, columns = page_table.shape
-    _check(seq_lens.dtype == _I32 and seq_lens.shape == (batch,) and seq_lens.is_contiguous(),
-           "seq_lens must be a contiguous int32 (B,)")
-    if q_starts is None:
-        _check(rows == batch, f"{rows} rows for {batch} sequences: ragged rows need q_starts")
-        starts = None
-    else:
-        _check(q_starts.dtype == _I32 and q_starts.shape == (batch + 1,) and q_starts.is_contiguous(),
-               "q_starts must be a contiguous int32 (B + 1,)")
-        starts = q_starts.data_ptr()
-    pages, hkv, size, dim = shape
-    _check(pages > 0 and hkv > 0 and columns > 0 and batch > 0, "empty cache or batch")
-    return (batch, hkv, dim, size, pages, columns, _lib._DT[dtype], 0, k_pages.data_ptr(), ks[0], ks[1], ks[2],
-            v_pages.data_ptr(), vs[0], vs[1], vs[2], page_table.data_ptr(),
-            page_table.stride(0) if batch > 1 else columns, seq_lens.data_ptr(), starts)
-
-
-def _row_tensor(t: torch.Tensor, name: str) -> int:
+def _row_stride(t: torch.Tensor, name: str) -> int:
     """Row stride of a 2-D tensor with contiguous rows."""
-    _check(t.dim() == 2 and t.stride(1) == 1, f"{name} must be a 2-D tensor with unit stride in the last dimension")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    st = t.stride()
+    if len(st) != 2 or st[1] != 1:
+        raise ValueError(f"{name} must be a 2-D tensor with unit stride in the last dimension")
+    return st[0] if t.shape[0] > 1 else t.shape[1]
+
+
+def _cache_fields(x: torch.Tensor, rows: int, k_pages, v_pages, page_table, seq_lens, q_starts):
+    """The leading fields of both descriptors, after the checks both calls share."""
+    dev, dtype = x.get_device(), x.dtype
+    if dev < 0:
+        raise RuntimeError("breeze_b200 kernels need CUDA tensors (there is no CPU path)")
+    if (k_pages.get_device() != dev or v_pages.get_device() != dev or page_table.get_device() != dev
+            or seq_lens.get_device() != dev or (q_starts is not None and q_starts.get_device() != dev)):
+        raise RuntimeError(f"tensors on different devices: rows on {x.device}, cache or lengths elsewhere")
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"paged caches are bf16 or fp16 (got {dtype})")
+    if k_pages.dtype != dtype or v_pages.dtype != dtype:
+        raise ValueError(f"rows and pages must have one dtype (got {dtype}, {k_pages.dtype}, {v_pages.dtype})")
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
+        raise ValueError("k_pages and v_pages must be (pages, HKV, page size, D) of one shape")
+    ks, vs, ts = k_pages.stride(), v_pages.stride(), page_table.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise ValueError("the last dimension of the pages must be contiguous")
+    if page_table.dtype != _I32 or len(ts) != 2 or ts[1] != 1:
+        raise ValueError("page_table must be int32 (B, columns) with contiguous rows")
+    batch, columns = page_table.shape
+    if seq_lens.dtype != _I32 or seq_lens.shape != (batch,) or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be a contiguous int32 (B,)")
+    starts = 0
+    if q_starts is not None:
+        if q_starts.dtype != _I32 or q_starts.shape != (batch + 1,) or not q_starts.is_contiguous():
+            raise ValueError("q_starts must be a contiguous int32 (B + 1,)")
+        starts = q_starts.data_ptr()
+    elif rows != batch:
+        raise ValueError(f"{rows} rows for {batch} sequences: ragged rows need q_starts")
+    pages, hkv, size, dim = shape
+    if pages == 0 or hkv == 0 or dim == 0 or columns == 0 or batch == 0:
+        raise ValueError("empty cache or batch")
+    return (batch, hkv, dim, size, pages, columns, _lib._DT[dtype], 0, k_pages.data_ptr(), ks[0], ks[1], ks[2],
+            v_pages.data_ptr(), vs[0], vs[1], vs[2], page_table.data_ptr(), ts[0] if batch > 1 else columns,
+            seq_lens.data_ptr(), starts)
+
+
+def _on_device(dev: int, call, *args):
+    """call(*args) with ``dev`` as the current device."""
+    if dev == torch.cuda.current_device():
+        return call(*args)
+    with torch.cuda.device(dev):
+        return call(*args)
 
 
 def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -100,70 +114,78 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_page
     takes them. The math is fp32 with one rounding at the end. ``out`` may be
     ``qkv[:, :HQ * D]`` itself. Tokens of an unused batch slot (seq_lens[b] less
     than its new tokens) are skipped where their position would be negative."""
-    dev, dtype = qkv.device, qkv.dtype
-    ldqkv = _row_tensor(qkv, "qkv")
+    ldqkv = _row_stride(qkv, "qkv")
     rows, width = qkv.shape
-    fields = _cache_fields(rows, dtype, dev, k_pages, v_pages, page_table, seq_lens, q_starts)
+    dev, dtype = qkv.get_device(), qkv.dtype
+    fields = _cache_fields(qkv, rows, k_pages, v_pages, page_table, seq_lens, q_starts)
     hkv, dim = fields[1], fields[2]
     hq = width // dim - 2 * hkv
-    _check(hq > 0 and (hq + 2 * hkv) * dim == width, f"qkv width {width} does not split into heads of {dim}")
-    _check(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == dim and cos.dtype == sin.dtype,
-           "cos and sin must be (positions, D) tables of one shape and dtype")
-    _check(cos.dtype == dtype or cos.dtype == torch.float32, "cos and sin must be fp32 or the cache's dtype")
-    ldcs = _row_tensor(cos, "cos")
-    _check(_row_tensor(sin, "sin") == ldcs, "cos and sin must have equal strides")
-    _check((q_norm_w is None) == (k_norm_w is None), "q_norm_w and k_norm_w go together")
-    for t in (cos, sin, q_norm_w, k_norm_w, out):
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
-    if q_norm_w is not None:
+    if hq <= 0 or (hq + 2 * hkv) * dim != width:
+        raise ValueError(f"qkv width {width} does not split into q, k and v heads of {dim}")
+    ldcs, cs_dtype = _row_stride(cos, "cos"), cos.dtype
+    if cos.shape != sin.shape or cos.shape[1] != dim or cs_dtype != sin.dtype or _row_stride(sin, "sin") != ldcs:
+        raise ValueError("cos and sin must be (positions, D) tables of one shape, stride and dtype")
+    if cs_dtype != dtype and cs_dtype != _F32:
+        raise ValueError(f"cos and sin must be fp32 or the cache's dtype (got {cs_dtype})")
+    if cos.get_device() != dev or sin.get_device() != dev:
+        raise RuntimeError("cos and sin are on another device than qkv")
+    qn = kn = 0
+    if q_norm_w is not None and k_norm_w is not None:
         for t in (q_norm_w, k_norm_w):
-            _check(t.dtype == dtype and t.shape == (dim,) and t.is_contiguous(),
-                   "norm weights must be contiguous (D,) vectors of the cache's dtype")
+            if t.dtype != dtype or t.shape != (dim,) or not t.is_contiguous() or t.get_device() != dev:
+                raise ValueError("norm weights must be contiguous (D,) vectors of the cache's dtype and device")
+        qn, kn = q_norm_w.data_ptr(), k_norm_w.data_ptr()
+    elif q_norm_w is not None or k_norm_w is not None:
+        raise ValueError("q_norm_w and k_norm_w go together")
     if out is None:
-        out = torch.empty(rows, hq * dim, device=dev, dtype=dtype)
-    else:
-        _check(out.shape == (rows, hq * dim) and out.dtype == dtype, "out must be (T, HQ D) of the cache's dtype")
-    desc = _lib.PagedAppendDesc(
-        *fields, rows, hq, _lib._DT[cos.dtype], cos.shape[0], eps, _lib.default_flags(), qkv.data_ptr(), ldqkv,
-        cos.data_ptr(), sin.data_ptr(), ldcs, None if q_norm_w is None else q_norm_w.data_ptr(),
-        None if k_norm_w is None else k_norm_w.data_ptr(), out.data_ptr(), _row_tensor(out, "out"))
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().bq_paged_append(ctypes.byref(desc), _lib._stream(dev)), "bq_paged_append")
+        out = qkv.new_empty((rows, hq * dim))
+    elif out.shape != (rows, hq * dim) or out.dtype != dtype or out.get_device() != dev:
+        raise ValueError("out must be (T, HQ D) of the cache's dtype and device")
+    desc = _pack_append(*fields, rows, hq, _lib._DT[cs_dtype], cos.shape[0], eps, _lib.default_flags(), qkv.data_ptr(),
+                        ldqkv, cos.data_ptr(), sin.data_ptr(), ldcs, qn, kn, out.data_ptr(), _row_stride(out, "out"))
+    _lib.check(_on_device(dev, _lib.load().bq_paged_append, desc, torch._C._cuda_getCurrentRawStream(dev)),
+               "bq_paged_append")
     return out
 
 
+def _workspace_bytes(desc: bytes) -> int:
+    need = ctypes.c_size_t(0)
+    _lib.check(_lib.load().bq_paged_attention_workspace_bytes(desc, ctypes.byref(need)),
+               "bq_paged_attention_workspace_bytes")
+    return need.value
+
+
 def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, causal, max_q, out, lse):
-    dev, dtype = q.device, q.dtype
-    ldq = _row_tensor(q, "q")
+    ldq = _row_stride(q, "q")
     rows, width = q.shape
-    fields = _cache_fields(rows, dtype, dev, k_pages, v_pages, page_table, seq_lens, q_starts)
+    dev = q.get_device()
+    fields = _cache_fields(q, rows, k_pages, v_pages, page_table, seq_lens, q_starts)
     hkv, dim = fields[1], fields[2]
     hq = width // dim
-    _check(hq > 0 and hq * dim == width and hq % hkv == 0,
-           f"q width {width} does not split into heads of {dim} over {hkv} kv heads")
+    if hq == 0 or hq * dim != width or hq % hkv:
+        raise ValueError(f"q width {width} does not split into heads of {dim} over {hkv} kv heads")
     if out is None:
-        out = torch.empty(rows, width, device=dev, dtype=dtype)
-    else:
-        _check(out.shape == (rows, width) and out.dtype == dtype and out.device == dev,
-               "out must be (T, HQ D) of q's dtype and device")
-    lse_ptr, ldl = None, 0
+        out = q.new_empty((rows, width))
+    elif out.shape != (rows, width) or out.dtype != q.dtype or out.get_device() != dev:
+        raise ValueError("out must be (T, HQ D) of q's dtype and device")
+    lse_ptr = ldl = 0
     if lse is not None:
-        _check(lse.shape == (rows, hq) and lse.dtype == torch.float32 and lse.device == dev,
-               "lse must be fp32 (T, HQ) on q's device")
-        lse_ptr, ldl = lse.data_ptr(), _row_tensor(lse, "lse")
-    desc = _lib.PagedAttnDesc(
-        *fields, rows, hq, prefix_len, 0 if max_q is None else max_q, dim ** -0.5 if scale is None else scale,
-        _lib.default_flags() | (0 if causal else _lib.PAGED_FULL), q.data_ptr(), ldq, out.data_ptr(),
-        _row_tensor(out, "out"), lse_ptr, ldl)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        need = ctypes.c_size_t(0)
-        _lib.check(lib.bq_paged_attention_workspace_bytes(ctypes.byref(desc), ctypes.byref(need)),
-                   "bq_paged_attention_workspace_bytes")
-        ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
-        _lib.check(lib.bq_paged_attention(ctypes.byref(desc), None if ws is None else ws.data_ptr(), need.value,
-                                          _lib._stream(dev)), "bq_paged_attention")
+        if lse.shape != (rows, hq) or lse.dtype != _F32 or lse.get_device() != dev:
+            raise ValueError("lse must be fp32 (T, HQ) on q's device")
+        lse_ptr, ldl = lse.data_ptr(), _row_stride(lse, "lse")
+    max_q = 0 if max_q is None else max_q
+    desc = _pack_attn(*fields, rows, hq, prefix_len, max_q, dim ** -0.5 if scale is None else scale,
+                      _lib.default_flags() | (0 if causal else _lib.PAGED_FULL), q.data_ptr(), ldq, out.data_ptr(),
+                      _row_stride(out, "out"), lse_ptr, ldl)
+    key = (dev, rows, hq, hkv, dim, fields[0], prefix_len > 0, max_q, q_starts is None)
+    need = _WORKSPACE.get(key)
+    if need is None:
+        if len(_WORKSPACE) >= 4096:
+            _WORKSPACE.clear()
+        need = _WORKSPACE[key] = _on_device(dev, _workspace_bytes, desc)
+    ws = torch.empty(need, device=q.device, dtype=torch.uint8)
+    _lib.check(_on_device(dev, _lib.load().bq_paged_attention, desc, ws.data_ptr(), need,
+                          torch._C._cuda_getCurrentRawStream(dev)), "bq_paged_attention")
     return out
 
 

@@ -342,7 +342,7 @@ int validate_attention(const bq_paged_attn_desc* d) {
     const int rc = paged_validate(&d->kv, d->T, d->HQ);
     if (rc) return rc;
     const int width = d->HQ * d->kv.D;
-    if (!d->q || !d->out) return set_error(BQ_ERR_INVALID_ARG, "q and out must be non-NULL");
+    if (d->T && (!d->q || !d->out)) return set_error(BQ_ERR_INVALID_ARG, "q and out must be non-NULL");
     if (d->ldq < width || d->ldo < width)
         return set_error(BQ_ERR_SHAPE, "row strides %lld / %lld < %d", (long long)d->ldq, (long long)d->ldo, width);
     if (d->lse && d->ldl < d->HQ) return set_error(BQ_ERR_SHAPE, "lse row stride %lld < %d", (long long)d->ldl, d->HQ);

@@ -394,3 +394,61 @@ def test_append_then_attention_follows_a_growing_batch():
         torch.cuda.synchronize()
         case = dict(c, q=q.cpu(), k=k.cpu(), v=v.cpu(), table=table, lens=torch.tensor(lens), starts=starts, rows=rows)
         compare(case, out.cpu(), lse.cpu())
+
+
+def test_python_refusals():
+    P = _api()
+    c = pc.to(pc.batch([40, 20], None, 4, 2, 64, 16, BF, seed=1), DEV)
+    cos, sin = (t.to(DEV) for t in rope(64, 64, BF))
+    qkv = torch.zeros(2, 8 * 64, dtype=BF, device=DEV)
+    good = dict(q=c["q"], k_pages=c["k"], v_pages=c["v"], page_table=c["table"], seq_lens=c["lens"])
+    for change, error, text in [
+        (dict(q=c["q"].float()), ValueError, "bf16 or fp16"),
+        (dict(q=c["q"].half()), ValueError, "one dtype"),
+        (dict(q=c["q"][:, :100]), ValueError, "does not split"),
+        (dict(q=c["q"][:, ::2]), ValueError, "unit stride"),
+        (dict(q=c["q"][:1]), ValueError, "ragged rows need q_starts"),
+        (dict(q=c["q"][:, :192]), ValueError, "does not split"),
+        (dict(v_pages=c["v"][1:]), ValueError, "one shape"),
+        (dict(k_pages=c["k"].transpose(2, 3)), ValueError, "one shape|contiguous"),
+        (dict(page_table=c["table"].long()), ValueError, "int32"),
+        (dict(page_table=c["table"].t()), ValueError, "contiguous rows|seq_lens"),
+        (dict(seq_lens=c["lens"].long()), ValueError, "int32"),
+        (dict(seq_lens=c["lens"][:1]), ValueError, "int32"),
+        (dict(q_starts=torch.zeros(2, dtype=torch.int32, device=DEV)), ValueError, "q_starts"),
+        (dict(seq_lens=c["lens"].cpu()), RuntimeError, "different devices"),
+        (dict(out=torch.empty(2, 128, dtype=BF, device=DEV)), ValueError, "out must be"),
+        (dict(lse=torch.empty(2, 4, dtype=BF, device=DEV)), ValueError, "lse must be"),
+        (dict(scale=-1.0), ValueError, "scale"),
+    ]:
+        with pytest.raises(error, match=text):
+            P.paged_attention(**{**good, **change})
+    with pytest.raises(ValueError, match="multiple of the page size"):
+        P.prefix_attention(**good, prefix_len=17)
+    put = dict(qkv=qkv, cos=cos, sin=sin, k_pages=c["k"], v_pages=c["v"], page_table=c["table"], seq_lens=c["lens"])
+    for change, error, text in [
+        (dict(qkv=qkv[:, :4 * 64]), ValueError, "does not split"),
+        (dict(qkv=qkv[:, :500]), ValueError, "does not split"),
+        (dict(cos=cos.half()), ValueError, "cos and sin"),
+        (dict(cos=cos.half(), sin=sin.half()), ValueError, "fp32 or the cache's dtype"),
+        (dict(cos=cos[:, :32], sin=sin[:, :32]), ValueError, "cos and sin"),
+        (dict(q_norm_w=cos[0]), ValueError, "go together"),
+        (dict(q_norm_w=cos[0], k_norm_w=sin[0].float()), ValueError, "norm weights"),
+        (dict(out=qkv), ValueError, "out must be"),
+        (dict(sin=sin.cpu()), RuntimeError, "another device"),
+    ]:
+        with pytest.raises(error, match=text):
+            P.paged_append(**{**put, **change})
+
+
+def test_no_rows():
+    """A ragged call without new rows is answered without a launch."""
+    P = _api()
+    c = pc.to(pc.batch([40, 20], None, 4, 2, 64, 16, BF, seed=1), DEV)
+    starts = torch.zeros(3, dtype=torch.int32, device=DEV)
+    cos, sin = (t.to(DEV) for t in rope(64, 64, BF))
+    args = (c["k"], c["v"], c["table"], c["lens"])
+    empty = torch.empty(0, 8 * 64, dtype=BF, device=DEV)
+    assert P.paged_append(empty, cos, sin, *args, q_starts=starts).shape == (0, 4 * 64)
+    assert P.paged_attention(empty[:, :256], *args, q_starts=starts).shape == (0, 256)
+    assert P.prefix_attention(empty[:, :256], *args, 16, q_starts=starts).shape == (0, 256)
