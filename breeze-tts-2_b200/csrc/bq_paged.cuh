@@ -78,7 +78,9 @@ struct FastDiv {
 // query heads that share a kv head share a tile -- and each tile's positions
 // into units of UNIT. All units of the batch, in (sequence, kv head, tile,
 // position) order, are dealt to the CTAs in equal contiguous shares: however
-// uneven the lengths, every CTA reads the same number of positions. A tile
+// uneven the lengths, every CTA has the same work. A tile costs its units plus
+// OVERHEAD more for its start and end (queries in, outputs out): the CTA whose
+// share holds only those does nothing for the tile. A tile
 // that ends up in several CTAs leaves one partial (largest score, sum of
 // exponentials, unnormalized output) per CTA; a CTA can only share its first
 // and its last tile, so two partial slots per CTA hold them all, and a second
@@ -151,9 +153,10 @@ __device__ __forceinline__ int paged_tile_units(const PagedWork& p, const PagedS
     return max(1, (n + UNIT - 1) / UNIT);
 }
 
-template <int ROWS, int UNIT>
-__device__ __forceinline__ int paged_head_units(const PagedWork& p, const PagedSeq& s, int tiles) {
-    int n = 0;
+// Cost of the tiles of one kv head, in units.
+template <int ROWS, int UNIT, int OVERHEAD>
+__device__ __forceinline__ int paged_head_cost(const PagedWork& p, const PagedSeq& s, int tiles) {
+    int n = tiles * OVERHEAD;
     for (int i = 0; i < tiles; ++i) n += paged_tile_units<ROWS, UNIT>(p, s, i);
     return n;
 }
@@ -181,16 +184,35 @@ struct PagedShare {
     }
 };
 
-// Place of a CTA's first unit.
+// Place in a CTA's share.
 struct PagedCursor {
-    int b, j, i, k;        // sequence, kv head, tile, unit within the tile
-    int tiles, head_units; // of sequence b
-    long long u, hi;       // next unit, end of the share
+    int b, j, i, k;   // sequence, kv head, tile, cost units of the tile that lie before
+    int tiles;        // of sequence b
+    long long u, hi;  // cost units of the batch that lie before, end of the share
     PagedShare share;
 };
 
+// The part of the tile at the cursor that lies in the share: units [k0, k0 + nu)
+// of `units`; nu = 0: only overhead.
+template <int ROWS, int UNIT, int OVERHEAD>
+struct PagedSegment {
+    int units, k0, nu, cost;
+    PagedSegment() = default;
+    __device__ __forceinline__ PagedSegment(const PagedWork& p, const PagedSeq& s, const PagedCursor& c) {
+        units = paged_tile_units<ROWS, UNIT>(p, s, c.i);
+        cost = int(min((long long)(units + OVERHEAD - c.k), c.hi - c.u));
+        k0 = max(0, c.k - OVERHEAD);
+        nu = max(0, c.k + cost - OVERHEAD) - k0;
+    }
+    __device__ __forceinline__ bool whole() const { return nu == units; }
+    // CTAs that hold the tile when it begins in this one and goes on, else 0
+    __device__ __forceinline__ int parts(const PagedCursor& c, int cta) const {
+        return whole() || k0 > 0 ? 0 : c.share.owner(c.u - c.k + units + OVERHEAD - 1) - cta + 1;
+    }
+};
+
 // All NT threads: finds the share of CTA `cta`.
-template <int ROWS, int UNIT, int NT>
+template <int ROWS, int UNIT, int OVERHEAD, int NT>
 __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, int grid) {
     __shared__ long long s_sum[NT / 32];
     __shared__ long long s_rem;
@@ -203,7 +225,7 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
         bool cut;
         const PagedSeq s = paged_seq(p, b, cut);
         if (cut && cta == 0) atomicOr(&g_device_error, BQ_DEVERR_POSITION_BIT);
-        mine += (long long)paged_head_units<ROWS, UNIT>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
+        mine += (long long)paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
     }
     long long incl = mine;
 #pragma unroll
@@ -230,7 +252,7 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
             bool cut;
             const PagedSeq s = paged_seq(p, b, cut);
             const long long n =
-                (long long)paged_head_units<ROWS, UNIT>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
+                (long long)paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
             if (c.u >= at && c.u < at + n) {
                 s_b = b;
                 s_rem = c.u - at;
@@ -240,7 +262,7 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
     }
     __syncthreads();
     c.b = s_b;
-    c.i = c.j = c.k = c.tiles = c.head_units = 0;
+    c.i = c.j = c.k = c.tiles = 0;
     if (c.b < 0) {
         c.hi = c.u;  // nothing for this CTA
         return c;
@@ -248,12 +270,12 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
     bool cut;
     const PagedSeq s = paged_seq(p, c.b, cut);
     c.tiles = (s.rows + ROWS - 1) / ROWS;
-    c.head_units = paged_head_units<ROWS, UNIT>(p, s, c.tiles);
-    long long rem = s_rem;
-    c.j = (rem >> 32) ? int(rem / c.head_units) : int(uint32_t(rem) / uint32_t(c.head_units));
-    int left = int(rem - (long long)c.j * c.head_units);
+    const int head = paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, c.tiles);
+    const long long rem = s_rem;
+    c.j = (rem >> 32) ? int(rem / head) : int(uint32_t(rem) / uint32_t(head));
+    int left = int(rem - (long long)c.j * head);
     for (;; ++c.i) {
-        const int n = paged_tile_units<ROWS, UNIT>(p, s, c.i);
+        const int n = paged_tile_units<ROWS, UNIT>(p, s, c.i) + OVERHEAD;
         if (left < n) break;
         left -= n;
     }
@@ -261,9 +283,10 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
     return c;
 }
 
-// The tile after the cursor's (sequences without rows have none).
-template <int ROWS, int UNIT>
-__device__ __forceinline__ void paged_next(const PagedWork& p, PagedCursor& c) {
+// To the tile after the cursor's, `cost` units on (sequences without rows have none).
+template <int ROWS>
+__device__ __forceinline__ void paged_next(const PagedWork& p, PagedCursor& c, int cost) {
+    c.u += cost;
     c.k = 0;
     if (++c.i < c.tiles) return;
     c.i = 0;

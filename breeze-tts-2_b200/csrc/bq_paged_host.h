@@ -8,10 +8,11 @@ namespace bq {
 struct PagedKV;
 struct PagedWork;
 
-// Tile and unit of the kernel for few rows (bq_paged_narrow.cu) and its warps.
-constexpr int kNarrowRows = 16, kNarrowUnit = 64, kNarrowWarps = 4;
-// Tile and unit of the kernel for many rows (bq_paged_wide.cu).
-constexpr int kWideRows = 256, kWideUnit = 128;
+// Tile and unit of the kernel for few rows (bq_paged_narrow.cu), what a tile's
+// start and end cost in units, and its warps.
+constexpr int kNarrowRows = 16, kNarrowUnit = 64, kNarrowOverhead = 1, kNarrowWarps = 4;
+// The same of the kernel for many rows (bq_paged_wide.cu).
+constexpr int kWideRows = 256, kWideUnit = 128, kWideOverhead = 1;
 int paged_launch_wide(const PagedWork& w, const bq_paged_kv* kv, int grid, uint32_t flags, void* stream);
 int paged_launch_narrow(const PagedWork& w, int dtype, int D, int grid, uint32_t flags, void* stream);
 

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
     const PagedKV& kv = p.kv;
     pdl_launch_dependents();
     pdl_wait();
-    PagedCursor c = paged_find<ROWS, UNIT, kThreads>(p, blockIdx.x, gridDim.x);
+    PagedCursor c = paged_find<ROWS, UNIT, kNarrowOverhead, kThreads>(p, blockIdx.x, gridDim.x);
     bool shares = false;  // the last tile goes on in the next CTA
     const int kv_lo = p.prefix_pass ? 0 : p.prefix_len;
     const uint32_t ring = sb + warp * SM::kRing;
@@ -91,9 +91,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
         bool cut, pages_ok = true;
         const PagedSeq s = paged_seq(p, c.b, cut);
         const int limit = paged_tile_limit<ROWS>(p, s, c.i);
-        const int units = paged_tile_units<ROWS, UNIT>(p, s, c.i);
-        const int nu = int(min((long long)(units - c.k), c.hi - c.u));
-        const int p0 = kv_lo + c.k * UNIT, p1 = min(p0 + nu * UNIT, limit);
+        const PagedSegment<ROWS, UNIT, kNarrowOverhead> sg(p, s, c);
+        if (sg.nu == 0) {
+            paged_next<ROWS>(p, c, sg.cost);
+            continue;
+        }
+        const int p0 = kv_lo + sg.k0 * UNIT, p1 = min(p0 + sg.nu * UNIT, limit);
         const int r0 = c.i * ROWS, nrows = min(ROWS, s.rows - r0);
         const int blocks = max(0, (p1 - p0 + 15) >> 4);
         const int steps = (blocks - warp + kNarrowWarps - 1) / kNarrowWarps;
@@ -235,9 +238,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
             if (tq == 0) s_ml[warp][g + 8] = make_float2(m1, l1);
         }
         __syncthreads();
-        const bool whole = c.k == 0 && nu == units;
-        const int slot = 2 * blockIdx.x + (c.k == 0 ? 1 : 0);
-        const int parts = whole || c.k ? 0 : c.share.owner(c.u + units - 1) - int(blockIdx.x) + 1;
+        const bool whole = sg.whole();
+        const int slot = 2 * blockIdx.x + (sg.k0 == 0 ? 1 : 0), parts = sg.parts(c, blockIdx.x);
         if (parts) {
             shares = true;
             if (threadIdx.x == 0) p.shared[blockIdx.x] = PagedShared{parts, nrows, r0, s.begin, c.j};
@@ -268,13 +270,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
                 *reinterpret_cast<float4*>((whole ? p.row_o : p.part_o) + at * D + d) = a;
                 if (d == 0) {
                     (whole ? p.row_ml : p.part_ml)[at] = make_float2(mm, ll);
-                    if (p.row_at && c.k == 0) p.row_at[row * kv.HQ + head] = paged_row_at(blockIdx.x, parts, r);
+                    if (p.row_at && sg.k0 == 0) p.row_at[row * kv.HQ + head] = paged_row_at(blockIdx.x, parts, r);
                 }
             }
         }
         __syncthreads();  // the rings are free again
-        c.u += nu;
-        paged_next<ROWS, UNIT>(p, c);
+        paged_next<ROWS>(p, c, sg.cost);
     }
     if (!shares && threadIdx.x == 0) p.shared[blockIdx.x].parts = 0;
 }

@@ -9,7 +9,7 @@
 // multiply for the other. Both halves use the same k / v tiles, which halves
 // what the tiles cost in L2 reads (32 bytes per cycle and SM).
 //
-// Roles (10 warps, one CTA per SM, all 512 tensor-memory columns):
+// Roles (one CTA per SM, all 512 tensor-memory columns):
 //   warps 0-3, 4-7  softmax of half 0 / 1, one row per thread: the row's 128
 //                   scores from tensor memory, running maximum and sum, the
 //                   probabilities back to tensor memory in 16 bits over the
@@ -48,7 +48,7 @@ struct PagedWideParams {
 
 namespace {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 320;  // 168 registers per thread: a scheduler holds up to three of the ten warps
 constexpr int kRows = kWideRows, kUnit = kWideUnit;
 constexpr uint32_t kCols = 512;
 
@@ -103,21 +103,83 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // What every role derives for the tile at the cursor.
-struct WideTile {
+struct WideTile : PagedSegment<kRows, kUnit, kWideOverhead> {
     PagedSeq s;
-    int units, nu, p0, p1, r0, nrows;
-    __device__ __forceinline__ WideTile(const PagedWork& w, const PagedCursor& c) {
-        bool cut;
-        s = paged_seq(w, c.b, cut);
-        const int limit = paged_tile_limit<kRows>(w, s, c.i);
-        units = paged_tile_units<kRows, kUnit>(w, s, c.i);
-        nu = int(min((long long)(units - c.k), c.hi - c.u));
-        p0 = (w.prefix_pass ? 0 : w.prefix_len) + c.k * kUnit;
-        p1 = min(p0 + nu * kUnit, limit);
+    int p0, p1, r0, nrows;
+    WideTile() = default;
+    __device__ __forceinline__ WideTile(const PagedWork& w, const PagedSeq& seq, const PagedCursor& c)
+        : PagedSegment<kRows, kUnit, kWideOverhead>(w, seq, c), s(seq) {
+        p0 = (w.prefix_pass ? 0 : w.prefix_len) + k0 * kUnit;
+        p1 = min(p0 + nu * kUnit, paged_tile_limit<kRows>(w, s, c.i));
         r0 = c.i * kRows;
         nrows = min(kRows, s.rows - r0);
     }
 };
+
+__device__ __forceinline__ bool wide_more(const PagedWork& w, const PagedCursor& c) {
+    return c.u < c.hi && c.b < (w.prefix_pass ? 1 : w.kv.B);
+}
+// Moves the cursor past tiles of which this share holds only overhead; false at the end of the share.
+__device__ __forceinline__ bool wide_skip(const PagedWork& w, PagedCursor& c) {
+    while (wide_more(w, c)) {
+        bool cut;
+        const PagedSegment<kRows, kUnit, kWideOverhead> g(w, paged_seq(w, c.b, cut), c);
+        if (g.nu > 0) return true;
+        paged_next<kRows>(w, c, g.cost);
+    }
+    return false;
+}
+__device__ __forceinline__ WideTile wide_tile(const PagedWork& w, const PagedCursor& c) {
+    bool cut;
+    return WideTile(w, paged_seq(w, c.b, cut), c);
+}
+
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool full) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
+}
+
+// Two fp32 values in a register pair: one instruction for both.
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unf2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// A softmax warp's place and tile.
+struct WideState {
+    PagedCursor c;
+    WideTile t;
+};
+
+// Queries of half h of tile t into shared memory (128 threads, thread `row`), in
+// the 128-byte-swizzled K-major layout; rows that do not exist are zeros.
+template <typename E, int D>
+__device__ __forceinline__ void wide_queries(const PagedWork& w, const PagedCursor& c, const WideTile& t, int h, int row, uint32_t dst) {
+    constexpr int CH = D / 8;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int idx = row + 128 * i, r = idx / CH, ch = idx % CH;
+        const int rr = t.r0 + min(128 * h + r, t.nrows - 1), tok = w.by_G(rr);
+        const E* src = static_cast<const E*>(w.q) + int64_t(t.s.begin + tok) * w.ldq + (c.j * w.G + rr - tok * w.G) * D + ch * 8;
+        cp_async16_zfill(dst + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src, 128 * h + r < t.nrows);
+    }
+}
 
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_constant__ PagedWideParams p) {
@@ -126,6 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
+    __shared__ WideState s_state[8];  // of each softmax warp: its registers are for the scores
     const uint32_t sraw = smem_u32(smem_raw), sb = (sraw + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (sb - sraw);
     const PagedWork& w = p.w;
@@ -152,179 +215,209 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
         fence_barrier_init();
     }
     pdl_wait();  // before the tensor memory is taken: a kernel before this one may still need its own
-    PagedCursor c = paged_find<kRows, kUnit, kThreads>(w, blockIdx.x, gridDim.x);
+    PagedCursor c = paged_find<kRows, kUnit, kWideOverhead, kThreads>(w, blockIdx.x, gridDim.x);
     if (warp == 9) tmem_alloc(smem_u32(&s_tmem), kCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     pdl_launch_dependents();
     const uint32_t tmem = s_tmem;  // scores / probabilities of half h at columns 128 h, outputs at 256 + 128 h
-    const int sequences = w.prefix_pass ? 1 : kv.B;
 
     if (warp < 8) {
         // ------------------------------------------------------------ softmax of one half
         const int h = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
         const uint32_t t_s = lanes + 128 * h, t_o = lanes + 256 + 128 * h;
+        const uint32_t qs = sb + h * SM::kTile;
         int seg = 0, ph_s = 0, it = 0;  // tiles of this half done, score phases, ring stages passed
         bool ok = true, shares = false;  // shares: the last tile goes on in the next CTA
-        for (; ok && c.u < c.hi && c.b < sequences;) {
-            const WideTile t(w, c);
-            const int hrows = t.nrows - 128 * h;  // valid rows of this half
-            if (hrows > 0) {
-                for (int idx = row; idx < 128 * CH; idx += 128) {
-                    const int r = idx / CH, ch = idx - r * CH;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (r < hrows) {
-                        const int rr = t.r0 + 128 * h + r, tok = w.by_G(rr);
-                        v = *reinterpret_cast<const uint4*>(static_cast<const E*>(w.q) + int64_t(t.s.begin + tok) * w.ldq +
-                                                            (c.j * w.G + rr - tok * w.G) * D + ch * 8);
-                    }
-                    *reinterpret_cast<uint4*>(smem + h * SM::kTile + (ch >> 3) * (128 * 128) + r * 128 +
-                                              (((ch & 7) ^ (r & 7)) << 4)) = v;
-                }
-                fence_async_smem();
-                mbar_arrive(bar_q + 8 * h);
-                const int myrow = t.r0 + 128 * h + row;
-                const int limit = row < hrows ? paged_row_limit(w, t.s, myrow) : 0;
-                const bool idle = (warp & 3) * 32 >= hrows;  // no row of this warp exists
-                __syncwarp();
-                float mref = -INFINITY, l = 0.f;
-                for (int u = 0; u < t.nu; ++u) {
-                    ok = __all_sync(0xffffffffu, tc_wait(bar_s + 8 * h, ph_s & 1, abort, lim));
-                    if (!ok) break;
-                    ++ph_s;
-                    tc_fence_after();
-                    const int base = t.p0 + u * kUnit;
-                    if (!idle) {
-                        float s[128];
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) tmem_ld32(t_s + 32 * q, s + 32 * q);
-                        tmem_wait_ld();
-                        if (base + kUnit > limit) {
-                            const int n = limit - base;
-#pragma unroll
-                            for (int i = 0; i < 128; ++i) s[i] = i < n ? s[i] : -INFINITY;
-                        }
-                        __syncwarp();  // tensor-memory instructions below are warp-wide
-                        float m = s[0];
-#pragma unroll
-                        for (int i = 1; i < 128; ++i) m = fmaxf(m, s[i]);
-                        m *= w.scale_log2;
-                        const bool move = m > mref + 8.f;  // also the first finite maximum
-                        if (__any_sync(0xffffffffu, move)) {
-                            const float f = move ? ex2(mref - m) : 1.f;
-                            if (move) mref = m;
-                            l *= f;
-                            if (u > 0) {
-#pragma unroll
-                                for (int q = 0; q < D / 16; ++q) {
-                                    float o[16];
-                                    tmem_ld16(t_o + 16 * q, o);
-                                    uint32_t o2[16];
-#pragma unroll
-                                    for (int i = 0; i < 16; ++i) o2[i] = __float_as_uint(o[i] * f);
-                                    tmem_st16(t_o + 16 * q, o2);
-                                }
-                            }
-                        }
-                        const float off = mref == -INFINITY ? 0.f : mref;
-                        float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            uint32_t pk[16];
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const float a = ex2(fmaf(s[32 * q + 2 * i], w.scale_log2, -off));
-                                const float b = ex2(fmaf(s[32 * q + 2 * i + 1], w.scale_log2, -off));
-                                l0 += a;
-                                l1 += b;
-                                pk[i] = pack2<E>(a, b);
-                            }
-                            tmem_st16(t_s + 16 * q, pk);
-                        }
-                        l += l0 + l1;
-                        tmem_wait_st();
-                    }
-                    if (h == 0 && base + kUnit > t.p1) {  // rows of v that no position owns
-                        const int st = (it + 1) % ST, from = max(0, t.p1 - base);
-                        ok = __all_sync(0xffffffffu, tc_wait(bar_full + 8 * st, ((it + 1) / ST) & 1, abort, lim));
-                        if (!ok) break;
-                        const uint4 z = make_uint4(0, 0, 0, 0);
-                        for (int idx = row; idx < (128 - from) * CH; idx += 128) {
-                            const int r = from + idx / CH, ch = idx % CH;
-                            *reinterpret_cast<uint4*>(smem + SM::kRing + st * SM::kTile + (ch >> 3) * (128 * 128) + r * 128 +
-                                                      ((ch & 7) << 4)) = z;
-                        }
-                        fence_async_smem();
-                        __syncwarp();
-                    }
-                    it += 2;
-                    tc_fence_before();
-                    mbar_arrive(bar_p + 8 * h);
-                }
-                if (ok) ok = __all_sync(0xffffffffu, tc_wait(bar_o + 8 * h, seg & 1, abort, lim));
-                if (!ok) break;
-                ++seg;
-                tc_fence_after();
-                const bool whole = c.k == 0 && t.nu == t.units, final = whole && !w.row_o;
-                const int parts = whole || c.k ? 0 : c.share.owner(c.u + t.units - 1) - int(blockIdx.x) + 1;
-                if (parts) {
-                    shares = true;
-                    if (threadIdx.x == 0) w.shared[blockIdx.x] = PagedShared{parts, t.nrows, t.r0, t.s.begin, c.j};
-                }
-                if (!idle) {
-                    const int tok = w.by_G(myrow), head = c.j * w.G + myrow - tok * w.G;
-                    const int64_t orow = t.s.begin + tok;
-                    const int64_t at = whole ? orow * kv.HQ + head
-                                             : int64_t(2 * blockIdx.x + (c.k == 0 ? 1 : 0)) * kRows + 128 * h + row;
-                    const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-                    for (int q = 0; q < D / 16; ++q) {
-                        float o[16];
-                        __syncwarp();
-                        tmem_ld16(t_o + 16 * q, o);
-                        if (row < hrows && final) {
-                            uint4* dst = reinterpret_cast<uint4*>(static_cast<E*>(w.out) + orow * w.ldo + head * D + 16 * q);
-                            uint4 a, b;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] *= inv;
-                            a = make_uint4(pack2<E>(o[0], o[1]), pack2<E>(o[2], o[3]), pack2<E>(o[4], o[5]), pack2<E>(o[6], o[7]));
-                            b = make_uint4(pack2<E>(o[8], o[9]), pack2<E>(o[10], o[11]), pack2<E>(o[12], o[13]),
-                                           pack2<E>(o[14], o[15]));
-                            dst[0] = a;
-                            dst[1] = b;
-                        } else if (row < hrows) {
-                            float4* dst = reinterpret_cast<float4*>((whole ? w.row_o : w.part_o) + at * D + 16 * q);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                        }
-                    }
-                    if (row < hrows) {
-                        if (!final) {
-                            (whole ? w.row_ml : w.part_ml)[at] = make_float2(mref, l);
-                            if (w.row_at && c.k == 0)
-                                w.row_at[orow * kv.HQ + head] = paged_row_at(blockIdx.x, parts, 128 * h + row);
-                        } else if (w.lse) {
-                            w.lse[orow * w.ldl + head] = l > 0.f ? (mref + log2f(l)) * kLn2 : -INFINITY;
-                        }
-                    }
-                }
-                __syncwarp();
-                tc_fence_before();  // ordered before the next tile's first product by its bar_p arrivals
-            } else {
-                it += 2 * t.nu;
+        bool more = wide_skip(w, c);
+        WideState& state = s_state[warp];
+        auto staged = [&] {  // this thread's queries have landed; tell the tensor cores
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async_smem();
+            mbar_arrive(bar_q + 8 * h);
+        };
+        if (more) {
+            const WideTile t = wide_tile(w, c);
+            if (lane == 0) {
+                state.c = c;
+                state.t = t;
             }
-            c.u += t.nu;
-            paged_next<kRows, kUnit>(w, c);
+            if (t.nrows > 128 * h) {
+                wide_queries<E, D>(w, c, t, h, row, qs);
+                staged();
+            }
         }
+        while (ok && more) {
+            __syncwarp();
+            const int hrows = state.t.nrows - 128 * h;  // valid rows of this half
+            const int myrow = state.t.r0 + 128 * h + row, units = state.t.nu, p0 = state.t.p0, p1 = state.t.p1;
+            const bool idle = (warp & 3) * 32 >= hrows;  // no row of this warp exists
+            const int limit = row < hrows ? paged_row_limit(w, state.t.s, myrow) : 0;
+            float mref = -INFINITY, l = 0.f;
+            __syncwarp();  // tensor-memory instructions below are warp-wide
+            for (int u = 0; hrows > 0 && u < units; ++u) {
+                ok = __all_sync(0xffffffffu, tc_wait(bar_s + 8 * h, ph_s & 1, abort, lim));
+                if (!ok) break;
+                ++ph_s;
+                tc_fence_after();
+                const int base = p0 + u * kUnit;
+                if (!idle) {
+                    float s[128];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) tmem_ld32(t_s + 32 * q, s + 32 * q);
+                    tmem_wait_ld();
+                    if (base + kUnit > limit) {
+                        const int n = limit - base;
+#pragma unroll
+                        for (int i = 0; i < 128; ++i) s[i] = i < n ? s[i] : -INFINITY;
+                    }
+                    __syncwarp();
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int i = 4; i + 8 <= 124 + 4; i += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[i + e], s[i + 4 + e]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[124 + e]);
+                    const float m = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * w.scale_log2;
+                    const bool move = m > mref + 8.f;  // also the first finite maximum
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float f = move ? ex2(mref - m) : 1.f;
+                        if (move) mref = m;
+                        l *= f;
+                        if (u > 0) {
+#pragma unroll
+                            for (int q = 0; q < D / 16; ++q) {
+                                float o[16];
+                                tmem_ld16(t_o + 16 * q, o);
+                                uint32_t o2[16];
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) o2[i] = __float_as_uint(o[i] * f);
+                                tmem_st16(t_o + 16 * q, o2);
+                            }
+                        }
+                    }
+                    const float off = mref == -INFINITY ? 0.f : -mref;
+                    const uint64_t sc2 = f2(w.scale_log2, w.scale_log2), off2 = f2(off, off);
+                    uint64_t sum[2] = {0, 0};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float a, b;
+                            unf2(fma2(f2(s[32 * q + 2 * i], s[32 * q + 2 * i + 1]), sc2, off2), a, b);
+                            a = ex2(a);
+                            b = ex2(b);
+                            sum[i & 1] = add2(sum[i & 1], f2(a, b));
+                            pk[i] = pack2<E>(a, b);
+                        }
+                        tmem_st16(t_s + 16 * q, pk);
+                    }
+                    float l0, l1;
+                    unf2(add2(sum[0], sum[1]), l0, l1);
+                    l += l0 + l1;
+                    tmem_wait_st();
+                }
+                if (h == 0 && base + kUnit > p1) {  // rows of v that no position owns
+                    const int st = (it + 1) % ST, from = max(0, p1 - base);
+                    ok = __all_sync(0xffffffffu, tc_wait(bar_full + 8 * st, ((it + 1) / ST) & 1, abort, lim));
+                    if (!ok) break;
+                    const uint4 z = make_uint4(0, 0, 0, 0);
+                    for (int idx = row; idx < (128 - from) * CH; idx += 128) {
+                        const int r = from + idx / CH, ch = idx % CH;
+                        *reinterpret_cast<uint4*>(smem + SM::kRing + st * SM::kTile + (ch >> 3) * (128 * 128) + r * 128 +
+                                                  ((ch & 7) << 4)) = z;
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                }
+                it += 2;
+                tc_fence_before();
+                mbar_arrive(bar_p + 8 * h);
+            }
+            if (!ok) break;
+            // This half's queries have been used: the next tile's are fetched behind the last product.
+            PagedCursor at_next = state.c;
+            const WideTile done = state.t;
+            const bool whole = done.whole();
+            const int parts = done.parts(at_next, blockIdx.x), j = at_next.j;
+            paged_next<kRows>(w, at_next, done.cost);
+            more = wide_skip(w, at_next);
+            bool next = false;
+            __syncwarp();  // every lane has read the state
+            if (more) {
+                const WideTile t = wide_tile(w, at_next);
+                if (lane == 0) {
+                    state.c = at_next;
+                    state.t = t;
+                }
+                next = t.nrows > 128 * h;
+                if (next) wide_queries<E, D>(w, at_next, t, h, row, qs);
+            }
+            if (parts) {
+                shares = true;
+                if (threadIdx.x == 0) w.shared[blockIdx.x] = PagedShared{parts, done.nrows, done.r0, done.s.begin, j};
+            }
+            if (hrows <= 0) {
+                it += 2 * done.nu;
+                if (next) staged();
+                continue;
+            }
+            __syncwarp();
+            ok = __all_sync(0xffffffffu, tc_wait(bar_o + 8 * h, seg & 1, abort, lim));
+            if (!ok) break;
+            ++seg;
+            if (next) staged();
+            tc_fence_after();
+            if (!idle) {
+                const bool final = whole && !w.row_o;
+                const int tok = w.by_G(myrow), head = j * w.G + myrow - tok * w.G;
+                const int64_t orow = done.s.begin + tok;
+                const int64_t at = whole ? orow * kv.HQ + head
+                                         : int64_t(2 * blockIdx.x + (done.k0 == 0 ? 1 : 0)) * kRows + 128 * h + row;
+                const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+                for (int q = 0; q < D / 32; ++q) {
+                    float o[32];
+                    __syncwarp();
+                    tmem_ld32(t_o + 32 * q, o);
+                    tmem_wait_ld();
+                    if (row < hrows && final) {
+                        uint4* dst = reinterpret_cast<uint4*>(static_cast<E*>(w.out) + orow * w.ldo + head * D + 32 * q);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            dst[i] = make_uint4(pack2<E>(o[8 * i] * inv, o[8 * i + 1] * inv), pack2<E>(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                                                pack2<E>(o[8 * i + 4] * inv, o[8 * i + 5] * inv), pack2<E>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+                    } else if (row < hrows) {
+                        float4* dst = reinterpret_cast<float4*>((whole ? w.row_o : w.part_o) + at * D + 32 * q);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                }
+                if (row < hrows) {
+                    if (!final) {
+                        (whole ? w.row_ml : w.part_ml)[at] = make_float2(mref, l);
+                        if (w.row_at && done.k0 == 0)
+                            w.row_at[orow * kv.HQ + head] = paged_row_at(blockIdx.x, parts, 128 * h + row);
+                    } else if (w.lse) {
+                        w.lse[orow * w.ldl + head] = l > 0.f ? (mref + log2f(l)) * kLn2 : -INFINITY;
+                    }
+                }
+            }
+            __syncwarp();
+            tc_fence_before();  // ordered before the next tile's first product by its bar_p arrivals
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         if (threadIdx.x == 0 && !shares) w.shared[blockIdx.x].parts = 0;
     } else if (warp == 8) {
         // ------------------------------------------------------------ k / v loads
         int it = 0;
         bool ok = true, pages_ok = true;
-        for (; ok && c.u < c.hi && c.b < sequences;) {
-            const WideTile t(w, c);
+        while (ok && wide_skip(w, c)) {
+            const WideTile t = wide_tile(w, c);
             for (int u = 0; ok && u < t.nu; ++u) {
                 const int base = t.p0 + u * kUnit;
                 const int nb = max(0, (min(kUnit, t.p1 - base) + p.box - 1) / p.box);  // boxes that hold positions
@@ -351,8 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     }
                 }
             }
-            c.u += t.nu;
-            paged_next<kRows, kUnit>(w, c);
+            paged_next<kRows>(w, c, t.cost);
         }
         if (!pages_ok) atomicOr(&g_device_error, BQ_DEVERR_PAGE_BIT);
         // no tile may still be landing when the CTA leaves (an abort skips the products)
@@ -372,8 +464,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 }
                 tc_commit(bar_s + 8 * h);
             };
-            for (; ok && c.u < c.hi && c.b < sequences;) {
-                const WideTile t(w, c);
+            while (ok && wide_skip(w, c)) {
+                const WideTile t = wide_tile(w, c);
                 const int halves = t.nrows > 128 ? 2 : 1;
                 ok = tc_wait(bar_full + 8 * (it % ST), (it / ST) & 1, abort, lim);
                 for (int h = 0; ok && h < halves; ++h) {
@@ -406,8 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                         }
                     }
                 }
-                c.u += t.nu;
-                paged_next<kRows, kUnit>(w, c);
+                paged_next<kRows>(w, c, t.cost);
             }
             tc_commit(bar_done);  // every product issued above has finished once this completes
             tc_wait(bar_done, 0, nullptr, lim);
