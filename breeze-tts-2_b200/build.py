@@ -2,7 +2,8 @@
 
     python breeze-tts-2_b200/build.py [--force] [--jobs N]
 
-Compiles every csrc/*.cu as relocatable device code for
+Compiles every csrc/*.cu as relocatable device code (``WHOLE``: as a whole
+program) for
 ``-gencode arch=compute_100a,code=sm_100a`` and links them, with the CUDA
 runtime linked statically, into breeze_b200/libbreeze_b200.so next to the
 Python package that loads it. Objects go to _build/ (git-ignored). The
@@ -26,6 +27,8 @@ OUT = HERE / "breeze_b200" / "libbreeze_b200.so"
 BUILD = HERE / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
+# compiled as whole programs: relocatable code ignores register reallocation (setmaxnreg)
+WHOLE = {"bq_paged_wide"}
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-rdc=true", "--expt-relaxed-constexpr",
           f"-I{INCLUDE}", f"-I{CSRC}"]
 
@@ -52,7 +55,8 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
 
     def compile_one(so):
         s, o = so
-        cmd = [nvcc(), *ARCH, *CFLAGS, "-c", str(s), "-o", str(o)]
+        flags = [f for f in CFLAGS if f != "-rdc=true"] if s.stem in WHOLE else CFLAGS
+        cmd = [nvcc(), *ARCH, *flags, "-c", str(s), "-o", str(o)]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
         r = subprocess.run(cmd, capture_output=True, text=True)

@@ -58,6 +58,13 @@ const DeviceInfo* device_info() {
     return &d;
 }
 
+unsigned int* device_error_word() {
+    void* word = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&word, g_device_error);
+    if (e != cudaSuccess) set_error(BQ_ERR_CUDA, "cudaGetSymbolAddress: %s", cudaGetErrorString(e));
+    return static_cast<unsigned int*>(word);
+}
+
 int dtype_size(int dt) { return dt == BQ_DT_F32 ? 4 : 2; }
 
 int ensure_smem_attr(const void* fn, uint32_t bytes) {

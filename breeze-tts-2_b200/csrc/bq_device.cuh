@@ -12,8 +12,11 @@
 
 namespace bq {
 
-// Device error word, one per device (set by bounded waits that give up).
+// Device error word, one per device (set by bounded waits that give up). A file
+// compiled as a whole program (not relocatable) gets its address as an argument.
+#ifdef __CUDACC_RDC__
 extern __device__ unsigned int g_device_error;
+#endif
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -58,9 +61,10 @@ __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
+constexpr long long kWaitCycles = 4ll << 30;  // ~2 s at 1.9 GHz
+#ifdef __CUDACC_RDC__
 // Bounded wait: gives up after ~kWaitCycles SM cycles, records the failure in
 // the device error word and returns false. Never spins forever.
-constexpr long long kWaitCycles = 4ll << 30;  // ~2 s at 1.9 GHz
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
@@ -72,6 +76,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
     }
     return true;
 }
+#endif
 
 // ---------------------------------------------------------------- cp.async
 // 16-byte asynchronous global -> shared copy, L2 only (both addresses 16-byte aligned).

@@ -24,6 +24,9 @@ const DeviceInfo* device_info();
 
 int dtype_size(int dt);
 
+// Address of the current device's error word (nullptr + error set on failure).
+unsigned int* device_error_word();
+
 // Raises the kernel's dynamic shared memory limit once per (kernel, device).
 int ensure_smem_attr(const void* fn, uint32_t bytes);
 

@@ -49,7 +49,7 @@ int paged_check_device() {
     return BQ_OK;
 }
 
-void paged_fill(PagedKV* o, const bq_paged_kv* kv, int T, int HQ) {
+int paged_fill(PagedKV* o, const bq_paged_kv* kv, int T, int HQ) {
     o->B = kv->B;
     o->HKV = kv->HKV;
     o->page_shift = __builtin_ctz(unsigned(kv->page_size));
@@ -70,6 +70,8 @@ void paged_fill(PagedKV* o, const bq_paged_kv* kv, int T, int HQ) {
     o->ld_table = kv->ld_table;
     o->lens = kv->seq_lens;
     o->starts = kv->q_starts;
+    o->errors = device_error_word();
+    return o->errors ? BQ_OK : BQ_ERR_CUDA;
 }
 
 int paged_launch(const void* fn, dim3 grid, dim3 block, uint32_t smem, void** args, uint32_t flags, void* stream,
@@ -390,7 +392,8 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
     char* ws = static_cast<char*>(workspace);
     PagedWork w;
     std::memset(&w, 0, sizeof(w));
-    paged_fill(&w.kv, &d->kv, d->T, d->HQ);
+    rc = paged_fill(&w.kv, &d->kv, d->T, d->HQ);
+    if (rc) return rc;
     w.G = d->HQ / d->kv.HKV;
     w.by_G.set(uint32_t(w.G));
     w.causal = (d->flags & BQ_PAGED_FULL) ? 0 : 1;

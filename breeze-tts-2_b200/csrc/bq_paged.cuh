@@ -24,6 +24,7 @@ struct PagedKV {
     int64_t ld_table;
     const int32_t* lens;
     const int32_t* starts;  // NULL: one new token per sequence
+    unsigned int* errors;   // the device error word
 };
 
 // Rows [begin, begin + count) of the new tokens belong to sequence b. Values
@@ -224,7 +225,7 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
     for (int b = b0; b < b1; ++b) {
         bool cut;
         const PagedSeq s = paged_seq(p, b, cut);
-        if (cut && cta == 0) atomicOr(&g_device_error, BQ_DEVERR_POSITION_BIT);
+        if (cut && cta == 0) atomicOr(p.kv.errors, BQ_DEVERR_POSITION_BIT);
         mine += (long long)paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
     }
     long long incl = mine;

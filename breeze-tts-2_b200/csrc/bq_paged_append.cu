@@ -81,12 +81,12 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
     if (pos < 0) return;  // an unused batch slot
     bool ok = pos < p.rope_rows && (pos >> kv.page_shift) < kv.max_pages;
     if (!ok) {
-        if (threadIdx.x == 0) atomicOr(&g_device_error, BQ_DEVERR_POSITION_BIT);
+        if (threadIdx.x == 0) atomicOr(kv.errors, BQ_DEVERR_POSITION_BIT);
         return;
     }
     const int page = paged_page(kv, b, pos, ok);
     if (!ok) {
-        if (threadIdx.x == 0) atomicOr(&g_device_error, BQ_DEVERR_PAGE_BIT);
+        if (threadIdx.x == 0) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
         return;
     }
     const int slot = pos & kv.page_mask;
@@ -165,7 +165,8 @@ extern "C" int32_t bq_paged_append(const bq_paged_append_desc* d, void* stream) 
     if (rc) return rc;
     AppendParams p;
     std::memset(&p, 0, sizeof(p));
-    paged_fill(&p.kv, &d->kv, d->T, d->HQ);
+    rc = paged_fill(&p.kv, &d->kv, d->T, d->HQ);
+    if (rc) return rc;
     p.rope_rows = d->rope_rows;
     p.has_norm = d->q_norm != nullptr;
     p.eps = d->eps;

@@ -20,7 +20,7 @@ int paged_launch_narrow(const PagedWork& w, int dtype, int D, int grid, uint32_t
 int paged_validate(const bq_paged_kv* kv, int T, int HQ);
 // BQ_OK when the current device is the one this library is built for.
 int paged_check_device();
-void paged_fill(PagedKV* out, const bq_paged_kv* kv, int T, int HQ);
+int paged_fill(PagedKV* out, const bq_paged_kv* kv, int T, int HQ);
 // 16-byte aligned base and row stride (NULL counts as aligned).
 inline bool paged_aligned(const void* p, int64_t ld, int elem) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * elem) % 16 == 0;

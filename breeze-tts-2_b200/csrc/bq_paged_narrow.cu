@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
             }
         }
         cp_wait<0>();
-        if (!pages_ok) atomicOr(&g_device_error, BQ_DEVERR_PAGE_BIT);
+        if (!pages_ok) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);

@@ -4,24 +4,25 @@
 //
 // Bound: tensor cores and, as close, the exponentials: a half's unit is two
 // products of 128 x 128 x D (512 cycles each at D = 128) and 128 x 128
-// exponentials (1024 cycles on an SM's 16 lanes). So the two halves take turns:
-// while one half's scores go through the softmax warps, the tensor cores
-// multiply for the other. Both halves use the same k / v tiles, which halves
-// what the tiles cost in L2 reads (32 bytes per cycle and SM).
+// exponentials (1024 cycles on an SM's 16 lanes). So everything has to overlap.
+// The halves take turns in one score buffer: as soon as a half's softmax warps
+// have its scores in registers, the next scores (the other half's) are computed
+// over them, and a half's second product runs while its next scores are being
+// worked on. Both halves use the same k / v tiles, which halves what the tiles
+// cost in L2 reads (32 bytes per cycle and SM).
 //
 // Roles (one CTA per SM, all 512 tensor-memory columns):
 //   warps 0-3, 4-7  softmax of half 0 / 1, one row per thread: the row's 128
 //                   scores from tensor memory, running maximum and sum, the
-//                   probabilities back to tensor memory in 16 bits over the
-//                   scores' columns (they are the A operand of the second
-//                   product). The output accumulator stays in tensor memory; a
+//                   probabilities back to tensor memory in 16 bits (the A
+//                   operand of the second product). The output accumulator stays in tensor memory; a
 //                   row's reference maximum may lag behind the true one by up
 //                   to a factor 2^8 (probabilities up to 256 are exact enough
 //                   in either type, and the factor cancels), so the accumulator
 //                   is rescaled only when a maximum really moves.
 //   warp 8          k and v by tiled TMA, one box per page (or 128 positions of
 //                   one) and 64 dims, into a ring of 32 KB stages
-//   warp 9          one thread issues the products: S = Q K^T (both operands in
+//   warp 9          (of the third warpgroup; its last two warps only complete it) one thread issues the products: S = Q K^T (both operands in
 //                   shared memory, K-major) and O += P V (A in tensor memory, V
 //                   as stored, dims contiguous)
 // Page slots behind the last position arrive with the last page, whatever they
@@ -48,7 +49,11 @@ struct PagedWideParams {
 
 namespace {
 
-constexpr int kThreads = 320;  // 168 registers per thread: a scheduler holds up to three of the ten warps
+constexpr int kThreads = 384;
+// Registers: the CTA starts with 384 x 168; the third warpgroup gives up what the softmax warps, a row of 128
+// scores per thread, need more (256 x 216 + 128 x 72). The file is compiled as a whole program, since relocatable
+// code may not move registers.
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 constexpr int kRows = kWideRows, kUnit = kWideUnit;
 constexpr uint32_t kCols = 512;
 
@@ -196,9 +201,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort = &s_abort;
     const long long lim = p.wait_cycles;
-    // full / empty per ring stage; per half: queries staged, scores ready, probabilities written, output complete
+    // full / empty per ring stage; per half: queries staged, scores ready, probabilities written, second product
+    // complete; scores read
     const uint32_t bar_full = sb + SM::kBars, bar_empty = bar_full + 64, bar_q = bar_full + 128, bar_s = bar_full + 144,
-                   bar_p = bar_full + 160, bar_o = bar_full + 176, bar_done = bar_full + 192;
+                   bar_p = bar_full + 160, bar_pv = bar_full + 176, bar_read = bar_full + 192, bar_done = bar_full + 200;
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) {
             mbar_init(bar_full + 8 * i, 1);
@@ -208,8 +214,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             mbar_init(bar_q + 8 * h, 128);
             mbar_init(bar_s + 8 * h, 1);
             mbar_init(bar_p + 8 * h, 128);
-            mbar_init(bar_o + 8 * h, 1);
+            mbar_init(bar_pv + 8 * h, 1);
         }
+        mbar_init(bar_read, 128);
         mbar_init(bar_done, 1);
         s_abort = 0;
         fence_barrier_init();
@@ -221,15 +228,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
     __syncthreads();
     tc_fence_after();
     pdl_launch_dependents();
-    const uint32_t tmem = s_tmem;  // scores / probabilities of half h at columns 128 h, outputs at 256 + 128 h
+    const uint32_t tmem = s_tmem;  // scores at columns 0, probabilities of half h at 128 + 64 h, outputs at 256 + 128 h
 
     if (warp < 8) {
         // ------------------------------------------------------------ softmax of one half
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int h = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
-        const uint32_t t_s = lanes + 128 * h, t_o = lanes + 256 + 128 * h;
+        const uint32_t t_p = lanes + 128 + 64 * h, t_o = lanes + 256 + 128 * h;
         const uint32_t qs = sb + h * SM::kTile;
-        int seg = 0, ph_s = 0, it = 0;  // tiles of this half done, score phases, ring stages passed
+        int done_units = 0, it = 0;  // units of this half (phases of bar_s, bar_p, bar_pv), ring stages passed
         bool ok = true, shares = false;  // shares: the last tile goes on in the next CTA
         bool more = wide_skip(w, c);
         WideState& state = s_state[warp];
@@ -258,63 +266,80 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             float mref = -INFINITY, l = 0.f;
             __syncwarp();  // tensor-memory instructions below are warp-wide
             for (int u = 0; hrows > 0 && u < units; ++u) {
-                ok = __all_sync(0xffffffffu, tc_wait(bar_s + 8 * h, ph_s & 1, abort, lim));
+                ok = __all_sync(0xffffffffu, tc_wait(bar_s + 8 * h, done_units & 1, abort, lim, kv.errors));
                 if (!ok) break;
-                ++ph_s;
                 tc_fence_after();
                 const int base = p0 + u * kUnit;
+                float s[128];
                 if (!idle) {
-                    float s[128];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) tmem_ld32(t_s + 32 * q, s + 32 * q);
+                    for (int q = 0; q < 4; ++q) tmem_ld32(lanes + 32 * q, s + 32 * q);
                     tmem_wait_ld();
+                }
+                tc_fence_before();
+                mbar_arrive(bar_read);  // the score buffer may be written again
+                float f = 1.f;
+                bool move = false;
+                if (!idle) {
                     if (base + kUnit > limit) {
                         const int n = limit - base;
 #pragma unroll
                         for (int i = 0; i < 128; ++i) s[i] = i < n ? s[i] : -INFINITY;
                     }
-                    __syncwarp();
                     float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int i = 4; i + 8 <= 124 + 4; i += 8)
+                    for (int i = 4; i < 124; i += 8)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[i + e], s[i + 4 + e]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[124 + e]);
                     const float m = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * w.scale_log2;
-                    const bool move = m > mref + 8.f;  // also the first finite maximum
-                    if (__any_sync(0xffffffffu, move)) {
-                        const float f = move ? ex2(mref - m) : 1.f;
-                        if (move) mref = m;
+                    move = m > mref + 8.f;  // also the first finite maximum
+                    if (move) {
+                        f = ex2(mref - m);
+                        mref = m;
                         l *= f;
-                        if (u > 0) {
+                    }
+                }
+                __syncwarp();
+                move = __any_sync(0xffffffffu, move);
+                const float off = mref == -INFINITY ? 0.f : -mref;
+                const uint64_t sc2 = f2(w.scale_log2, w.scale_log2), off2 = f2(off, off);
+                uint64_t sum[2] = {0, 0};
+                uint32_t pk[16];
+                auto exponentials = [&](int q) {  // of scores 32 q .. 32 q + 31
 #pragma unroll
-                            for (int q = 0; q < D / 16; ++q) {
-                                float o[16];
-                                tmem_ld16(t_o + 16 * q, o);
-                                uint32_t o2[16];
+                    for (int i = 0; i < 16; ++i) {
+                        float a, b;
+                        unf2(fma2(f2(s[32 * q + 2 * i], s[32 * q + 2 * i + 1]), sc2, off2), a, b);
+                        a = ex2(a);
+                        b = ex2(b);
+                        sum[i & 1] = add2(sum[i & 1], f2(a, b));
+                        pk[i] = pack2<E>(a, b);
+                    }
+                };
+                if (!idle) exponentials(0);
+                // the product before this one has read its probabilities and written its outputs
+                if (u > 0) ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
+                if (!ok) break;
+                tc_fence_after();
+                if (!idle) {
+                    if (move && u > 0) {
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) o2[i] = __float_as_uint(o[i] * f);
-                                tmem_st16(t_o + 16 * q, o2);
-                            }
+                        for (int q = 0; q < D / 16; ++q) {
+                            float o[16];
+                            tmem_ld16(t_o + 16 * q, o);
+                            uint32_t o2[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o2[i] = __float_as_uint(o[i] * f);
+                            tmem_st16(t_o + 16 * q, o2);
                         }
                     }
-                    const float off = mref == -INFINITY ? 0.f : -mref;
-                    const uint64_t sc2 = f2(w.scale_log2, w.scale_log2), off2 = f2(off, off);
-                    uint64_t sum[2] = {0, 0};
+                    tmem_st16(t_p, pk);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            float a, b;
-                            unf2(fma2(f2(s[32 * q + 2 * i], s[32 * q + 2 * i + 1]), sc2, off2), a, b);
-                            a = ex2(a);
-                            b = ex2(b);
-                            sum[i & 1] = add2(sum[i & 1], f2(a, b));
-                            pk[i] = pack2<E>(a, b);
-                        }
-                        tmem_st16(t_s + 16 * q, pk);
+                    for (int q = 1; q < 4; ++q) {
+                        exponentials(q);
+                        tmem_st16(t_p + 16 * q, pk);
                     }
                     float l0, l1;
                     unf2(add2(sum[0], sum[1]), l0, l1);
@@ -323,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 }
                 if (h == 0 && base + kUnit > p1) {  // rows of v that no position owns
                     const int st = (it + 1) % ST, from = max(0, p1 - base);
-                    ok = __all_sync(0xffffffffu, tc_wait(bar_full + 8 * st, ((it + 1) / ST) & 1, abort, lim));
+                    ok = __all_sync(0xffffffffu, tc_wait(bar_full + 8 * st, ((it + 1) / ST) & 1, abort, lim, kv.errors));
                     if (!ok) break;
                     const uint4 z = make_uint4(0, 0, 0, 0);
                     for (int idx = row; idx < (128 - from) * CH; idx += 128) {
@@ -335,6 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     __syncwarp();
                 }
                 it += 2;
+                ++done_units;
                 tc_fence_before();
                 mbar_arrive(bar_p + 8 * h);
             }
@@ -367,9 +393,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 continue;
             }
             __syncwarp();
-            ok = __all_sync(0xffffffffu, tc_wait(bar_o + 8 * h, seg & 1, abort, lim));
+            ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
             if (!ok) break;
-            ++seg;
             if (next) staged();
             tc_fence_after();
             if (!idle) {
@@ -414,6 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
         if (threadIdx.x == 0 && !shares) w.shared[blockIdx.x].parts = 0;
     } else if (warp == 8) {
         // ------------------------------------------------------------ k / v loads
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         int it = 0;
         bool ok = true, pages_ok = true;
         while (ok && wide_skip(w, c)) {
@@ -428,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 for (int x = 0; x < 2; ++x, ++it) {
                     const int st = it % ST;
                     const uint32_t bar = bar_full + 8 * st;
-                    if (it >= ST) ok = __all_sync(0xffffffffu, tc_wait(bar_empty + 8 * st, ((it / ST) + 1) & 1, abort, lim));
+                    if (it >= ST) ok = __all_sync(0xffffffffu, tc_wait(bar_empty + 8 * st, ((it / ST) + 1) & 1, abort, lim, kv.errors));
                     if (!ok) break;
                     if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(nb * p.box) * (D * 2));
                     __syncwarp();
@@ -446,62 +472,55 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             }
             paged_next<kRows>(w, c, t.cost);
         }
-        if (!pages_ok) atomicOr(&g_device_error, BQ_DEVERR_PAGE_BIT);
+        if (!pages_ok) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
         // no tile may still be landing when the CTA leaves (an abort skips the products)
-        for (int i = max(0, it - ST); i < it; ++i) tc_wait(bar_full + 8 * (i % ST), (i / ST) & 1, nullptr, lim);
+        for (int i = max(0, it - ST); i < it; ++i) tc_wait(bar_full + 8 * (i % ST), (i / ST) & 1, nullptr, lim, kv.errors);
         __syncwarp();
     } else {
         // ------------------------------------------------------------ products
-        if (lane == 0) {
-            int it = 0, ph_q[2] = {0, 0}, ph_p[2] = {0, 0};
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == 9 && lane == 0) {
+            int it = 0, tiles[2] = {0, 0}, units[2] = {0, 0}, scored = 0;  // of each half; score tiles so far
             bool ok = true;
-            auto scores = [&](int h, int st) {  // S(h) = Q(h) K^T
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t at = (k >> 2) * (128 * 128) + 32 * (k & 3);
-                    tc_mma_ss(tmem + 128 * h, tc_bdesc(sb + h * SM::kTile + at), tc_bdesc(sb + SM::kRing + st * SM::kTile + at),
-                              p.idesc_qk, k > 0);
-                }
-                tc_commit(bar_s + 8 * h);
-            };
             while (ok && wide_skip(w, c)) {
                 const WideTile t = wide_tile(w, c);
-                const int halves = t.nrows > 128 ? 2 : 1;
-                ok = tc_wait(bar_full + 8 * (it % ST), (it / ST) & 1, abort, lim);
-                for (int h = 0; ok && h < halves; ++h) {
-                    ok = tc_wait(bar_q + 8 * h, ph_q[h]++ & 1, abort, lim);
-                    if (!ok) break;
-                    tc_fence_after();
-                    scores(h, it % ST);
-                }
-                if (ok) tc_commit(bar_empty + 8 * (it % ST));
-                for (int u = 0; ok && u < t.nu; ++u, it += 2) {
-                    const int vs = (it + 1) % ST, ks = (it + 2) % ST;
-                    const bool more = u + 1 < t.nu;
-                    for (int h = 0; h < halves; ++h) {
-                        ok = tc_wait(bar_p + 8 * h, ph_p[h]++ & 1, abort, lim);
-                        if (ok && h == 0) ok = tc_wait(bar_full + 8 * vs, ((it + 1) / ST) & 1, abort, lim);
+                const int both = t.nrows > 128 ? 1 : 0, n_items = t.nu << both;  // item n: unit n >> both, half n & both
+                for (int h = 0; ok && h <= both; ++h) ok = tc_wait(bar_q + 8 * h, tiles[h]++ & 1, abort, lim, kv.errors);
+                int q = 0;
+                for (int n = 0; ok && n < n_items; ++n) {
+                    // scores run one unit ahead of the second products
+                    for (; ok && q < n_items && q <= n + 1 + both; ++q, ++scored) {
+                        const int h = q & both, ring = it + 2 * (q >> both), st = ring % ST;
+                        if (h == 0) ok = tc_wait(bar_full + 8 * st, (ring / ST) & 1, abort, lim, kv.errors);
+                        if (ok && scored > 0) ok = tc_wait(bar_read, (scored - 1) & 1, abort, lim, kv.errors);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)  // O(h) += P(h) V, 16 positions per step
-                            tc_mma(tmem + 256 + 128 * h, tmem + 128 * h + 8 * k,
-                                   tc_vdesc(sb + SM::kRing + vs * SM::kTile + 2048 * k), p.idesc_pv, (u > 0 || k > 0) ? 1u : 0u);
-                        if (h == halves - 1) tc_commit(bar_empty + 8 * vs);
-                        if (more) {
-                            if (h == 0) ok = tc_wait(bar_full + 8 * ks, ((it + 2) / ST) & 1, abort, lim);
-                            if (!ok) break;
-                            scores(h, ks);
-                            if (h == halves - 1) tc_commit(bar_empty + 8 * ks);
-                        } else {
-                            tc_commit(bar_o + 8 * h);
+                        for (int k = 0; k < D / 16; ++k) {  // S = Q(h) K^T
+                            const uint32_t at = (k >> 2) * (128 * 128) + 32 * (k & 3);
+                            tc_mma_ss(tmem, tc_bdesc(sb + h * SM::kTile + at), tc_bdesc(sb + SM::kRing + st * SM::kTile + at),
+                                      p.idesc_qk, k > 0);
                         }
+                        tc_commit(bar_s + 8 * h);
+                        if (h == both) tc_commit(bar_empty + 8 * st);
                     }
+                    const int h = n & both, ring = it + 2 * (n >> both) + 1, st = ring % ST;
+                    if (ok) ok = tc_wait(bar_p + 8 * h, units[h]++ & 1, abort, lim, kv.errors);
+                    if (ok && h == 0) ok = tc_wait(bar_full + 8 * st, (ring / ST) & 1, abort, lim, kv.errors);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)  // O(h) += P(h) V, 16 positions per step
+                        tc_mma(tmem + 256 + 128 * h, tmem + 128 + 64 * h + 8 * k, tc_vdesc(sb + SM::kRing + st * SM::kTile + 2048 * k),
+                               p.idesc_pv, ((n >> both) > 0 || k > 0) ? 1u : 0u);
+                    tc_commit(bar_pv + 8 * h);
+                    if (h == both) tc_commit(bar_empty + 8 * st);
                 }
+                it += 2 * t.nu;
                 paged_next<kRows>(w, c, t.cost);
             }
             tc_commit(bar_done);  // every product issued above has finished once this completes
-            tc_wait(bar_done, 0, nullptr, lim);
+            tc_wait(bar_done, 0, nullptr, lim, kv.errors);
         }
         __syncwarp();
     }

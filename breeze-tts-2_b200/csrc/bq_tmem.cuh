@@ -77,8 +77,10 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // Waits for a phase of `bar` with a bound; gives up when another role has
-// already given up (abort flag) or after p.wait_cycles, recording the timeout.
-__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit) {
+// already given up (abort flag) or after `limit` cycles, recording the timeout
+// in the device error word `errors`.
+__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit,
+                                        unsigned int* errors) {
     if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
     for (int it = 0;; ++it) {
@@ -86,12 +88,17 @@ __device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile 
         if ((it & 15) == 15) {
             if (abort && *abort) return false;
             if (clock64() - t0 > limit) {
-                atomicOr(&g_device_error, BQ_DEVERR_WAIT_TIMEOUT_BIT);
+                atomicOr(errors, BQ_DEVERR_WAIT_TIMEOUT_BIT);
                 if (abort) *abort = 1;
                 return false;
             }
         }
     }
 }
+#ifdef __CUDACC_RDC__
+__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit) {
+    return tc_wait(bar, parity, abort, limit, &g_device_error);
+}
+#endif
 
 }  // namespace bq
