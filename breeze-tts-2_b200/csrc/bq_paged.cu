@@ -141,17 +141,52 @@ __device__ __forceinline__ RowParts shared_row(const PagedParts& p, int cta, int
     return x;
 }
 
-// Joins output rows: out = sum f_i o_i / sum f_i l_i with f_i = 2^(m_i - max m),
-// over the prefix's parts, then the sequence's own, in CTA order. WPR warps work
-// on a row, each on every WPR-th part: eight for tiles of few rows, which may be
-// spread over all CTAs, one where rows are many. Without a prefix, block (c, y)
-// takes rows of the shared tile that begins in CTA c -- tiles that one CTA held
-// are finished already; with one, blocks take all rows in turn.
-// Bound: latency (a record, the statistics, then all parts' rows in flight).
-template <typename E, int D, int WPR, bool PREFIX>
+// Running join of parts of one row: largest score, sum of exponentials, and this
+// lane's outputs.
+template <int DPL>
+struct JoinRow {
+    float m, l, acc[DPL];
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) acc[e] = 0.f;
+    }
+    __device__ __forceinline__ void add(float m2, float l2, const float (&o)[DPL]) {
+        const float nm = fmaxf(m, m2), u = nm == -INFINITY ? 0.f : nm, f = ex2(m - u), g = ex2(m2 - u);
+        m = nm;
+        l = l * f + l2 * g;
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) acc[e] = acc[e] * f + o[e] * g;
+    }
+};
+
+template <int DPL>
+__device__ __forceinline__ void load_lane(const float* src, float (&o)[DPL]) {
+    if constexpr (DPL == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
+    } else {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        o[0] = v.x, o[1] = v.y;
+    }
+}
+
+// Joins output rows from their parts -- the prefix's, then the sequence's own, in
+// CTA order -- by a running maximum, so that a part's statistics and outputs are
+// one round of loads. WPR warps work on a row, each on every WPR-th part: eight for
+// tiles of few rows, which may be spread over all CTAs, one where rows are many; a
+// warp then has R rows and always kParts parts of each in flight. Without a prefix,
+// block (c, y) takes rows of the shared tile that begins in CTA c -- tiles that one
+// CTA held are finished already; with one, blocks take all rows in turn.
+// Bound: latency of two rounds of loads (a record, then the parts), or L2 for the
+// prompts' tiles.
+template <typename E, int D, int WPR, int R, bool PREFIX>
 __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __grid_constant__ PagedJoin p) {
-    constexpr int DPL = D / 32, RPB = kJoinWarps / WPR;  // rows per block at a time
+    constexpr int DPL = D / 32, RPB = kJoinWarps / WPR * R;  // rows per block at a time
+    constexpr int kParts = R > 1 ? 2 : 4;
     __shared__ float s_acc[kJoinWarps][D];
+    __shared__ float2 s_ml[kJoinWarps];
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WPR;
@@ -159,12 +194,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __gri
     int total, first, stride;
     if constexpr (PREFIX) {
         total = p.T * p.HQ;
-        first = blockIdx.x * RPB + warp / WPR;
+        first = blockIdx.x * RPB + warp / WPR * R;
         stride = gridDim.x * RPB;
     } else {
         sh = p.shared[blockIdx.x];
         total = sh.parts ? sh.rows : 0;
-        first = blockIdx.y * RPB + warp / WPR;
+        first = blockIdx.y * RPB + warp / WPR * R;
         stride = gridDim.y * RPB;
     }
     const int rounds = (total + stride - 1) / stride;  // the same for all warps: they meet at barriers
@@ -176,13 +211,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __gri
     for (int k = 0; k < rounds; ++k) {
         const int idx = first + k * stride;
         bool live = idx < total;
-        int t = 0, h = 0;
         RowParts part[2];
         part[0].n = part[1].n = 0;
         if (PREFIX) {
             if (live) {
-                t = p.by_HQ(idx);
-                h = idx - t * p.HQ;
+                const int t = p.by_HQ(idx);
                 live = t >= row_lo && t < row_hi;
             }
             if (live) {
@@ -203,79 +236,85 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __gri
                 }
             }
         } else if (live) {
-            const int rr = sh.r0 + idx, tok = p.by_G(rr);
-            t = sh.begin + tok;
-            h = sh.j * p.G + rr - tok * p.G;
             part[1] = shared_row(p.pass[0], blockIdx.x, sh.parts, idx);
         }
-        float M = -INFINITY, L = 0.f, acc[DPL] = {};
-        if (live) {
+        JoinRow<DPL> row[R];
 #pragma unroll
-            for (int a = PREFIX ? 0 : 1; a < 2; ++a)
-                for (int i = lane; i < part[a].n; i += 32) M = fmaxf(M, part[a].ml[part[a].at(i)].x);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const float u = M == -INFINITY ? 0.f : M;
+        for (int r = 0; r < R; ++r) row[r].clear();
+        const int rows = PREFIX ? 1 : min(R, total - idx);  // of this warp
 #pragma unroll
         for (int a = PREFIX ? 0 : 1; a < 2; ++a) {
-            for (int i0 = 0; i0 < part[a].n; i0 += 32) {  // the statistics of 32 parts at once, one per lane
-                const int n = min(32, part[a].n - i0);
-                float f = 0.f, l = 0.f;
-                if (lane < n) {
-                    const float2 ml = part[a].ml[part[a].at(i0 + lane)];
-                    f = ex2(ml.x - u);
-                    l = f * ml.y;
-                }
+            for (int i0 = sub; i0 < part[a].n; i0 += WPR * kParts) {
+                float2 ml[kParts][R];
+                float o[kParts][R][DPL];
 #pragma unroll
-                for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-                L += l;
-#pragma unroll 4
-                for (int i = sub; i < n; i += WPR) {
-                    const float fa = __shfl_sync(0xffffffffu, f, i);
-                    const float* src = part[a].o + part[a].at(i0 + i) * D + lane * DPL;
-                    if constexpr (DPL == 4) {
-                        const float4 v = *reinterpret_cast<const float4*>(src);
-                        acc[0] = fmaf(fa, v.x, acc[0]), acc[1] = fmaf(fa, v.y, acc[1]);
-                        acc[2] = fmaf(fa, v.z, acc[2]), acc[3] = fmaf(fa, v.w, acc[3]);
-                    } else {
-                        const float2 v = *reinterpret_cast<const float2*>(src);
-                        acc[0] = fmaf(fa, v.x, acc[0]), acc[1] = fmaf(fa, v.y, acc[1]);
+                for (int i = 0; i < kParts; ++i) {
+                    const int64_t at = part[a].at(min(i0 + i * WPR, part[a].n - 1));
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const int64_t from = at + min(r, rows - 1);  // rows of a slot follow one another
+                        ml[i][r] = part[a].ml[from];
+                        load_lane<DPL>(part[a].o + from * D + lane * DPL, o[i][r]);
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < kParts; ++i)
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+                        if (i0 + i * WPR < part[a].n) row[r].add(ml[i][r].x, ml[i][r].y, o[i][r]);
             }
         }
         if constexpr (WPR > 1) {
             __syncthreads();
 #pragma unroll
-            for (int e = 0; e < DPL; ++e) s_acc[warp][lane * DPL + e] = acc[e];
+            for (int e = 0; e < DPL; ++e) s_acc[warp][lane * DPL + e] = row[0].acc[e];
+            if (lane == 0) s_ml[warp] = make_float2(row[0].m, row[0].l);
             __syncthreads();
             if (sub == 0) {
 #pragma unroll
-                for (int q = 1; q < WPR; ++q)
+                for (int q = 1; q < WPR; ++q) {
+                    float o[DPL];
 #pragma unroll
-                    for (int e = 0; e < DPL; ++e) acc[e] += s_acc[warp + q][lane * DPL + e];
+                    for (int e = 0; e < DPL; ++e) o[e] = s_acc[warp + q][lane * DPL + e];
+                    row[0].add(s_ml[warp + q].x, s_ml[warp + q].y, o);
+                }
             }
         }
         if (live && sub == 0) {
-            const float inv = L > 0.f ? 1.f / L : 0.f;
-            E* dst = static_cast<E*>(p.out) + int64_t(t) * p.ldo + h * D + lane * DPL;
-            if constexpr (DPL == 4)
-                *reinterpret_cast<uint2*>(dst) = pack4<E>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
-            else
-                *reinterpret_cast<uint32_t*>(dst) = pack2<E>(acc[0] * inv, acc[1] * inv);
-            if (p.lse && lane == 0) p.lse[int64_t(t) * p.ldl + h] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if (r >= rows) break;
+                int t, h;
+                if (PREFIX) {
+                    t = p.by_HQ(idx);
+                    h = idx - t * p.HQ;
+                } else {
+                    const int rr = sh.r0 + idx + r, tok = p.by_G(rr);
+                    t = sh.begin + tok;
+                    h = sh.j * p.G + rr - tok * p.G;
+                }
+                const float l = row[r].l, inv = l > 0.f ? 1.f / l : 0.f;
+                const float (&acc)[DPL] = row[r].acc;
+                E* dst = static_cast<E*>(p.out) + int64_t(t) * p.ldo + h * D + lane * DPL;
+                if constexpr (DPL == 4)
+                    *reinterpret_cast<uint2*>(dst) = pack4<E>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+                else
+                    *reinterpret_cast<uint32_t*>(dst) = pack2<E>(acc[0] * inv, acc[1] * inv);
+                if (p.lse && lane == 0) p.lse[int64_t(t) * p.ldl + h] = l > 0.f ? (row[r].m + log2f(l)) * kLn2 : -INFINITY;
+            }
         }
     }
 }
 
+constexpr int kJoinRows = 4;  // rows of a warp where rows are many
+
 template <typename E, int D>
 const void* join_kernel(bool prefix, bool many) {
     if (prefix)
-        return many ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1, true>)
-                    : reinterpret_cast<const void*>(&paged_join_kernel<E, D, kJoinWarps, true>);
-    return many ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1, false>)
-                : reinterpret_cast<const void*>(&paged_join_kernel<E, D, kJoinWarps, false>);
+        return many ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1, 1, true>)
+                    : reinterpret_cast<const void*>(&paged_join_kernel<E, D, kJoinWarps, 1, true>);
+    return many ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1, kJoinRows, false>)
+                : reinterpret_cast<const void*>(&paged_join_kernel<E, D, kJoinWarps, 1, false>);
 }
 
 // One pass over positions: its kernel and its CTAs.
@@ -438,7 +477,7 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
     // warps per row: see paged_join_kernel; with a prefix 1024 rows give every SM a row per warp
     const int64_t rows = int64_t(d->T) * d->HQ;
     const bool many = prefix ? rows >= 1024 : pl.pass[0].wide;
-    const int rpb = many ? kJoinWarps : 1;
+    const int rpb = !many ? 1 : prefix ? kJoinWarps : kJoinWarps * kJoinRows;
     const dim3 grid = prefix ? dim3(unsigned(std::min<int64_t>((rows + rpb - 1) / rpb, 1 << 20)))
                              : dim3(pl.pass[0].grid, unsigned(std::min<int64_t>(pl.pass[0].rows, pl.tile_rows) + rpb - 1) / rpb);
     const bool bf = d->kv.dtype == BQ_DT_BF16;

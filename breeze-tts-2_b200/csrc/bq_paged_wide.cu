@@ -22,9 +22,12 @@
 //                   is rescaled only when a maximum really moves.
 //   warp 8          k and v by tiled TMA, one box per page (or 128 positions of
 //                   one) and 64 dims, into a ring of 32 KB stages
-//   warp 9          (of the third warpgroup; its last two warps only complete it) one thread issues the products: S = Q K^T (both operands in
+//   warps 9, 10     issue the products, each its own: S = Q K^T (both operands in
 //                   shared memory, K-major) and O += P V (A in tensor memory, V
-//                   as stored, dims contiguous)
+//                   as stored, dims contiguous). Issuing blocks until the tensor
+//                   cores take the product, so while one warp is between two
+//                   products the other's keep them busy
+//   warp 11         completes the third warpgroup
 // Page slots behind the last position arrive with the last page, whatever they
 // hold; before the product that would multiply them by zero probabilities the
 // softmax warps of half 0 clear those rows of v. Scores there are never used.
@@ -73,23 +76,105 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
-// D[tmem] (+)= A[smem] . B[smem]^T, one 128 x N x 16 step.
-__device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// Shared-memory matrix descriptors are a constant upper half and a lower half that
+// only differs in the address.
+// K-major tile (queries, keys): rows of 64 dims (128 B, 128-byte swizzle), groups
+// of 8 rows 1024 B apart (stride offset; the leading offset is not used); version
+// bit 46, layout type 2.
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kDescLoK = 1u << 16;
+// v tile as the B operand with its dims (N) contiguous: one row of 64 dims per
+// position, groups of 8 positions 1024 B apart (stride offset), the second 64 dims
+// 128 rows further (leading offset).
+constexpr uint32_t kDescLoV = uint32_t((128 * 128) >> 4) << 16;
+
+// The products of a unit. One thread of the (converged) warp issues, by a predicate
+// and not a branch, so that the operands can stay in uniform registers. Completion
+// arrives on `bar`, and on `bar2` unless it is 0.
+// S = Q K^T: D / 16 steps of 128 x 128 x 16, 32 B apart within a swizzled 64-dim row,
+// then in the second 64 dims 128 rows on.
+template <int D>
+__device__ __forceinline__ void scores_product(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t bar, uint32_t bar2) {
+    if constexpr (D == 128) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred e, no, yes;\n\t.reg .b32 x, y;\n\t.reg .b64 a, b;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 no, 0, 0;\n\tsetp.eq.b32 yes, 0, 0;\n\t"
+        "add.u32 x, %1, 0;\n\tadd.u32 y, %2, 0;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, no;\n\t"
+        "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
+        "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
+        "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
+        "add.u32 x, %1, 1024;\n\tadd.u32 y, %2, 1024;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
+        "add.u32 x, %1, 1026;\n\tadd.u32 y, %2, 1026;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
+        "add.u32 x, %1, 1028;\n\tadd.u32 y, %2, 1028;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
+        "add.u32 x, %1, 1030;\n\tadd.u32 y, %2, 1030;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t"
+        "setp.ne.and.b32 e, %7, 0, e;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"(0), "r"(bar), "r"(bar2)
+        : "memory");
+    } else {
+    asm volatile(
+        "{\n\t.reg .pred e, no, yes;\n\t.reg .b32 x, y;\n\t.reg .b64 a, b;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 no, 0, 0;\n\tsetp.eq.b32 yes, 0, 0;\n\t"
+        "add.u32 x, %1, 0;\n\tadd.u32 y, %2, 0;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, no;\n\t"
+        "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
+        "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
+        "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t"
+        "setp.ne.and.b32 e, %7, 0, e;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"(0), "r"(bar), "r"(bar2)
+        : "memory");
+    }
+}
+// O (+)= P V: 8 steps of 128 x D x 16, 16 positions (2048 B) and 8 columns of P apart.
+__device__ __forceinline__ void output_product(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool accumulate,
+                                               uint32_t bar, uint32_t bar2) {
+    asm volatile(
+        "{\n\t.reg .pred e, first, yes;\n\t.reg .b32 x, y;\n\t.reg .b64 b;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 first, %5, 0;\n\tsetp.eq.b32 yes, 0, 0;\n\t"
+        "add.u32 x, %1, 0;\n\tadd.u32 y, %2, 0;\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, first;\n\t"
+        "add.u32 x, %1, 8;\n\tadd.u32 y, %2, 128;\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, yes;\n\t"
+        "add.u32 x, %1, 16;\n\tadd.u32 y, %2, 256;\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, yes;\n\t"
+        "add.u32 x, %1, 24;\n\tadd.u32 y, %2, 384;\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, yes;\n\t"
+        "add.u32 x, %1, 32;\n\tadd.u32 y, %2, 512;\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, yes;\n\t"
+        "add.u32 x, %1, 40;\n\tadd.u32 y, %2, 640;\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, yes;\n\t"
+        "add.u32 x, %1, 48;\n\tadd.u32 y, %2, 768;\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, yes;\n\t"
+        "add.u32 x, %1, 56;\n\tadd.u32 y, %2, 896;\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, yes;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t"
+        "setp.ne.and.b32 e, %7, 0, e;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"(uint32_t(accumulate)), "r"(bar), "r"(bar2)
         : "memory");
 }
-
-// Descriptor of a v tile as the B operand with its dims (N) contiguous: rows of
-// 64 dims (128 B, 128-byte swizzle), one row per position; groups of 8
-// positions are 1024 B apart (stride offset), the second 64 dims 128 rows
-// further (leading offset).
-__device__ __forceinline__ uint64_t tc_vdesc(uint32_t saddr) {
-    return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t((128 * 128) >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) |
-           (uint64_t(2) << 61);
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+// The rest of a wait whose first look failed, out of line: the roles' registers are few.
+__device__ __noinline__ bool wide_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit, unsigned int* errors) {
+    return tc_wait(bar, parity, abort, limit, errors);
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {  // completes at tmem_wait_ld
@@ -211,13 +296,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             mbar_init(bar_empty + 8 * i, 1);
         }
         for (int h = 0; h < 2; ++h) {
-            mbar_init(bar_q + 8 * h, 128);
+            mbar_init(bar_q + 8 * h, 4);  // an arrival per warp
             mbar_init(bar_s + 8 * h, 1);
-            mbar_init(bar_p + 8 * h, 128);
+            mbar_init(bar_p + 8 * h, 4);
             mbar_init(bar_pv + 8 * h, 1);
         }
-        mbar_init(bar_read, 128);
+        mbar_init(bar_read, 4);
         mbar_init(bar_done, 1);
+        mbar_init(bar_done + 8, 1);
         s_abort = 0;
         fence_barrier_init();
     }
@@ -230,6 +316,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
     pdl_launch_dependents();
     const uint32_t tmem = s_tmem;  // scores at columns 0, probabilities of half h at 128 + 64 h, outputs at 256 + 128 h
 
+    bool ok = true;
+    // warp-wide; clears ok when the wait gave up (the softmax warps wait in line: a call would cost them registers)
+    auto wait = [&](uint32_t bar, int phase) {
+        if (!__all_sync(0xffffffffu, mbar_try_wait(bar, phase & 1)))
+            ok = __all_sync(0xffffffffu, wide_wait(bar, phase & 1, abort, lim, kv.errors));
+    };
+
     if (warp < 8) {
         // ------------------------------------------------------------ softmax of one half
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -238,13 +331,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
         const uint32_t t_p = lanes + 128 + 64 * h, t_o = lanes + 256 + 128 * h;
         const uint32_t qs = sb + h * SM::kTile;
         int done_units = 0, it = 0;  // units of this half (phases of bar_s, bar_p, bar_pv), ring stages passed
-        bool ok = true, shares = false;  // shares: the last tile goes on in the next CTA
+        bool shares = false;  // shares: the last tile goes on in the next CTA
         bool more = wide_skip(w, c);
         WideState& state = s_state[warp];
         auto staged = [&] {  // this thread's queries have landed; tell the tensor cores
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_async_smem();
-            mbar_arrive(bar_q + 8 * h);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_q + 8 * h);
         };
         if (more) {
             const WideTile t = wide_tile(w, c);
@@ -277,7 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     tmem_wait_ld();
                 }
                 tc_fence_before();
-                mbar_arrive(bar_read);  // the score buffer may be written again
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_read);  // the score buffer may be written again
                 float f = 1.f;
                 bool move = false;
                 if (!idle) {
@@ -362,7 +457,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 it += 2;
                 ++done_units;
                 tc_fence_before();
-                mbar_arrive(bar_p + 8 * h);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_p + 8 * h);
             }
             if (!ok) break;
             // This half's queries have been used: the next tile's are fetched behind the last product.
@@ -441,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
         // ------------------------------------------------------------ k / v loads
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         int it = 0;
-        bool ok = true, pages_ok = true;
+        bool pages_ok = true;
         while (ok && wide_skip(w, c)) {
             const WideTile t = wide_tile(w, c);
             for (int u = 0; ok && u < t.nu; ++u) {
@@ -454,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 for (int x = 0; x < 2; ++x, ++it) {
                     const int st = it % ST;
                     const uint32_t bar = bar_full + 8 * st;
-                    if (it >= ST) ok = __all_sync(0xffffffffu, tc_wait(bar_empty + 8 * st, ((it / ST) + 1) & 1, abort, lim, kv.errors));
+                    if (it >= ST) wait(bar_empty + 8 * st, it / ST + 1);
                     if (!ok) break;
                     if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(nb * p.box) * (D * 2));
                     __syncwarp();
@@ -479,48 +575,60 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
     } else {
         // ------------------------------------------------------------ products
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (warp == 9 && lane == 0) {
-            int it = 0, tiles[2] = {0, 0}, units[2] = {0, 0}, scored = 0;  // of each half; score tiles so far
-            bool ok = true;
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        int it = 0;  // ring stages before the tile
+        if (warp == 9) {
+            int tiles0 = 0, tiles1 = 0, scored = 0;  // tiles of each half, score tiles so far
             while (ok && wide_skip(w, c)) {
                 const WideTile t = wide_tile(w, c);
-                const int both = t.nrows > 128 ? 1 : 0, n_items = t.nu << both;  // item n: unit n >> both, half n & both
-                for (int h = 0; ok && h <= both; ++h) ok = tc_wait(bar_q + 8 * h, tiles[h]++ & 1, abort, lim, kv.errors);
-                int q = 0;
-                for (int n = 0; ok && n < n_items; ++n) {
-                    // scores run one unit ahead of the second products
-                    for (; ok && q < n_items && q <= n + 1 + both; ++q, ++scored) {
-                        const int h = q & both, ring = it + 2 * (q >> both), st = ring % ST;
-                        if (h == 0) ok = tc_wait(bar_full + 8 * st, (ring / ST) & 1, abort, lim, kv.errors);
-                        if (ok && scored > 0) ok = tc_wait(bar_read, (scored - 1) & 1, abort, lim, kv.errors);
+                const int both = __shfl_sync(0xffffffffu, t.nrows > 128 ? 1 : 0, 0);
+                const int nu = __shfl_sync(0xffffffffu, t.nu, 0);
+                wait(bar_q, tiles0++);
+                if (ok && both) wait(bar_q + 8, tiles1++);
+                for (int u = 0; ok && u < nu; ++u) {
+                    const int ring = it + 2 * u, st = ring % ST;
+                    const uint32_t k_lo = ((sb + SM::kRing + st * SM::kTile) >> 4) | kDescLoK;
+                    wait(bar_full + 8 * st, ring / ST);
+                    for (int h = 0; ok && h <= both; ++h, ++scored) {
+                        if (scored > 0) wait(bar_read, scored - 1);
                         if (!ok) break;
                         tc_fence_after();
-#pragma unroll
-                        for (int k = 0; k < D / 16; ++k) {  // S = Q(h) K^T
-                            const uint32_t at = (k >> 2) * (128 * 128) + 32 * (k & 3);
-                            tc_mma_ss(tmem, tc_bdesc(sb + h * SM::kTile + at), tc_bdesc(sb + SM::kRing + st * SM::kTile + at),
-                                      p.idesc_qk, k > 0);
-                        }
-                        tc_commit(bar_s + 8 * h);
-                        if (h == both) tc_commit(bar_empty + 8 * st);
+                        scores_product<D>(tm, ((sb + h * SM::kTile) >> 4) | kDescLoK, k_lo, p.idesc_qk, bar_s + 8 * h,
+                                          h == both ? bar_empty + 8 * st : 0u);
                     }
-                    const int h = n & both, ring = it + 2 * (n >> both) + 1, st = ring % ST;
-                    if (ok) ok = tc_wait(bar_p + 8 * h, units[h]++ & 1, abort, lim, kv.errors);
-                    if (ok && h == 0) ok = tc_wait(bar_full + 8 * st, (ring / ST) & 1, abort, lim, kv.errors);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)  // O(h) += P(h) V, 16 positions per step
-                        tc_mma(tmem + 256 + 128 * h, tmem + 128 + 64 * h + 8 * k, tc_vdesc(sb + SM::kRing + st * SM::kTile + 2048 * k),
-                               p.idesc_pv, ((n >> both) > 0 || k > 0) ? 1u : 0u);
-                    tc_commit(bar_pv + 8 * h);
-                    if (h == both) tc_commit(bar_empty + 8 * st);
                 }
-                it += 2 * t.nu;
+                it += 2 * nu;
                 paged_next<kRows>(w, c, t.cost);
             }
-            tc_commit(bar_done);  // every product issued above has finished once this completes
-            tc_wait(bar_done, 0, nullptr, lim, kv.errors);
+        } else if (warp == 10) {
+            int units0 = 0, units1 = 0;  // units of each half before the tile
+            while (ok && wide_skip(w, c)) {
+                const WideTile t = wide_tile(w, c);
+                const int both = __shfl_sync(0xffffffffu, t.nrows > 128 ? 1 : 0, 0);
+                const int nu = __shfl_sync(0xffffffffu, t.nu, 0);
+                for (int u = 0; ok && u < nu; ++u) {
+                    const int ring = it + 2 * u + 1, st = ring % ST;
+                    const uint32_t v_lo = ((sb + SM::kRing + st * SM::kTile) >> 4) | kDescLoV;
+                    wait(bar_full + 8 * st, ring / ST);
+                    for (int h = 0; ok && h <= both; ++h) {
+                        wait(bar_p + 8 * h, (h ? units1 : units0) + u);
+                        if (!ok) break;
+                        tc_fence_after();
+                        output_product(tm + 256 + 128 * h, tm + 128 + 64 * h, v_lo, p.idesc_pv, u > 0, bar_pv + 8 * h,
+                                       h == both ? bar_empty + 8 * st : 0u);
+                    }
+                }
+                it += 2 * nu;
+                units0 += nu;
+                units1 += both ? nu : 0;
+                paged_next<kRows>(w, c, t.cost);
+            }
+        }
+        if (warp <= 10) {  // every product issued above has finished once this completes
+            const uint32_t done = bar_done + 8 * (warp - 9);
+            if (elect_one()) tc_commit(done);
+            __syncwarp();
+            tc_wait(done, 0, nullptr, lim, kv.errors);
         }
         __syncwarp();
     }
