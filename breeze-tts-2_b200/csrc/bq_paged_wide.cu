@@ -373,74 +373,79 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_read);  // the score buffer may be written again
-                float f = 1.f;
-                bool move = false;
-                if (!idle) {
-                    if (base + kUnit > limit) {
-                        const int n = limit - base;
+                if (!idle && base + kUnit > limit) {
+                    const int n = limit - base;
 #pragma unroll
-                        for (int i = 0; i < 128; ++i) s[i] = i < n ? s[i] : -INFINITY;
-                    }
+                    for (int i = 0; i < 128; ++i) s[i] = i < n ? s[i] : -INFINITY;
+                }
+                if (!idle && u == 0) {  // the tile's first reference
                     float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int i = 4; i < 124; i += 8)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[i + e], s[i + 4 + e]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[124 + e]);
-                    const float m = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * w.scale_log2;
-                    move = m > mref + 8.f;  // also the first finite maximum
-                    if (move) {
-                        f = ex2(mref - m);
-                        mref = m;
-                        l *= f;
-                    }
+                    for (int i = 4; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                    mref = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * w.scale_log2;
                 }
                 __syncwarp();
-                move = __any_sync(0xffffffffu, move);
-                const float off = mref == -INFINITY ? 0.f : -mref;
-                const uint64_t sc2 = f2(w.scale_log2, w.scale_log2), off2 = f2(off, off);
-                uint64_t sum[2] = {0, 0};
-                uint32_t pk[16];
-                auto exponentials = [&](int q) {  // of scores 32 q .. 32 q + 31
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float a, b;
-                        unf2(fma2(f2(s[32 * q + 2 * i], s[32 * q + 2 * i + 1]), sc2, off2), a, b);
-                        a = ex2(a);
-                        b = ex2(b);
-                        sum[i & 1] = add2(sum[i & 1], f2(a, b));
-                        pk[i] = pack2<E>(a, b);
-                    }
-                };
-                if (!idle) exponentials(0);
-                // the product before this one has read its probabilities and written its outputs
-                if (u > 0) ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
+                // A warp without rows arrives with the others all the same, and never a unit ahead of them: it, too, waits
+                // for the product before (its early arrival would count as another warp's).
+                if (idle && u > 0) ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
                 if (!ok) break;
-                tc_fence_after();
-                if (!idle) {
-                    if (move && u > 0) {
+                // Probabilities against the reference as it stands, and the maximum beside them; only where a
+                // maximum turns out to have moved by more than the allowance are they computed once more.
+                bool again = !idle, first = u > 0;
+                while (again) {
+                    const float off = mref == -INFINITY ? 0.f : -mref;
+                    const uint64_t sc2 = f2(w.scale_log2, w.scale_log2), off2 = f2(off, off);
+                    uint64_t sum[2] = {0, 0};
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int q = 0; q < D / 16; ++q) {
-                            float o[16];
-                            tmem_ld16(t_o + 16 * q, o);
-                            uint32_t o2[16];
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t pk[16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o2[i] = __float_as_uint(o[i] * f);
-                            tmem_st16(t_o + 16 * q, o2);
+                        for (int i = 0; i < 16; ++i) {
+                            const float x = s[32 * q + 2 * i], y = s[32 * q + 2 * i + 1];
+                            mx[i & 3] = max3(mx[i & 3], x, y);
+                            float a, b;
+                            unf2(fma2(f2(x, y), sc2, off2), a, b);
+                            a = ex2(a);
+                            b = ex2(b);
+                            sum[i & 1] = add2(sum[i & 1], f2(a, b));
+                            pk[i] = pack2<E>(a, b);
                         }
-                    }
-                    tmem_st16(t_p, pk);
-#pragma unroll
-                    for (int q = 1; q < 4; ++q) {
-                        exponentials(q);
+                        if (q == 0 && first) {  // the product before has read its probabilities and written its outputs
+                            ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
+                            if (!ok) break;
+                            tc_fence_after();
+                            first = false;
+                        }
                         tmem_st16(t_p + 16 * q, pk);
                     }
-                    float l0, l1;
-                    unf2(add2(sum[0], sum[1]), l0, l1);
-                    l += l0 + l1;
-                    tmem_wait_st();
+                    if (!ok) break;
+                    const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * w.scale_log2;
+                    const bool move = m > mref + 8.f;  // also the first finite maximum
+                    again = __any_sync(0xffffffffu, move);
+                    if (again) {
+                        const float f = move ? ex2(mref - m) : 1.f;
+                        mref = move ? m : mref;
+                        l *= f;
+                        if (u > 0) {
+#pragma unroll 1
+                            for (int q = 0; q < D / 16; ++q) {
+                                float o[16];
+                                tmem_ld16(t_o + 16 * q, o);
+                                uint32_t o2[16];
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) o2[i] = __float_as_uint(o[i] * f);
+                                tmem_st16(t_o + 16 * q, o2);
+                            }
+                        }
+                    } else {
+                        float l0, l1;
+                        unf2(add2(sum[0], sum[1]), l0, l1);
+                        l += l0 + l1;
+                        tmem_wait_st();
+                    }
                 }
+                if (!ok) break;
                 if (h == 0 && base + kUnit > p1) {  // rows of v that no position owns
                     const int st = (it + 1) % ST, from = max(0, p1 - base);
                     ok = __all_sync(0xffffffffu, tc_wait(bar_full + 8 * st, ((it + 1) / ST) & 1, abort, lim, kv.errors));
