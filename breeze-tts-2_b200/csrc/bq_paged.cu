@@ -172,149 +172,157 @@ __device__ __forceinline__ void load_lane(const float* src, float (&o)[DPL]) {
     }
 }
 
-// Joins output rows from their parts -- the prefix's, then the sequence's own, in
-// CTA order -- by a running maximum, so that a part's statistics and outputs are
-// one round of loads. WPR warps work on a row, each on every WPR-th part: eight for
-// tiles of few rows, which may be spread over all CTAs, one where rows are many; a
-// warp then has R rows and always kParts parts of each in flight. Without a prefix,
-// block (c, y) takes rows of the shared tile that begins in CTA c -- tiles that one
-// CTA held are finished already; with one, blocks take all rows in turn.
-// Bound: latency of two rounds of loads (a record, then the parts), or L2 for the
-// prompts' tiles.
-template <typename E, int D, int WPR, int R, bool PREFIX>
-__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __grid_constant__ PagedJoin p) {
-    constexpr int DPL = D / 32, RPB = kJoinWarps / WPR * R;  // rows per block at a time
-    constexpr int kParts = R > 1 ? 2 : 4;
-    __shared__ float s_acc[kJoinWarps][D];
-    __shared__ float2 s_ml[kJoinWarps];
-    pdl_launch_dependents();
-    pdl_wait();
+// One output row (R = 1) or R neighbouring rows of a tile: WPR warps, each on every
+// WPR-th part, kParts parts of each row in flight. Every thread of the block calls
+// it. `place` gives row r's output row and head.
+constexpr int kFewParts = 8;
+
+template <typename E, int D, int WPR, int R, typename Place>
+__device__ __forceinline__ void join_rows(const PagedJoin& p, const RowParts (&part)[2], int rows, const Place& place) {
+    constexpr int DPL = D / 32, kParts = R > 1 ? 2 : 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WPR;
-    PagedShared sh{};
-    int total, first, stride;
-    if constexpr (PREFIX) {
-        total = p.T * p.HQ;
-        first = blockIdx.x * RPB + warp / WPR * R;
-        stride = gridDim.x * RPB;
-    } else {
-        sh = p.shared[blockIdx.x];
-        total = sh.parts ? sh.rows : 0;
-        first = blockIdx.y * RPB + warp / WPR * R;
-        stride = gridDim.y * RPB;
+    JoinRow<DPL> row[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) row[r].clear();
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+        for (int i0 = sub; i0 < part[a].n; i0 += WPR * kParts) {
+            float2 ml[kParts][R];
+            float o[kParts][R][DPL];
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                const int64_t at = part[a].at(min(i0 + i * WPR, part[a].n - 1));
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const int64_t from = at + min(r, rows - 1);  // rows of a slot follow one another
+                    ml[i][r] = part[a].ml[from];
+                    load_lane<DPL>(part[a].o + from * D + lane * DPL, o[i][r]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kParts; ++i)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if (i0 + i * WPR < part[a].n) row[r].add(ml[i][r].x, ml[i][r].y, o[i][r]);
+        }
     }
-    const int rounds = (total + stride - 1) / stride;  // the same for all warps: they meet at barriers
-    int row_lo = 0, row_hi = p.T;  // rows of sequences
-    if (PREFIX && p.starts) {
-        row_lo = p.starts[0];
-        row_hi = p.starts[p.B];
+    if constexpr (WPR > 1) {
+        __shared__ float s_acc[kJoinWarps][D];
+        __shared__ float2 s_ml[kJoinWarps];
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) s_acc[warp][lane * DPL + e] = row[0].acc[e];
+        if (lane == 0) s_ml[warp] = make_float2(row[0].m, row[0].l);
+        __syncthreads();
+        if (sub == 0) {
+#pragma unroll
+            for (int q = 1; q < WPR; ++q) {
+                float o[DPL];
+#pragma unroll
+                for (int e = 0; e < DPL; ++e) o[e] = s_acc[warp + q][lane * DPL + e];
+                row[0].add(s_ml[warp + q].x, s_ml[warp + q].y, o);
+            }
+        }
     }
-    for (int k = 0; k < rounds; ++k) {
-        const int idx = first + k * stride;
-        bool live = idx < total;
-        RowParts part[2];
-        part[0].n = part[1].n = 0;
-        if (PREFIX) {
-            if (live) {
-                const int t = p.by_HQ(idx);
-                live = t >= row_lo && t < row_hi;
-            }
-            if (live) {
+    if (sub != 0) return;
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {  // a = 0: the prefix, which comes first
-                    const PagedParts& ps = p.pass[1 - a];
-                    const int2 at = ps.row_at[idx];
-                    const int n = at.y >> 8;
-                    if (n > 0) {  // clamped: a row that ill-ordered starts left out reads no address outside
-                        const int cta = min(max(at.x, 0), ps.grid - 1);
-                        part[a] = shared_row(ps, cta, min(n, ps.grid - cta), min(at.y & 255, ps.rows - 1));
-                    } else {
-                        part[a].o = ps.row_o;
-                        part[a].ml = ps.row_ml;
-                        part[a].first = idx;
-                        part[a].n = 1;
-                    }
-                }
-            }
-        } else if (live) {
-            part[1] = shared_row(p.pass[0], blockIdx.x, sh.parts, idx);
-        }
-        JoinRow<DPL> row[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) row[r].clear();
-        const int rows = PREFIX ? 1 : min(R, total - idx);  // of this warp
-#pragma unroll
-        for (int a = PREFIX ? 0 : 1; a < 2; ++a) {
-            for (int i0 = sub; i0 < part[a].n; i0 += WPR * kParts) {
-                float2 ml[kParts][R];
-                float o[kParts][R][DPL];
-#pragma unroll
-                for (int i = 0; i < kParts; ++i) {
-                    const int64_t at = part[a].at(min(i0 + i * WPR, part[a].n - 1));
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        const int64_t from = at + min(r, rows - 1);  // rows of a slot follow one another
-                        ml[i][r] = part[a].ml[from];
-                        load_lane<DPL>(part[a].o + from * D + lane * DPL, o[i][r]);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < kParts; ++i)
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-                        if (i0 + i * WPR < part[a].n) row[r].add(ml[i][r].x, ml[i][r].y, o[i][r]);
-            }
-        }
-        if constexpr (WPR > 1) {
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < DPL; ++e) s_acc[warp][lane * DPL + e] = row[0].acc[e];
-            if (lane == 0) s_ml[warp] = make_float2(row[0].m, row[0].l);
-            __syncthreads();
-            if (sub == 0) {
-#pragma unroll
-                for (int q = 1; q < WPR; ++q) {
-                    float o[DPL];
-#pragma unroll
-                    for (int e = 0; e < DPL; ++e) o[e] = s_acc[warp + q][lane * DPL + e];
-                    row[0].add(s_ml[warp + q].x, s_ml[warp + q].y, o);
-                }
-            }
-        }
-        if (live && sub == 0) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if (r >= rows) break;
-                int t, h;
-                if (PREFIX) {
-                    t = p.by_HQ(idx);
-                    h = idx - t * p.HQ;
-                } else {
-                    const int rr = sh.r0 + idx + r, tok = p.by_G(rr);
-                    t = sh.begin + tok;
-                    h = sh.j * p.G + rr - tok * p.G;
-                }
-                const float l = row[r].l, inv = l > 0.f ? 1.f / l : 0.f;
-                const float (&acc)[DPL] = row[r].acc;
-                E* dst = static_cast<E*>(p.out) + int64_t(t) * p.ldo + h * D + lane * DPL;
-                if constexpr (DPL == 4)
-                    *reinterpret_cast<uint2*>(dst) = pack4<E>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
-                else
-                    *reinterpret_cast<uint32_t*>(dst) = pack2<E>(acc[0] * inv, acc[1] * inv);
-                if (p.lse && lane == 0) p.lse[int64_t(t) * p.ldl + h] = l > 0.f ? (row[r].m + log2f(l)) * kLn2 : -INFINITY;
-            }
-        }
+    for (int r = 0; r < R; ++r) {
+        if (r >= rows) break;
+        int t, h;
+        place(r, t, h);
+        const float l = row[r].l, inv = l > 0.f ? 1.f / l : 0.f;
+        const float (&acc)[DPL] = row[r].acc;
+        E* dst = static_cast<E*>(p.out) + int64_t(t) * p.ldo + h * D + lane * DPL;
+        if constexpr (DPL == 4)
+            *reinterpret_cast<uint2*>(dst) = pack4<E>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+        else
+            *reinterpret_cast<uint32_t*>(dst) = pack2<E>(acc[0] * inv, acc[1] * inv);
+        if (p.lse && lane == 0) p.lse[int64_t(t) * p.ldl + h] = l > 0.f ? (row[r].m + log2f(l)) * kLn2 : -INFINITY;
     }
 }
 
-constexpr int kJoinRows = 4;  // rows of a warp where rows are many
+// Joins the tiles that CTAs share: block (c, y) takes rows of the one that begins in
+// CTA c (tiles that one CTA held are finished already), R per warp, or, where the
+// tile is spread over more than kFewParts CTAs, one row at a time with all its
+// warps. Parts are added in CTA order within a warp, warps in order: deterministic.
+// Bound: latency of two rounds of loads (a record, then the parts), or L2 for the
+// prompts' tiles.
+template <typename E, int D, int R>
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __grid_constant__ PagedJoin p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const PagedShared sh = p.shared[blockIdx.x];
+    if (sh.parts == 0) return;
+    const bool few = sh.parts <= kFewParts;
+    const int per = few ? kJoinWarps * R : 1;  // rows of a block at a time
+    for (int r0 = blockIdx.y * per; r0 < sh.rows; r0 += gridDim.y * per) {
+        const int idx = few ? r0 + (threadIdx.x >> 5) * R : r0;
+        RowParts part[2];
+        part[0].n = part[1].n = 0;
+        if (idx < sh.rows) part[1] = shared_row(p.pass[0], blockIdx.x, sh.parts, idx);
+        auto place = [&](int r, int& t, int& h) {
+            const int rr = sh.r0 + idx + r, tok = p.by_G(rr);
+            t = sh.begin + tok;
+            h = sh.j * p.G + rr - tok * p.G;
+        };
+        if (few)
+            join_rows<E, D, 1, R>(p, part, max(0, min(R, sh.rows - idx)), place);
+        else
+            join_rows<E, D, kJoinWarps, 1>(p, part, 1, place);
+    }
+}
+
+// Joins every row from the prefix's parts and its own: WPR warps per row.
+template <typename E, int D, int WPR>
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_prefix_kernel(const __grid_constant__ PagedJoin p) {
+    constexpr int RPB = kJoinWarps / WPR;
+    pdl_launch_dependents();
+    pdl_wait();
+    int row_lo = 0, row_hi = p.T;  // rows of sequences
+    if (p.starts) {
+        row_lo = p.starts[0];
+        row_hi = p.starts[p.B];
+    }
+    const int total = p.T * p.HQ;
+    for (int r0 = blockIdx.x * RPB; r0 < total; r0 += gridDim.x * RPB) {
+        const int idx = r0 + (threadIdx.x >> 5) / WPR;
+        const int t = p.by_HQ(min(idx, total - 1));
+        const bool live = idx < total && t >= row_lo && t < row_hi;
+        RowParts part[2];
+        part[0].n = part[1].n = 0;
+        if (live) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {  // a = 0: the prefix, which comes first
+                const PagedParts& ps = p.pass[1 - a];
+                const int2 at = ps.row_at[idx];
+                const int n = at.y >> 8;
+                if (n > 0) {  // clamped: a row that ill-ordered starts left out reads no address outside
+                    const int cta = min(max(at.x, 0), ps.grid - 1);
+                    part[a] = shared_row(ps, cta, min(n, ps.grid - cta), min(at.y & 255, ps.rows - 1));
+                } else {
+                    part[a].o = ps.row_o;
+                    part[a].ml = ps.row_ml;
+                    part[a].first = idx;
+                    part[a].n = 1;
+                }
+            }
+        }
+        join_rows<E, D, WPR, 1>(p, part, live ? 1 : 0, [&](int, int& tt, int& h) {
+            tt = t;
+            h = idx - t * p.HQ;
+        });
+    }
+}
+
+constexpr int kJoinRows = 2;  // rows of a warp where tiles have many
 
 template <typename E, int D>
 const void* join_kernel(bool prefix, bool many) {
     if (prefix)
-        return many ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1, 1, true>)
-                    : reinterpret_cast<const void*>(&paged_join_kernel<E, D, kJoinWarps, 1, true>);
-    return many ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1, kJoinRows, false>)
-                : reinterpret_cast<const void*>(&paged_join_kernel<E, D, kJoinWarps, 1, false>);
+        return many ? reinterpret_cast<const void*>(&paged_join_prefix_kernel<E, D, 1>)
+                    : reinterpret_cast<const void*>(&paged_join_prefix_kernel<E, D, kJoinWarps>);
+    return many ? reinterpret_cast<const void*>(&paged_join_kernel<E, D, kJoinRows>)
+                : reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1>);
 }
 
 // One pass over positions: its kernel and its CTAs.
@@ -335,10 +343,14 @@ struct PagedPlan {
     size_t total;
 };
 
-// rows: rows of one tile as far as is known. Tiles of up to 16 rows take the
-// kernel for few rows, two CTAs per SM; larger ones the 256-row kernel, one per SM.
-PagedPass paged_pass(int64_t rows, int sms) {
-    if (rows <= kNarrowRows) return PagedPass{false, kNarrowRows, kNarrowUnit, 2 * sms};
+// rows: rows that share a kv head as far as is known. Up to 16 take the kernel for
+// few rows (two CTAs per SM), and up to 32 of 64 dims, though it then reads the
+// cache twice, the second time from L2 (24 rows: 32 sequences of 700 and 6000
+// positions 26 and 63 us, against 46 and 90 us with the 256-row kernel; of 128
+// dims 38 and 135 us against 55 and 94 us, where they take the latter). More go to
+// the 256-row kernel, one CTA per SM (48 rows of 64 dims, 6000 positions: 112 / 90 us).
+PagedPass paged_pass(int64_t rows, int D, int sms) {
+    if (rows <= kNarrowRows * (D == 64 ? 2 : 1)) return PagedPass{false, kNarrowRows, kNarrowUnit, 2 * sms};
     return PagedPass{true, kWideRows, kWideUnit, sms};
 }
 
@@ -349,8 +361,8 @@ int plan_paged(const bq_paged_attn_desc* d, PagedPlan* pl) {
     *pl = PagedPlan{};
     const int64_t most = !d->kv.q_starts ? 1 : d->max_q > 0 ? d->max_q : (int64_t(d->T) + d->kv.B - 1) / d->kv.B;
     pl->tile_rows = most * G;
-    pl->pass[0] = paged_pass(most * G, di->sm_count);
-    pl->pass[1] = paged_pass(int64_t(d->T) * G, di->sm_count);
+    pl->pass[0] = paged_pass(most * G, d->kv.D, di->sm_count);
+    pl->pass[1] = paged_pass(int64_t(d->T) * G, d->kv.D, di->sm_count);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -474,12 +486,13 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
     p.G = w.G;
     p.by_G = w.by_G;
     p.by_HQ.set(uint32_t(d->HQ));
-    // warps per row: see paged_join_kernel; with a prefix 1024 rows give every SM a row per warp
+    // With a prefix, 1024 rows give every SM a row per warp; fewer are shared among a block's warps.
     const int64_t rows = int64_t(d->T) * d->HQ;
     const bool many = prefix ? rows >= 1024 : pl.pass[0].wide;
-    const int rpb = !many ? 1 : prefix ? kJoinWarps : kJoinWarps * kJoinRows;
-    const dim3 grid = prefix ? dim3(unsigned(std::min<int64_t>((rows + rpb - 1) / rpb, 1 << 20)))
-                             : dim3(pl.pass[0].grid, unsigned(std::min<int64_t>(pl.pass[0].rows, pl.tile_rows) + rpb - 1) / rpb);
+    const int per = prefix ? (many ? kJoinWarps : 1) : kJoinWarps * (many ? kJoinRows : 1);
+    const int64_t tile = std::min<int64_t>(pl.pass[0].rows, pl.tile_rows);  // (a tile spread over many CTAs: a block per row)
+    const dim3 grid = prefix ? dim3(unsigned(std::min<int64_t>((rows + per - 1) / per, 1 << 20)))
+                             : dim3(pl.pass[0].grid, unsigned(std::max((tile + per - 1) / per, std::min<int64_t>(tile, 4))));
     const bool bf = d->kv.dtype == BQ_DT_BF16;
     const void* fn = d->kv.D == 128 ? (bf ? join_kernel<__nv_bfloat16, 128>(prefix, many) : join_kernel<__half, 128>(prefix, many))
                                     : (bf ? join_kernel<__nv_bfloat16, 64>(prefix, many) : join_kernel<__half, 64>(prefix, many));

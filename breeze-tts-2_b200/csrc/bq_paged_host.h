@@ -10,7 +10,7 @@ struct PagedWork;
 
 // Tile and unit of the kernel for few rows (bq_paged_narrow.cu), what a tile's
 // start and end cost in units, and its warps.
-constexpr int kNarrowRows = 16, kNarrowUnit = 64, kNarrowOverhead = 1, kNarrowWarps = 4;
+constexpr int kNarrowRows = 16, kNarrowUnit = 64, kNarrowOverhead = 2, kNarrowWarps = 4;
 // The same of the kernel for many rows (bq_paged_wide.cu).
 constexpr int kWideRows = 256, kWideUnit = 128, kWideOverhead = 1;
 int paged_launch_wide(const PagedWork& w, const bq_paged_kv* kv, int grid, uint32_t flags, void* stream);
