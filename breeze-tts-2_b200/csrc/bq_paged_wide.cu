@@ -257,6 +257,13 @@ struct WideState {
     WideTile t;
 };
 
+// Eight fp32 values, 32-byte aligned: a row's lane writes whole sectors.
+__device__ __forceinline__ void store8(float* dst, const float* v) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+                 "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+}
+
 // Queries of half h of tile t into shared memory (128 threads, thread `row`), in
 // the 128-byte-swizzled K-major layout; rows that do not exist are zeros.
 template <typename E, int D>
@@ -518,9 +525,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                             dst[i] = make_uint4(pack2<E>(o[8 * i] * inv, o[8 * i + 1] * inv), pack2<E>(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
                                                 pack2<E>(o[8 * i + 4] * inv, o[8 * i + 5] * inv), pack2<E>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
                     } else if (row < hrows) {
-                        float4* dst = reinterpret_cast<float4*>((whole ? w.row_o : w.part_o) + at * D + 32 * q);
+                        float* dst = (whole ? w.row_o : w.part_o) + at * D + 32 * q;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        for (int i = 0; i < 4; ++i) store8(dst + 8 * i, o + 8 * i);
                     }
                 }
                 if (row < hrows) {
