@@ -13,7 +13,8 @@ reference keeps its output heads in fp32, cudagraph/backbone_graph.py:70).
 ``attn`` is the attention output: with ``attention=True`` each layer runs the
 decode attention step (bq_attention_step: q/k RMSNorm, RoPE, KV-cache write,
 flash-decode over the cache) between QKV and O, as FusedDecoderLayer does
-(layer.py:89-90); otherwise the first ``attn_cols`` columns of ``qkv`` (the
+(layer.py:89-90); with ``page_size`` the rows are streams of their own length over
+a paged cache (breeze_b200.fused.paged: append, then attention); otherwise the first ``attn_cols`` columns of ``qkv`` (the
 query block) stand in for it, which keeps the QKV -> O data dependency.
 
 Every projection is one bq_gemv launch (int4 tinygemm / plain, fp8 or int8
@@ -29,6 +30,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import _lib
+from . import paged
 
 
 @dataclass
@@ -150,8 +152,20 @@ class DecodeStack:
     def __init__(self, layers: list[DecodeLayer], head: QWeight | None, ln_f: torch.Tensor, rows: int,
                  eps: float = 1e-6, attn_cols: int | None = None, chain: bool = False, attention: bool = False,
                  head_dim: int = 128, kv_heads: int | None = None, kv_len: int = 256,
-                 lm_head: torch.Tensor | None = None, sampling: dict | None = None):
-        """``lm_head``: an fp32 nn.Linear weight (V, hidden) used instead of the
+                 lm_head: torch.Tensor | None = None, sampling: dict | None = None, page_size: int | None = None,
+                 num_pages: int | None = None, prefix_len: int = 0):
+        """``page_size`` (needs ``attention``): every row is a stream of its own
+        length, up to ``kv_len`` positions, in pages of that size. ``seq_lens``
+        (rows,) int32 holds each row's length with this step's token (add 1
+        before each step; 0: an unused row), ``page_table`` (rows, kv_len /
+        page_size) int32 its pages out of ``num_pages`` per layer, ``cos`` /
+        ``sin`` (kv_len, head_dim) the rotary table by position (1 and 0 until
+        filled). ``prefix_len``: the first so many positions are the same pages
+        in every row and are read once for all. Initially all rows are full and
+        take consecutive pages, the prefix's first; with fewer pages than that
+        takes, the rows start unused and without pages (-1) of their own.
+
+        ``lm_head``: an fp32 nn.Linear weight (V, hidden) used instead of the
         quantized ``head``, as the backbone graph casts lm_head to fp32
         (backbone_graph.py:70, 272-273). ``sampling`` (needs ``lm_head``):
         the token is drawn in the graph (bq_sample) instead of on the host
@@ -218,6 +232,11 @@ class DecodeStack:
         self.graph = None
         self.chain = None
         self.attention = attention
+        self.page_size, self.prefix_len = page_size, prefix_len
+        if page_size is not None and not attention:
+            raise ValueError("a paged cache needs attention=True")
+        if prefix_len and page_size is None:
+            raise ValueError("a shared prefix needs a paged cache (page_size)")
         if attention:
             if chain:
                 raise ValueError("the decode chain runs GEMVs only; attention=True needs chain=False")
@@ -226,13 +245,32 @@ class DecodeStack:
             if (hq + 2 * hkv) * head_dim != layers[0].wqkv.N:
                 raise ValueError("QKV width does not split into q / k / v heads of head_dim")
             self.hq, self.hkv, self.head_dim, self.kv_len = hq, hkv, head_dim, kv_len
-            cache = dict(device=dev, dtype=torch.bfloat16)
-            self.k_cache = [torch.zeros(rows, hkv, kv_len, head_dim, **cache) for _ in layers]
-            self.v_cache = [torch.zeros(rows, hkv, kv_len, head_dim, **cache) for _ in layers]
-            self.cos = torch.ones(rows, 1, head_dim, **cache)
-            self.sin = torch.zeros(rows, 1, head_dim, **cache)
-            self.pos = torch.full((1,), kv_len - 1, device=dev, dtype=torch.int64)  # attend over the whole cache
             self.attn_out = torch.zeros(rows, hq * head_dim, **bf)
+            if page_size is None:
+                self.k_cache = [torch.zeros(rows, hkv, kv_len, head_dim, **bf) for _ in layers]
+                self.v_cache = [torch.zeros(rows, hkv, kv_len, head_dim, **bf) for _ in layers]
+                self.cos = torch.ones(rows, 1, head_dim, **bf)
+                self.sin = torch.zeros(rows, 1, head_dim, **bf)
+                self.pos = torch.full((1,), kv_len - 1, device=dev, dtype=torch.int64)  # attend over the whole cache
+            else:
+                if kv_len % page_size or prefix_len % page_size or not 0 <= prefix_len <= kv_len:
+                    raise ValueError(f"kv_len={kv_len} and prefix_len={prefix_len} must be whole pages of {page_size}")
+                shared, cols = prefix_len // page_size, kv_len // page_size
+                need = shared + rows * (cols - shared)
+                pages = need if num_pages is None else num_pages
+                if pages <= shared:
+                    raise ValueError(f"{pages} pages hold no position behind a prefix of {shared}")
+                shape = (pages, hkv, page_size, head_dim)
+                self.k_pages = [torch.zeros(shape, **bf) for _ in layers]
+                self.v_pages = [torch.zeros(shape, **bf) for _ in layers]
+                enough = pages >= need
+                own = torch.arange(shared, need, dtype=torch.int32) if enough else torch.full((need - shared,), -1, dtype=torch.int32)
+                prefix = torch.arange(shared, dtype=torch.int32).expand(rows, shared)
+                self.page_table = torch.cat([prefix, own.reshape(rows, cols - shared)], 1).to(dev)
+                self.seq_lens = torch.full((rows,), kv_len if enough else 0, device=dev, dtype=torch.int32)
+                self.cos = torch.ones(kv_len, head_dim, **bf)
+                self.sin = torch.zeros(kv_len, head_dim, **bf)
+                self.q = torch.zeros(rows, hq * head_dim, **bf)
         if chain:
             descs = [_lib.gemv_desc(x, qw.w, qw.wfmt, qw.N, out=out, scale=qw.scale, group=qw.group, gamma=g,
                                     eps=eps, epilogue=epi, residual=res, flags=_lib.default_flags())
@@ -251,13 +289,20 @@ class DecodeStack:
         """KV-cache bytes the attention steps read per decode step."""
         if not self.attention:
             return 0
+        if self.page_size is not None:
+            lens = self.seq_lens.clamp(min=0)
+            positions = int((lens - self.prefix_len).clamp(min=0).sum()) + min(self.prefix_len, int(lens.max()))
+            return len(self.layers) * 2 * positions * self.hkv * self.head_dim * 2
         return len(self.layers) * 2 * self.rows * self.hkv * (int(self.pos.item()) + 1) * self.head_dim * 2
 
     @property
     def launches(self) -> int:
         if self.chain is not None:
             return 1
-        return (5 if self.attention else 4) * len(self.layers) + 1 + (1 if self.sampling is not None else 0)
+        per_layer = 4
+        if self.attention:  # one step; or append, attention (twice with a prefix) and its join
+            per_layer += 1 if self.page_size is None else 4 if self.prefix_len else 3
+        return per_layer * len(self.layers) + 1 + (1 if self.sampling is not None else 0)
 
     def _ops(self):
         """(x, weight, out, gamma, epilogue, residual) of every launch, in order."""
@@ -278,9 +323,20 @@ class DecodeStack:
             self._final = x
         return ops
 
+    def _paged_attention(self, li: int) -> None:
+        """Layer li's attention over the paged caches: qkv -> attn_out."""
+        l = self.layers[li]
+        where = (self.k_pages[li], self.v_pages[li], self.page_table, self.seq_lens)
+        paged.paged_append(self.qkv[:, : l.wqkv.N], self.cos, self.sin, *where, q_norm_w=l.q_norm, k_norm_w=l.k_norm,
+                           eps=self.eps, out=self.q)
+        if self.prefix_len:
+            paged.prefix_attention(self.q, *where, self.prefix_len, out=self.attn_out)
+        else:
+            paged.paged_attention(self.q, *where, out=self.attn_out)
+
     def run(self) -> torch.Tensor:
         """Enqueue the step: one bq_gemv launch per projection (and one
-        bq_attention_step per layer with ``attention=True``), or the whole
+        bq_attention_step, or the paged operators, per layer with ``attention=True``), or the whole
         step as one decode-chain launch (``chain=True``)."""
         if self.chain is not None:
             self.chain.launch()
@@ -290,9 +346,12 @@ class DecodeStack:
             if self.attention and k % 4 == 1 and k < 4 * len(self.layers):
                 li = k // 4
                 l = self.layers[li]
-                _lib.attention_step(self.qkv[:, : l.wqkv.N], self.cos, self.sin, self.pos, self.k_cache[li],
-                                    self.v_cache[li], None, l.q_norm, l.k_norm, self.eps, out=self.attn_out,
-                                    flags=_lib.default_flags())
+                if self.page_size is not None:
+                    self._paged_attention(li)
+                else:
+                    _lib.attention_step(self.qkv[:, : l.wqkv.N], self.cos, self.sin, self.pos, self.k_cache[li],
+                                        self.v_cache[li], None, l.q_norm, l.k_norm, self.eps, out=self.attn_out,
+                                        flags=_lib.default_flags())
                 x = self.attn_out
             _lib.gemv(x, qw.w, qw.wfmt, qw.N, scale=qw.scale, group=qw.group, gamma=gamma, eps=self.eps,
                       epilogue=epi, residual=res, out=out, flags=_lib.default_flags())
