@@ -44,6 +44,8 @@ import torch
 from .. import _lib
 
 _I32, _F32 = torch.int32, torch.float32
+_UNIT = (1,)  # stride of a contiguous vector
+_CACHE_DT = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 _pack_append = _lib.packer(_lib.PagedAppendDesc)
 _pack_attn = _lib.packer(_lib.PagedAttnDesc)
 _WORKSPACE: dict = {}  # bytes by shape; a decode loop asks once
@@ -57,50 +59,57 @@ def _row_stride(t: torch.Tensor, name: str) -> int:
     return st[0] if t.shape[0] > 1 else t.shape[1]
 
 
-def _cache_fields(x: torch.Tensor, rows: int, k_pages, v_pages, page_table, seq_lens, q_starts):
+def _cache_fields(dev: int, dtype: torch.dtype, rows: int, k_pages, v_pages, page_table, seq_lens, q_starts):
     """The leading fields of both descriptors, after the checks both calls share."""
-    dev, dtype = x.get_device(), x.dtype
     if dev < 0:
         raise RuntimeError("breeze_b200 kernels need CUDA tensors (there is no CPU path)")
-    if (k_pages.get_device() != dev or v_pages.get_device() != dev or page_table.get_device() != dev
-            or seq_lens.get_device() != dev or (q_starts is not None and q_starts.get_device() != dev)):
-        raise RuntimeError(f"tensors on different devices: rows on {x.device}, cache or lengths elsewhere")
-    if dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"paged caches are bf16 or fp16 (got {dtype})")
-    if k_pages.dtype != dtype or v_pages.dtype != dtype:
+    if not (k_pages.get_device() == v_pages.get_device() == page_table.get_device() == seq_lens.get_device() == dev):
+        raise RuntimeError("tensors on different devices: the rows, the cache and the lengths must share one")
+    if not (k_pages.dtype == v_pages.dtype == dtype):
         raise ValueError(f"rows and pages must have one dtype (got {dtype}, {k_pages.dtype}, {v_pages.dtype})")
+    code = _CACHE_DT.get(dtype)
+    if code is None:
+        raise ValueError(f"paged caches are bf16 or fp16 (got {dtype})")
     shape = k_pages.shape
     if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must be (pages, HKV, page size, D) of one shape")
-    ks, vs, ts = k_pages.stride(), v_pages.stride(), page_table.stride()
-    if ks[3] != 1 or vs[3] != 1:
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    ts = page_table.stride()
+    if k3 != 1 or v3 != 1:
         raise ValueError("the last dimension of the pages must be contiguous")
     if page_table.dtype != _I32 or len(ts) != 2 or ts[1] != 1:
         raise ValueError("page_table must be int32 (B, columns) with contiguous rows")
     batch, columns = page_table.shape
-    if seq_lens.dtype != _I32 or seq_lens.shape != (batch,) or not seq_lens.is_contiguous():
+    if seq_lens.dtype != _I32 or seq_lens.shape != (batch,) or seq_lens.stride() != _UNIT:
         raise ValueError("seq_lens must be a contiguous int32 (B,)")
-    starts = 0
-    if q_starts is not None:
-        if q_starts.dtype != _I32 or q_starts.shape != (batch + 1,) or not q_starts.is_contiguous():
+    if q_starts is None:
+        if rows != batch:
+            raise ValueError(f"{rows} rows for {batch} sequences: ragged rows need q_starts")
+        starts = 0
+    else:
+        if q_starts.dtype != _I32 or q_starts.shape != (batch + 1,) or q_starts.stride() != _UNIT:
             raise ValueError("q_starts must be a contiguous int32 (B + 1,)")
+        if q_starts.get_device() != dev:
+            raise RuntimeError("tensors on different devices: q_starts is not where the rows are")
         starts = q_starts.data_ptr()
-    elif rows != batch:
-        raise ValueError(f"{rows} rows for {batch} sequences: ragged rows need q_starts")
     pages, hkv, size, dim = shape
     if pages == 0 or hkv == 0 or dim == 0 or columns == 0 or batch == 0:
         raise ValueError("empty cache or batch")
-    return (batch, hkv, dim, size, pages, columns, _lib._DT[dtype], 0, k_pages.data_ptr(), ks[0], ks[1], ks[2],
-            v_pages.data_ptr(), vs[0], vs[1], vs[2], page_table.data_ptr(), ts[0] if batch > 1 else columns,
-            seq_lens.data_ptr(), starts)
+    return (batch, hkv, dim, size, pages, columns, code, 0, k_pages.data_ptr(), k0, k1, k2, v_pages.data_ptr(), v0, v1, v2,
+            page_table.data_ptr(), ts[0] if batch > 1 else columns, seq_lens.data_ptr(), starts)
 
 
-def _on_device(dev: int, call, *args):
-    """call(*args) with ``dev`` as the current device."""
-    if dev == torch.cuda.current_device():
-        return call(*args)
-    with torch.cuda.device(dev):
-        return call(*args)
+def _launch(dev: int, what: str, call, *args) -> None:
+    """call(*args, stream): a library entry on the current stream of ``dev``, made the current device for it."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch._C._cuda_getDevice():
+        rc = call(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = call(*args, stream)
+    if rc:
+        _lib.check(rc, what)
 
 
 def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -117,75 +126,78 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_page
     ldqkv = _row_stride(qkv, "qkv")
     rows, width = qkv.shape
     dev, dtype = qkv.get_device(), qkv.dtype
-    fields = _cache_fields(qkv, rows, k_pages, v_pages, page_table, seq_lens, q_starts)
+    fields = _cache_fields(dev, dtype, rows, k_pages, v_pages, page_table, seq_lens, q_starts)
     hkv, dim = fields[1], fields[2]
     hq = width // dim - 2 * hkv
     if hq <= 0 or (hq + 2 * hkv) * dim != width:
         raise ValueError(f"qkv width {width} does not split into q, k and v heads of {dim}")
-    ldcs, cs_dtype = _row_stride(cos, "cos"), cos.dtype
-    if cos.shape != sin.shape or cos.shape[1] != dim or cs_dtype != sin.dtype or _row_stride(sin, "sin") != ldcs:
+    ldcs, cs_dtype, cs_shape = _row_stride(cos, "cos"), cos.dtype, cos.shape
+    if cs_shape[1] != dim or sin.shape != cs_shape or sin.dtype != cs_dtype or _row_stride(sin, "sin") != ldcs:
         raise ValueError("cos and sin must be (positions, D) tables of one shape, stride and dtype")
     if cs_dtype != dtype and cs_dtype != _F32:
         raise ValueError(f"cos and sin must be fp32 or the cache's dtype (got {cs_dtype})")
-    if cos.get_device() != dev or sin.get_device() != dev:
+    if not (cos.get_device() == sin.get_device() == dev):
         raise RuntimeError("cos and sin are on another device than qkv")
     qn = kn = 0
     if q_norm_w is not None and k_norm_w is not None:
         for t in (q_norm_w, k_norm_w):
-            if t.dtype != dtype or t.shape != (dim,) or not t.is_contiguous() or t.get_device() != dev:
+            if t.dtype != dtype or t.shape != (dim,) or t.stride() != _UNIT or t.get_device() != dev:
                 raise ValueError("norm weights must be contiguous (D,) vectors of the cache's dtype and device")
         qn, kn = q_norm_w.data_ptr(), k_norm_w.data_ptr()
     elif q_norm_w is not None or k_norm_w is not None:
         raise ValueError("q_norm_w and k_norm_w go together")
+    ldq = hq * dim
     if out is None:
-        out = qkv.new_empty((rows, hq * dim))
-    elif out.shape != (rows, hq * dim) or out.dtype != dtype or out.get_device() != dev:
+        out = qkv.new_empty((rows, ldq))
+    elif out.shape != (rows, ldq) or out.dtype != dtype or out.get_device() != dev:
         raise ValueError("out must be (T, HQ D) of the cache's dtype and device")
-    desc = _pack_append(*fields, rows, hq, _lib._DT[cs_dtype], cos.shape[0], eps, _lib.default_flags(), qkv.data_ptr(),
-                        ldqkv, cos.data_ptr(), sin.data_ptr(), ldcs, qn, kn, out.data_ptr(), _row_stride(out, "out"))
-    _lib.check(_on_device(dev, _lib.load().bq_paged_append, desc, torch._C._cuda_getCurrentRawStream(dev)),
-               "bq_paged_append")
+    else:
+        ldq = _row_stride(out, "out")
+    desc = _pack_append(*fields, rows, hq, _lib._DT[cs_dtype], cs_shape[0], eps, _lib.default_flags(), qkv.data_ptr(), ldqkv,
+                        cos.data_ptr(), sin.data_ptr(), ldcs, qn, kn, out.data_ptr(), ldq)
+    _launch(dev, "bq_paged_append", _lib.load().bq_paged_append, desc)
     return out
 
 
-def _workspace_bytes(desc: bytes) -> int:
-    need = ctypes.c_size_t(0)
-    _lib.check(_lib.load().bq_paged_attention_workspace_bytes(desc, ctypes.byref(need)),
-               "bq_paged_attention_workspace_bytes")
-    return need.value
+def _workspace_bytes(desc: bytes, need, stream) -> int:  # noqa: ARG001 - _launch passes the stream
+    return _lib.load().bq_paged_attention_workspace_bytes(desc, need)
 
 
 def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, causal, max_q, out, lse):
     ldq = _row_stride(q, "q")
     rows, width = q.shape
-    dev = q.get_device()
-    fields = _cache_fields(q, rows, k_pages, v_pages, page_table, seq_lens, q_starts)
+    dev, dtype = q.get_device(), q.dtype
+    fields = _cache_fields(dev, dtype, rows, k_pages, v_pages, page_table, seq_lens, q_starts)
     hkv, dim = fields[1], fields[2]
     hq = width // dim
     if hq == 0 or hq * dim != width or hq % hkv:
         raise ValueError(f"q width {width} does not split into heads of {dim} over {hkv} kv heads")
+    ldo = width
     if out is None:
         out = q.new_empty((rows, width))
-    elif out.shape != (rows, width) or out.dtype != q.dtype or out.get_device() != dev:
+    elif out.shape != (rows, width) or out.dtype != dtype or out.get_device() != dev:
         raise ValueError("out must be (T, HQ D) of q's dtype and device")
+    else:
+        ldo = _row_stride(out, "out")
     lse_ptr = ldl = 0
     if lse is not None:
         if lse.shape != (rows, hq) or lse.dtype != _F32 or lse.get_device() != dev:
             raise ValueError("lse must be fp32 (T, HQ) on q's device")
         lse_ptr, ldl = lse.data_ptr(), _row_stride(lse, "lse")
     max_q = 0 if max_q is None else max_q
+    flags = _lib.default_flags()
     desc = _pack_attn(*fields, rows, hq, prefix_len, max_q, dim ** -0.5 if scale is None else scale,
-                      _lib.default_flags() | (0 if causal else _lib.PAGED_FULL), q.data_ptr(), ldq, out.data_ptr(),
-                      _row_stride(out, "out"), lse_ptr, ldl)
+                      flags if causal else flags | _lib.PAGED_FULL, q.data_ptr(), ldq, out.data_ptr(), ldo, lse_ptr, ldl)
     key = (dev, rows, hq, hkv, dim, fields[0], prefix_len > 0, max_q, q_starts is None)
     need = _WORKSPACE.get(key)
     if need is None:
         if len(_WORKSPACE) >= 4096:
             _WORKSPACE.clear()
-        need = _WORKSPACE[key] = _on_device(dev, _workspace_bytes, desc)
+        size = ctypes.c_size_t(0)
+        _launch(dev, "bq_paged_attention_workspace_bytes", _workspace_bytes, desc, ctypes.byref(size))
+        need = _WORKSPACE[key] = size.value
     ws = torch.empty(need, device=q.device, dtype=torch.uint8)
-    _lib.check(_on_device(dev, _lib.load().bq_paged_attention, desc, ws.data_ptr(), need,
-                          torch._C._cuda_getCurrentRawStream(dev)), "bq_paged_attention")
+    _launch(dev, "bq_paged_attention", _lib.load().bq_paged_attention, desc, ws.data_ptr(), need)
     return out
 
 

@@ -63,21 +63,27 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
     uint4 raw = make_uint4(0, 0, 0, 0);
     if (live) raw = *reinterpret_cast<const uint4*>(static_cast<const E*>(p.qkv) + int64_t(t) * p.ldqkv + h * D + l * 8);
 
-    // sequence of row t: with ragged rows, the number of sequences that end at or before it
-    int b = t;
+    // Sequence of row t. With ragged rows every thread looks at some sequences, and the one that finds the row's
+    // passes on what it read: one round of loads and a barrier, whatever the batch.
+    int b = t, pos;
     if (kv.starts) {
-        int n = 0;
-        for (int i0 = 0; i0 < kv.B; i0 += kAppendThreads) {
-            const int i = i0 + int(threadIdx.x);
-            n += __syncthreads_count(i < kv.B && kv.starts[i + 1] <= t);
+        __shared__ int s_seq, s_pos;
+        if (threadIdx.x == 0) s_seq = -1;
+        __syncthreads();
+        for (int i = threadIdx.x; i < kv.B; i += kAppendThreads) {
+            const int begin = kv.starts[i], end = kv.starts[i + 1], len = kv.lens[i];
+            if (t >= begin && t < end) {
+                s_seq = i;
+                s_pos = len - (min(end, kv.T) - max(begin, 0)) + (t - max(begin, 0));
+            }
         }
-        b = n;
-        if (b >= kv.B) return;  // a row behind the last sequence
+        __syncthreads();
+        b = s_seq;
+        if (b < 0) return;  // a row of no sequence
+        pos = s_pos;
+    } else {
+        pos = kv.lens[b] - 1;
     }
-    int begin, count;
-    paged_rows(kv, b, begin, count);
-    if (t < begin || t >= begin + count) return;
-    const int pos = kv.lens[b] - count + (t - begin);
     if (pos < 0) return;  // an unused batch slot
     bool ok = pos < p.rope_rows && (pos >> kv.page_shift) < kv.max_pages;
     if (!ok) {
@@ -104,7 +110,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
             for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
             for (int m = LG / 2; m; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-            const float inv = 1.0f / sqrtf(ss / float(D) + p.eps);
+            const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * g[i];
         }

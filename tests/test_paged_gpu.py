@@ -403,7 +403,8 @@ def test_python_refusals():
     qkv = torch.zeros(2, 8 * 64, dtype=BF, device=DEV)
     good = dict(q=c["q"], k_pages=c["k"], v_pages=c["v"], page_table=c["table"], seq_lens=c["lens"])
     for change, error, text in [
-        (dict(q=c["q"].float()), ValueError, "bf16 or fp16"),
+        (dict(q=c["q"].float()), ValueError, "one dtype"),
+        (dict(q=c["q"].float(), k_pages=c["k"].float(), v_pages=c["v"].float()), ValueError, "bf16 or fp16"),
         (dict(q=c["q"].half()), ValueError, "one dtype"),
         (dict(q=c["q"][:, :100]), ValueError, "does not split"),
         (dict(q=c["q"][:, ::2]), ValueError, "unit stride"),
