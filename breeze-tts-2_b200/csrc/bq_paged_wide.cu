@@ -27,7 +27,10 @@
 //                   as stored, dims contiguous). Issuing blocks until the tensor
 //                   cores take the product, so while one warp is between two
 //                   products the other's keep them busy
-//   warp 11         completes the third warpgroup
+//   warp 11         walks the tiles of the CTA's share, passes each on to the other
+//                   roles through shared memory and fetches its queries (by TMA
+//                   when the query heads of a kv head are a power of two: then
+//                   128 rows are a box of whole tokens)
 // Page slots behind the last position arrive with the last page, whatever they
 // hold; before the product that would multiply them by zero probabilities the
 // softmax warps of half 0 clear those rows of v. Scores there are never used.
@@ -42,10 +45,11 @@
 namespace bq {
 
 struct PagedWideParams {
-    CUtensorMap kmap, vmap;  // (D, then slot, head and page in order of stride); boxes of 64 dims x positions of one page
+    CUtensorMap qmap, kmap, vmap;  // (D, then slot, head and page in order of stride); boxes of 64 dims x positions of one page
     PagedWork w;
     int32_t box;                          // positions per box: min(page size, 128)
     int32_t k_slot, k_head, v_slot, v_head;  // which of coordinates 1 .. 3 is the slot, the head (the third is the page)
+    int32_t q_tma;                        // the queries come by TMA: qmap is (D, heads, rows), boxes of 64 dims x 128 rows
     uint32_t idesc_qk, idesc_pv;
     long long wait_cycles;
 };
@@ -66,7 +70,7 @@ struct WideSmem {
     static constexpr int kStages = D == 128 ? 4 : 8;
     static constexpr uint32_t kRing = 2 * kTile;
     static constexpr uint32_t kBars = kRing + kStages * kTile;
-    static constexpr uint32_t kTotal = kBars + 256 + 1024;           // + slack to align the tiles to 1024 bytes
+    static constexpr uint32_t kTotal = kBars + 512 + 1024;           // + slack to align the tiles to 1024 bytes
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
@@ -192,37 +196,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {  // comple
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// What every role derives for the tile at the cursor.
-struct WideTile : PagedSegment<kRows, kUnit, kWideOverhead> {
+// A tile as warp 11 passes it on: units k0 .. k0 + nu of the rows r0 .. r0 + nrows of sequence b and kv head j.
+struct WideTile {
     PagedSeq s;
-    int p0, p1, r0, nrows;
-    WideTile() = default;
-    __device__ __forceinline__ WideTile(const PagedWork& w, const PagedSeq& seq, const PagedCursor& c)
-        : PagedSegment<kRows, kUnit, kWideOverhead>(w, seq, c), s(seq) {
-        p0 = (w.prefix_pass ? 0 : w.prefix_len) + k0 * kUnit;
-        p1 = min(p0 + nu * kUnit, paged_tile_limit<kRows>(w, s, c.i));
-        r0 = c.i * kRows;
-        nrows = min(kRows, s.rows - r0);
-    }
+    int b, j, r0, nrows, k0, nu, p0, p1;
+    int whole, parts;  // one CTA has all of it; CTAs that share it when it begins here
+    int ring;          // ring stages before it
+    int valid;         // 0: the share has ended
 };
-
-__device__ __forceinline__ bool wide_more(const PagedWork& w, const PagedCursor& c) {
-    return c.u < c.hi && c.b < (w.prefix_pass ? 1 : w.kv.B);
-}
-// Moves the cursor past tiles of which this share holds only overhead; false at the end of the share.
-__device__ __forceinline__ bool wide_skip(const PagedWork& w, PagedCursor& c) {
-    while (wide_more(w, c)) {
-        bool cut;
-        const PagedSegment<kRows, kUnit, kWideOverhead> g(w, paged_seq(w, c.b, cut), c);
-        if (g.nu > 0) return true;
-        paged_next<kRows>(w, c, g.cost);
-    }
-    return false;
-}
-__device__ __forceinline__ WideTile wide_tile(const PagedWork& w, const PagedCursor& c) {
-    bool cut;
-    return WideTile(w, paged_seq(w, c.b, cut), c);
-}
+constexpr int kTiles = 4;  // tiles on their way
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool full) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
@@ -251,12 +233,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// A softmax warp's place and tile.
-struct WideState {
-    PagedCursor c;
-    WideTile t;
-};
-
 // Eight fp32 values, 32-byte aligned: a row's lane writes whole sectors.
 __device__ __forceinline__ void store8(float* dst, const float* v) {
     asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
@@ -264,18 +240,42 @@ __device__ __forceinline__ void store8(float* dst, const float* v) {
                  : "memory");
 }
 
-// Queries of half h of tile t into shared memory (128 threads, thread `row`), in
-// the 128-byte-swizzled K-major layout; rows that do not exist are zeros.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+                 : "memory");
+}
+
+// Queries of half h of tile t into shared memory (one warp), in the
+// 128-byte-swizzled K-major layout, arriving on `bar`. By TMA the box may reach
+// into rows of other sequences or behind the last: those rows are not looked at.
 template <typename E, int D>
-__device__ __forceinline__ void wide_queries(const PagedWork& w, const PagedCursor& c, const WideTile& t, int h, int row, uint32_t dst) {
+__device__ __forceinline__ void wide_queries(const PagedWideParams& p, const WideTile& t, int h, int lane, uint32_t dst, uint32_t bar) {
     constexpr int CH = D / 8;
+    const PagedWork& w = p.w;
+    const int first = t.r0 + 128 * h;
+    if (p.q_tma) {
+        if (lane == 0) {
+            mbar_arrive_expect_tx(bar, 128 * D * 2);
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        const int idx = row + 128 * i, r = idx / CH, ch = idx % CH;
-        const int rr = t.r0 + min(128 * h + r, t.nrows - 1), tok = w.by_G(rr);
-        const E* src = static_cast<const E*>(w.q) + int64_t(t.s.begin + tok) * w.ldq + (c.j * w.G + rr - tok * w.G) * D + ch * 8;
-        cp_async16_zfill(dst + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src, 128 * h + r < t.nrows);
+            for (int half = 0; half < D / 64; ++half)
+                tma_load_3d(dst + half * (128 * 128), &p.qmap, half * 64, t.j * w.G, t.s.begin + w.by_G(first), bar);
+        }
+        __syncwarp();
+        return;
     }
+    const int ch = lane % CH, last = t.r0 + t.nrows - 1;
+    const E* base = static_cast<const E*>(w.q) + t.j * w.G * D + ch * 8;
+#pragma unroll 4
+    for (int r = lane / CH; r < 128; r += 32 / CH) {
+        const int rr = min(first + r, last), tok = w.by_G(rr);
+        cp_async16_zfill(dst + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
+                         base + int64_t(t.s.begin + tok) * w.ldq + (rr - tok * w.G) * D, first + r <= last);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
 }
 
 template <typename E, int D>
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    __shared__ WideState s_state[8];  // of each softmax warp: its registers are for the scores
+    __shared__ WideTile s_tile[kTiles];
     const uint32_t sraw = smem_u32(smem_raw), sb = (sraw + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (sb - sraw);
     const PagedWork& w = p.w;
@@ -294,23 +294,29 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
     volatile int* abort = &s_abort;
     const long long lim = p.wait_cycles;
     // full / empty per ring stage; per half: queries staged, scores ready, probabilities written, second product
-    // complete; scores read
+    // complete, queries used; scores read; per tile in s_tile: written, read by all eleven other warps
     const uint32_t bar_full = sb + SM::kBars, bar_empty = bar_full + 64, bar_q = bar_full + 128, bar_s = bar_full + 144,
-                   bar_p = bar_full + 160, bar_pv = bar_full + 176, bar_read = bar_full + 192, bar_done = bar_full + 200;
+                   bar_p = bar_full + 160, bar_pv = bar_full + 176, bar_read = bar_full + 192, bar_done = bar_full + 200,
+                   bar_used = bar_full + 216, bar_tile = bar_full + 232, bar_free = bar_full + 264;
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) {
             mbar_init(bar_full + 8 * i, 1);
             mbar_init(bar_empty + 8 * i, 1);
         }
         for (int h = 0; h < 2; ++h) {
-            mbar_init(bar_q + 8 * h, 4);  // an arrival per warp
+            mbar_init(bar_q + 8 * h, 1);
+            mbar_init(bar_used + 8 * h, 1);
             mbar_init(bar_s + 8 * h, 1);
-            mbar_init(bar_p + 8 * h, 4);
+            mbar_init(bar_p + 8 * h, 4);  // an arrival per warp
             mbar_init(bar_pv + 8 * h, 1);
         }
         mbar_init(bar_read, 4);
         mbar_init(bar_done, 1);
         mbar_init(bar_done + 8, 1);
+        for (int i = 0; i < kTiles; ++i) {
+            mbar_init(bar_tile + 8 * i, 1);
+            mbar_init(bar_free + 8 * i, 11);
+        }
         s_abort = 0;
         fence_barrier_init();
     }
@@ -330,43 +336,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             ok = __all_sync(0xffffffffu, wide_wait(bar, phase & 1, abort, lim, kv.errors));
     };
 
+    // The n-th tile of the share, and having read it.
+    auto tile = [&](int n) -> const WideTile& { return s_tile[n % kTiles]; };
+    auto release = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_free + 8 * (n % kTiles));
+    };
+
     if (warp < 8) {
         // ------------------------------------------------------------ softmax of one half
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int h = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
         const uint32_t t_p = lanes + 128 + 64 * h, t_o = lanes + 256 + 128 * h;
-        const uint32_t qs = sb + h * SM::kTile;
-        int done_units = 0, it = 0;  // units of this half (phases of bar_s, bar_p, bar_pv), ring stages passed
-        bool shares = false;  // shares: the last tile goes on in the next CTA
-        bool more = wide_skip(w, c);
-        WideState& state = s_state[warp];
-        auto staged = [&] {  // this thread's queries have landed; tell the tensor cores
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_q + 8 * h);
-        };
-        if (more) {
-            const WideTile t = wide_tile(w, c);
-            if (lane == 0) {
-                state.c = c;
-                state.t = t;
+        int done_units = 0;  // units of this half (phases of bar_s, bar_p, bar_pv)
+        for (int n = 0;; ++n) {
+            ok = __all_sync(0xffffffffu, tc_wait(bar_tile + 8 * (n % kTiles), (n / kTiles) & 1, abort, lim, kv.errors));
+            if (!ok) break;
+            const WideTile& t = tile(n);
+            if (!t.valid) break;
+            const int hrows = t.nrows - 128 * h;  // valid rows of this half
+            if (hrows <= 0) {
+                release(n);
+                continue;
             }
-            if (t.nrows > 128 * h) {
-                wide_queries<E, D>(w, c, t, h, row, qs);
-                staged();
-            }
-        }
-        while (ok && more) {
-            __syncwarp();
-            const int hrows = state.t.nrows - 128 * h;  // valid rows of this half
-            const int myrow = state.t.r0 + 128 * h + row, units = state.t.nu, p0 = state.t.p0, p1 = state.t.p1;
+            const int myrow = t.r0 + 128 * h + row, units = t.nu, p0 = t.p0, p1 = t.p1;
             const bool idle = (warp & 3) * 32 >= hrows;  // no row of this warp exists
-            const int limit = row < hrows ? paged_row_limit(w, state.t.s, myrow) : 0;
+            const int limit = row < hrows ? paged_row_limit(w, t.s, myrow) : 0;
             float mref = -INFINITY, l = 0.f;
             __syncwarp();  // tensor-memory instructions below are warp-wide
-            for (int u = 0; hrows > 0 && u < units; ++u) {
+            for (int u = 0; u < units; ++u) {
                 ok = __all_sync(0xffffffffu, tc_wait(bar_s + 8 * h, done_units & 1, abort, lim, kv.errors));
                 if (!ok) break;
                 tc_fence_after();
@@ -454,8 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 }
                 if (!ok) break;
                 if (h == 0 && base + kUnit > p1) {  // rows of v that no position owns
-                    const int st = (it + 1) % ST, from = max(0, p1 - base);
-                    ok = __all_sync(0xffffffffu, tc_wait(bar_full + 8 * st, ((it + 1) / ST) & 1, abort, lim, kv.errors));
+                    const int ring = t.ring + 2 * u + 1, st = ring % ST, from = max(0, p1 - base);
+                    ok = __all_sync(0xffffffffu, tc_wait(bar_full + 8 * st, (ring / ST) & 1, abort, lim, kv.errors));
                     if (!ok) break;
                     const uint4 z = make_uint4(0, 0, 0, 0);
                     for (int idx = row; idx < (128 - from) * CH; idx += 128) {
@@ -466,51 +465,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     fence_async_smem();
                     __syncwarp();
                 }
-                it += 2;
                 ++done_units;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_p + 8 * h);
             }
             if (!ok) break;
-            // This half's queries have been used: the next tile's are fetched behind the last product.
-            PagedCursor at_next = state.c;
-            const WideTile done = state.t;
-            const bool whole = done.whole();
-            const int parts = done.parts(at_next, blockIdx.x), j = at_next.j;
-            paged_next<kRows>(w, at_next, done.cost);
-            more = wide_skip(w, at_next);
-            bool next = false;
-            __syncwarp();  // every lane has read the state
-            if (more) {
-                const WideTile t = wide_tile(w, at_next);
-                if (lane == 0) {
-                    state.c = at_next;
-                    state.t = t;
-                }
-                next = t.nrows > 128 * h;
-                if (next) wide_queries<E, D>(w, at_next, t, h, row, qs);
-            }
-            if (parts) {
-                shares = true;
-                if (threadIdx.x == 0) w.shared[blockIdx.x] = PagedShared{parts, done.nrows, done.r0, done.s.begin, j};
-            }
-            if (hrows <= 0) {
-                it += 2 * done.nu;
-                if (next) staged();
-                continue;
-            }
-            __syncwarp();
             ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
             if (!ok) break;
-            if (next) staged();
             tc_fence_after();
             if (!idle) {
-                const bool final = whole && !w.row_o;
-                const int tok = w.by_G(myrow), head = j * w.G + myrow - tok * w.G;
-                const int64_t orow = done.s.begin + tok;
+                const bool whole = t.whole, final = whole && !w.row_o;
+                const int tok = w.by_G(myrow), head = t.j * w.G + myrow - tok * w.G;
+                const int64_t orow = t.s.begin + tok;
                 const int64_t at = whole ? orow * kv.HQ + head
-                                         : int64_t(2 * blockIdx.x + (done.k0 == 0 ? 1 : 0)) * kRows + 128 * h + row;
+                                         : int64_t(2 * blockIdx.x + (t.k0 == 0 ? 1 : 0)) * kRows + 128 * h + row;
                 const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
                 for (int q = 0; q < D / 32; ++q) {
@@ -533,8 +502,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 if (row < hrows) {
                     if (!final) {
                         (whole ? w.row_ml : w.part_ml)[at] = make_float2(mref, l);
-                        if (w.row_at && done.k0 == 0)
-                            w.row_at[orow * kv.HQ + head] = paged_row_at(blockIdx.x, parts, 128 * h + row);
+                        if (w.row_at && t.k0 == 0)
+                            w.row_at[orow * kv.HQ + head] = paged_row_at(blockIdx.x, t.parts, 128 * h + row);
                     } else if (w.lse) {
                         w.lse[orow * w.ldl + head] = l > 0.f ? (mref + log2f(l)) * kLn2 : -INFINITY;
                     }
@@ -542,21 +511,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             }
             __syncwarp();
             tc_fence_before();  // ordered before the next tile's first product by its bar_p arrivals
+            release(n);
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        if (threadIdx.x == 0 && !shares) w.shared[blockIdx.x].parts = 0;
     } else if (warp == 8) {
         // ------------------------------------------------------------ k / v loads
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         int it = 0;
         bool pages_ok = true;
-        while (ok && wide_skip(w, c)) {
-            const WideTile t = wide_tile(w, c);
-            for (int u = 0; ok && u < t.nu; ++u) {
-                const int base = t.p0 + u * kUnit;
-                const int nb = max(0, (min(kUnit, t.p1 - base) + p.box - 1) / p.box);  // boxes that hold positions
+        for (int n = 0;; ++n) {
+            wait(bar_tile + 8 * (n % kTiles), n / kTiles);
+            if (!ok || !tile(n).valid) break;
+            const int units = tile(n).nu, p0 = tile(n).p0, p1 = tile(n).p1, seq = tile(n).b, j = tile(n).j;
+            release(n);
+            for (int u = 0; ok && u < units; ++u) {
+                const int base = p0 + u * kUnit;
+                const int nb = max(0, (min(kUnit, p1 - base) + p.box - 1) / p.box);  // boxes that hold positions
                 int page = 0;
-                if (lane < nb) page = paged_page(kv, c.b, base + lane * p.box, pages_ok);
+                if (lane < nb) page = paged_page(kv, seq, base + lane * p.box, pages_ok);
                 const int slot = (base + lane * p.box) & kv.page_mask;
 #pragma unroll
                 for (int x = 0; x < 2; ++x, ++it) {
@@ -569,8 +540,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     if (lane < nb) {
                         const CUtensorMap* map = x ? &p.vmap : &p.kmap;
                         const int ps = x ? p.v_slot : p.k_slot, ph = x ? p.v_head : p.k_head;
-                        const int c1 = ps == 1 ? slot : ph == 1 ? c.j : page, c2 = ps == 2 ? slot : ph == 2 ? c.j : page,
-                                  c3 = ps == 3 ? slot : ph == 3 ? c.j : page;
+                        const int c1 = ps == 1 ? slot : ph == 1 ? j : page, c2 = ps == 2 ? slot : ph == 2 ? j : page,
+                                  c3 = ps == 3 ? slot : ph == 3 ? j : page;
                         const uint32_t dst = sb + SM::kRing + st * SM::kTile + uint32_t(lane * p.box) * 128u;
 #pragma unroll
                         for (int half = 0; half < D / 64; ++half)
@@ -578,7 +549,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     }
                 }
             }
-            paged_next<kRows>(w, c, t.cost);
         }
         if (!pages_ok) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
         // no tile may still be landing when the CTA leaves (an abort skips the products)
@@ -588,13 +558,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
         // ------------------------------------------------------------ products
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        int it = 0;  // ring stages before the tile
         if (warp == 9) {
             int tiles0 = 0, tiles1 = 0, scored = 0;  // tiles of each half, score tiles so far
-            while (ok && wide_skip(w, c)) {
-                const WideTile t = wide_tile(w, c);
-                const int both = __shfl_sync(0xffffffffu, t.nrows > 128 ? 1 : 0, 0);
-                const int nu = __shfl_sync(0xffffffffu, t.nu, 0);
+            for (int n = 0;; ++n) {
+                wait(bar_tile + 8 * (n % kTiles), n / kTiles);
+                if (!ok || !tile(n).valid) break;
+                const int both = __shfl_sync(0xffffffffu, tile(n).nrows > 128 ? 1 : 0, 0);
+                const int nu = __shfl_sync(0xffffffffu, tile(n).nu, 0), it = __shfl_sync(0xffffffffu, tile(n).ring, 0);
+                release(n);
                 wait(bar_q, tiles0++);
                 if (ok && both) wait(bar_q + 8, tiles1++);
                 for (int u = 0; ok && u < nu; ++u) {
@@ -607,17 +578,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                         tc_fence_after();
                         scores_product<D>(tm, ((sb + h * SM::kTile) >> 4) | kDescLoK, k_lo, p.idesc_qk, bar_s + 8 * h,
                                           h == both ? bar_empty + 8 * st : 0u);
+                        if (u + 1 == nu && elect_one()) tc_commit(bar_used + 8 * h);
+                        __syncwarp();
                     }
                 }
-                it += 2 * nu;
-                paged_next<kRows>(w, c, t.cost);
+                if (!ok) break;
             }
         } else if (warp == 10) {
             int units0 = 0, units1 = 0;  // units of each half before the tile
-            while (ok && wide_skip(w, c)) {
-                const WideTile t = wide_tile(w, c);
-                const int both = __shfl_sync(0xffffffffu, t.nrows > 128 ? 1 : 0, 0);
-                const int nu = __shfl_sync(0xffffffffu, t.nu, 0);
+            for (int n = 0;; ++n) {
+                wait(bar_tile + 8 * (n % kTiles), n / kTiles);
+                if (!ok || !tile(n).valid) break;
+                const int both = __shfl_sync(0xffffffffu, tile(n).nrows > 128 ? 1 : 0, 0);
+                const int nu = __shfl_sync(0xffffffffu, tile(n).nu, 0), it = __shfl_sync(0xffffffffu, tile(n).ring, 0);
+                release(n);
                 for (int u = 0; ok && u < nu; ++u) {
                     const int ring = it + 2 * u + 1, st = ring % ST;
                     const uint32_t v_lo = ((sb + SM::kRing + st * SM::kTile) >> 4) | kDescLoV;
@@ -630,11 +604,66 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                                        h == both ? bar_empty + 8 * st : 0u);
                     }
                 }
-                it += 2 * nu;
+                if (!ok) break;
                 units0 += nu;
                 units1 += both ? nu : 0;
-                paged_next<kRows>(w, c, t.cost);
             }
+        } else {
+            // -------------------------------------------------------- tiles and queries
+            int used0 = 0, used1 = 0, ring = 0;  // tiles of each half, ring stages so far
+            bool shares = false;                 // the last tile goes on in the next CTA
+            const int sequences = w.prefix_pass ? 1 : kv.B;
+            for (int n = 0; ok; ++n) {
+                if (n >= kTiles) wait(bar_free + 8 * (n % kTiles), n / kTiles - 1);
+                if (!ok) break;
+                WideTile t;
+                t.valid = 0;
+                while (c.u < c.hi && c.b < sequences) {  // past tiles of which this share holds only overhead
+                    bool cut;
+                    t.s = paged_seq(w, c.b, cut);
+                    const PagedSegment<kRows, kUnit, kWideOverhead> g(w, t.s, c);
+                    if (g.nu > 0) {
+                        t.b = c.b;
+                        t.j = c.j;
+                        t.r0 = c.i * kRows;
+                        t.nrows = min(kRows, t.s.rows - t.r0);
+                        t.k0 = g.k0;
+                        t.nu = g.nu;
+                        t.p0 = (w.prefix_pass ? 0 : w.prefix_len) + g.k0 * kUnit;
+                        t.p1 = min(t.p0 + g.nu * kUnit, paged_tile_limit<kRows>(w, t.s, c.i));
+                        t.whole = g.whole();
+                        t.parts = g.parts(c, blockIdx.x);
+                        t.ring = ring;
+                        t.valid = 1;
+                        paged_next<kRows>(w, c, g.cost);
+                        break;
+                    }
+                    paged_next<kRows>(w, c, g.cost);
+                }
+                if (lane == 0) {
+                    s_tile[n % kTiles] = t;
+                    mbar_arrive(bar_tile + 8 * (n % kTiles));
+                }
+                __syncwarp();
+                if (!t.valid) break;
+                ring += 2 * t.nu;
+                if (t.parts) {
+                    shares = true;
+                    if (lane == 0) w.shared[blockIdx.x] = PagedShared{t.parts, t.nrows, t.r0, t.s.begin, t.j};
+                }
+                for (int h = 0; ok && h <= (t.nrows > 128 ? 1 : 0); ++h) {
+                    int& used = h ? used1 : used0;
+                    if (used > 0) wait(bar_used + 8 * h, used - 1);  // the tile before it has been multiplied
+                    if (!ok) break;
+                    wide_queries<E, D>(p, t, h, lane, sb + h * SM::kTile, bar_q + 8 * h);
+                    ++used;
+                }
+            }
+            if (lane == 0 && !shares) w.shared[blockIdx.x].parts = 0;
+            // no queries may still be landing when the CTA leaves
+            if (used0 > 0) tc_wait(bar_q, (used0 - 1) & 1, nullptr, lim, kv.errors);
+            if (used1 > 0) tc_wait(bar_q + 8, (used1 - 1) & 1, nullptr, lim, kv.errors);
+            __syncwarp();
         }
         if (warp <= 10) {  // every product issued above has finished once this completes
             const uint32_t done = bar_done + 8 * (warp - 9);
@@ -679,6 +708,22 @@ int encode_pages(const bq_paged_kv* kv, const void* base, const int64_t* st, int
     return BQ_OK;
 }
 
+// Tensor map of the query rows, (D, heads, rows): a box is 64 dims of the G heads of
+// a kv head and of 128 / G tokens, which are 128 rows of a tile in their order.
+int encode_queries(const PagedWork& w, const bq_paged_kv* kv, CUtensorMap* map) {
+    EncodeTiledFn enc = tensor_map_encoder();
+    if (!enc) return set_error(BQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[3] = {cuuint64_t(kv->D), cuuint64_t(w.kv.HQ), cuuint64_t(w.kv.T)};
+    const cuuint64_t strides[2] = {cuuint64_t(kv->D) * 2, cuuint64_t(w.ldq) * 2};
+    const cuuint32_t box[3] = {64, cuuint32_t(w.G), cuuint32_t(128 / w.G)};
+    const cuuint32_t es[3] = {1, 1, 1};
+    const CUresult r = enc(map, kv->dtype == BQ_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                           const_cast<void*>(w.q), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(BQ_ERR_CUDA, "cuTensorMapEncodeTiled (queries) failed (%d)", int(r));
+    return BQ_OK;
+}
+
 }  // namespace
 
 int paged_launch_wide(const PagedWork& w, const bq_paged_kv* kv, int grid, uint32_t flags, void* stream) {
@@ -689,6 +734,11 @@ int paged_launch_wide(const PagedWork& w, const bq_paged_kv* kv, int grid, uint3
     int rc = encode_pages(kv, kv->k_pages, kv->k_stride, p.box, &p.kmap, &p.k_slot, &p.k_head);
     if (!rc) rc = encode_pages(kv, kv->v_pages, kv->v_stride, p.box, &p.vmap, &p.v_slot, &p.v_head);
     if (rc) return rc;
+    if (128 % w.G == 0) {
+        rc = encode_queries(w, kv, &p.qmap);
+        if (rc) return rc;
+        p.q_tma = 1;
+    }
     // kind::f16, fp32 accumulate; A and B of the pages' type; M = 128; N = 128 positions / D dims (B dims-contiguous)
     const uint32_t type = kv->dtype == BQ_DT_BF16 ? 1u : 0u;
     const uint32_t common = (1u << 4) | (type << 7) | (type << 10) | (uint32_t(128 >> 4) << 24);
