@@ -188,7 +188,7 @@ def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, 
     flags = _lib.default_flags()
     desc = _pack_attn(*fields, rows, hq, prefix_len, max_q, dim ** -0.5 if scale is None else scale,
                       flags if causal else flags | _lib.PAGED_FULL, q.data_ptr(), ldq, out.data_ptr(), ldo, lse_ptr, ldl)
-    key = (dev, rows, hq, hkv, dim, fields[0], prefix_len > 0, max_q, q_starts is None)
+    key = (dev, rows, hq, hkv, dim, fields[0], fields[3] * fields[5], prefix_len > 0, max_q, q_starts is None)
     need = _WORKSPACE.get(key)
     if need is None:
         if len(_WORKSPACE) >= 4096:
@@ -196,8 +196,8 @@ def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, 
         size = ctypes.c_size_t(0)
         _launch(dev, "bq_paged_attention_workspace_bytes", _workspace_bytes, desc, ctypes.byref(size))
         need = _WORKSPACE[key] = size.value
-    ws = torch.empty(need, device=q.device, dtype=torch.uint8)
-    _launch(dev, "bq_paged_attention", _lib.load().bq_paged_attention, desc, ws.data_ptr(), need)
+    ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+    _launch(dev, "bq_paged_attention", _lib.load().bq_paged_attention, desc, ws.data_ptr() if need else None, need)
     return out
 
 
@@ -223,5 +223,6 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     positions (a multiple of the page size): the first prefix_len / page size
     entries of every table row name the same pages. They are read once for all
     rows together, through row 0 of the table, and joined with each sequence's
-    own positions; the value is paged_attention's."""
+    own positions (a few short sequences read them each); the value is
+    paged_attention's."""
     return _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, causal, max_q, out, lse)

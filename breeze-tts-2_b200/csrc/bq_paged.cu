@@ -75,19 +75,24 @@ int paged_fill(PagedKV* o, const bq_paged_kv* kv, int T, int HQ) {
 }
 
 int paged_launch(const void* fn, dim3 grid, dim3 block, uint32_t smem, void** args, uint32_t flags, void* stream,
-                 const char* what) {
+                 const char* what, int cluster) {
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
     if (flags & BQ_FLAG_PDL) {
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = unsigned(cluster);
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs++].val.clusterDim.z = 1;
     }
     const cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
     if (e != cudaSuccess) return set_error(BQ_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
@@ -325,6 +330,13 @@ const void* join_kernel(bool prefix, bool many) {
                 : reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1>);
 }
 
+// Most positions per CTA of a cluster that the page table may hold. Clusters against
+// equal shares, 128 dims, all sequences of the table's length: two sequences of 16
+// heads, 256 / 1024 / 4096 positions 5.4 / 6.4 / 11.8 us and 8.4 / 10.7 / 17.2 us; 9
+// sequences of 8 (four CTAs per pair), 1024 / 2048 positions 13.2 / 19.0 and 14.2 /
+// 18.7 us. Uneven lengths cost a cluster its longest, hence the limit.
+constexpr int kClusterPositions = 512;
+
 // One pass over positions: its kernel and its CTAs.
 struct PagedPass {
     bool wide;
@@ -340,6 +352,7 @@ struct PagedPlan {
     PagedPass pass[2];  // own positions, the prefix
     PagedScratch at[2];
     int64_t tile_rows;  // rows of one own tile as far as is known
+    int ranks;          // > 0: one cluster of so many CTAs per (sequence, kv head) instead
     size_t total;
 };
 
@@ -361,6 +374,15 @@ int plan_paged(const bq_paged_attn_desc* d, PagedPlan* pl) {
     *pl = PagedPlan{};
     const int64_t most = !d->kv.q_starts ? 1 : d->max_q > 0 ? d->max_q : (int64_t(d->T) + d->kv.B - 1) / d->kv.B;
     pl->tile_rows = most * G;
+    if (most * G <= kNarrowRows) {
+        const int64_t pairs = int64_t(d->kv.B) * d->kv.HKV, room = int64_t(d->kv.max_pages) * d->kv.page_size;
+        int ranks = kNarrowRanks;
+        while (ranks > 1 && pairs * ranks > 2 * di->sm_count) ranks >>= 1;
+        if (ranks > 1 && room <= int64_t(kClusterPositions) * ranks) {
+            pl->ranks = ranks;
+            return BQ_OK;
+        }
+    }
     pl->pass[0] = paged_pass(most * G, d->kv.D, di->sm_count);
     pl->pass[1] = paged_pass(int64_t(d->T) * G, d->kv.D, di->sm_count);
     size_t at = 0;
@@ -437,7 +459,7 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
     PagedPlan pl;
     rc = plan_paged(d, &pl);
     if (rc) return rc;
-    if (!workspace || workspace_bytes < pl.total)
+    if (pl.total && (!workspace || workspace_bytes < pl.total))
         return set_error(BQ_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", workspace_bytes, pl.total);
     if (reinterpret_cast<uintptr_t>(workspace) & 255) return set_error(BQ_ERR_ALIGN, "workspace must be 256-byte aligned");
     char* ws = static_cast<char*>(workspace);
@@ -456,6 +478,7 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
     w.ldo = d->ldo;
     w.lse = d->lse;
     w.ldl = d->ldl;
+    if (pl.ranks) return paged_launch_cluster(w, d->kv.dtype, d->kv.D, pl.ranks, d->flags, stream);
     PagedJoin p;
     std::memset(&p, 0, sizeof(p));
     const bool prefix = d->prefix_len > 0;

@@ -19,6 +19,10 @@ constexpr int kWideRows = 256, kWideUnit = 128, kWideOverhead = 3;
 int paged_launch_wide(const PagedWork& w, const bq_paged_kv* kv, int grid, uint32_t flags, void* stream);
 int paged_launch_narrow(const PagedWork& w, int dtype, int D, int grid, uint32_t flags, void* stream);
 
+// The form of the few-row kernel with a cluster of `ranks` CTAs per (sequence, kv head).
+constexpr int kNarrowRanks = 8;
+int paged_launch_cluster(const PagedWork& w, int dtype, int D, int ranks, uint32_t flags, void* stream);
+
 // Checks the cache part of a descriptor with T new rows of HQ query heads.
 int paged_validate(const bq_paged_kv* kv, int T, int HQ);
 // BQ_OK when the current device is the one this library is built for.
@@ -28,7 +32,8 @@ int paged_fill(PagedKV* out, const bq_paged_kv* kv, int T, int HQ);
 inline bool paged_aligned(const void* p, int64_t ld, int elem) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * elem) % 16 == 0;
 }
+// cluster: CTAs per cluster along x (1: none).
 int paged_launch(const void* fn, dim3 grid, dim3 block, uint32_t smem, void** args, uint32_t flags, void* stream,
-                 const char* what);
+                 const char* what, int cluster = 1);
 
 }  // namespace bq

@@ -24,6 +24,7 @@ namespace bq {
 namespace {
 
 constexpr int kThreads = 32 * kNarrowWarps;
+constexpr int kMaxRanks = kNarrowRanks;
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool full) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
@@ -69,197 +70,221 @@ struct NarrowSmem {
     static_assert(kNarrowWarps * 16 * kPitch * 4 <= kQ, "the warps' outputs fit the rings");
 };
 
+// Positions [p0, p1) of rows r0 .. r0 + nrows of sequence b and kv head j.
+struct NarrowTile {
+    PagedSeq s;
+    int b, j, r0, nrows, p0, p1;
+};
+
+// One tile with the whole CTA: emit(r, d, m, l, o) receives dims d .. d + 3 of row r,
+// unnormalized, with the row's largest score (base 2) and sum of exponentials.
+template <typename E, int D, typename Emit>
+__device__ __forceinline__ void narrow_tile(const PagedWork& p, const NarrowTile& t, unsigned char* smem, int* s_lim,
+                                            float2 (*s_ml)[kNarrowRows], const Emit& emit) {
+    using SM = NarrowSmem<D>;
+    constexpr int ROWS = kNarrowRows, CH = D / 8, ST = SM::kStages;
+    const uint32_t sb = smem_u32(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+    const PagedKV& kv = p.kv;
+    const uint32_t ring = sb + warp * SM::kRing;
+    const PagedSeq& s = t.s;
+    const int p0 = t.p0, p1 = t.p1, r0 = t.r0, nrows = t.nrows;
+    bool pages_ok = true;
+    const int blocks = max(0, (p1 - p0 + 15) >> 4);
+    const int steps = (blocks - warp + kNarrowWarps - 1) / kNarrowWarps;
+    const E* kh = static_cast<const E*>(kv.k) + t.j * kv.ks_head;
+    const E* vh = static_cast<const E*>(kv.v) + t.j * kv.vs_head;
+
+    // query tile: row r0 + r is head j G + (r0 + r) % G of token (r0 + r) / G
+    for (int idx = threadIdx.x; idx < ROWS * CH; idx += kThreads) {
+        const int r = idx / CH, ch = idx - r * CH, rr = r0 + min(r, nrows - 1), tok = p.by_G(rr);
+        const E* src = static_cast<const E*>(p.q) + int64_t(s.begin + tok) * p.ldq + (t.j * p.G + rr - tok * p.G) * D + ch * 8;
+        cp_async16_zfill(sb + SM::kQ + r * (D * 2) + ((ch ^ (r & 7)) << 4), src, r < nrows);
+    }
+    cp_commit();
+
+    int pages = 0;  // lane i: page of the warp's step (32 n + i)
+    auto issue = [&](int st) {
+        if ((st & 31) == 0) {
+            const int mine = st + lane;
+            pages = mine < steps ? paged_page(kv, t.b, p0 + 16 * (warp + kNarrowWarps * mine), pages_ok) : 0;
+        }
+        const int page = __shfl_sync(0xffffffffu, pages, st & 31);
+        if (st < steps) {
+            const int pb = p0 + 16 * (warp + kNarrowWarps * st), slot = pb & kv.page_mask;
+            const E* kp = kh + page * kv.ks_page + slot * kv.ks_slot;
+            const E* vp = vh + page * kv.vs_page + slot * kv.vs_slot;
+            const uint32_t dst = ring + (st % ST) * (2 * SM::kBlock);
+#pragma unroll
+            for (int i = 0; i < 16 * CH / 32; ++i) {
+                const int idx = lane + 32 * i, r = idx / CH, ch = idx % CH;
+                const uint32_t at = r * (D * 2) + ((ch ^ (r & 7)) << 4);
+                cp_async16_zfill(dst + at, kp + r * kv.ks_slot + ch * 8, pb + r < p1);
+                cp_async16_zfill(dst + SM::kBlock + at, vp + r * kv.vs_slot + ch * 8, pb + r < p1);
+            }
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int st = 0; st < ST - 1; ++st) issue(st);
+    if (threadIdx.x < ROWS) s_lim[threadIdx.x] = int(threadIdx.x) < nrows ? paged_row_limit(p, s, r0 + threadIdx.x) : 0;
+    cp_wait<ST - 1>();  // the query tile
+    __syncthreads();
+    uint32_t qf[D / 16][4];
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        const int r = (lane & 7) + (lane & 8), ch = 2 * ks + (lane >> 4);
+        ldsm4(qf[ks], sb + SM::kQ + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+    }
+    const int lim0 = s_lim[g], lim1 = s_lim[g + 8];
+    float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+
+    for (int st = 0; st < steps; ++st) {
+        cp_wait<ST - 2>();
+        __syncwarp();  // every lane's copies of this stage have landed, and every lane is done with the one before
+        issue(st + ST - 1);
+        const uint32_t kb = ring + (st % ST) * (2 * SM::kBlock), vb = kb + SM::kBlock;
+        float sc[2][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t bf[4];
+            const int r = (lane & 7) + ((lane >> 4) << 3), ch = 2 * ks + ((lane >> 3) & 1);
+            ldsm4(bf, kb + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+            mma<E>(sc[0], qf[ks], bf[0], bf[1]);
+            mma<E>(sc[1], qf[ks], bf[2], bf[3]);
+        }
+        const int pb = p0 + 16 * (warp + kNarrowWarps * st) + 2 * tq;
+        float n0 = m0, n1 = m1;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int pos = pb + 8 * n + e;
+                sc[n][e] = pos < lim0 ? sc[n][e] * p.scale_log2 : -INFINITY;
+                sc[n][2 + e] = pos < lim1 ? sc[n][2 + e] * p.scale_log2 : -INFINITY;
+                n0 = fmaxf(n0, sc[n][e]);
+                n1 = fmaxf(n1, sc[n][2 + e]);
+            }
+        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
+        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
+        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
+        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
+        if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {  // a maximum moved: rescale what was summed
+            const float a0 = n0 == m0 ? 1.f : ex2(m0 - n0), a1 = n1 == m1 ? 1.f : ex2(m1 - n1);
+            l0 *= a0;
+            l1 *= a1;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+                o[n][0] *= a0;
+                o[n][1] *= a0;
+                o[n][2] *= a1;
+                o[n][3] *= a1;
+            }
+            m0 = n0;
+            m1 = n1;
+        }
+        const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;  // rows that see nothing yet
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                sc[n][e] = ex2(sc[n][e] - u0);
+                sc[n][2 + e] = ex2(sc[n][2 + e] - u1);
+                l0 += sc[n][e];
+                l1 += sc[n][2 + e];
+            }
+        const uint32_t pf[4] = {pack2<E>(sc[0][0], sc[0][1]), pack2<E>(sc[0][2], sc[0][3]),
+                                pack2<E>(sc[1][0], sc[1][1]), pack2<E>(sc[1][2], sc[1][3])};
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+            uint32_t bf[4];
+            const int r = (lane & 7) + (lane & 8), ch = 2 * dt + (lane >> 4);
+            ldsm4t(bf, vb + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+            mma<E>(o[2 * dt], pf, bf[0], bf[1]);
+            mma<E>(o[2 * dt + 1], pf, bf[2], bf[3]);
+        }
+    }
+    cp_wait<0>();
+    if (!pages_ok) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    __syncthreads();  // every warp is done with its ring: it now takes the warps' outputs
+    float* red = reinterpret_cast<float*>(smem);
+    if (g < nrows) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(red + (warp * 16 + g) * SM::kPitch + 8 * n + 2 * tq) = make_float2(o[n][0], o[n][1]);
+        if (tq == 0) s_ml[warp][g] = make_float2(m0, l0);
+    }
+    if (g + 8 < nrows) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(red + (warp * 16 + g + 8) * SM::kPitch + 8 * n + 2 * tq) =
+                make_float2(o[n][2], o[n][3]);
+        if (tq == 0) s_ml[warp][g + 8] = make_float2(m1, l1);
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < nrows * (D / 4); idx += kThreads) {
+        const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
+        float mm = -INFINITY, ll = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kNarrowWarps; ++w) mm = fmaxf(mm, s_ml[w][r].x);
+        const float u = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+        for (int w = 0; w < kNarrowWarps; ++w) {
+            const float f = ex2(s_ml[w][r].x - u);
+            const float4 v = *reinterpret_cast<const float4*>(red + (w * 16 + r) * SM::kPitch + d);
+            ll = fmaf(f, s_ml[w][r].y, ll);
+            a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
+        }
+        emit(r, d, mm, ll, a);
+    }
+    __syncthreads();  // the rings are free again
+}
+
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_constant__ PagedWork p) {
-    using SM = NarrowSmem<D>;
-    constexpr int ROWS = kNarrowRows, UNIT = kNarrowUnit, CH = D / 8, ST = SM::kStages;
+    constexpr int ROWS = kNarrowRows, UNIT = kNarrowUnit;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int s_lim[ROWS];
     __shared__ float2 s_ml[kNarrowWarps][ROWS];
-    const uint32_t sb = smem_u32(smem);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
     const PagedKV& kv = p.kv;
     pdl_launch_dependents();
     pdl_wait();
     PagedCursor c = paged_find<ROWS, UNIT, kNarrowOverhead, kThreads>(p, blockIdx.x, gridDim.x);
     bool shares = false;  // the last tile goes on in the next CTA
-    const int kv_lo = p.prefix_pass ? 0 : p.prefix_len;
-    const uint32_t ring = sb + warp * SM::kRing;
-
-    const int sequences = p.prefix_pass ? 1 : kv.B;
+    const int kv_lo = p.prefix_pass ? 0 : p.prefix_len, sequences = p.prefix_pass ? 1 : kv.B;
     while (c.u < c.hi && c.b < sequences) {
-        bool cut, pages_ok = true;
-        const PagedSeq s = paged_seq(p, c.b, cut);
-        const int limit = paged_tile_limit<ROWS>(p, s, c.i);
-        const PagedSegment<ROWS, UNIT, kNarrowOverhead> sg(p, s, c);
+        bool cut;
+        NarrowTile t;
+        t.s = paged_seq(p, c.b, cut);
+        const PagedSegment<ROWS, UNIT, kNarrowOverhead> sg(p, t.s, c);
         if (sg.nu == 0) {
             paged_next<ROWS>(p, c, sg.cost);
             continue;
         }
-        const int p0 = kv_lo + sg.k0 * UNIT, p1 = min(p0 + sg.nu * UNIT, limit);
-        const int r0 = c.i * ROWS, nrows = min(ROWS, s.rows - r0);
-        const int blocks = max(0, (p1 - p0 + 15) >> 4);
-        const int steps = (blocks - warp + kNarrowWarps - 1) / kNarrowWarps;
-        const E* kh = static_cast<const E*>(kv.k) + c.j * kv.ks_head;
-        const E* vh = static_cast<const E*>(kv.v) + c.j * kv.vs_head;
-
-        // query tile: row r0 + r is head j G + (r0 + r) % G of token (r0 + r) / G
-        for (int idx = threadIdx.x; idx < ROWS * CH; idx += kThreads) {
-            const int r = idx / CH, ch = idx - r * CH, rr = r0 + min(r, nrows - 1), tok = p.by_G(rr);
-            const E* src = static_cast<const E*>(p.q) + int64_t(s.begin + tok) * p.ldq + (c.j * p.G + rr - tok * p.G) * D + ch * 8;
-            cp_async16_zfill(sb + SM::kQ + r * (D * 2) + ((ch ^ (r & 7)) << 4), src, r < nrows);
-        }
-        cp_commit();
-
-        int pages = 0;  // lane i: page of the warp's step (32 n + i)
-        auto issue = [&](int st) {
-            if ((st & 31) == 0) {
-                const int mine = st + lane;
-                pages = mine < steps ? paged_page(kv, c.b, p0 + 16 * (warp + kNarrowWarps * mine), pages_ok) : 0;
-            }
-            const int page = __shfl_sync(0xffffffffu, pages, st & 31);
-            if (st < steps) {
-                const int pb = p0 + 16 * (warp + kNarrowWarps * st), slot = pb & kv.page_mask;
-                const E* kp = kh + page * kv.ks_page + slot * kv.ks_slot;
-                const E* vp = vh + page * kv.vs_page + slot * kv.vs_slot;
-                const uint32_t dst = ring + (st % ST) * (2 * SM::kBlock);
-#pragma unroll
-                for (int i = 0; i < 16 * CH / 32; ++i) {
-                    const int idx = lane + 32 * i, r = idx / CH, ch = idx % CH;
-                    const uint32_t at = r * (D * 2) + ((ch ^ (r & 7)) << 4);
-                    cp_async16_zfill(dst + at, kp + r * kv.ks_slot + ch * 8, pb + r < p1);
-                    cp_async16_zfill(dst + SM::kBlock + at, vp + r * kv.vs_slot + ch * 8, pb + r < p1);
-                }
-            }
-            cp_commit();
-        };
-#pragma unroll
-        for (int st = 0; st < ST - 1; ++st) issue(st);
-        if (threadIdx.x < ROWS) s_lim[threadIdx.x] = int(threadIdx.x) < nrows ? paged_row_limit(p, s, r0 + threadIdx.x) : 0;
-        cp_wait<ST - 1>();  // the query tile
-        __syncthreads();
-        uint32_t qf[D / 16][4];
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            const int r = (lane & 7) + (lane & 8), ch = 2 * ks + (lane >> 4);
-            ldsm4(qf[ks], sb + SM::kQ + r * (D * 2) + ((ch ^ (r & 7)) << 4));
-        }
-        const int lim0 = s_lim[g], lim1 = s_lim[g + 8];
-        float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-
-        for (int st = 0; st < steps; ++st) {
-            cp_wait<ST - 2>();
-            __syncwarp();  // every lane's copies of this stage have landed, and every lane is done with the one before
-            issue(st + ST - 1);
-            const uint32_t kb = ring + (st % ST) * (2 * SM::kBlock), vb = kb + SM::kBlock;
-            float sc[2][4] = {};
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-                uint32_t bf[4];
-                const int r = (lane & 7) + ((lane >> 4) << 3), ch = 2 * ks + ((lane >> 3) & 1);
-                ldsm4(bf, kb + r * (D * 2) + ((ch ^ (r & 7)) << 4));
-                mma<E>(sc[0], qf[ks], bf[0], bf[1]);
-                mma<E>(sc[1], qf[ks], bf[2], bf[3]);
-            }
-            const int pb = p0 + 16 * (warp + kNarrowWarps * st) + 2 * tq;
-            float n0 = m0, n1 = m1;
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int pos = pb + 8 * n + e;
-                    sc[n][e] = pos < lim0 ? sc[n][e] * p.scale_log2 : -INFINITY;
-                    sc[n][2 + e] = pos < lim1 ? sc[n][2 + e] * p.scale_log2 : -INFINITY;
-                    n0 = fmaxf(n0, sc[n][e]);
-                    n1 = fmaxf(n1, sc[n][2 + e]);
-                }
-            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
-            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
-            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
-            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
-            if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {  // a maximum moved: rescale what was summed
-                const float a0 = n0 == m0 ? 1.f : ex2(m0 - n0), a1 = n1 == m1 ? 1.f : ex2(m1 - n1);
-                l0 *= a0;
-                l1 *= a1;
-#pragma unroll
-                for (int n = 0; n < D / 8; ++n) {
-                    o[n][0] *= a0;
-                    o[n][1] *= a0;
-                    o[n][2] *= a1;
-                    o[n][3] *= a1;
-                }
-                m0 = n0;
-                m1 = n1;
-            }
-            const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;  // rows that see nothing yet
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    sc[n][e] = ex2(sc[n][e] - u0);
-                    sc[n][2 + e] = ex2(sc[n][2 + e] - u1);
-                    l0 += sc[n][e];
-                    l1 += sc[n][2 + e];
-                }
-            const uint32_t pf[4] = {pack2<E>(sc[0][0], sc[0][1]), pack2<E>(sc[0][2], sc[0][3]),
-                                    pack2<E>(sc[1][0], sc[1][1]), pack2<E>(sc[1][2], sc[1][3])};
-#pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt) {
-                uint32_t bf[4];
-                const int r = (lane & 7) + (lane & 8), ch = 2 * dt + (lane >> 4);
-                ldsm4t(bf, vb + r * (D * 2) + ((ch ^ (r & 7)) << 4));
-                mma<E>(o[2 * dt], pf, bf[0], bf[1]);
-                mma<E>(o[2 * dt + 1], pf, bf[2], bf[3]);
-            }
-        }
-        cp_wait<0>();
-        if (!pages_ok) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        __syncthreads();  // every warp is done with its ring: it now takes the warps' outputs
-        float* red = reinterpret_cast<float*>(smem);
-        if (g < nrows) {
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-                *reinterpret_cast<float2*>(red + (warp * 16 + g) * SM::kPitch + 8 * n + 2 * tq) = make_float2(o[n][0], o[n][1]);
-            if (tq == 0) s_ml[warp][g] = make_float2(m0, l0);
-        }
-        if (g + 8 < nrows) {
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-                *reinterpret_cast<float2*>(red + (warp * 16 + g + 8) * SM::kPitch + 8 * n + 2 * tq) =
-                    make_float2(o[n][2], o[n][3]);
-            if (tq == 0) s_ml[warp][g + 8] = make_float2(m1, l1);
-        }
-        __syncthreads();
+        t.b = c.b;
+        t.j = c.j;
+        t.p0 = kv_lo + sg.k0 * UNIT;
+        t.p1 = min(t.p0 + sg.nu * UNIT, paged_tile_limit<ROWS>(p, t.s, c.i));
+        t.r0 = c.i * ROWS;
+        t.nrows = min(ROWS, t.s.rows - t.r0);
         const bool whole = sg.whole();
         const int slot = 2 * blockIdx.x + (sg.k0 == 0 ? 1 : 0), parts = sg.parts(c, blockIdx.x);
         if (parts) {
             shares = true;
-            if (threadIdx.x == 0) p.shared[blockIdx.x] = PagedShared{parts, nrows, r0, s.begin, c.j};
+            if (threadIdx.x == 0) p.shared[blockIdx.x] = PagedShared{parts, t.nrows, t.r0, t.s.begin, c.j};
         }
-        for (int idx = threadIdx.x; idx < nrows * (D / 4); idx += kThreads) {
-            const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
-            float mm = -INFINITY, ll = 0.f;
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kNarrowWarps; ++w) mm = fmaxf(mm, s_ml[w][r].x);
-            const float u = mm == -INFINITY ? 0.f : mm;
-#pragma unroll
-            for (int w = 0; w < kNarrowWarps; ++w) {
-                const float f = ex2(s_ml[w][r].x - u);
-                const float4 v = *reinterpret_cast<const float4*>(red + (w * 16 + r) * SM::kPitch + d);
-                ll = fmaf(f, s_ml[w][r].y, ll);
-                a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
-            }
-            const int rr = r0 + r, tok = p.by_G(rr), head = c.j * p.G + rr - tok * p.G;
-            const int64_t row = s.begin + tok;
+        narrow_tile<E, D>(p, t, smem, s_lim, s_ml, [&](int r, int d, float mm, float ll, const float4& a) {
+            const int rr = t.r0 + r, tok = p.by_G(rr), head = c.j * p.G + rr - tok * p.G;
+            const int64_t row = t.s.begin + tok;
             if (whole && !p.row_o) {
                 const float inv = ll > 0.f ? 1.f / ll : 0.f;
                 *reinterpret_cast<uint2*>(static_cast<E*>(p.out) + row * p.ldo + head * D + d) =
@@ -273,11 +298,80 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
                     if (p.row_at && sg.k0 == 0) p.row_at[row * kv.HQ + head] = paged_row_at(blockIdx.x, parts, r);
                 }
             }
-        }
-        __syncthreads();  // the rings are free again
+        });
         paged_next<ROWS>(p, c, sg.cost);
     }
     if (!shares && threadIdx.x == 0) p.shared[blockIdx.x].parts = 0;
+}
+
+// Few (sequence, kv head) pairs and a short cache: a cluster of CTAs per pair takes
+// equal pieces of its positions and joins them through distributed shared memory
+// (rank order, deterministic). No schedule to work out, no partials in memory and
+// no second kernel. A shared prefix is read by each pair, mostly from L2.
+template <typename E, int D>
+__global__ void __launch_bounds__(kThreads, 2) paged_cluster_kernel(const __grid_constant__ PagedWork p, int ranks) {
+    using SM = NarrowSmem<D>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int s_lim[kNarrowRows];
+    __shared__ float2 s_ml[kNarrowWarps][kNarrowRows];
+    __shared__ float2 s_row[kNarrowRows];
+    constexpr int kOut = 40960;  // of the rings, behind the warps' outputs: this CTA's rows
+    static_assert(kNarrowWarps * 16 * SM::kPitch * 4 <= kOut && kOut + 16 * D * 4 <= SM::kQ, "the rows fit the rings");
+    float* out = reinterpret_cast<float*>(smem + kOut);
+    pdl_launch_dependents();
+    pdl_wait();
+    const int pair = blockIdx.x / ranks, rank = blockIdx.x - pair * ranks;
+    NarrowTile t;
+    t.b = pair / p.kv.HKV;
+    t.j = pair - t.b * p.kv.HKV;
+    bool cut;
+    t.s = paged_seq(p, t.b, cut);
+    if (cut && rank == 0 && t.j == 0 && threadIdx.x == 0) atomicOr(p.kv.errors, BQ_DEVERR_POSITION_BIT);
+    for (int i = 0; i * kNarrowRows < t.s.rows; ++i) {  // one tile, unless max_q was told too low
+        t.r0 = i * kNarrowRows;
+        t.nrows = min(kNarrowRows, t.s.rows - t.r0);
+        const int limit = paged_tile_limit<kNarrowRows>(p, t.s, i), units = (limit + kNarrowUnit - 1) / kNarrowUnit;
+        t.p0 = rank * units / ranks * kNarrowUnit;
+        t.p1 = min((rank + 1) * units / ranks * kNarrowUnit, limit);
+        narrow_tile<E, D>(p, t, smem, s_lim, s_ml, [&](int r, int d, float mm, float ll, const float4& a) {
+            *reinterpret_cast<float4*>(out + r * D + d) = a;
+            if (d == 0) s_row[r] = make_float2(mm, ll);
+        });
+        cluster_sync_all();  // every rank's rows are in its shared memory
+        for (int idx = rank * kThreads + threadIdx.x; idx < t.nrows * (D / 4); idx += ranks * kThreads) {
+            const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
+            const uint32_t a_out = smem_u32(out + r * D + d), a_row = smem_u32(&s_row[r]);
+            float m[kMaxRanks], l[kMaxRanks], mm = -INFINITY, ll = 0.f;
+            float4 o[kMaxRanks], a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < kMaxRanks; ++q) {
+                if (q < ranks) {
+                    const uint32_t from = dsmem_addr(a_row, uint32_t(q));
+                    m[q] = dsmem_ld_f32(from);
+                    l[q] = dsmem_ld_f32(from + 4);
+                    o[q] = dsmem_ld4(dsmem_addr(a_out, uint32_t(q)));
+                    mm = fmaxf(mm, m[q]);
+                }
+            }
+            const float u = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+            for (int q = 0; q < kMaxRanks; ++q) {
+                if (q < ranks) {
+                    const float f = ex2(m[q] - u);
+                    ll = fmaf(f, l[q], ll);
+                    a.x = fmaf(f, o[q].x, a.x), a.y = fmaf(f, o[q].y, a.y), a.z = fmaf(f, o[q].z, a.z), a.w = fmaf(f, o[q].w, a.w);
+                }
+            }
+            const int rr = t.r0 + r, tok = p.by_G(rr), head = t.j * p.G + rr - tok * p.G;
+            const int64_t row = t.s.begin + tok;
+            const float inv = ll > 0.f ? 1.f / ll : 0.f;
+            *reinterpret_cast<uint2*>(static_cast<E*>(p.out) + row * p.ldo + head * D + d) =
+                pack4<E>(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+            if (p.lse && d == 0) p.lse[row * p.ldl + head] = ll > 0.f ? (mm + log2f(ll)) * kLn2 : -INFINITY;
+        }
+        cluster_sync_relaxed();  // rows are not written over, nor does a rank leave, while another reads them (the reads
+                                 // were consumed by the stores)
+    }
 }
 
 }  // namespace
@@ -292,6 +386,19 @@ int paged_launch_narrow(const PagedWork& w, int dtype, int D, int grid, uint32_t
     if (rc) return rc;
     void* args[] = {const_cast<PagedWork*>(&w)};
     return paged_launch(fn, dim3(grid), dim3(kThreads), smem, args, flags, stream, "paged attention");
+}
+
+int paged_launch_cluster(const PagedWork& w, int dtype, int D, int ranks, uint32_t flags, void* stream) {
+    const void* fn = D == 128 ? (dtype == BQ_DT_BF16 ? reinterpret_cast<const void*>(&paged_cluster_kernel<__nv_bfloat16, 128>)
+                                                     : reinterpret_cast<const void*>(&paged_cluster_kernel<__half, 128>))
+                              : (dtype == BQ_DT_BF16 ? reinterpret_cast<const void*>(&paged_cluster_kernel<__nv_bfloat16, 64>)
+                                                     : reinterpret_cast<const void*>(&paged_cluster_kernel<__half, 64>));
+    const uint32_t smem = D == 128 ? NarrowSmem<128>::kTotal : NarrowSmem<64>::kTotal;
+    const int rc = ensure_smem_attr(fn, smem);
+    if (rc) return rc;
+    void* args[] = {const_cast<PagedWork*>(&w), &ranks};
+    return paged_launch(fn, dim3(unsigned(w.kv.B) * w.kv.HKV * ranks), dim3(kThreads), smem, args, flags, stream, "paged attention",
+                        ranks);
 }
 
 }  // namespace bq

@@ -343,7 +343,8 @@ int32_t bq_paged_append(const bq_paged_append_desc* desc, void* stream);
  * given, is the natural logarithm of each row's sum of exponentials.
  * prefix_len > 0: the first prefix_len positions (a multiple of page_size) are
  * the same pages in every row of the table and are read once for the whole
- * batch, through row 0; the value is the same. */
+ * batch, through row 0, where that pays (few short sequences read them each);
+ * the value is the same. */
 #define BQ_PAGED_FULL 2u
 
 typedef struct bq_paged_attn_desc {

@@ -67,6 +67,19 @@ def compare(c, out, lse, causal=True, scale=None):
     assert (o[rows:] == 3.0).all() and (lse[rows:] == 7.0).all()  # rows behind the last sequence
 
 
+@pytest.fixture(params=["tight", "roomy"])
+def table_room(request):
+    """A table that ends with its longest sequence, and one with room for another
+    32768 positions: the room decides how a sequence is divided among CTAs."""
+
+    def apply(c):
+        if request.param == "roomy":
+            c["table"] = torch.nn.functional.pad(c["table"], (0, 32768 // c["page"]), value=-(2 ** 30))
+        return c
+
+    return apply
+
+
 DECODE = [
     # lens, hq, hkv, dim, page, dtype
     ([1], 1, 1, 128, 16, BF),
@@ -84,8 +97,8 @@ DECODE = [
 
 
 @pytest.mark.parametrize("lens,hq,hkv,dim,page,dtype", DECODE)
-def test_one_token_per_sequence(lens, hq, hkv, dim, page, dtype):
-    c = pc.batch(lens, None, hq, hkv, dim, page, dtype, seed=hq + dim + len(lens))
+def test_one_token_per_sequence(lens, hq, hkv, dim, page, dtype, table_room):
+    c = table_room(pc.batch(lens, None, hq, hkv, dim, page, dtype, seed=hq + dim + len(lens)))
     compare(c, *run(c))
 
 
@@ -105,17 +118,17 @@ RAGGED = [
 
 @pytest.mark.parametrize("lens,new,hq,hkv,dim,page,dtype", RAGGED)
 @pytest.mark.parametrize("causal", [True, False])
-def test_ragged_rows(lens, new, hq, hkv, dim, page, dtype, causal):
-    c = pc.batch(lens, new, hq, hkv, dim, page, dtype, seed=hq + dim + sum(new), spare_rows=3)
+def test_ragged_rows(lens, new, hq, hkv, dim, page, dtype, causal, table_room):
+    c = table_room(pc.batch(lens, new, hq, hkv, dim, page, dtype, seed=hq + dim + sum(new), spare_rows=3))
     compare(c, *run(c, causal=causal), causal=causal)
 
 
 @pytest.mark.parametrize("max_q", [1, 3, 16, 1000])
-def test_the_hint_changes_no_value(max_q):
+def test_the_hint_changes_no_value(max_q, table_room):
     """max_q picks the kernel; a wrong one is still answered right."""
-    c = pc.batch([150, 300, 40], [40, 1, 17], 8, 4, 128, 32, BF, seed=3)
+    c = table_room(pc.batch([150, 300, 40], [40, 1, 17], 8, 4, 128, 32, BF, seed=3))
     compare(c, *run(c, max_q=max_q))
-    c = pc.batch([150, 300, 40], None, 8, 4, 64, 32, F16, seed=4)
+    c = table_room(pc.batch([150, 300, 40], None, 8, 4, 64, 32, F16, seed=4))
     compare(c, *run(c, max_q=max_q))
 
 
@@ -136,8 +149,9 @@ PREFIX = [
 
 
 @pytest.mark.parametrize("lens,new,prefix,hq,hkv,dim,page,dtype", PREFIX)
-def test_shared_prefix(lens, new, prefix, hq, hkv, dim, page, dtype):
-    c = pc.batch(lens, new, hq, hkv, dim, page, dtype, seed=len(lens) + prefix, prefix=prefix, spare_rows=0 if new is None else 2)
+def test_shared_prefix(lens, new, prefix, hq, hkv, dim, page, dtype, table_room):
+    c = table_room(pc.batch(lens, new, hq, hkv, dim, page, dtype, seed=len(lens) + prefix, prefix=prefix,
+                            spare_rows=0 if new is None else 2))
     out, lse = run(c)
     compare(c, out, lse)
     compare(c, *run(c, prefix=0))  # the same table without naming the prefix
@@ -145,16 +159,16 @@ def test_shared_prefix(lens, new, prefix, hq, hkv, dim, page, dtype):
 
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("new", [None, [40, 90]])
-def test_large_scores(dtype, new):
+def test_large_scores(dtype, new, table_room):
     """Scores of some thousands: one position takes all, nothing overflows."""
-    c = pc.batch([700, 260], new, 4, 2, 128, 64, dtype, seed=8, qscale=60.0)
+    c = table_room(pc.batch([700, 260], new, 4, 2, 128, 64, dtype, seed=8, qscale=60.0))
     compare(c, *run(c, scale=3.0), scale=3.0)
 
 
 @pytest.mark.parametrize("new", [None, [40, 90]])
-def test_rising_scores(new):
+def test_rising_scores(new, table_room):
     """Every position's score is above all before it: the running maximum moves at each step."""
-    c = pc.batch([900, 333], new, 2, 1, 64, 32, BF, seed=9)
+    c = table_room(pc.batch([900, 333], new, 2, 1, 64, 32, BF, seed=9))
     c["q"][:] = 1.0
     for b in range(2):
         for p in range(int(c["lens"][b])):
@@ -188,9 +202,9 @@ def test_strides(new, prefix):
 
 
 @pytest.mark.parametrize("new", [None, [3, 70]])
-def test_offsets_behind_two_gigabytes(new):
+def test_offsets_behind_two_gigabytes(new, table_room):
     """Pages more than 2^31 elements from the base."""
-    c = pc.batch([200, 131], new, 4, 2, 128, 64, BF, seed=2)
+    c = table_room(pc.batch([200, 131], new, 4, 2, 128, 64, BF, seed=2))
     pages, step = c["k"].shape[0], (1 << 31) // (c["k"].shape[0] - 1) // 8 * 8 + 64
     k, v = (torch.empty(pages * step, dtype=BF, device=DEV).as_strided((pages, 2, 64, 128), (step, 8192, 128, 1))
             for _ in range(2))
@@ -204,8 +218,8 @@ def test_offsets_behind_two_gigabytes(new):
 
 
 @pytest.mark.parametrize("new,prefix", [(None, 0), ([9, 150, 1], 0), (None, 128), ([9, 150, 1], 128)])
-def test_reruns_are_bit_identical(new, prefix):
-    c = pc.batch([900, 2000, 400], new, 16, 4, 128, 64, BF, seed=6, prefix=prefix)
+def test_reruns_are_bit_identical(new, prefix, table_room):
+    c = table_room(pc.batch([900, 2000, 400], new, 16, 4, 128, 64, BF, seed=6, prefix=prefix))
     first = run(c)
     for _ in range(3):
         again = run(c)
@@ -213,11 +227,11 @@ def test_reruns_are_bit_identical(new, prefix):
 
 
 @pytest.mark.parametrize("new,prefix", [(None, 0), ([4, 80], 0), (None, 64)])
-def test_captured_graphs(new, prefix):
+def test_captured_graphs(new, prefix, table_room):
     """Two graphs captured once, replayed at the same time on two streams with
     lengths, tables and rows changed in place after the capture."""
     P = _api()
-    cases = [pc.batch([300, 500], new, 8, 4, 128, 64, BF, seed=s, prefix=prefix) for s in (1, 2)]
+    cases = [table_room(pc.batch([300, 500], new, 8, 4, 128, 64, BF, seed=s, prefix=prefix)) for s in (1, 2)]
     devs, graphs, outs, streams = [], [], [], []
     for c in cases:
         d = pc.to({k: c[k] for k in ("q", "k", "v", "table", "lens")}, DEV)
@@ -259,11 +273,11 @@ def test_captured_graphs(new, prefix):
 
 
 @pytest.mark.parametrize("new", [None, [5, 70, 1]])
-def test_a_bad_page_is_flagged_and_harms_no_other_sequence(new):
+def test_a_bad_page_is_flagged_and_harms_no_other_sequence(new, table_room):
     from breeze_b200 import _lib
 
     for bad in (-1, 10 ** 9):
-        c = pc.batch([300, 200, 150], new, 4, 2, 128, 64, BF, seed=5)
+        c = table_room(pc.batch([300, 200, 150], new, 4, 2, 128, 64, BF, seed=5))
         whole = c["table"].clone()
         c["table"][1, 1] = bad
         out, lse = run(c)
@@ -284,6 +298,30 @@ def test_a_length_behind_the_table_is_flagged(new):
     c["lens"][1] = 10 ** 6
     run(c, causal=False)
     assert _status() == _lib.BQ_DEVERR_POSITION
+
+
+def test_a_mixed_batch_with_tiles_of_few_rows():
+    """Running streams of one token beside long new pieces, in the kernel for many
+    rows: most of a tile's warps have no row, and must stay in step with the
+    others over many units; repeated, since a step out of turn is a matter of time."""
+    new = [200, 1, 3, 1, 130, 2, 1, 1, 40, 1, 1, 5]
+    lens = [1500, 900, 2100, 1024, 700, 1300, 1700, 640, 2000, 129, 128, 1999]
+    c = pc.batch(lens, new, 16, 4, 128, 64, BF, seed=21)
+    first = run(c)
+    compare(c, *first)
+    for _ in range(20):
+        again = run(c)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_many_short_sequences():
+    """More tiles than CTAs, most of them whole in one; some empty; repeated."""
+    g = torch.Generator().manual_seed(1)
+    lens = torch.randint(0, 90, (300,), generator=g).tolist()
+    for new in (None, [min(n, 1 + i % 23) for i, n in enumerate(lens)]):
+        c = pc.batch(lens, new, 12, 6, 64, 16, F16, seed=22)
+        compare(c, *run(c))
+        compare(c, *run(c, max_q=100))
 
 
 # ------------------------------------------------------------------ append
