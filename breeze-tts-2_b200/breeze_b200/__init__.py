@@ -8,6 +8,7 @@ decode kernels, backed by hand-written CUDA kernels in libbreeze_b200.so
   breeze_b200.fp8_linear    Fp8Linear, quantize_module_fp8
   breeze_b200.int8_linear   Int8Linear, quantize_module_int8
   breeze_b200.fused.kernels FusedWeight, rms_gemv, rmsnorm, silu_mul
+  breeze_b200.fused.paged   paged_append, paged_attention, prefix_attention
 
 Put the ``breeze-tts-2_b200`` directory on sys.path to import it.
 """

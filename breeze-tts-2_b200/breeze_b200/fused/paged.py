@@ -163,7 +163,7 @@ def _workspace_bytes(desc: bytes, need, stream) -> int:  # noqa: ARG001 - _launc
     return _lib.load().bq_paged_attention_workspace_bytes(desc, need)
 
 
-def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, causal, max_q, out, lse):
+def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, causal, max_q, out, lse, extra=0):
     ldq = _row_stride(q, "q")
     rows, width = q.shape
     dev, dtype = q.get_device(), q.dtype
@@ -185,10 +185,10 @@ def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, 
             raise ValueError("lse must be fp32 (T, HQ) on q's device")
         lse_ptr, ldl = lse.data_ptr(), _row_stride(lse, "lse")
     max_q = 0 if max_q is None else max_q
-    flags = _lib.default_flags()
+    flags = _lib.default_flags() | extra
     desc = _pack_attn(*fields, rows, hq, prefix_len, max_q, dim ** -0.5 if scale is None else scale,
                       flags if causal else flags | _lib.PAGED_FULL, q.data_ptr(), ldq, out.data_ptr(), ldo, lse_ptr, ldl)
-    key = (dev, rows, hq, hkv, dim, fields[0], fields[3] * fields[5], prefix_len > 0, max_q, q_starts is None)
+    key = (dev, rows, hq, hkv, dim, fields[0], fields[3] * fields[5], prefix_len, max_q, q_starts is None, extra)
     need = _WORKSPACE.get(key)
     if need is None:
         if len(_WORKSPACE) >= 4096:
@@ -218,11 +218,14 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                      seq_lens: torch.Tensor, prefix_len: int, q_starts: torch.Tensor | None = None,
                      scale: float | None = None, causal: bool = True, max_q: int | None = None,
-                     out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
+                     out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                     always: bool = False) -> torch.Tensor:
     """paged_attention for a batch that shares its first ``prefix_len``
     positions (a multiple of the page size): the first prefix_len / page size
     entries of every table row name the same pages. They are read once for all
     rows together, through row 0 of the table, and joined with each sequence's
-    own positions (a few short sequences read them each); the value is
+    own positions, where that pays (a short prefix of few sequences is read by
+    each; ``always=True`` shares it all the same); the value is
     paged_attention's."""
-    return _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, causal, max_q, out, lse)
+    return _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, causal, max_q, out, lse,
+                      _lib.PAGED_SHARE if always else 0)

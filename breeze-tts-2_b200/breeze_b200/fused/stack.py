@@ -297,6 +297,9 @@ class DecodeStack:
 
     @property
     def launches(self) -> int:
+        """Kernel launches of one step; with a paged cache the most it can take (few
+        streams of a short cache join in the attention kernel itself, and a prefix
+        that does not pay gets no pass of its own)."""
         if self.chain is not None:
             return 1
         per_layer = 4

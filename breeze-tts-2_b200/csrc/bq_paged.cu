@@ -337,6 +337,12 @@ const void* join_kernel(bool prefix, bool many) {
 // 18.7 us. Uneven lengths cost a cluster its longest, hence the limit.
 constexpr int kClusterPositions = 512;
 
+// Bytes of repeated reads that a shared prefix must save for its second pass and
+// the join of every row to pay. Shared against not, 128 dims, prefix of 1024 / 4096
+// positions: 16 sequences of 8 heads (63 / 252 MB saved) 25 / 27 us against 20 / 42
+// us, 48 sequences of 2 heads (49 / 197 MB) 28 / 29 us against 18 / 35 us.
+constexpr int64_t kSharedBytes = 96ll << 20;
+
 // One pass over positions: its kernel and its CTAs.
 struct PagedPass {
     bool wide;
@@ -353,6 +359,7 @@ struct PagedPlan {
     PagedScratch at[2];
     int64_t tile_rows;  // rows of one own tile as far as is known
     int ranks;          // > 0: one cluster of so many CTAs per (sequence, kv head) instead
+    int prefix;         // shared positions that get a pass of their own
     size_t total;
 };
 
@@ -374,7 +381,8 @@ int plan_paged(const bq_paged_attn_desc* d, PagedPlan* pl) {
     *pl = PagedPlan{};
     const int64_t most = !d->kv.q_starts ? 1 : d->max_q > 0 ? d->max_q : (int64_t(d->T) + d->kv.B - 1) / d->kv.B;
     pl->tile_rows = most * G;
-    if (most * G <= kNarrowRows) {
+    const bool share = d->prefix_len > 0 && (d->flags & BQ_PAGED_SHARE);
+    if (most * G <= kNarrowRows && !share) {
         const int64_t pairs = int64_t(d->kv.B) * d->kv.HKV, room = int64_t(d->kv.max_pages) * d->kv.page_size;
         int ranks = kNarrowRanks;
         while (ranks > 1 && pairs * ranks > 2 * di->sm_count) ranks >>= 1;
@@ -383,6 +391,8 @@ int plan_paged(const bq_paged_attn_desc* d, PagedPlan* pl) {
             return BQ_OK;
         }
     }
+    const int64_t saved = int64_t(d->kv.B - 1) * d->prefix_len * d->kv.HKV * d->kv.D * 4;
+    pl->prefix = share || saved >= kSharedBytes ? d->prefix_len : 0;
     pl->pass[0] = paged_pass(most * G, d->kv.D, di->sm_count);
     pl->pass[1] = paged_pass(int64_t(d->T) * G, d->kv.D, di->sm_count);
     size_t at = 0;
@@ -391,13 +401,13 @@ int plan_paged(const bq_paged_attn_desc* d, PagedPlan* pl) {
         at += (bytes + 255) & ~size_t(255);
         return here;
     };
-    for (int i = 0; i < (d->prefix_len > 0 ? 2 : 1); ++i) {
+    for (int i = 0; i < (pl->prefix > 0 ? 2 : 1); ++i) {
         const size_t slots = size_t(2) * pl->pass[i].grid * pl->pass[i].rows, rows = size_t(d->T) * d->HQ;
         PagedScratch& s = pl->at[i];
         s.part_o = take(slots * d->kv.D * 4);
         s.part_ml = take(slots * 8);
         s.shared = take(size_t(pl->pass[i].grid) * sizeof(PagedShared));
-        if (d->prefix_len > 0) {
+        if (pl->prefix > 0) {
             s.row_o = take(rows * d->kv.D * 4);
             s.row_ml = take(rows * 8);
             s.row_at = take(rows * 8);
@@ -470,7 +480,7 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
     w.G = d->HQ / d->kv.HKV;
     w.by_G.set(uint32_t(w.G));
     w.causal = (d->flags & BQ_PAGED_FULL) ? 0 : 1;
-    w.prefix_len = d->prefix_len;
+    w.prefix_len = pl.prefix;
     w.scale_log2 = d->scale * 1.4426950408889634f;
     w.q = d->q;
     w.ldq = d->ldq;
@@ -481,7 +491,7 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
     if (pl.ranks) return paged_launch_cluster(w, d->kv.dtype, d->kv.D, pl.ranks, d->flags, stream);
     PagedJoin p;
     std::memset(&p, 0, sizeof(p));
-    const bool prefix = d->prefix_len > 0;
+    const bool prefix = pl.prefix > 0;
     for (int i = prefix ? 1 : 0; i >= 0; --i) {  // the prefix first
         const PagedScratch& s = pl.at[i];
         w.prefix_pass = i;

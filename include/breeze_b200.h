@@ -343,9 +343,10 @@ int32_t bq_paged_append(const bq_paged_append_desc* desc, void* stream);
  * given, is the natural logarithm of each row's sum of exponentials.
  * prefix_len > 0: the first prefix_len positions (a multiple of page_size) are
  * the same pages in every row of the table and are read once for the whole
- * batch, through row 0, where that pays (few short sequences read them each);
+ * batch, through row 0, where that pays (else each sequence reads them);
  * the value is the same. */
-#define BQ_PAGED_FULL 2u
+#define BQ_PAGED_FULL 2u  /* every new row sees all of its sequence */
+#define BQ_PAGED_SHARE 4u /* the prefix gets its one pass even where that does not pay (for comparisons) */
 
 typedef struct bq_paged_attn_desc {
     bq_paged_kv kv;
@@ -354,7 +355,7 @@ typedef struct bq_paged_attn_desc {
     int32_t max_q;             /* most new rows of one sequence as far as the caller knows (a hint that
                                   picks the kernel, not a limit); 0 = T / B rounded up */
     float scale;
-    uint32_t flags;            /* BQ_FLAG_PDL | BQ_PAGED_FULL */
+    uint32_t flags;            /* BQ_FLAG_PDL | BQ_PAGED_FULL | BQ_PAGED_SHARE */
     const void* q;             /* [T, ldq]: HQ * D elements a row */
     int64_t ldq;
     void* out;                 /* [T, ldo] */

@@ -52,7 +52,7 @@ def test_descriptors_have_the_headers_layout():
     for desc in (L.PagedAppendDesc, L.PagedAttnDesc):  # packed values and a filled Structure are the same bytes
         values = [i + 1 if t is not ctypes.c_float else 0.5 for i, (_, t) in enumerate(desc._fields_)]
         assert L.packer(desc)(*values) == bytes(desc(*values))
-    for name, value in (("BQ_PAGED_FULL", L.PAGED_FULL), ("BQ_DEVERR_PAGE", L.BQ_DEVERR_PAGE)):
+    for name, value in (("BQ_PAGED_FULL", L.PAGED_FULL), ("BQ_PAGED_SHARE", L.PAGED_SHARE), ("BQ_DEVERR_PAGE", L.BQ_DEVERR_PAGE)):
         assert int(re.search(rf"#define {name} (\d+)u", HEADER).group(1)) == value
 
 

@@ -34,7 +34,7 @@ def _clean_status():
     assert _status() == 0
 
 
-def run(c, causal=True, scale=None, prefix=None, out=None, lse=None, max_q=None):
+def run(c, causal=True, scale=None, prefix=None, out=None, lse=None, max_q=None, always=True):
     d = pc.to({k: c[k] for k in ("q", "k", "v", "table", "lens")}, DEV)
     starts = None if c["starts"] is None else c["starts"].to(DEV)
     prefix = c["prefix"] if prefix is None else prefix
@@ -44,7 +44,7 @@ def run(c, causal=True, scale=None, prefix=None, out=None, lse=None, max_q=None)
         out = torch.full((c["rows"], c["hq"] * c["dim"]), 3.0, device=DEV, dtype=c["dtype"])
     kw = dict(q_starts=starts, scale=scale, causal=causal, max_q=max_q, out=out, lse=lse)
     if prefix:
-        _api().prefix_attention(d["q"], d["k"], d["v"], d["table"], d["lens"], prefix, **kw)
+        _api().prefix_attention(d["q"], d["k"], d["v"], d["table"], d["lens"], prefix, always=always, **kw)
     else:
         _api().paged_attention(d["q"], d["k"], d["v"], d["table"], d["lens"], **kw)
     torch.cuda.synchronize()
@@ -154,7 +154,19 @@ def test_shared_prefix(lens, new, prefix, hq, hkv, dim, page, dtype, table_room)
                             spare_rows=0 if new is None else 2))
     out, lse = run(c)
     compare(c, out, lse)
+    compare(c, *run(c, always=False))  # where sharing does not pay
     compare(c, *run(c, prefix=0))  # the same table without naming the prefix
+
+
+def test_a_prefix_worth_sharing():
+    """51 repeated readings of 4096 positions saved: shared without being told to."""
+    lens = [4096 + 1 + 5 * i for i in range(52)]
+    c = pc.batch(lens, None, 4, 1, 128, 64, BF, seed=31, prefix=4096)
+    out, lse = run(c, always=False)
+    compare(c, out, lse)
+    told = run(c)
+    assert torch.equal(out, told[0]) and torch.equal(lse, told[1])
+    assert not torch.equal(lse, run(c, prefix=0)[1])  # another order of the same sums
 
 
 @pytest.mark.parametrize("dtype", [BF, F16])
@@ -195,7 +207,7 @@ def test_strides(new, prefix):
     starts = None if c["starts"] is None else c["starts"].to(DEV)
     args = (wide[:, 1024:2048], d[:, 0], d[:, 1], table[:, 2:-3], c["lens"].to(DEV))
     kw = dict(q_starts=starts, out=out[:, 64:], lse=lse[:, 16:24])
-    _api().prefix_attention(*args, prefix, **kw) if prefix else _api().paged_attention(*args, **kw)
+    _api().prefix_attention(*args, prefix, always=True, **kw) if prefix else _api().paged_attention(*args, **kw)
     torch.cuda.synchronize()
     assert (out[:, :64] == 3.0).all() and (lse[:, :16] == 7.0).all() and (lse[:, 24:] == 7.0).all()
     compare(c, out[:, 64:].cpu(), lse[:, 16:24].cpu())
@@ -242,7 +254,7 @@ def test_captured_graphs(new, prefix, table_room):
         def call():
             a = (d["q"], d["k"], d["v"], d["table"], d["lens"])
             kw = dict(q_starts=d["starts"], out=out, lse=lse)
-            P.prefix_attention(*a, prefix, **kw) if prefix else P.paged_attention(*a, **kw)
+            P.prefix_attention(*a, prefix, always=True, **kw) if prefix else P.paged_attention(*a, **kw)
 
         call()
         torch.cuda.synchronize()
