@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "bq_device.cuh"
 
 namespace bq {
@@ -323,29 +325,33 @@ __device__ __forceinline__ int paged_row_limit(const PagedWork& p, const PagedSe
     return max(0, min(lim, p.prefix_len));
 }
 
-// Eight elements of a 16-byte vector <-> fp32.
+// What is infinite or NaN among two packed elements: 0xffff in its half.
+template <typename E>
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {
+    constexpr uint32_t exps = std::is_same_v<E, __half> ? 0x7C007C00u : 0x7F807F80u;
+    return __vcmpeq2(x & exps, exps);
+}
+
+// Two or eight elements <-> fp32.
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& r, float (&v)[8]);
-template <>
-__device__ __forceinline__ void unpack8<__nv_bfloat16>(const uint4& r, float (&v)[8]) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+    if constexpr (std::is_same_v<T, __half>) {
+        __half2 h;
+        memcpy(&h, &w, 4);
+        const float2 f = __half22float2(h);
+        lo = f.x;
+        hi = f.y;
+    } else {
+        lo = __uint_as_float(w << 16);
+        hi = __uint_as_float(w & 0xFFFF0000u);
     }
 }
-template <>
-__device__ __forceinline__ void unpack8<__half>(const uint4& r, float (&v)[8]) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        __half2 h;
-        memcpy(&h, &w[i], 4);
-        const float2 f = __half22float2(h);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& r, float (&v)[8]) {
+    unpack2<T>(r.x, v[0], v[1]);
+    unpack2<T>(r.y, v[2], v[3]);
+    unpack2<T>(r.z, v[4], v[5]);
+    unpack2<T>(r.w, v[6], v[7]);
 }
 
 template <typename T>

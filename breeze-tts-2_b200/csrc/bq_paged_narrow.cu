@@ -11,7 +11,10 @@
 // page. Rows of a page are stored 16-byte chunk ^ (row & 7), so that the
 // ldmatrix reads of eight rows fall on different banks. Positions behind the
 // share are zero-filled by the copy (0 bytes read): what lies behind a
-// sequence's last position, NaN or not, never enters a product.
+// sequence's last position, NaN or not, never enters a product. Where some rows
+// see a position and others do not, its probabilities are zero for the latter, but
+// zero times an infinite or NaN v is NaN: such entries are taken out of the product
+// and added to the rows that see them (narrow_nonfinite).
 //
 // Scores, statistics and outputs are fp32; the probabilities are rounded to the
 // element type for the second product (relative error of half a step of that
@@ -46,6 +49,9 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
                  : "r"(a)
                  : "memory");
 }
+__device__ __forceinline__ void lds128(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
 template <typename E>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
@@ -75,6 +81,46 @@ struct NarrowTile {
     PagedSeq s;
     int b, j, r0, nrows, p0, p1;
 };
+
+// Infinite and NaN entries of the v block at vb (positions pb .. pb + 15): added to
+// the outputs of the rows that see their position, then cleared. A warp calls it.
+template <typename E, int D>
+__device__ __forceinline__ void narrow_nonfinite(uint32_t vb, int pb, int lim0, int lim1, float (&o)[D / 8][4]) {
+    constexpr int CH = D / 8;
+    const int lane = threadIdx.x & 31;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 16 * CH / 32; ++i) {
+        uint32_t x[4];
+        lds128(x, vb + (lane + 32 * i) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= nonfinite2<E>(x[e]);
+    }
+    if (!__any_sync(0xffffffffu, bad)) return;
+#pragma unroll 1
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int n = 0; n < CH; ++n) {
+            uint32_t x;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(vb + r * (D * 2) + ((n ^ (r & 7)) << 4) + (lane & 3) * 4));
+            float a, b;
+            unpack2<E>(x & nonfinite2<E>(x), a, b);  // 0 for the finite ones
+            if (pb + r < lim0) o[n][0] += a, o[n][1] += b;
+            if (pb + r < lim1) o[n][2] += a, o[n][3] += b;
+        }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16 * CH / 32; ++i) {
+        uint32_t x[4];
+        lds128(x, vb + (lane + 32 * i) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] &= ~nonfinite2<E>(x[e]);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(vb + (lane + 32 * i) * 16), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+                     "r"(x[3])
+                     : "memory");
+    }
+    __syncwarp();
+}
 
 // One tile with the whole CTA: emit(r, d, m, l, o) receives dims d .. d + 3 of row r,
 // unnormalized, with the row's largest score (base 2) and sum of exponentials.
@@ -137,6 +183,7 @@ __device__ __forceinline__ void narrow_tile(const PagedWork& p, const NarrowTile
         ldsm4(qf[ks], sb + SM::kQ + r * (D * 2) + ((ch ^ (r & 7)) << 4));
     }
     const int lim0 = s_lim[g], lim1 = s_lim[g + 8];
+    const int seen = __reduce_min_sync(0xffffffffu, min(g < nrows ? lim0 : p1, g + 8 < nrows ? lim1 : p1));  // by every row
     float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
     for (int n = 0; n < D / 8; ++n)
@@ -197,6 +244,8 @@ __device__ __forceinline__ void narrow_tile(const PagedWork& p, const NarrowTile
                 l0 += sc[n][e];
                 l1 += sc[n][2 + e];
             }
+        const int blk = p0 + 16 * (warp + kNarrowWarps * st);
+        if (min(blk + 16, p1) > seen) narrow_nonfinite<E, D>(vb, blk, lim0, lim1, o);
         const uint32_t pf[4] = {pack2<E>(sc[0][0], sc[0][1]), pack2<E>(sc[0][2], sc[0][3]),
                                 pack2<E>(sc[1][0], sc[1][1]), pack2<E>(sc[1][2], sc[1][3])};
 #pragma unroll
@@ -286,10 +335,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
             const int rr = t.r0 + r, tok = p.by_G(rr), head = c.j * p.G + rr - tok * p.G;
             const int64_t row = t.s.begin + tok;
             if (whole && !p.row_o) {
-                const float inv = ll > 0.f ? 1.f / ll : 0.f;
+                const float inv = ll != 0.f ? 1.f / ll : 0.f;
                 *reinterpret_cast<uint2*>(static_cast<E*>(p.out) + row * p.ldo + head * D + d) =
                     pack4<E>(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-                if (p.lse && d == 0) p.lse[row * p.ldl + head] = ll > 0.f ? (mm + log2f(ll)) * kLn2 : -INFINITY;
+                if (p.lse && d == 0) p.lse[row * p.ldl + head] = ll != 0.f ? (mm + log2f(ll)) * kLn2 : -INFINITY;
             } else {
                 const int64_t at = whole ? row * kv.HQ + head : int64_t(slot) * ROWS + r;
                 *reinterpret_cast<float4*>((whole ? p.row_o : p.part_o) + at * D + d) = a;
@@ -364,10 +413,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_cluster_kernel(const __grid
             }
             const int rr = t.r0 + r, tok = p.by_G(rr), head = t.j * p.G + rr - tok * p.G;
             const int64_t row = t.s.begin + tok;
-            const float inv = ll > 0.f ? 1.f / ll : 0.f;
+            const float inv = ll != 0.f ? 1.f / ll : 0.f;
             *reinterpret_cast<uint2*>(static_cast<E*>(p.out) + row * p.ldo + head * D + d) =
                 pack4<E>(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-            if (p.lse && d == 0) p.lse[row * p.ldl + head] = ll > 0.f ? (mm + log2f(ll)) * kLn2 : -INFINITY;
+            if (p.lse && d == 0) p.lse[row * p.ldl + head] = ll != 0.f ? (mm + log2f(ll)) * kLn2 : -INFINITY;
         }
         cluster_sync_relaxed();  // rows are not written over, nor does a rank leave, while another reads them (the reads
                                  // were consumed by the stores)

@@ -34,6 +34,9 @@
 // Page slots behind the last position arrive with the last page, whatever they
 // hold; before the product that would multiply them by zero probabilities the
 // softmax warps of half 0 clear those rows of v. Scores there are never used.
+// Infinite and NaN entries of v at positions that only some rows of a tile see
+// are cleared likewise, and added in memory to the outputs of the rows that see
+// them (not in the prefix pass: there every sequence sees the same positions).
 #include <algorithm>
 #include <cstring>
 
@@ -286,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ WideTile s_tile[kTiles];
+    __shared__ volatile int s_bad[kTiles];  // n + 1: entries of v were cleared from tile n
     const uint32_t sraw = smem_u32(smem_raw), sb = (sraw + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (sb - sraw);
     const PagedWork& w = p.w;
@@ -314,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
         mbar_init(bar_done, 1);
         mbar_init(bar_done + 8, 1);
         for (int i = 0; i < kTiles; ++i) {
+            s_bad[i] = 0;
             mbar_init(bar_tile + 8 * i, 1);
             mbar_init(bar_free + 8 * i, 11);
         }
@@ -363,6 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             const int myrow = t.r0 + 128 * h + row, units = t.nu, p0 = t.p0, p1 = t.p1;
             const bool idle = (warp & 3) * 32 >= hrows;  // no row of this warp exists
             const int limit = row < hrows ? paged_row_limit(w, t.s, myrow) : 0;
+            const int seen = w.prefix_pass ? p1 : paged_row_limit(w, t.s, t.r0);  // by every row: limits ascend
             float mref = -INFINITY, l = 0.f;
             __syncwarp();  // tensor-memory instructions below are warp-wide
             for (int u = 0; u < units; ++u) {
@@ -380,9 +386,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_read);  // the score buffer may be written again
                 if (!idle && base + kUnit > limit) {
-                    const int n = limit - base;
+                    const int sees = limit - base;
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) s[i] = i < n ? s[i] : -INFINITY;
+                    for (int i = 0; i < 128; ++i) s[i] = i < sees ? s[i] : -INFINITY;
                 }
                 if (!idle && u == 0) {  // the tile's first reference
                     float mx[4] = {s[0], s[1], s[2], s[3]};
@@ -452,15 +458,26 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     }
                 }
                 if (!ok) break;
-                if (h == 0 && base + kUnit > p1) {  // rows of v that no position owns
+                if (h == 0 && base + kUnit > min(p1, seen)) {  // rows of v that no position owns, or not every row sees
                     const int ring = t.ring + 2 * u + 1, st = ring % ST, from = max(0, p1 - base);
                     ok = __all_sync(0xffffffffu, tc_wait(bar_full + 8 * st, (ring / ST) & 1, abort, lim, kv.errors));
                     if (!ok) break;
-                    const uint4 z = make_uint4(0, 0, 0, 0);
-                    for (int idx = row; idx < (128 - from) * CH; idx += 128) {
-                        const int r = from + idx / CH, ch = idx % CH;
-                        *reinterpret_cast<uint4*>(smem + SM::kRing + st * SM::kTile + (ch >> 3) * (128 * 128) + r * 128 +
-                                                  ((ch & 7) << 4)) = z;
+                    const int some = max(0, min(from, seen - base));
+#pragma unroll 1
+                    for (int idx = row; idx < (128 - some) * CH; idx += 128) {
+                        const int r = some + idx / CH, ch = idx % CH;
+                        uint4* at = reinterpret_cast<uint4*>(smem + SM::kRing + st * SM::kTile + (ch >> 3) * (128 * 128) + r * 128 +
+                                                             ((ch & 7) << 4));
+                        if (r >= from) {
+                            *at = make_uint4(0, 0, 0, 0);
+                        } else {
+                            const uint4 x = *at;
+                            const uint4 bad = make_uint4(nonfinite2<E>(x.x), nonfinite2<E>(x.y), nonfinite2<E>(x.z), nonfinite2<E>(x.w));
+                            if (bad.x | bad.y | bad.z | bad.w) {
+                                *at = make_uint4(x.x & ~bad.x, x.y & ~bad.y, x.z & ~bad.z, x.w & ~bad.w);
+                                s_bad[n % kTiles] = n + 1;
+                            }
+                        }
                     }
                     fence_async_smem();
                     __syncwarp();
@@ -480,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 const int64_t orow = t.s.begin + tok;
                 const int64_t at = whole ? orow * kv.HQ + head
                                          : int64_t(2 * blockIdx.x + (t.k0 == 0 ? 1 : 0)) * kRows + 128 * h + row;
-                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
                 for (int q = 0; q < D / 32; ++q) {
                     float o[32];
@@ -505,7 +522,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                         if (w.row_at && t.k0 == 0)
                             w.row_at[orow * kv.HQ + head] = paged_row_at(blockIdx.x, t.parts, 128 * h + row);
                     } else if (w.lse) {
-                        w.lse[orow * w.ldl + head] = l > 0.f ? (mref + log2f(l)) * kLn2 : -INFINITY;
+                        w.lse[orow * w.ldl + head] = l != 0.f ? (mref + log2f(l)) * kLn2 : -INFINITY;
+                    }
+                }
+            }
+            if (s_bad[n % kTiles] == n + 1 && row < hrows) {
+                const int tok = w.by_G(myrow), head = t.j * w.G + myrow - tok * w.G;
+                const int64_t orow = t.s.begin + tok;
+                const bool final = t.whole && !w.row_o;
+                const int64_t at = t.whole ? orow * kv.HQ + head
+                                           : int64_t(2 * blockIdx.x + (t.k0 == 0 ? 1 : 0)) * kRows + 128 * h + row;
+                bool page_ok = true;
+#pragma unroll 1
+                for (int pos = max(p0, seen); pos < min(p1, limit); ++pos) {
+                    const E* v = static_cast<const E*>(kv.v) + paged_page(kv, t.b, pos, page_ok) * kv.vs_page + t.j * kv.vs_head +
+                                 int64_t(pos & kv.page_mask) * kv.vs_slot;
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 2) {
+                        const uint32_t x = *reinterpret_cast<const uint32_t*>(v + d);
+                        float a, b;
+                        unpack2<E>(x & nonfinite2<E>(x), a, b);
+                        if (final) {
+                            uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<E*>(w.out) + orow * w.ldo + head * D + d);
+                            float oa, ob;
+                            unpack2<E>(*o, oa, ob);
+                            *o = pack2<E>(oa + a, ob + b);
+                        } else {
+                            float* o = (t.whole ? w.row_o : w.part_o) + at * D + d;
+                            o[0] += a;
+                            o[1] += b;
+                        }
                     }
                 }
             }

@@ -188,6 +188,55 @@ def test_rising_scores(new, table_room):
     compare(c, *run(c))
 
 
+@pytest.mark.parametrize("lens,new,hq,hkv,dim,page,dtype", [
+    ([90, 700, 33], [3, 2, 3], 10, 2, 128, 32, BF),      # a few drafted tokens
+    ([2600, 41], [16, 16], 3, 3, 64, 16, F16),
+    ([400, 131], [150, 131], 4, 2, 128, 64, BF),         # prompts
+    ([700, 300], [260, 41], 5, 1, 64, 16, F16),
+    ([3900], [600], 2, 1, 128, 128, F16),                # shared by many CTAs
+])
+def test_what_a_row_does_not_see_may_be_infinite_or_nan(lens, new, hq, hkv, dim, page, dtype, table_room):
+    """Keys and values of later tokens reach no earlier row, whatever they hold; the rows that see them show it."""
+    c = table_room(pc.batch(lens, new, hq, hkv, dim, page, dtype, seed=41))
+    clean = dict(c, k=c["k"].clone(), v=c["v"].clone())
+    table, ls, starts = pc.lists(c)
+    kinds = [float("inf"), float("-inf"), float("nan")]
+    for b, (n, m) in enumerate(zip(lens, new)):
+        for i, back in enumerate(sorted({1, 2, m // 2, m - 1} & set(range(1, m)))):  # `back` - 1 rows later than the last
+            pos = n - back
+            where = (table[b][pos // page], i % hkv, pos % page)
+            c["v"][where][(7 * i) % dim] = kinds[i % 3]
+            c["v"][where][dim - 1 - i] = kinds[(i + 1) % 3]
+            clean["v"][where][(7 * i) % dim] = clean["v"][where][dim - 1 - i] = 0.0
+        last = (table[b][(n - 1) // page], 0, (n - 1) % page)
+        c["k"][last][3] = kinds[b % 3]
+        clean["k"][last][3] = 0.0
+    ref, fine = (op.attention(x["q"], x["k"], x["v"], table, ls, starts) for x in (c, clean))
+    tol, ltol = op.attention_bounds(fine, dim, dtype)
+    out, lse = run(c)
+    o = out.double().reshape(c["rows"], hq, dim)
+    sees_k = torch.zeros(c["rows"], hq, dtype=torch.bool)  # an unusual key: the sequences' last rows, kv head 0
+    sees_k[[s - 1 for s in starts[1:]], :hq // hkv] = True
+    odd = ~torch.isfinite(ref["out"]) & ~sees_k[..., None]
+    assert odd.any() and torch.equal(torch.isnan(o)[odd], torch.isnan(ref["out"])[odd])
+    inf = odd & torch.isinf(ref["out"])
+    assert torch.equal(o[inf], ref["out"][inf])
+    good = torch.isfinite(ref["out"]) & ~sees_k[..., None]
+    assert ((o - ref["out"]).abs() <= tol)[good].all()
+    assert ((lse.double() - ref["lse"]).abs() <= ltol)[~sees_k].all()
+
+
+@pytest.mark.parametrize("new", [None, [40, 30]])
+def test_a_nan_query_stays_in_its_row(new, table_room):
+    c = table_room(pc.batch([300, 90], new, 4, 2, 128, 32, BF, seed=43))
+    c["q"][1, 130] = float("nan")  # head 1 of row 1
+    out, lse = run(c)
+    odd = torch.zeros_like(lse, dtype=torch.bool)
+    odd[1, 1] = True
+    assert torch.equal(torch.isnan(lse), odd)
+    assert torch.equal(torch.isnan(out.reshape(c["rows"], 4, 128)), odd[..., None].expand(-1, -1, 128))
+
+
 @pytest.mark.parametrize("new", [None, [21, 64]])
 @pytest.mark.parametrize("prefix", [0, 64])
 def test_strides(new, prefix):
