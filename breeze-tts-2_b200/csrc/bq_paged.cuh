@@ -158,8 +158,8 @@ __device__ __forceinline__ int paged_tile_units(const PagedWork& p, const PagedS
 
 // Cost of the tiles of one kv head, in units.
 template <int ROWS, int UNIT, int OVERHEAD>
-__device__ __forceinline__ int paged_head_cost(const PagedWork& p, const PagedSeq& s, int tiles) {
-    int n = tiles * OVERHEAD;
+__device__ __forceinline__ long long paged_head_cost(const PagedWork& p, const PagedSeq& s, int tiles) {
+    long long n = (long long)tiles * OVERHEAD;
     for (int i = 0; i < tiles; ++i) n += paged_tile_units<ROWS, UNIT>(p, s, i);
     return n;
 }
@@ -228,7 +228,7 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
         bool cut;
         const PagedSeq s = paged_seq(p, b, cut);
         if (cut && cta == 0) atomicOr(p.kv.errors, BQ_DEVERR_POSITION_BIT);
-        mine += (long long)paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
+        mine += paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
     }
     long long incl = mine;
 #pragma unroll
@@ -254,8 +254,7 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
         for (int b = b0; b < b1; ++b) {
             bool cut;
             const PagedSeq s = paged_seq(p, b, cut);
-            const long long n =
-                (long long)paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
+            const long long n = paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
             if (c.u >= at && c.u < at + n) {
                 s_b = b;
                 s_rem = c.u - at;
@@ -273,16 +272,16 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
     bool cut;
     const PagedSeq s = paged_seq(p, c.b, cut);
     c.tiles = (s.rows + ROWS - 1) / ROWS;
-    const int head = paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, c.tiles);
+    const long long head = paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, c.tiles);
     const long long rem = s_rem;
     c.j = (rem >> 32) ? int(rem / head) : int(uint32_t(rem) / uint32_t(head));
-    int left = int(rem - (long long)c.j * head);
+    long long left = rem - c.j * head;
     for (;; ++c.i) {
         const int n = paged_tile_units<ROWS, UNIT>(p, s, c.i) + OVERHEAD;
         if (left < n) break;
         left -= n;
     }
-    c.k = left;
+    c.k = int(left);
     return c;
 }
 
