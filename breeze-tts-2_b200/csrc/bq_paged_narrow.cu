@@ -19,6 +19,15 @@
 // Scores, statistics and outputs are fp32; the probabilities are rounded to the
 // element type for the second product (relative error of half a step of that
 // type each, as the values they weight).
+//
+// Measured, join included (B200, copies run at 6554 GB/s): 8 sequences of 24 to 32
+// thousand positions, 8 kv heads of 128, 881 MB in 158 us (5.6 TB/s); 48 of 17 to
+// 6000, 184 MB in 42 us (4.4 TB/s), where finding the shares (2 us), each tile's
+// start and end and the join (5 us) show. The shares are equal, the SMs' speeds are
+// not: on average an SM is done after 85 % of the time. Two, four and eight times
+// as many smaller shares, dealt out as CTAs end, cost more in starts than they
+// gain (158, 160, 174 us); fetching the next tile's first 128 positions into L2
+// meanwhile changes nothing (42 / 43 us).
 #include "bq_host.h"
 #include "bq_paged.cuh"
 #include "bq_paged_host.h"
@@ -356,7 +365,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
 // Few (sequence, kv head) pairs and a short cache: a cluster of CTAs per pair takes
 // equal pieces of its positions and joins them through distributed shared memory
 // (rank order, deterministic). No schedule to work out, no partials in memory and
-// no second kernel. A shared prefix is read by each pair, mostly from L2.
+// no second kernel. A shared prefix is read by each pair, mostly from L2. Bound:
+// latency (length, page, keys, cluster barrier, output). Two sequences of 16 heads
+// of 128, 300 to 700 positions: 6.8 us (equal shares and join: 10.6 us); four that
+// share 512 of 520 to 800 positions: 8.2 us (two passes and join: 16.7 us).
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads, 2) paged_cluster_kernel(const __grid_constant__ PagedWork p, int ranks) {
     using SM = NarrowSmem<D>;

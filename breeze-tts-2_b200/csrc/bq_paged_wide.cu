@@ -15,11 +15,12 @@
 //   warps 0-3, 4-7  softmax of half 0 / 1, one row per thread: the row's 128
 //                   scores from tensor memory, running maximum and sum, the
 //                   probabilities back to tensor memory in 16 bits (the A
-//                   operand of the second product). The output accumulator stays in tensor memory; a
-//                   row's reference maximum may lag behind the true one by up
-//                   to a factor 2^8 (probabilities up to 256 are exact enough
-//                   in either type, and the factor cancels), so the accumulator
-//                   is rescaled only when a maximum really moves.
+//                   operand of the second product). The output accumulator
+//                   stays in tensor memory; a row's reference maximum may lag
+//                   behind the true one by up to a factor 2^8 (probabilities up
+//                   to 256 are exact enough in either type, and the factor
+//                   cancels), so the accumulator is rescaled only when a maximum
+//                   really moves.
 //   warp 8          k and v by tiled TMA, one box per page (or 128 positions of
 //                   one) and 64 dims, into a ring of 32 KB stages
 //   warps 9, 10     issue the products, each its own: S = Q K^T (both operands in
@@ -37,6 +38,15 @@
 // Infinite and NaN entries of v at positions that only some rows of a tile see
 // are cleared likewise, and added in memory to the outputs of the rows that see
 // them (not in the prefix pass: there every sequence sees the same positions).
+//
+// Measured, join included (B200): 7000 new positions of 16 query and 8 kv heads of
+// 128, causal, 201 GFLOP in 217 us (0.92 PFLOP/s; library products of 8192^3 run at
+// 1.65); 1474 ragged ones of 32 heads over 18 thousand in 113 us. The tensor cores
+// and the exponential units are each busy half of the time; without the softmax's
+// arithmetic the same pipeline takes 163 us, and a change of tile 7700 cycles.
+// Dropped: units of 64 positions with a score buffer per half (271 against then 238
+// us), two threads per row (291), outputs staged through shared memory (245 against
+// 237), a peeled unit loop (266).
 #include <algorithm>
 #include <cstring>
 
