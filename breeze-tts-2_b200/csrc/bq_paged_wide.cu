@@ -40,13 +40,15 @@
 // them (not in the prefix pass: there every sequence sees the same positions).
 //
 // Measured, join included (B200): 7000 new positions of 16 query and 8 kv heads of
-// 128, causal, 201 GFLOP in 217 us (0.92 PFLOP/s; library products of 8192^3 run at
+// 128, causal, 201 GFLOP in 210 us (0.96 PFLOP/s; library products of 8192^3 run at
 // 1.65); 1474 ragged ones of 32 heads over 18 thousand in 113 us. The tensor cores
 // and the exponential units are each busy half of the time; without the softmax's
 // arithmetic the same pipeline takes 163 us, and a change of tile 7700 cycles.
 // Dropped: units of 64 positions with a score buffer per half (271 against then 238
 // us), two threads per row (291), outputs staged through shared memory (245 against
-// 237), a peeled unit loop (266).
+// 237), a peeled unit loop (266), every fourth, third or eighth pair of exponentials
+// as a polynomial (211, 218 and 207 against 210): what the softmax warps wait for is
+// mostly not the exponential units but their own chains of instructions.
 #include <algorithm>
 #include <cstring>
 
@@ -419,9 +421,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     const uint64_t sc2 = f2(w.scale_log2, w.scale_log2), off2 = f2(off, off);
                     uint64_t sum[2] = {0, 0};
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    // The first kHeld quarters wait in registers for the product before, which still reads its probabilities.
+                    constexpr int kHeld = 2;
+                    uint32_t held[kHeld][16], now[16];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        uint32_t pk[16];
+                        uint32_t(&pk)[16] = q < kHeld ? held[q < kHeld ? q : 0] : now;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const float x = s[32 * q + 2 * i], y = s[32 * q + 2 * i + 1];
@@ -433,13 +438,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                             sum[i & 1] = add2(sum[i & 1], f2(a, b));
                             pk[i] = pack2<E>(a, b);
                         }
-                        if (q == 0 && first) {  // the product before has read its probabilities and written its outputs
+                        if (q == kHeld - 1 && first) {  // it has read its probabilities and written its outputs
                             ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
                             if (!ok) break;
                             tc_fence_after();
                             first = false;
                         }
-                        tmem_st16(t_p + 16 * q, pk);
+                        if (q == kHeld - 1) {
+#pragma unroll
+                            for (int e = 0; e < kHeld; ++e) tmem_st16(t_p + 16 * e, held[e]);
+                        } else if (q >= kHeld) {
+                            tmem_st16(t_p + 16 * q, now);
+                        }
                     }
                     if (!ok) break;
                     const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * w.scale_log2;
