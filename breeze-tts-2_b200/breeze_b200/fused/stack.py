@@ -13,9 +13,10 @@ reference keeps its output heads in fp32, cudagraph/backbone_graph.py:70).
 ``attn`` is the attention output: with ``attention=True`` each layer runs the
 decode attention step (bq_attention_step: q/k RMSNorm, RoPE, KV-cache write,
 flash-decode over the cache) between QKV and O, as FusedDecoderLayer does
-(layer.py:89-90); with ``page_size`` the rows are streams of their own length over
-a paged cache (breeze_b200.fused.paged: append, then attention); otherwise the first ``attn_cols`` columns of ``qkv`` (the
-query block) stand in for it, which keeps the QKV -> O data dependency.
+(layer.py:89-90); with ``page_size`` the rows are streams of their own length
+over a paged cache (breeze_b200.fused.paged: append, then attention); otherwise
+the first ``attn_cols`` columns of ``qkv`` (the query block) stand in for it,
+which keeps the QKV -> O data dependency.
 
 Every projection is one bq_gemv launch (int4 tinygemm / plain, fp8 or int8
 weight-only, bf16), launched with programmatic dependent launch so each
@@ -339,8 +340,9 @@ class DecodeStack:
 
     def run(self) -> torch.Tensor:
         """Enqueue the step: one bq_gemv launch per projection (and one
-        bq_attention_step, or the paged operators, per layer with ``attention=True``), or the whole
-        step as one decode-chain launch (``chain=True``)."""
+        bq_attention_step, or the paged operators, per layer with
+        ``attention=True``), or the whole step as one decode-chain launch
+        (``chain=True``)."""
         if self.chain is not None:
             self.chain.launch()
             return self.logits

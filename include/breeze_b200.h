@@ -288,8 +288,9 @@ int32_t bq_attention_o_step(const bq_attn_o_desc* desc, void* workspace, size_t 
  *     BQ_DEVERR_PAGE; the append skips the token, the attention reads page 0,
  *     so the outputs of that sequence mean nothing. Entries that no position
  *     needs may hold anything.
- * Slots that hold no position may hold anything, NaN included; the positions'
- * own k and v must be finite. */
+ * Slots that hold no position may hold anything, NaN included, and infinite or
+ * NaN keys and values reach only the rows that see their position (of a shared
+ * prefix that gets its own pass: all rows whose sequence ends in it, too). */
 typedef struct bq_paged_kv {
     int32_t B;             /* sequences, >= 1 */
     int32_t HKV, D;        /* kv heads, head dim (64 or 128) */
