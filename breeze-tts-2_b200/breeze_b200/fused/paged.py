@@ -48,7 +48,26 @@ _UNIT = (1,)  # stride of a contiguous vector
 _CACHE_DT = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 _pack_append = _lib.packer(_lib.PagedAppendDesc)
 _pack_attn = _lib.packer(_lib.PagedAttnDesc)
-_WORKSPACE: dict = {}  # bytes by shape; a decode loop asks once
+_bound = None
+
+
+def _native():
+    """The compiled calls (csrc/bind_paged.cpp), bound to the loaded library:
+    plain calls in a few microseconds of host time. They answer None where
+    something is to be refused or is out of the ordinary (another device is
+    current): then the functions below check, raise or launch."""
+    global _bound
+    if _bound is None:
+        lib = _lib.load()
+        try:
+            from .. import _paged_bind
+        except ImportError as e:
+            raise RuntimeError(f"breeze_b200/_paged_bind.so does not load ({e}): build it with "
+                               "`python breeze-tts-2_b200/build.py`") from e
+        _paged_bind.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.bq_paged_append, lib.bq_paged_attention, lib.bq_paged_attention_workspace_bytes)))
+        _bound = _paged_bind
+    return _bound
 
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
@@ -123,6 +142,10 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_page
     takes them. The math is fp32 with one rounding at the end. ``out`` may be
     ``qkv[:, :HQ * D]`` itself. Tokens of an unused batch slot (seq_lens[b] less
     than its new tokens) are skipped where their position would be negative."""
+    done = (_bound or _native()).append(qkv, cos, sin, k_pages, v_pages, page_table, seq_lens, q_starts, q_norm_w, k_norm_w,
+                                        eps, out, _lib.default_flags())
+    if done is not None:
+        return done if done.__class__ is not int else _lib.check(done, "bq_paged_append")
     ldqkv = _row_stride(qkv, "qkv")
     rows, width = qkv.shape
     dev, dtype = qkv.get_device(), qkv.dtype
@@ -164,6 +187,13 @@ def _workspace_bytes(desc: bytes, need, stream) -> int:  # noqa: ARG001 - _launc
 
 
 def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, causal, max_q, out, lse, extra=0):
+    flags = _lib.default_flags() | extra
+    if not causal:
+        flags |= _lib.PAGED_FULL
+    done = (_bound or _native()).attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, max_q, out,
+                                           lse, flags)
+    if done is not None:
+        return done if done.__class__ is not int else _lib.check(done, "bq_paged_attention")
     ldq = _row_stride(q, "q")
     rows, width = q.shape
     dev, dtype = q.get_device(), q.dtype
@@ -185,17 +215,11 @@ def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, 
             raise ValueError("lse must be fp32 (T, HQ) on q's device")
         lse_ptr, ldl = lse.data_ptr(), _row_stride(lse, "lse")
     max_q = 0 if max_q is None else max_q
-    flags = _lib.default_flags() | extra
     desc = _pack_attn(*fields, rows, hq, prefix_len, max_q, dim ** -0.5 if scale is None else scale,
-                      flags if causal else flags | _lib.PAGED_FULL, q.data_ptr(), ldq, out.data_ptr(), ldo, lse_ptr, ldl)
-    key = (dev, rows, hq, hkv, dim, fields[0], fields[3] * fields[5], prefix_len, max_q, q_starts is None, extra)
-    need = _WORKSPACE.get(key)
-    if need is None:
-        if len(_WORKSPACE) >= 4096:
-            _WORKSPACE.clear()
-        size = ctypes.c_size_t(0)
-        _launch(dev, "bq_paged_attention_workspace_bytes", _workspace_bytes, desc, ctypes.byref(size))
-        need = _WORKSPACE[key] = size.value
+                      flags, q.data_ptr(), ldq, out.data_ptr(), ldo, lse_ptr, ldl)
+    size = ctypes.c_size_t(0)
+    _launch(dev, "bq_paged_attention_workspace_bytes", _workspace_bytes, desc, ctypes.byref(size))
+    need = size.value
     ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
     _launch(dev, "bq_paged_attention", _lib.load().bq_paged_attention, desc, ws.data_ptr() if need else None, need)
     return out

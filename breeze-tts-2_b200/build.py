@@ -3,20 +3,23 @@
     python breeze-tts-2_b200/build.py [--force] [--jobs N]
 
 Compiles every csrc/*.cu as relocatable device code (``WHOLE``: as a whole
-program) for
-``-gencode arch=compute_100a,code=sm_100a`` and links them, with the CUDA
-runtime linked statically, into breeze_b200/libbreeze_b200.so next to the
-Python package that loads it. Objects go to _build/ (git-ignored). The
-library depends on nothing from PyTorch.
+program) for ``-gencode arch=compute_100a,code=sm_100a`` and links them, with
+the CUDA runtime linked statically, into breeze_b200/libbreeze_b200.so next to
+the Python package that loads it. Objects go to _build/ (git-ignored). The
+library depends on nothing from PyTorch; breeze_b200/_paged_bind.so, the Python
+side of the paged operators (csrc/bind_paged.cpp, host code), is compiled
+against torch's headers.
 """
 
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -24,6 +27,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 OUT = HERE / "breeze_b200" / "libbreeze_b200.so"
+BIND_SRC, BIND_OUT = CSRC / "bind_paged.cpp", HERE / "breeze_b200" / "_paged_bind.so"
 BUILD = HERE / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -47,6 +51,20 @@ def _stale(obj: Path, src: Path) -> bool:
     return any(d.stat().st_mtime > obj.stat().st_mtime for d in deps)
 
 
+def build_bind() -> Path:
+    """The Python side of the paged operators, against the installed torch."""
+    torch = Path(importlib.util.find_spec("torch").origin).parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{torch / 'include'}", f"-I{torch / 'include/torch/csrc/api/include'}",
+           f"-I{cuda / 'include'}", f"-I{INCLUDE}", str(BIND_SRC), "-o", str(BIND_OUT), f"-L{torch / 'lib'}",
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{torch / 'lib'}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {BIND_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    return BIND_OUT
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
@@ -65,9 +83,12 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         return r.stderr
 
     with ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 1)) as ex:
+        bind = ex.submit(build_bind) if force or _stale(BIND_OUT, BIND_SRC) else None
         for log in ex.map(compile_one, todo):
             if verbose and log:
                 print(log)
+        if bind is not None:
+            bind.result()
     if todo or force or not OUT.exists():
         cmd = [nvcc(), *ARCH, "-shared", "-rdc=true", "-Xcompiler", "-fPIC", "-cudart", "static",
                *map(str, objs), "-o", str(OUT)]

@@ -139,6 +139,20 @@ def test_cpu_tensors_are_refused():
                            c["table"], c["lens"])
 
 
+def test_the_compiled_calls_leave_what_is_not_plain_to_python():
+    native = paged._native()
+    c = pc.batch([5, 9], None, 2, 1, 64, 16)
+    assert native.attention(c["q"], c["k"], c["v"], c["table"], c["lens"], 0, None, None, None, None, None, 0) is None  # no GPU
+    assert native.append(torch.zeros(2, 256, dtype=torch.bfloat16), torch.ones(9, 64), torch.zeros(9, 64), c["k"], c["v"],
+                         c["table"], c["lens"], None, None, None, 1e-6, None, 0) is None
+    assert native.attention() is None and native.attention(*[None] * 12) is None
+    assert native.append(c["q"]) is None and native.append(*["x"] * 13) is None
+    with pytest.raises(TypeError, match="three addresses"):
+        native.bind(1)
+    with pytest.raises(ValueError, match="address 0"):
+        native.bind(1, 0, 1)
+
+
 def test_oracle_agrees_with_the_dense_step():
     """A paged batch whose rows are all at one position is the static cache's step."""
     from oracle import attention as oa

@@ -541,6 +541,51 @@ def test_python_refusals():
             P.paged_append(**{**put, **change})
 
 
+class _Aside:
+    """Stands in for the compiled calls: leaves every call to Python."""
+
+    @staticmethod
+    def append(*args):
+        assert len(args) == 13
+
+    @staticmethod
+    def attention(*args):
+        assert len(args) == 12
+
+
+@pytest.mark.parametrize("new", [None, [3, 70]])
+def test_compiled_calls_and_python_do_the_same(new, monkeypatch):
+    P = _api()
+    c = pc.batch([600, 131], new, 4, 2, 64, 32, BF, seed=51, prefix=64)
+    cos, sin = (t.to(DEV) for t in rope(600, 64, BF))
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn(c["rows"], 8 * 64, generator=g).to(BF).to(DEV)
+    gain = torch.nn.Parameter((1 + 0.1 * torch.randn(64, generator=g)).to(BF).to(DEV))  # weights come as parameters
+
+    def calls():
+        d = pc.to(c, DEV)
+        where = (d["k"], d["v"], d["table"], d["lens"])
+        kw = dict(q_starts=d["starts"])
+        q = P.paged_append(qkv, cos, sin, *where, q_norm_w=gain, k_norm_w=gain, eps=1e-5, **kw)
+        inplace = torch.empty_like(q)
+        assert P.paged_append(qkv, cos, sin, *where, out=inplace, **kw) is inplace
+        lse = torch.empty(c["rows"], 4, device=DEV)
+        outs = [q, inplace, lse, d["k"], d["v"], P.paged_attention(q, *where, scale=0.2, causal=False, max_q=2, **kw),
+                P.paged_attention(q, *where, lse=lse, **kw), P.prefix_attention(q, *where, 64, always=True, **kw)]
+        out = torch.empty_like(q)
+        assert P.paged_attention(q, *where, out=out, **kw) is out
+        assert not q.requires_grad
+        torch.cuda.synchronize()
+        return outs + [out]
+
+    with monkeypatch.context() as m:
+        m.setattr(P, "_cache_fields", None)  # plain calls never reach Python's checks
+        fast = calls()
+    monkeypatch.setattr(P, "_bound", _Aside)
+    for a, b in zip(fast, calls(), strict=True):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num()) and a.dtype == b.dtype and a.stride() == b.stride()
+
+
 def test_no_rows():
     """A ragged call without new rows is answered without a launch."""
     P = _api()
