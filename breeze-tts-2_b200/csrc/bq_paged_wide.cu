@@ -48,7 +48,8 @@
 // us), two threads per row (291), outputs staged through shared memory (245 against
 // 237), a peeled unit loop (266), every fourth, third or eighth pair of exponentials
 // as a polynomial (211, 218 and 207 against 210): what the softmax warps wait for is
-// mostly not the exponential units but their own chains of instructions.
+// mostly not the exponential units but their own chains of instructions. A score
+// buffer per half, the probabilities through shared memory instead: 266.
 #include <algorithm>
 #include <cstring>
 
