@@ -214,21 +214,31 @@ struct PagedSegment {
     }
 };
 
-// All NT threads: finds the share of CTA `cta`.
+// All NT threads: finds the share of CTA `cta`. The thread whose sequences hold its
+// first unit finds the place with what it has read and tells the others (when every
+// thread read the sequence once more and divided for itself, 48 sequences of 17 to
+// 6000 positions took 42.1 us instead of 38.4, 8 of 24 to 32 thousand 158 instead of
+// 146).
 template <int ROWS, int UNIT, int OVERHEAD, int NT>
 __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, int grid) {
     __shared__ long long s_sum[NT / 32];
-    __shared__ long long s_rem;
-    __shared__ int s_b;
+    __shared__ int s_at[5];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int B = p.prefix_pass ? 1 : p.kv.B;
     const int per = (B + NT - 1) / NT, b0 = min(int(threadIdx.x) * per, B), b1 = min(b0 + per, B);
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) {
+    PagedSeq s;
+    int tiles = 0;
+    long long head = 0, mine = 0;
+    auto read = [&](int b) {
         bool cut;
-        const PagedSeq s = paged_seq(p, b, cut);
-        if (cut && cta == 0) atomicOr(p.kv.errors, BQ_DEVERR_POSITION_BIT);
-        mine += paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
+        s = paged_seq(p, b, cut);
+        tiles = (s.rows + ROWS - 1) / ROWS;
+        head = paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, tiles);
+        return cut;
+    };
+    for (int b = b0; b < b1; ++b) {
+        if (read(b) && cta == 0) atomicOr(p.kv.errors, BQ_DEVERR_POSITION_BIT);
+        mine += head * p.kv.HKV;
     }
     long long incl = mine;
 #pragma unroll
@@ -237,7 +247,7 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
         if (lane >= o) incl += v;
     }
     if (lane == 31) s_sum[warp] = incl;
-    if (threadIdx.x == 0) s_b = -1;
+    if (threadIdx.x == 0) s_at[0] = -1;
     __syncthreads();
     long long before = incl - mine, U = 0;
 #pragma unroll
@@ -249,39 +259,40 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
     c.share = PagedShare(U, grid);
     c.u = c.share.lo(cta);
     c.hi = c.share.lo(cta + 1);
-    if (mine > 0 && c.u < c.hi && c.u >= before && c.u < before + mine) {
-        long long at = before;
-        for (int b = b0; b < b1; ++b) {
-            bool cut;
-            const PagedSeq s = paged_seq(p, b, cut);
-            const long long n = paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, (s.rows + ROWS - 1) / ROWS) * p.kv.HKV;
-            if (c.u >= at && c.u < at + n) {
-                s_b = b;
-                s_rem = c.u - at;
+    if (c.u < c.hi && c.u >= before && c.u < before + mine) {
+        int b = b0;
+        if (per > 1)
+            for (;; ++b) {
+                read(b);
+                if (c.u < before + head * p.kv.HKV) break;
+                before += head * p.kv.HKV;
             }
-            at += n;
+        const long long rem = c.u - before;
+        const int j = (rem >> 32) || (head >> 32) ? int(rem / head) : int(uint32_t(rem) / uint32_t(head));
+        long long left = rem - j * head;
+        int i = 0;
+        for (;; ++i) {
+            const int n = paged_tile_units<ROWS, UNIT>(p, s, i) + OVERHEAD;
+            if (left < n) break;
+            left -= n;
         }
+        s_at[0] = b;
+        s_at[1] = j;
+        s_at[2] = i;
+        s_at[3] = int(left);
+        s_at[4] = tiles;
     }
     __syncthreads();
-    c.b = s_b;
-    c.i = c.j = c.k = c.tiles = 0;
+    c.b = s_at[0];
+    c.j = c.i = c.k = c.tiles = 0;
     if (c.b < 0) {
         c.hi = c.u;  // nothing for this CTA
         return c;
     }
-    bool cut;
-    const PagedSeq s = paged_seq(p, c.b, cut);
-    c.tiles = (s.rows + ROWS - 1) / ROWS;
-    const long long head = paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, c.tiles);
-    const long long rem = s_rem;
-    c.j = (rem >> 32) ? int(rem / head) : int(uint32_t(rem) / uint32_t(head));
-    long long left = rem - c.j * head;
-    for (;; ++c.i) {
-        const int n = paged_tile_units<ROWS, UNIT>(p, s, c.i) + OVERHEAD;
-        if (left < n) break;
-        left -= n;
-    }
-    c.k = int(left);
+    c.j = s_at[1];
+    c.i = s_at[2];
+    c.k = s_at[3];
+    c.tiles = s_at[4];
     return c;
 }
 
