@@ -181,11 +181,11 @@ __device__ __forceinline__ void load_lane(const float* src, float (&o)[DPL]) {
 // One output row (R = 1) or R neighbouring rows of a tile: WPR warps, each on every
 // WPR-th part, kParts parts of each row in flight. Every thread of the block calls
 // it. `place` gives row r's output row and head.
-constexpr int kFewParts = 8;
+constexpr int kFewParts = 8, kFewRows = 32;
 
-template <typename E, int D, int WPR, int R, typename Place>
+template <typename E, int D, int WPR, int R, int kParts, typename Place>
 __device__ __forceinline__ void join_rows(const PagedJoin& p, const RowParts (&part)[2], int rows, const Place& place) {
-    constexpr int DPL = D / 32, kParts = R > 1 ? 2 : 4;
+    constexpr int DPL = D / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WPR;
     JoinRow<DPL> row[R];
 #pragma unroll
@@ -248,9 +248,12 @@ __device__ __forceinline__ void join_rows(const PagedJoin& p, const RowParts (&p
 }
 
 // Joins the tiles that CTAs share: block (c, y) takes rows of the one that begins in
-// CTA c (tiles that one CTA held are finished already), R per warp, or, where the
-// tile is spread over more than kFewParts CTAs, one row at a time with all its
-// warps. Parts are added in CTA order within a warp, warps in order: deterministic.
+// CTA c (tiles that one CTA held are finished already), R per warp; where the tile
+// is spread over more than kFewParts CTAs, one per warp, or, with few rows, one at a
+// time with all its warps. Parts are added in CTA order within a warp, warps in
+// order: deterministic. (A prompt of 1655 positions, one kv head of 64: 24 us; 38 us
+// with a row per block there. One row per warp throughout costs a prompt of 7000
+// tokens 213 instead of 207 us, eight parts in flight 211.)
 // Bound: latency of two rounds of loads (a record, then the parts), or L2 for the
 // prompts' tiles.
 template <typename E, int D, int R>
@@ -259,10 +262,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __gri
     pdl_wait();
     const PagedShared sh = p.shared[blockIdx.x];
     if (sh.parts == 0) return;
-    const bool few = sh.parts <= kFewParts;
-    const int per = few ? kJoinWarps * R : 1;  // rows of a block at a time
+    const bool few = sh.parts <= kFewParts, each = few || sh.rows > kFewRows;
+    const int mine = few ? R : 1;                // rows of a warp, or of the block
+    const int per = each ? kJoinWarps * mine : 1;  // rows of a block at a time
     for (int r0 = blockIdx.y * per; r0 < sh.rows; r0 += gridDim.y * per) {
-        const int idx = few ? r0 + (threadIdx.x >> 5) * R : r0;
+        const int idx = each ? r0 + (threadIdx.x >> 5) * mine : r0;
         RowParts part[2];
         part[0].n = part[1].n = 0;
         if (idx < sh.rows) part[1] = shared_row(p.pass[0], blockIdx.x, sh.parts, idx);
@@ -272,9 +276,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __gri
             h = sh.j * p.G + rr - tok * p.G;
         };
         if (few)
-            join_rows<E, D, 1, R>(p, part, max(0, min(R, sh.rows - idx)), place);
+            join_rows<E, D, 1, R, R == 1 ? 4 : 2>(p, part, max(0, min(R, sh.rows - idx)), place);
+        else if (each)
+            join_rows<E, D, 1, 1, 4>(p, part, max(0, min(1, sh.rows - idx)), place);
         else
-            join_rows<E, D, kJoinWarps, 1>(p, part, 1, place);
+            join_rows<E, D, kJoinWarps, 1, 4>(p, part, 1, place);
     }
 }
 
@@ -313,7 +319,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_prefix_kernel(cons
                 }
             }
         }
-        join_rows<E, D, WPR, 1>(p, part, live ? 1 : 0, [&](int, int& tt, int& h) {
+        join_rows<E, D, WPR, 1, 4>(p, part, live ? 1 : 0, [&](int, int& tt, int& h) {
             tt = t;
             h = idx - t * p.HQ;
         });

@@ -40,8 +40,8 @@
 // them (not in the prefix pass: there every sequence sees the same positions).
 //
 // Measured, join included (B200): 7000 new positions of 16 query and 8 kv heads of
-// 128, causal, 201 GFLOP in 210 us (0.96 PFLOP/s; library products of 8192^3 run at
-// 1.65); 1474 ragged ones of 32 heads over 18 thousand in 113 us. The tensor cores
+// 128, causal, 201 GFLOP in 207 us (0.97 PFLOP/s; library products of 8192^3 run at
+// 1.65); 1474 ragged ones of 32 heads over 18 thousand in 112 us. The tensor cores
 // and the exponential units are each busy half of the time; without the softmax's
 // arithmetic the same pipeline takes 163 us, and a change of tile 7700 cycles.
 // Dropped: units of 64 positions with a score buffer per half (271 against then 238
