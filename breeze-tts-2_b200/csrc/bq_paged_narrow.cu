@@ -24,7 +24,7 @@
 // thousand positions, 8 kv heads of 128, 881 MB in 145 us (6.1 TB/s); 48 of 17 to
 // 6000, 184 MB in 38 us (4.8 TB/s), where finding the shares (2 us), each tile's
 // start and end and the join (5 us) show. The shares are equal, the SMs' speeds are
-// not: on average an SM is done after 85 % of the time. Two, four and eight times
+// not: on average an SM is done after 87 % of the time. Two, four and eight times
 // as many smaller shares, dealt out as CTAs end, cost more in starts than they
 // gain (158, 160, 174 us against then 156); fetching the next tile's first 128 positions into L2
 // meanwhile changes nothing (43 / 42 us).
