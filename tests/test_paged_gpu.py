@@ -385,6 +385,39 @@ def test_many_short_sequences():
         compare(c, *run(c, max_q=100))
 
 
+def test_more_sequences_than_threads():
+    """Every thread that looks for a share's place has two sequences or more, in both kernels."""
+    g = torch.Generator().manual_seed(2)
+    lens = torch.randint(0, 60, (900,), generator=g).tolist()
+    c = pc.batch(lens, [min(n, i % 4) for i, n in enumerate(lens)], 3, 1, 64, 16, BF, seed=23)
+    compare(c, *run(c, max_q=3))
+    compare(c, *run(c, max_q=100))
+
+
+@pytest.mark.parametrize("new", [None, [40, 7, 300]])
+def test_two_streams_at_once(new):
+    """Calls that overlap on two streams share nothing."""
+    P = _api()
+    batches = [pc.to(pc.batch([900, 1300, 500], new, 8, 4, 128, 64, BF, seed=s), DEV) for s in (61, 62)]
+
+    def call(c):
+        lse = torch.empty(c["rows"], 8, device=DEV)
+        return P.paged_attention(c["q"], c["k"], c["v"], c["table"], c["lens"], q_starts=c["starts"], lse=lse), lse
+
+    alone = [call(c) for c in batches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in batches]
+    got = [[], []]
+    for _ in range(20):
+        for c, st, to in zip(batches, streams, got):
+            with torch.cuda.stream(st):
+                to.append(call(c))
+    torch.cuda.synchronize()
+    for (out, lse), runs in zip(alone, got):
+        for o2, l2 in runs:
+            assert torch.equal(out, o2) and torch.equal(lse, l2)
+
+
 # ------------------------------------------------------------------ append
 def rope(positions, dim, dtype):
     ang = torch.arange(positions, dtype=torch.float64)[:, None] * 1e4 ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
