@@ -10,7 +10,7 @@ decode kernels, backed by hand-written CUDA kernels in libbreeze_b200.so
   breeze_b200.fused.kernels FusedWeight, rms_gemv, rmsnorm, silu_mul
   breeze_b200.fused.paged   paged_append, paged_attention, prefix_attention
 
-Put the ``breeze-tts-2_b200`` directory on sys.path to import it.
+Put the ``breeze-tts-2_b200`` directory, or the repository's root, on sys.path to import it.
 """
 
 __version__ = "0.1.0"
