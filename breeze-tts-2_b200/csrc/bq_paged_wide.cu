@@ -580,165 +580,168 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             tc_fence_before();  // ordered before the next tile's first product by its bar_p arrivals
             release(n);
         }
-    } else if (warp == 8) {
-        // ------------------------------------------------------------ k / v loads
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        int it = 0;
-        bool pages_ok = true;
-        for (int n = 0;; ++n) {
-            wait(bar_tile + 8 * (n % kTiles), n / kTiles);
-            if (!ok || !tile(n).valid) break;
-            const int units = tile(n).nu, p0 = tile(n).p0, p1 = tile(n).p1, seq = tile(n).b, j = tile(n).j;
-            release(n);
-            for (int u = 0; ok && u < units; ++u) {
-                const int base = p0 + u * kUnit;
-                const int nb = max(0, (min(kUnit, p1 - base) + p.box - 1) / p.box);  // boxes that hold positions
-                int page = 0;
-                if (lane < nb) page = paged_page(kv, seq, base + lane * p.box, pages_ok);
-                const int slot = (base + lane * p.box) & kv.page_mask;
-#pragma unroll
-                for (int x = 0; x < 2; ++x, ++it) {
-                    const int st = it % ST;
-                    const uint32_t bar = bar_full + 8 * st;
-                    if (it >= ST) wait(bar_empty + 8 * st, it / ST + 1);
-                    if (!ok) break;
-                    if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(nb * p.box) * (D * 2));
-                    __syncwarp();
-                    if (lane < nb) {
-                        const CUtensorMap* map = x ? &p.vmap : &p.kmap;
-                        const int ps = x ? p.v_slot : p.k_slot, ph = x ? p.v_head : p.k_head;
-                        const int c1 = ps == 1 ? slot : ph == 1 ? j : page, c2 = ps == 2 ? slot : ph == 2 ? j : page,
-                                  c3 = ps == 3 ? slot : ph == 3 ? j : page;
-                        const uint32_t dst = sb + SM::kRing + st * SM::kTile + uint32_t(lane * p.box) * 128u;
-#pragma unroll
-                        for (int half = 0; half < D / 64; ++half)
-                            tma_load_4d(dst + half * (128 * 128), map, half * 64, c1, c2, c3, bar);
-                    }
-                }
-            }
-        }
-        if (!pages_ok) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
-        // no tile may still be landing when the CTA leaves (an abort skips the products)
-        for (int i = max(0, it - ST); i < it; ++i) tc_wait(bar_full + 8 * (i % ST), (i / ST) & 1, nullptr, lim, kv.errors);
-        __syncwarp();
     } else {
-        // ------------------------------------------------------------ products
+        // One instruction for the whole warpgroup, under a condition that its warps share: executed from different
+        // places by its warps, it would be undefined.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        if (warp == 9) {
-            int tiles0 = 0, tiles1 = 0, scored = 0;  // tiles of each half, score tiles so far
+        if (warp == 8) {
+            // -------------------------------------------------------- k / v loads
+            int it = 0;
+            bool pages_ok = true;
             for (int n = 0;; ++n) {
                 wait(bar_tile + 8 * (n % kTiles), n / kTiles);
                 if (!ok || !tile(n).valid) break;
-                const int both = __shfl_sync(0xffffffffu, tile(n).nrows > 128 ? 1 : 0, 0);
-                const int nu = __shfl_sync(0xffffffffu, tile(n).nu, 0), it = __shfl_sync(0xffffffffu, tile(n).ring, 0);
+                const int units = tile(n).nu, p0 = tile(n).p0, p1 = tile(n).p1, seq = tile(n).b, j = tile(n).j;
                 release(n);
-                wait(bar_q, tiles0++);
-                if (ok && both) wait(bar_q + 8, tiles1++);
-                for (int u = 0; ok && u < nu; ++u) {
-                    const int ring = it + 2 * u, st = ring % ST;
-                    const uint32_t k_lo = ((sb + SM::kRing + st * SM::kTile) >> 4) | kDescLoK;
-                    wait(bar_full + 8 * st, ring / ST);
-                    for (int h = 0; ok && h <= both; ++h, ++scored) {
-                        if (scored > 0) wait(bar_read, scored - 1);
+                for (int u = 0; ok && u < units; ++u) {
+                    const int base = p0 + u * kUnit;
+                    const int nb = max(0, (min(kUnit, p1 - base) + p.box - 1) / p.box);  // boxes that hold positions
+                    int page = 0;
+                    if (lane < nb) page = paged_page(kv, seq, base + lane * p.box, pages_ok);
+                    const int slot = (base + lane * p.box) & kv.page_mask;
+    #pragma unroll
+                    for (int x = 0; x < 2; ++x, ++it) {
+                        const int st = it % ST;
+                        const uint32_t bar = bar_full + 8 * st;
+                        if (it >= ST) wait(bar_empty + 8 * st, it / ST + 1);
                         if (!ok) break;
-                        tc_fence_after();
-                        scores_product<D>(tm, ((sb + h * SM::kTile) >> 4) | kDescLoK, k_lo, p.idesc_qk, bar_s + 8 * h,
-                                          h == both ? bar_empty + 8 * st : 0u);
-                        if (u + 1 == nu && elect_one()) tc_commit(bar_used + 8 * h);
+                        if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(nb * p.box) * (D * 2));
                         __syncwarp();
+                        if (lane < nb) {
+                            const CUtensorMap* map = x ? &p.vmap : &p.kmap;
+                            const int ps = x ? p.v_slot : p.k_slot, ph = x ? p.v_head : p.k_head;
+                            const int c1 = ps == 1 ? slot : ph == 1 ? j : page, c2 = ps == 2 ? slot : ph == 2 ? j : page,
+                                      c3 = ps == 3 ? slot : ph == 3 ? j : page;
+                            const uint32_t dst = sb + SM::kRing + st * SM::kTile + uint32_t(lane * p.box) * 128u;
+    #pragma unroll
+                            for (int half = 0; half < D / 64; ++half)
+                                tma_load_4d(dst + half * (128 * 128), map, half * 64, c1, c2, c3, bar);
+                        }
                     }
                 }
-                if (!ok) break;
             }
-        } else if (warp == 10) {
-            int units0 = 0, units1 = 0;  // units of each half before the tile
-            for (int n = 0;; ++n) {
-                wait(bar_tile + 8 * (n % kTiles), n / kTiles);
-                if (!ok || !tile(n).valid) break;
-                const int both = __shfl_sync(0xffffffffu, tile(n).nrows > 128 ? 1 : 0, 0);
-                const int nu = __shfl_sync(0xffffffffu, tile(n).nu, 0), it = __shfl_sync(0xffffffffu, tile(n).ring, 0);
-                release(n);
-                for (int u = 0; ok && u < nu; ++u) {
-                    const int ring = it + 2 * u + 1, st = ring % ST;
-                    const uint32_t v_lo = ((sb + SM::kRing + st * SM::kTile) >> 4) | kDescLoV;
-                    wait(bar_full + 8 * st, ring / ST);
-                    for (int h = 0; ok && h <= both; ++h) {
-                        wait(bar_p + 8 * h, (h ? units1 : units0) + u);
-                        if (!ok) break;
-                        tc_fence_after();
-                        output_product(tm + 256 + 128 * h, tm + 128 + 64 * h, v_lo, p.idesc_pv, u > 0, bar_pv + 8 * h,
-                                       h == both ? bar_empty + 8 * st : 0u);
-                    }
-                }
-                if (!ok) break;
-                units0 += nu;
-                units1 += both ? nu : 0;
-            }
+            if (!pages_ok) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
+            // no tile may still be landing when the CTA leaves (an abort skips the products)
+            for (int i = max(0, it - ST); i < it; ++i) tc_wait(bar_full + 8 * (i % ST), (i / ST) & 1, nullptr, lim, kv.errors);
+            __syncwarp();
         } else {
-            // -------------------------------------------------------- tiles and queries
-            int used0 = 0, used1 = 0, ring = 0;  // tiles of each half, ring stages so far
-            bool shares = false;                 // the last tile goes on in the next CTA
-            const int sequences = w.prefix_pass ? 1 : kv.B;
-            for (int n = 0; ok; ++n) {
-                if (n >= kTiles) wait(bar_free + 8 * (n % kTiles), n / kTiles - 1);
-                if (!ok) break;
-                WideTile t;
-                t.valid = 0;
-                while (c.u < c.hi && c.b < sequences) {  // past tiles of which this share holds only overhead
-                    bool cut;
-                    t.s = paged_seq(w, c.b, cut);
-                    const PagedSegment<kRows, kUnit, kWideOverhead> g(w, t.s, c);
-                    if (g.nu > 0) {
-                        t.b = c.b;
-                        t.j = c.j;
-                        t.r0 = c.i * kRows;
-                        t.nrows = min(kRows, t.s.rows - t.r0);
-                        t.k0 = g.k0;
-                        t.nu = g.nu;
-                        t.p0 = (w.prefix_pass ? 0 : w.prefix_len) + g.k0 * kUnit;
-                        t.p1 = min(t.p0 + g.nu * kUnit, paged_tile_limit<kRows>(w, t.s, c.i));
-                        t.whole = g.whole();
-                        t.parts = g.parts(c, blockIdx.x);
-                        t.ring = ring;
-                        t.valid = 1;
-                        paged_next<kRows>(w, c, g.cost);
-                        break;
+            // -------------------------------------------------------- products
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            if (warp == 9) {
+                int tiles0 = 0, tiles1 = 0, scored = 0;  // tiles of each half, score tiles so far
+                for (int n = 0;; ++n) {
+                    wait(bar_tile + 8 * (n % kTiles), n / kTiles);
+                    if (!ok || !tile(n).valid) break;
+                    const int both = __shfl_sync(0xffffffffu, tile(n).nrows > 128 ? 1 : 0, 0);
+                    const int nu = __shfl_sync(0xffffffffu, tile(n).nu, 0), it = __shfl_sync(0xffffffffu, tile(n).ring, 0);
+                    release(n);
+                    wait(bar_q, tiles0++);
+                    if (ok && both) wait(bar_q + 8, tiles1++);
+                    for (int u = 0; ok && u < nu; ++u) {
+                        const int ring = it + 2 * u, st = ring % ST;
+                        const uint32_t k_lo = ((sb + SM::kRing + st * SM::kTile) >> 4) | kDescLoK;
+                        wait(bar_full + 8 * st, ring / ST);
+                        for (int h = 0; ok && h <= both; ++h, ++scored) {
+                            if (scored > 0) wait(bar_read, scored - 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            scores_product<D>(tm, ((sb + h * SM::kTile) >> 4) | kDescLoK, k_lo, p.idesc_qk, bar_s + 8 * h,
+                                              h == both ? bar_empty + 8 * st : 0u);
+                            if (u + 1 == nu && elect_one()) tc_commit(bar_used + 8 * h);
+                            __syncwarp();
+                        }
                     }
-                    paged_next<kRows>(w, c, g.cost);
-                }
-                if (lane == 0) {
-                    s_tile[n % kTiles] = t;
-                    mbar_arrive(bar_tile + 8 * (n % kTiles));
-                }
-                __syncwarp();
-                if (!t.valid) break;
-                ring += 2 * t.nu;
-                if (t.parts) {
-                    shares = true;
-                    if (lane == 0) w.shared[blockIdx.x] = PagedShared{t.parts, t.nrows, t.r0, t.s.begin, t.j};
-                }
-                for (int h = 0; ok && h <= (t.nrows > 128 ? 1 : 0); ++h) {
-                    int& used = h ? used1 : used0;
-                    if (used > 0) wait(bar_used + 8 * h, used - 1);  // the tile before it has been multiplied
                     if (!ok) break;
-                    wide_queries<E, D>(p, t, h, lane, sb + h * SM::kTile, bar_q + 8 * h);
-                    ++used;
                 }
+            } else if (warp == 10) {
+                int units0 = 0, units1 = 0;  // units of each half before the tile
+                for (int n = 0;; ++n) {
+                    wait(bar_tile + 8 * (n % kTiles), n / kTiles);
+                    if (!ok || !tile(n).valid) break;
+                    const int both = __shfl_sync(0xffffffffu, tile(n).nrows > 128 ? 1 : 0, 0);
+                    const int nu = __shfl_sync(0xffffffffu, tile(n).nu, 0), it = __shfl_sync(0xffffffffu, tile(n).ring, 0);
+                    release(n);
+                    for (int u = 0; ok && u < nu; ++u) {
+                        const int ring = it + 2 * u + 1, st = ring % ST;
+                        const uint32_t v_lo = ((sb + SM::kRing + st * SM::kTile) >> 4) | kDescLoV;
+                        wait(bar_full + 8 * st, ring / ST);
+                        for (int h = 0; ok && h <= both; ++h) {
+                            wait(bar_p + 8 * h, (h ? units1 : units0) + u);
+                            if (!ok) break;
+                            tc_fence_after();
+                            output_product(tm + 256 + 128 * h, tm + 128 + 64 * h, v_lo, p.idesc_pv, u > 0, bar_pv + 8 * h,
+                                           h == both ? bar_empty + 8 * st : 0u);
+                        }
+                    }
+                    if (!ok) break;
+                    units0 += nu;
+                    units1 += both ? nu : 0;
+                }
+            } else {
+                // -------------------------------------------------------- tiles and queries
+                int used0 = 0, used1 = 0, ring = 0;  // tiles of each half, ring stages so far
+                bool shares = false;                 // the last tile goes on in the next CTA
+                const int sequences = w.prefix_pass ? 1 : kv.B;
+                for (int n = 0; ok; ++n) {
+                    if (n >= kTiles) wait(bar_free + 8 * (n % kTiles), n / kTiles - 1);
+                    if (!ok) break;
+                    WideTile t;
+                    t.valid = 0;
+                    while (c.u < c.hi && c.b < sequences) {  // past tiles of which this share holds only overhead
+                        bool cut;
+                        t.s = paged_seq(w, c.b, cut);
+                        const PagedSegment<kRows, kUnit, kWideOverhead> g(w, t.s, c);
+                        if (g.nu > 0) {
+                            t.b = c.b;
+                            t.j = c.j;
+                            t.r0 = c.i * kRows;
+                            t.nrows = min(kRows, t.s.rows - t.r0);
+                            t.k0 = g.k0;
+                            t.nu = g.nu;
+                            t.p0 = (w.prefix_pass ? 0 : w.prefix_len) + g.k0 * kUnit;
+                            t.p1 = min(t.p0 + g.nu * kUnit, paged_tile_limit<kRows>(w, t.s, c.i));
+                            t.whole = g.whole();
+                            t.parts = g.parts(c, blockIdx.x);
+                            t.ring = ring;
+                            t.valid = 1;
+                            paged_next<kRows>(w, c, g.cost);
+                            break;
+                        }
+                        paged_next<kRows>(w, c, g.cost);
+                    }
+                    if (lane == 0) {
+                        s_tile[n % kTiles] = t;
+                        mbar_arrive(bar_tile + 8 * (n % kTiles));
+                    }
+                    __syncwarp();
+                    if (!t.valid) break;
+                    ring += 2 * t.nu;
+                    if (t.parts) {
+                        shares = true;
+                        if (lane == 0) w.shared[blockIdx.x] = PagedShared{t.parts, t.nrows, t.r0, t.s.begin, t.j};
+                    }
+                    for (int h = 0; ok && h <= (t.nrows > 128 ? 1 : 0); ++h) {
+                        int& used = h ? used1 : used0;
+                        if (used > 0) wait(bar_used + 8 * h, used - 1);  // the tile before it has been multiplied
+                        if (!ok) break;
+                        wide_queries<E, D>(p, t, h, lane, sb + h * SM::kTile, bar_q + 8 * h);
+                        ++used;
+                    }
+                }
+                if (lane == 0 && !shares) w.shared[blockIdx.x].parts = 0;
+                // no queries may still be landing when the CTA leaves
+                if (used0 > 0) tc_wait(bar_q, (used0 - 1) & 1, nullptr, lim, kv.errors);
+                if (used1 > 0) tc_wait(bar_q + 8, (used1 - 1) & 1, nullptr, lim, kv.errors);
+                __syncwarp();
             }
-            if (lane == 0 && !shares) w.shared[blockIdx.x].parts = 0;
-            // no queries may still be landing when the CTA leaves
-            if (used0 > 0) tc_wait(bar_q, (used0 - 1) & 1, nullptr, lim, kv.errors);
-            if (used1 > 0) tc_wait(bar_q + 8, (used1 - 1) & 1, nullptr, lim, kv.errors);
+            if (warp <= 10) {  // every product issued above has finished once this completes
+                const uint32_t done = bar_done + 8 * (warp - 9);
+                if (elect_one()) tc_commit(done);
+                __syncwarp();
+                tc_wait(done, 0, nullptr, lim, kv.errors);
+            }
             __syncwarp();
         }
-        if (warp <= 10) {  // every product issued above has finished once this completes
-            const uint32_t done = bar_done + 8 * (warp - 9);
-            if (elect_one()) tc_commit(done);
-            __syncwarp();
-            tc_wait(done, 0, nullptr, lim, kv.errors);
-        }
-        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();

@@ -174,3 +174,12 @@ def test_oracle_agrees_with_the_dense_step():
     ref = op.attention(q.reshape(b, -1), kp, vp, table, lens, None)
     assert (ref["out"].reshape(b, -1) - dense.double()).abs().max() < 2e-2
     assert torch.equal(vp[table[0][2], :, pos % page], vd[0, :, pos])
+
+
+def test_registers_move_by_one_instruction_per_warpgroup():
+    """setmaxnreg is defined only where all warps of a warpgroup execute the same
+    one: a second place in the code means that some warps take another."""
+    for src in (Path(__file__).resolve().parents[1] / "breeze-tts-2_b200" / "csrc").glob("*.cu"):
+        text = src.read_text()
+        for kind in ("inc", "dec"):
+            assert len(re.findall(rf'"setmaxnreg\.{kind}\.', text)) <= 1, (src.name, kind)
