@@ -37,7 +37,7 @@
 // softmax warps of half 0 clear those rows of v. Scores there are never used.
 // Infinite and NaN entries of v at positions that only some rows of a tile see
 // are cleared likewise, and added in memory to the outputs of the rows that see
-// them (not in the prefix pass: there every sequence sees the same positions).
+// them.
 //
 // Measured, join included (B200): 7000 new positions of 16 query and 8 kv heads of
 // 128, causal, 201 GFLOP in 207 us (0.97 PFLOP/s; library products of 8192^3 run at
@@ -51,6 +51,7 @@
 // mostly not the exponential units but their own chains of instructions. A score
 // buffer per half, the probabilities through shared memory instead: 266.
 #include <algorithm>
+#include <climits>
 #include <cstring>
 
 #include "bq_host.h"
@@ -218,6 +219,7 @@ struct WideTile {
     int b, j, r0, nrows, k0, nu, p0, p1;
     int whole, parts;  // one CTA has all of it; CTAs that share it when it begins here
     int ring;          // ring stages before it
+    int seen;          // positions that every row sees (wide_seen)
     int valid;         // 0: the share has ended
 };
 constexpr int kTiles = 4;  // tiles on their way
@@ -260,6 +262,22 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
                  : "memory");
+}
+
+// Positions that every row of a tile sees (one warp). The rows of a sequence see ascending
+// numbers of positions. In the prefix pass, rows of many sequences, a row may see less of the
+// prefix than the one before it: the least of all of them, but for rows that see nothing, of
+// which the join takes nothing.
+__device__ __forceinline__ int wide_seen(const PagedWork& w, const PagedSeq& s, int r0, int nrows, int lane) {
+    if (!w.prefix_pass) return paged_row_limit(w, s, r0);
+    const int last = w.by_G(r0 + nrows - 1);
+    int least = INT_MAX;
+#pragma unroll 1
+    for (int tok = w.by_G(r0) + lane; tok <= last; tok += 32) {
+        const int limit = paged_row_limit(w, s, tok * w.G);
+        if (limit > 0) least = min(least, limit);
+    }
+    return __reduce_min_sync(0xffffffffu, least);
 }
 
 // Queries of half h of tile t into shared memory (one warp), in the
@@ -381,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             const int myrow = t.r0 + 128 * h + row, units = t.nu, p0 = t.p0, p1 = t.p1;
             const bool idle = (warp & 3) * 32 >= hrows;  // no row of this warp exists
             const int limit = row < hrows ? paged_row_limit(w, t.s, myrow) : 0;
-            const int seen = w.prefix_pass ? p1 : paged_row_limit(w, t.s, t.r0);  // by every row: limits ascend
+            const int seen = t.seen;
             float mref = -INFINITY, l = 0.f;
             __syncwarp();  // tensor-memory instructions below are warp-wide
             for (int u = 0; u < units; ++u) {
@@ -703,6 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                             t.whole = g.whole();
                             t.parts = g.parts(c, blockIdx.x);
                             t.ring = ring;
+                            t.seen = wide_seen(w, t.s, t.r0, t.nrows, lane);
                             t.valid = 1;
                             paged_next<kRows>(w, c, g.cost);
                             break;

@@ -289,8 +289,7 @@ int32_t bq_attention_o_step(const bq_attn_o_desc* desc, void* workspace, size_t 
  *     so the outputs of that sequence mean nothing. Entries that no position
  *     needs may hold anything.
  * Slots that hold no position may hold anything, NaN included, and infinite or
- * NaN keys and values reach only the rows that see their position (of a shared
- * prefix that gets its own pass: all rows whose sequence ends in it, too). */
+ * NaN keys and values reach only the rows that see their position. */
 typedef struct bq_paged_kv {
     int32_t B;             /* sequences, >= 1 */
     int32_t HKV, D;        /* kv heads, head dim (64 or 128) */

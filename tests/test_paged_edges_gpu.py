@@ -1,0 +1,47 @@
+"""Paged-cache operators where the definition is easily missed: values that only
+some rows of a shared prefix see, unused slots before it, scores of minus
+infinity, cut lengths, strides of dimensions of size one, long caches. Against
+the 64-bit oracle, within the bounds derived there."""
+
+import pytest
+import torch
+
+from oracle import paged as op
+from tests import paged_cases as pc
+from tests.test_paged_gpu import _clean_status, _status, compare, run  # noqa: F401 - fixtures
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F16 = pc.BF, pc.F16
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("lens,new,prefix,hq,hkv,dim,page,dtype,at", [
+    ([260, 258], [30, 1], 256, 4, 2, 128, 64, BF, [(250, INF), (235, NAN)]),         # new rows begin inside the prefix
+    ([256, 100, 300], [40, 40, 40], 256, 8, 2, 128, 32, BF, [(99, -INF), (200, NAN)]),  # one ends in it
+    ([700, 600], [150, 33], 640, 4, 2, 64, 64, F16, [(580, INF), (639, -INF), (555, NAN)]),
+    ([1500, 1033], [500, 20], 1024, 2, 2, 128, 16, BF, [(1001, INF), (1022, NAN), (1010, -INF)]),
+    ([70, 66, 40], None, 64, 2, 1, 128, 16, BF, [(50, INF), (39, NAN)]),             # few rows
+    ([70, 66, 40], [5, 3, 1], 64, 1, 1, 64, 16, F16, [(63, NAN), (39, INF)]),
+])
+def test_a_prefix_value_reaches_only_the_rows_that_see_it(lens, new, prefix, hq, hkv, dim, page, dtype, at):
+    c = pc.batch(lens, new, hq, hkv, dim, page, dtype, seed=47, prefix=prefix)
+    clean = dict(c, v=c["v"].clone())
+    table, ls, starts = pc.lists(c)
+    for i, (pos, what) in enumerate(at):
+        where = (table[0][pos // page], i % hkv, pos % page)
+        c["v"][where][5 * i + 1] = what
+        clean["v"][where][5 * i + 1] = 0.0
+    ref, fine = (op.attention(x["q"], x["k"], x["v"], table, ls, starts) for x in (c, clean))
+    tol, ltol = op.attention_bounds(fine, dim, dtype)
+    good = torch.isfinite(ref["out"])
+    assert not good.all() and good.any(-1).all()
+    for always in (True, False):
+        out, lse = run(c, always=always)
+        o = out.double().reshape(c["rows"], hq, dim)
+        assert torch.isfinite(o)[good].all()
+        assert ((o - ref["out"]).abs() <= tol)[good].all()
+        assert torch.equal(torch.isnan(o)[~good], torch.isnan(ref["out"])[~good])
+        inf = torch.isinf(ref["out"])
+        assert torch.equal(o[inf], ref["out"][inf])
+        assert ((lse.double() - ref["lse"]).abs() <= ltol).all()
