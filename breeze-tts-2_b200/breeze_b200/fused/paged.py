@@ -246,11 +246,12 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
                      out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
                      always: bool = False) -> torch.Tensor:
     """paged_attention for a batch that shares its first ``prefix_len``
-    positions (a multiple of the page size): the first prefix_len / page size
-    entries of every table row name the same pages. They are read once for all
-    rows together, through row 0 of the table, and joined with each sequence's
-    own positions, where that pays (a short prefix of few sequences is read by
-    each; ``always=True`` shares it all the same); the value is
-    paged_attention's."""
+    positions (a multiple of the page size): of every sequence with new rows the
+    first prefix_len / page size table entries name the same pages, as far as the
+    sequence goes (an unused slot's entries may hold anything). They are read once
+    for all rows together, through the table row of the longest such sequence, and
+    joined with each sequence's own positions, where that pays (a short prefix of
+    few sequences is read by each; ``always=True`` shares it all the same); the
+    value is paged_attention's."""
     return _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, causal, max_q, out, lse,
                       _lib.PAGED_SHARE if always else 0)

@@ -91,7 +91,9 @@ struct FastDiv {
 //
 // With a shared prefix there are two such schedules: the prefix over all rows
 // of the batch at once (one pseudo-sequence), and each sequence's own positions
-// from prefix_len on.
+// from prefix_len on. The prefix's pages are those of the longest sequence that
+// has new rows, as far as it goes (PagedPrefix): an unused slot's table entries
+// are not looked at.
 struct PagedShared {
     int32_t parts, rows, r0, begin, j;  // CTAs that hold it (0: none), its rows, first row, first token of the sequence, kv head
 };
@@ -122,16 +124,29 @@ __device__ __forceinline__ int2 paged_row_at(int cta, int parts, int row) { retu
 
 struct PagedSeq {
     int begin, count, rows, len, off;  // first row, new rows, rows * G, positions, position of the first new row
+    int table;                         // its row of the page table
 };
 
-__device__ __forceinline__ PagedSeq paged_seq(const PagedWork& p, int b, bool& cut) {
+// The prefix pass's sequence: the row of the table that it reads, the positions that any row sees, those that
+// every row sees (rows that see nothing aside).
+struct PagedPrefix {
+    int table, len, seen;
+};
+
+// PREFIX: the launch handles the prefix. A parameter of the kernels, since as a flag that they look at it takes the
+// few-row kernel without a prefix from 38.7 to 45 us (48 sequences of 17 to 6000 positions).
+
+template <bool PREFIX>
+__device__ __forceinline__ PagedSeq paged_seq(const PagedWork& p, const PagedPrefix& prefix, int b, bool& cut) {
     PagedSeq s;
     cut = false;
-    if (p.prefix_pass) {
+    s.table = b;
+    if (PREFIX) {
         s.begin = 0;
         s.count = p.kv.starts ? min(max(p.kv.starts[p.kv.B], 0), p.kv.T) : p.kv.T;
-        s.len = p.prefix_len;
+        s.len = prefix.len;
         s.off = 0;
+        s.table = prefix.table;
     } else {
         paged_rows(p.kv, b, s.begin, s.count);
         s.len = max(paged_len(p.kv, b, cut), 0);
@@ -142,25 +157,25 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedWork& p, int b, bool& c
 }
 
 // Positions that the last row of tile i sees (all that any row of it sees).
-template <int ROWS>
+template <bool PREFIX, int ROWS>
 __device__ __forceinline__ int paged_tile_limit(const PagedWork& p, const PagedSeq& s, int i) {
-    if (p.prefix_pass || !p.causal) return s.len;
+    if (PREFIX || !p.causal) return s.len;
     const int tok = p.by_G(min(s.rows, (i + 1) * ROWS) - 1);
     return max(0, min(s.len, s.off + tok + 1));
 }
 
 // Units of tile i: at least one, so that rows that see nothing are written too.
-template <int ROWS, int UNIT>
+template <bool PREFIX, int ROWS, int UNIT>
 __device__ __forceinline__ int paged_tile_units(const PagedWork& p, const PagedSeq& s, int i) {
-    const int n = paged_tile_limit<ROWS>(p, s, i) - (p.prefix_pass ? 0 : p.prefix_len);
+    const int n = paged_tile_limit<PREFIX, ROWS>(p, s, i) - (PREFIX ? 0 : p.prefix_len);
     return max(1, (n + UNIT - 1) / UNIT);
 }
 
 // Cost of the tiles of one kv head, in units.
-template <int ROWS, int UNIT, int OVERHEAD>
+template <bool PREFIX, int ROWS, int UNIT, int OVERHEAD>
 __device__ __forceinline__ long long paged_head_cost(const PagedWork& p, const PagedSeq& s, int tiles) {
     long long n = (long long)tiles * OVERHEAD;
-    for (int i = 0; i < tiles; ++i) n += paged_tile_units<ROWS, UNIT>(p, s, i);
+    for (int i = 0; i < tiles; ++i) n += paged_tile_units<PREFIX, ROWS, UNIT>(p, s, i);
     return n;
 }
 
@@ -187,6 +202,39 @@ struct PagedShare {
     }
 };
 
+// All NT threads, in the prefix pass: the longest sequence that has rows, of several the first.
+template <int NT>
+__device__ __forceinline__ PagedPrefix paged_prefix(const PagedWork& p) {
+    __shared__ unsigned long long s_key[NT / 32];
+    __shared__ int s_seen[NT / 32];
+    unsigned long long key = 0;  // length, then the smallest index
+    int seen = p.prefix_len;
+    for (int b = threadIdx.x; b < p.kv.B; b += NT) {
+        int begin, count;
+        paged_rows(p.kv, b, begin, count);
+        bool cut;
+        const int len = paged_len(p.kv, b, cut);
+        if (count == 0 || len <= 0) continue;
+        key = max(key, (unsigned long long)len << 32 | (0x7fffffffu - unsigned(b)));
+        seen = min(seen, p.causal ? min(len, max(1, p.kv.lens[b] - count + 1)) : len);  // its first row that sees any
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+    seen = __reduce_min_sync(0xffffffffu, seen);
+    if ((threadIdx.x & 31) == 0) {
+        s_key[threadIdx.x >> 5] = key;
+        s_seen[threadIdx.x >> 5] = seen;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+        key = max(key, s_key[w]);
+        seen = min(seen, s_seen[w]);
+    }
+    const int len = int(key >> 32);
+    return PagedPrefix{len ? int(0x7fffffffu - unsigned(key)) : 0, min(len, p.prefix_len), seen};
+}
+
 // Place in a CTA's share.
 struct PagedCursor {
     int b, j, i, k;   // sequence, kv head, tile, cost units of the tile that lie before
@@ -197,12 +245,12 @@ struct PagedCursor {
 
 // The part of the tile at the cursor that lies in the share: units [k0, k0 + nu)
 // of `units`; nu = 0: only overhead.
-template <int ROWS, int UNIT, int OVERHEAD>
+template <bool PREFIX, int ROWS, int UNIT, int OVERHEAD>
 struct PagedSegment {
     int units, k0, nu, cost;
     PagedSegment() = default;
     __device__ __forceinline__ PagedSegment(const PagedWork& p, const PagedSeq& s, const PagedCursor& c) {
-        units = paged_tile_units<ROWS, UNIT>(p, s, c.i);
+        units = paged_tile_units<PREFIX, ROWS, UNIT>(p, s, c.i);
         cost = int(min((long long)(units + OVERHEAD - c.k), c.hi - c.u));
         k0 = max(0, c.k - OVERHEAD);
         nu = max(0, c.k + cost - OVERHEAD) - k0;
@@ -214,26 +262,31 @@ struct PagedSegment {
     }
 };
 
-// All NT threads: finds the share of CTA `cta`. The thread whose sequences hold its
+// All NT threads: finds the share of CTA `cta` and, in the prefix pass, what `s_prefix` (shared memory) says. The thread whose sequences hold its
 // first unit finds the place with what it has read and tells the others (when every
 // thread read the sequence once more and divided for itself, 48 sequences of 17 to
 // 6000 positions took 42.1 us instead of 38.4, 8 of 24 to 32 thousand 158 instead of
 // 146).
-template <int ROWS, int UNIT, int OVERHEAD, int NT>
-__device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, int grid) {
+template <bool PREFIX, int ROWS, int UNIT, int OVERHEAD, int NT>
+__device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, int grid, PagedPrefix& s_prefix) {
     __shared__ long long s_sum[NT / 32];
     __shared__ int s_at[5];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int B = p.prefix_pass ? 1 : p.kv.B;
+    PagedPrefix prefix = {0, 0, 0};
+    if (PREFIX) {
+        prefix = paged_prefix<NT>(p);
+        if (threadIdx.x == 0) s_prefix = prefix;
+    }
+    const int B = PREFIX ? 1 : p.kv.B;
     const int per = (B + NT - 1) / NT, b0 = min(int(threadIdx.x) * per, B), b1 = min(b0 + per, B);
     PagedSeq s;
     int tiles = 0;
     long long head = 0, mine = 0;
     auto read = [&](int b) {
         bool cut;
-        s = paged_seq(p, b, cut);
+        s = paged_seq<PREFIX>(p, prefix, b, cut);
         tiles = (s.rows + ROWS - 1) / ROWS;
-        head = paged_head_cost<ROWS, UNIT, OVERHEAD>(p, s, tiles);
+        head = paged_head_cost<PREFIX, ROWS, UNIT, OVERHEAD>(p, s, tiles);
         return cut;
     };
     for (int b = b0; b < b1; ++b) {
@@ -272,7 +325,7 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
         long long left = rem - j * head;
         int i = 0;
         for (;; ++i) {
-            const int n = paged_tile_units<ROWS, UNIT>(p, s, i) + OVERHEAD;
+            const int n = paged_tile_units<PREFIX, ROWS, UNIT>(p, s, i) + OVERHEAD;
             if (left < n) break;
             left -= n;
         }
@@ -297,27 +350,28 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedWork& p, int cta, i
 }
 
 // To the tile after the cursor's, `cost` units on (sequences without rows have none).
-template <int ROWS>
-__device__ __forceinline__ void paged_next(const PagedWork& p, PagedCursor& c, int cost) {
+template <bool PREFIX, int ROWS>
+__device__ __forceinline__ void paged_next(const PagedWork& p, const PagedPrefix& prefix, PagedCursor& c, int cost) {
     c.u += cost;
     c.k = 0;
     if (++c.i < c.tiles) return;
     c.i = 0;
     if (++c.j < p.kv.HKV) return;
     c.j = 0;
-    const int B = p.prefix_pass ? 1 : p.kv.B;
+    const int B = PREFIX ? 1 : p.kv.B;
     for (++c.b; c.b < B; ++c.b) {
         bool cut;
-        const PagedSeq s = paged_seq(p, c.b, cut);
+        const PagedSeq s = paged_seq<PREFIX>(p, prefix, c.b, cut);
         c.tiles = (s.rows + ROWS - 1) / ROWS;
         if (c.tiles > 0) return;
     }
 }
 
 // Positions [0, limit) are seen by row r (of sequence s; in the prefix pass, of all rows).
+template <bool PREFIX>
 __device__ __forceinline__ int paged_row_limit(const PagedWork& p, const PagedSeq& s, int r) {
     const int tok = p.by_G(r);
-    if (!p.prefix_pass) return p.causal ? max(0, min(s.len, s.off + tok + 1)) : s.len;
+    if (!PREFIX) return p.causal ? max(0, min(s.len, s.off + tok + 1)) : s.len;
     int b = tok;
     if (p.kv.starts) {  // the sequence of row tok: starts[b] <= tok < starts[b + 1]
         int lo = 0, hi = p.kv.B;

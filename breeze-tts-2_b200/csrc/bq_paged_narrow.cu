@@ -85,10 +85,10 @@ struct NarrowSmem {
     static_assert(kNarrowWarps * 16 * kPitch * 4 <= kQ, "the warps' outputs fit the rings");
 };
 
-// Positions [p0, p1) of rows r0 .. r0 + nrows of sequence b and kv head j.
+// Positions [p0, p1) of rows r0 .. r0 + nrows of a sequence and kv head j.
 struct NarrowTile {
     PagedSeq s;
-    int b, j, r0, nrows, p0, p1;
+    int j, r0, nrows, p0, p1;
 };
 
 // Infinite and NaN entries of the v block at vb (positions pb .. pb + 15): added to
@@ -133,7 +133,7 @@ __device__ __forceinline__ void narrow_nonfinite(uint32_t vb, int pb, int lim0, 
 
 // One tile with the whole CTA: emit(r, d, m, l, o) receives dims d .. d + 3 of row r,
 // unnormalized, with the row's largest score (base 2) and sum of exponentials.
-template <typename E, int D, typename Emit>
+template <bool PREFIX, typename E, int D, typename Emit>
 __device__ __forceinline__ void narrow_tile(const PagedWork& p, const NarrowTile& t, unsigned char* smem, int* s_lim,
                                             float2 (*s_ml)[kNarrowRows], const Emit& emit) {
     using SM = NarrowSmem<D>;
@@ -162,7 +162,7 @@ __device__ __forceinline__ void narrow_tile(const PagedWork& p, const NarrowTile
     auto issue = [&](int st) {
         if ((st & 31) == 0) {
             const int mine = st + lane;
-            pages = mine < steps ? paged_page(kv, t.b, p0 + 16 * (warp + kNarrowWarps * mine), pages_ok) : 0;
+            pages = mine < steps ? paged_page(kv, s.table, p0 + 16 * (warp + kNarrowWarps * mine), pages_ok) : 0;
         }
         const int page = __shfl_sync(0xffffffffu, pages, st & 31);
         if (st < steps) {
@@ -182,7 +182,7 @@ __device__ __forceinline__ void narrow_tile(const PagedWork& p, const NarrowTile
     };
 #pragma unroll
     for (int st = 0; st < ST - 1; ++st) issue(st);
-    if (threadIdx.x < ROWS) s_lim[threadIdx.x] = int(threadIdx.x) < nrows ? paged_row_limit(p, s, r0 + threadIdx.x) : 0;
+    if (threadIdx.x < ROWS) s_lim[threadIdx.x] = int(threadIdx.x) < nrows ? paged_row_limit<PREFIX>(p, s, r0 + threadIdx.x) : 0;
     cp_wait<ST - 1>();  // the query tile
     __syncthreads();
     uint32_t qf[D / 16][4];
@@ -307,31 +307,31 @@ __device__ __forceinline__ void narrow_tile(const PagedWork& p, const NarrowTile
     __syncthreads();  // the rings are free again
 }
 
-template <typename E, int D>
+template <bool PREFIX, typename E, int D>
 __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_constant__ PagedWork p) {
     constexpr int ROWS = kNarrowRows, UNIT = kNarrowUnit;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int s_lim[ROWS];
     __shared__ float2 s_ml[kNarrowWarps][ROWS];
+    __shared__ PagedPrefix s_prefix;
     const PagedKV& kv = p.kv;
     pdl_launch_dependents();
     pdl_wait();
-    PagedCursor c = paged_find<ROWS, UNIT, kNarrowOverhead, kThreads>(p, blockIdx.x, gridDim.x);
+    PagedCursor c = paged_find<PREFIX, ROWS, UNIT, kNarrowOverhead, kThreads>(p, blockIdx.x, gridDim.x, s_prefix);
     bool shares = false;  // the last tile goes on in the next CTA
-    const int kv_lo = p.prefix_pass ? 0 : p.prefix_len, sequences = p.prefix_pass ? 1 : kv.B;
+    const int kv_lo = PREFIX ? 0 : p.prefix_len, sequences = PREFIX ? 1 : kv.B;
     while (c.u < c.hi && c.b < sequences) {
         bool cut;
         NarrowTile t;
-        t.s = paged_seq(p, c.b, cut);
-        const PagedSegment<ROWS, UNIT, kNarrowOverhead> sg(p, t.s, c);
+        t.s = paged_seq<PREFIX>(p, s_prefix, c.b, cut);
+        const PagedSegment<PREFIX, ROWS, UNIT, kNarrowOverhead> sg(p, t.s, c);
         if (sg.nu == 0) {
-            paged_next<ROWS>(p, c, sg.cost);
+            paged_next<PREFIX, ROWS>(p, s_prefix, c, sg.cost);
             continue;
         }
-        t.b = c.b;
         t.j = c.j;
         t.p0 = kv_lo + sg.k0 * UNIT;
-        t.p1 = min(t.p0 + sg.nu * UNIT, paged_tile_limit<ROWS>(p, t.s, c.i));
+        t.p1 = min(t.p0 + sg.nu * UNIT, paged_tile_limit<PREFIX, ROWS>(p, t.s, c.i));
         t.r0 = c.i * ROWS;
         t.nrows = min(ROWS, t.s.rows - t.r0);
         const bool whole = sg.whole();
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
             shares = true;
             if (threadIdx.x == 0) p.shared[blockIdx.x] = PagedShared{parts, t.nrows, t.r0, t.s.begin, c.j};
         }
-        narrow_tile<E, D>(p, t, smem, s_lim, s_ml, [&](int r, int d, float mm, float ll, const float4& a) {
+        narrow_tile<PREFIX, E, D>(p, t, smem, s_lim, s_ml, [&](int r, int d, float mm, float ll, const float4& a) {
             const int rr = t.r0 + r, tok = p.by_G(rr), head = c.j * p.G + rr - tok * p.G;
             const int64_t row = t.s.begin + tok;
             if (whole && !p.row_o) {
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
                 }
             }
         });
-        paged_next<ROWS>(p, c, sg.cost);
+        paged_next<PREFIX, ROWS>(p, s_prefix, c, sg.cost);
     }
     if (!shares && threadIdx.x == 0) p.shared[blockIdx.x].parts = 0;
 }
@@ -383,18 +383,18 @@ __global__ void __launch_bounds__(kThreads, 2) paged_cluster_kernel(const __grid
     pdl_wait();
     const int pair = blockIdx.x / ranks, rank = blockIdx.x - pair * ranks;
     NarrowTile t;
-    t.b = pair / p.kv.HKV;
-    t.j = pair - t.b * p.kv.HKV;
+    const int b = pair / p.kv.HKV;
+    t.j = pair - b * p.kv.HKV;
     bool cut;
-    t.s = paged_seq(p, t.b, cut);
+    t.s = paged_seq<false>(p, PagedPrefix{0, 0, 0}, b, cut);
     if (cut && rank == 0 && t.j == 0 && threadIdx.x == 0) atomicOr(p.kv.errors, BQ_DEVERR_POSITION_BIT);
     for (int i = 0; i * kNarrowRows < t.s.rows; ++i) {  // one tile, unless max_q was told too low
         t.r0 = i * kNarrowRows;
         t.nrows = min(kNarrowRows, t.s.rows - t.r0);
-        const int limit = paged_tile_limit<kNarrowRows>(p, t.s, i), units = (limit + kNarrowUnit - 1) / kNarrowUnit;
+        const int limit = paged_tile_limit<false, kNarrowRows>(p, t.s, i), units = (limit + kNarrowUnit - 1) / kNarrowUnit;
         t.p0 = rank * units / ranks * kNarrowUnit;
         t.p1 = min((rank + 1) * units / ranks * kNarrowUnit, limit);
-        narrow_tile<E, D>(p, t, smem, s_lim, s_ml, [&](int r, int d, float mm, float ll, const float4& a) {
+        narrow_tile<false, E, D>(p, t, smem, s_lim, s_ml, [&](int r, int d, float mm, float ll, const float4& a) {
             *reinterpret_cast<float4*>(out + r * D + d) = a;
             if (d == 0) s_row[r] = make_float2(mm, ll);
         });
@@ -435,13 +435,18 @@ __global__ void __launch_bounds__(kThreads, 2) paged_cluster_kernel(const __grid
     }
 }
 
+template <bool PREFIX>
+const void* narrow_kernel(int dtype, int D) {
+    return D == 128 ? (dtype == BQ_DT_BF16 ? reinterpret_cast<const void*>(&paged_narrow_kernel<PREFIX, __nv_bfloat16, 128>)
+                                           : reinterpret_cast<const void*>(&paged_narrow_kernel<PREFIX, __half, 128>))
+                    : (dtype == BQ_DT_BF16 ? reinterpret_cast<const void*>(&paged_narrow_kernel<PREFIX, __nv_bfloat16, 64>)
+                                           : reinterpret_cast<const void*>(&paged_narrow_kernel<PREFIX, __half, 64>));
+}
+
 }  // namespace
 
 int paged_launch_narrow(const PagedWork& w, int dtype, int D, int grid, uint32_t flags, void* stream) {
-    const void* fn = D == 128 ? (dtype == BQ_DT_BF16 ? reinterpret_cast<const void*>(&paged_narrow_kernel<__nv_bfloat16, 128>)
-                                                     : reinterpret_cast<const void*>(&paged_narrow_kernel<__half, 128>))
-                              : (dtype == BQ_DT_BF16 ? reinterpret_cast<const void*>(&paged_narrow_kernel<__nv_bfloat16, 64>)
-                                                     : reinterpret_cast<const void*>(&paged_narrow_kernel<__half, 64>));
+    const void* fn = w.prefix_pass ? narrow_kernel<true>(dtype, D) : narrow_kernel<false>(dtype, D);
     const uint32_t smem = D == 128 ? NarrowSmem<128>::kTotal : NarrowSmem<64>::kTotal;
     const int rc = ensure_smem_attr(fn, smem);
     if (rc) return rc;

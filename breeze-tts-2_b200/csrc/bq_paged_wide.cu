@@ -213,10 +213,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {  // comple
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// A tile as warp 11 passes it on: units k0 .. k0 + nu of the rows r0 .. r0 + nrows of sequence b and kv head j.
+// A tile as warp 11 passes it on: units k0 .. k0 + nu of the rows r0 .. r0 + nrows of a sequence and kv head j.
 struct WideTile {
     PagedSeq s;
-    int b, j, r0, nrows, k0, nu, p0, p1;
+    int j, r0, nrows, k0, nu, p0, p1;
     int whole, parts;  // one CTA has all of it; CTAs that share it when it begins here
     int ring;          // ring stages before it
     int seen;          // positions that every row sees (wide_seen)
@@ -267,14 +267,16 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 // Positions that every row of a tile sees (one warp). The rows of a sequence see ascending
 // numbers of positions. In the prefix pass, rows of many sequences, a row may see less of the
 // prefix than the one before it: the least of all of them, but for rows that see nothing, of
-// which the join takes nothing.
-__device__ __forceinline__ int wide_seen(const PagedWork& w, const PagedSeq& s, int r0, int nrows, int lane) {
-    if (!w.prefix_pass) return paged_row_limit(w, s, r0);
+// which the join takes nothing (mostly every row of the batch sees it all).
+template <bool PREFIX>
+__device__ __forceinline__ int wide_seen(const PagedWork& w, const PagedPrefix& prefix, const PagedSeq& s, int r0, int nrows, int lane) {
+    if (!PREFIX) return paged_row_limit<PREFIX>(w, s, r0);
+    if (prefix.seen >= prefix.len) return prefix.len;
     const int last = w.by_G(r0 + nrows - 1);
     int least = INT_MAX;
 #pragma unroll 1
     for (int tok = w.by_G(r0) + lane; tok <= last; tok += 32) {
-        const int limit = paged_row_limit(w, s, tok * w.G);
+        const int limit = paged_row_limit<PREFIX>(w, s, tok * w.G);
         if (limit > 0) least = min(least, limit);
     }
     return __reduce_min_sync(0xffffffffu, least);
@@ -312,13 +314,14 @@ __device__ __forceinline__ void wide_queries(const PagedWideParams& p, const Wid
     if (lane == 0) mbar_arrive(bar);
 }
 
-template <typename E, int D>
+template <bool PREFIX, typename E, int D>
 __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_constant__ PagedWideParams p) {
     using SM = WideSmem<D>;
     constexpr int ST = SM::kStages, CH = D / 8;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
+    __shared__ PagedPrefix s_prefix;
     __shared__ WideTile s_tile[kTiles];
     __shared__ volatile int s_bad[kTiles];  // n + 1: entries of v were cleared from tile n
     const uint32_t sraw = smem_u32(smem_raw), sb = (sraw + 1023u) & ~1023u;
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
         fence_barrier_init();
     }
     pdl_wait();  // before the tensor memory is taken: a kernel before this one may still need its own
-    PagedCursor c = paged_find<kRows, kUnit, kWideOverhead, kThreads>(w, blockIdx.x, gridDim.x);
+    PagedCursor c = paged_find<PREFIX, kRows, kUnit, kWideOverhead, kThreads>(w, blockIdx.x, gridDim.x, s_prefix);
     if (warp == 9) tmem_alloc(smem_u32(&s_tmem), kCols);
     tc_fence_before();
     __syncthreads();
@@ -398,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             }
             const int myrow = t.r0 + 128 * h + row, units = t.nu, p0 = t.p0, p1 = t.p1;
             const bool idle = (warp & 3) * 32 >= hrows;  // no row of this warp exists
-            const int limit = row < hrows ? paged_row_limit(w, t.s, myrow) : 0;
+            const int limit = row < hrows ? paged_row_limit<PREFIX>(w, t.s, myrow) : 0;
             const int seen = t.seen;
             float mref = -INFINITY, l = 0.f;
             __syncwarp();  // tensor-memory instructions below are warp-wide
@@ -574,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 bool page_ok = true;
 #pragma unroll 1
                 for (int pos = max(p0, seen); pos < min(p1, limit); ++pos) {
-                    const E* v = static_cast<const E*>(kv.v) + paged_page(kv, t.b, pos, page_ok) * kv.vs_page + t.j * kv.vs_head +
+                    const E* v = static_cast<const E*>(kv.v) + paged_page(kv, t.s.table, pos, page_ok) * kv.vs_page + t.j * kv.vs_head +
                                  int64_t(pos & kv.page_mask) * kv.vs_slot;
 #pragma unroll 1
                     for (int d = 0; d < D; d += 2) {
@@ -609,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
             for (int n = 0;; ++n) {
                 wait(bar_tile + 8 * (n % kTiles), n / kTiles);
                 if (!ok || !tile(n).valid) break;
-                const int units = tile(n).nu, p0 = tile(n).p0, p1 = tile(n).p1, seq = tile(n).b, j = tile(n).j;
+                const int units = tile(n).nu, p0 = tile(n).p0, p1 = tile(n).p1, seq = tile(n).s.table, j = tile(n).j;
                 release(n);
                 for (int u = 0; ok && u < units; ++u) {
                     const int base = p0 + u * kUnit;
@@ -699,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 // -------------------------------------------------------- tiles and queries
                 int used0 = 0, used1 = 0, ring = 0;  // tiles of each half, ring stages so far
                 bool shares = false;                 // the last tile goes on in the next CTA
-                const int sequences = w.prefix_pass ? 1 : kv.B;
+                const int sequences = PREFIX ? 1 : kv.B;
                 for (int n = 0; ok; ++n) {
                     if (n >= kTiles) wait(bar_free + 8 * (n % kTiles), n / kTiles - 1);
                     if (!ok) break;
@@ -707,26 +710,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     t.valid = 0;
                     while (c.u < c.hi && c.b < sequences) {  // past tiles of which this share holds only overhead
                         bool cut;
-                        t.s = paged_seq(w, c.b, cut);
-                        const PagedSegment<kRows, kUnit, kWideOverhead> g(w, t.s, c);
+                        t.s = paged_seq<PREFIX>(w, s_prefix, c.b, cut);
+                        const PagedSegment<PREFIX, kRows, kUnit, kWideOverhead> g(w, t.s, c);
                         if (g.nu > 0) {
-                            t.b = c.b;
-                            t.j = c.j;
+                                t.j = c.j;
                             t.r0 = c.i * kRows;
                             t.nrows = min(kRows, t.s.rows - t.r0);
                             t.k0 = g.k0;
                             t.nu = g.nu;
-                            t.p0 = (w.prefix_pass ? 0 : w.prefix_len) + g.k0 * kUnit;
-                            t.p1 = min(t.p0 + g.nu * kUnit, paged_tile_limit<kRows>(w, t.s, c.i));
+                            t.p0 = (PREFIX ? 0 : w.prefix_len) + g.k0 * kUnit;
+                            t.p1 = min(t.p0 + g.nu * kUnit, paged_tile_limit<PREFIX, kRows>(w, t.s, c.i));
                             t.whole = g.whole();
                             t.parts = g.parts(c, blockIdx.x);
                             t.ring = ring;
-                            t.seen = wide_seen(w, t.s, t.r0, t.nrows, lane);
+                            t.seen = wide_seen<PREFIX>(w, s_prefix, t.s, t.r0, t.nrows, lane);
                             t.valid = 1;
-                            paged_next<kRows>(w, c, g.cost);
+                            paged_next<PREFIX, kRows>(w, s_prefix, c, g.cost);
                             break;
                         }
-                        paged_next<kRows>(w, c, g.cost);
+                        paged_next<PREFIX, kRows>(w, s_prefix, c, g.cost);
                     }
                     if (lane == 0) {
                         s_tile[n % kTiles] = t;
@@ -813,6 +815,14 @@ int encode_queries(const PagedWork& w, const bq_paged_kv* kv, CUtensorMap* map) 
     return BQ_OK;
 }
 
+template <bool PREFIX>
+const void* wide_kernel(int dtype, int D) {
+    return D == 128 ? (dtype == BQ_DT_BF16 ? reinterpret_cast<const void*>(&paged_wide_kernel<PREFIX, __nv_bfloat16, 128>)
+                                           : reinterpret_cast<const void*>(&paged_wide_kernel<PREFIX, __half, 128>))
+                    : (dtype == BQ_DT_BF16 ? reinterpret_cast<const void*>(&paged_wide_kernel<PREFIX, __nv_bfloat16, 64>)
+                                           : reinterpret_cast<const void*>(&paged_wide_kernel<PREFIX, __half, 64>));
+}
+
 }  // namespace
 
 int paged_launch_wide(const PagedWork& w, const bq_paged_kv* kv, int grid, uint32_t flags, void* stream) {
@@ -834,11 +844,7 @@ int paged_launch_wide(const PagedWork& w, const bq_paged_kv* kv, int grid, uint3
     p.idesc_qk = common | (uint32_t(128 >> 3) << 17);
     p.idesc_pv = common | (1u << 16) | (uint32_t(kv->D >> 3) << 17);
     p.wait_cycles = kWaitCycles;
-    const bool bf = kv->dtype == BQ_DT_BF16;
-    const void* fn = kv->D == 128 ? (bf ? reinterpret_cast<const void*>(&paged_wide_kernel<__nv_bfloat16, 128>)
-                                        : reinterpret_cast<const void*>(&paged_wide_kernel<__half, 128>))
-                                  : (bf ? reinterpret_cast<const void*>(&paged_wide_kernel<__nv_bfloat16, 64>)
-                                        : reinterpret_cast<const void*>(&paged_wide_kernel<__half, 64>));
+    const void* fn = w.prefix_pass ? wide_kernel<true>(kv->dtype, kv->D) : wide_kernel<false>(kv->dtype, kv->D);
     const uint32_t smem = kv->D == 128 ? WideSmem<128>::kTotal : WideSmem<64>::kTotal;
     rc = ensure_smem_attr(fn, smem);
     if (rc) return rc;

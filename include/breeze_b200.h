@@ -342,9 +342,11 @@ int32_t bq_paged_append(const bq_paged_append_desc* desc, void* stream);
  * kv head h / (HQ / HKV). fp32 softmax statistics and accumulation; lse, when
  * given, is the natural logarithm of each row's sum of exponentials.
  * prefix_len > 0: the first prefix_len positions (a multiple of page_size) are
- * the same pages in every row of the table and are read once for the whole
- * batch, through row 0, where that pays (else each sequence reads them);
- * the value is the same. */
+ * the same pages in every sequence that has new rows, as far as it goes, and are
+ * read once for the whole batch, through the table row of the longest of them,
+ * where that pays (else each sequence reads them); the value is the same. The
+ * entries of an unused slot, or behind a sequence's end, may hold anything here
+ * too. */
 #define BQ_PAGED_FULL 2u  /* every new row sees all of its sequence */
 #define BQ_PAGED_SHARE 4u /* the prefix gets its one pass even where that does not pay (for comparisons) */
 

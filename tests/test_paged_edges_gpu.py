@@ -45,3 +45,30 @@ def test_a_prefix_value_reaches_only_the_rows_that_see_it(lens, new, prefix, hq,
         inf = torch.isinf(ref["out"])
         assert torch.equal(o[inf], ref["out"][inf])
         assert ((lse.double() - ref["lse"]).abs() <= ltol).all()
+
+
+@pytest.mark.parametrize("hole", [2 ** 30, -1])
+@pytest.mark.parametrize("lens,new,prefix,hq,hkv,dim,page,dtype", [
+    ([0, 300, 290, 257], None, 256, 8, 2, 64, 16, F16),           # slot 0 is unused
+    ([0, 0, 1100, 1024, 1300], None, 1024, 32, 8, 128, 64, BF),
+    ([100, 256, 300], None, 256, 8, 2, 128, 32, BF),              # slot 0 ends in the prefix
+    ([0, 700, 600], [0, 150, 33], 448, 4, 2, 64, 64, F16),        # no new rows in slot 0
+    ([200, 260, 258], [90, 30, 1], 256, 4, 2, 128, 64, BF),
+    ([40, 90, 33], None, 128, 4, 2, 128, 16, BF),                 # nobody reaches the prefix's end
+    ([0, 0], None, 64, 4, 2, 64, 16, BF),                         # nobody at all
+])
+def test_unused_slots_need_no_prefix_pages(lens, new, prefix, hq, hkv, dim, page, dtype, hole):
+    c = pc.batch(lens, new, hq, hkv, dim, page, dtype, seed=len(lens) + prefix, prefix=prefix)
+    for b, n in enumerate(lens):
+        c["table"][b, -(-n // page):] = hole
+    if new is not None and new[0] == 0:  # nor does a sequence without new rows, whatever its length says
+        c["table"][0, :] = hole
+        c["lens"][0] = 10 ** 6 if hole < 0 else 2
+        lens = c["lens"].tolist()
+    out, lse = run(c, always=True)
+    if new is not None and new[0] == 0 and hole < 0:
+        from breeze_b200 import _lib
+
+        assert _status() == _lib.BQ_DEVERR_POSITION
+    compare(c, out, lse)
+    compare(c, *run(dict(c, lens=c["lens"].clamp(max=c["table"].shape[1] * page)), always=False))
