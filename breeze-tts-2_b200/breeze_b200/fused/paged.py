@@ -232,7 +232,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """q (T, HQ D) of the new tokens (already in the cache: paged_append first)
     -> (T, HQ D). Row i of the n new rows of sequence b sees positions
     [0, seq_lens[b] - n + i + 1); with ``causal=False`` all seq_lens[b]. A row
-    that sees none gets zeros; infinite or NaN keys and values at positions it does
+    that sees none gets zeros, one whose scores are all -inf gets NaN; infinite or NaN keys and values at positions it does
     not see stay without effect. Query head h reads kv head h // (HQ / HKV).
     ``scale`` defaults to D^-0.5. ``max_q``: most new tokens of one sequence, a
     hint that picks the kernel (default: T / B rounded up). ``lse`` (T, HQ) fp32

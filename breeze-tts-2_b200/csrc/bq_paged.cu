@@ -158,7 +158,7 @@ struct JoinRow {
         for (int e = 0; e < DPL; ++e) acc[e] = 0.f;
     }
     __device__ __forceinline__ void add(float m2, float l2, const float (&o)[DPL]) {
-        if (l2 == 0.f) return;  // saw nothing (its outputs are zeros, or zeros times what it did not see)
+        if (l2 == 0.f && m2 == -INFINITY) return;  // saw nothing (its outputs are zeros, or zeros times what it did not see)
         const float nm = fmaxf(m, m2), u = nm == -INFINITY ? 0.f : nm, f = ex2(m - u), g = ex2(m2 - u);
         m = nm;
         l = l * f + l2 * g;
@@ -236,7 +236,7 @@ __device__ __forceinline__ void join_rows(const PagedJoin& p, const RowParts (&p
         if (r >= rows) break;
         int t, h;
         place(r, t, h);
-        const float l = row[r].l, inv = l != 0.f ? 1.f / l : 0.f;
+        const float l = row[r].l, inv = paged_inverse(row[r].m, l);
         const float (&acc)[DPL] = row[r].acc;
         E* dst = static_cast<E*>(p.out) + int64_t(t) * p.ldo + h * D + lane * DPL;
         if constexpr (DPL == 4)

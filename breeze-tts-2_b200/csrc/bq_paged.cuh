@@ -118,6 +118,12 @@ struct PagedWork {
     int2* row_at;      // [T][HQ] where the row's parts are (paged_row_at)
 };
 
+// A part of a row is its largest score m, its sum of exponentials l and its unnormalized outputs. A part that saw no
+// position has m = -inf, l = 0; one that saw nothing but scores of -inf has m = kLowest, l = 0. A row of which no part
+// saw any position is zeros, a row of which all scores are -inf is 0 / 0.
+constexpr float kLowest = -3.402823466e38f;
+__device__ __forceinline__ float paged_inverse(float m, float l) { return l != 0.f || m != -INFINITY ? 1.f / l : 0.f; }
+
 // Where a row's parts of one pass are: x = CTA of the first, y = parts << 8 | row
 // within the tile; no parts: in the row buffers.
 __device__ __forceinline__ int2 paged_row_at(int cta, int parts, int row) { return make_int2(cta, parts << 8 | row); }

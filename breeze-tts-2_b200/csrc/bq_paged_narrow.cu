@@ -302,6 +302,7 @@ __device__ __forceinline__ void narrow_tile(const PagedWork& p, const NarrowTile
             ll = fmaf(f, s_ml[w][r].y, ll);
             a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
         }
+        if (ll == 0.f && min(s_lim[r], p1) > p0) mm = kLowest;  // no score but -inf
         emit(r, d, mm, ll, a);
     }
     __syncthreads();  // the rings are free again
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
             const int rr = t.r0 + r, tok = p.by_G(rr), head = c.j * p.G + rr - tok * p.G;
             const int64_t row = t.s.begin + tok;
             if (whole && !p.row_o) {
-                const float inv = ll != 0.f ? 1.f / ll : 0.f;
+                const float inv = paged_inverse(mm, ll);
                 *reinterpret_cast<uint2*>(static_cast<E*>(p.out) + row * p.ldo + head * D + d) =
                     pack4<E>(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
                 if (p.lse && d == 0) p.lse[row * p.ldl + head] = ll != 0.f ? (mm + log2f(ll)) * kLn2 : -INFINITY;
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_cluster_kernel(const __grid
             }
             const int rr = t.r0 + r, tok = p.by_G(rr), head = t.j * p.G + rr - tok * p.G;
             const int64_t row = t.s.begin + tok;
-            const float inv = ll != 0.f ? 1.f / ll : 0.f;
+            const float inv = paged_inverse(mm, ll);
             *reinterpret_cast<uint2*>(static_cast<E*>(p.out) + row * p.ldo + head * D + d) =
                 pack4<E>(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
             if (p.lse && d == 0) p.lse[row * p.ldl + head] = ll != 0.f ? (mm + log2f(ll)) * kLn2 : -INFINITY;

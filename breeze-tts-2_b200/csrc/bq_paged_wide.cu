@@ -539,7 +539,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                 const int64_t orow = t.s.begin + tok;
                 const int64_t at = whole ? orow * kv.HQ + head
                                          : int64_t(2 * blockIdx.x + (t.k0 == 0 ? 1 : 0)) * kRows + 128 * h + row;
-                const float inv = l != 0.f ? 1.f / l : 0.f;
+                if (l == 0.f && min(limit, p1) > p0) mref = kLowest;  // no score but -inf
+                const float inv = paged_inverse(mref, l);
 #pragma unroll
                 for (int q = 0; q < D / 32; ++q) {
                     float o[32];

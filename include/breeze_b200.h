@@ -338,7 +338,8 @@ int32_t bq_paged_append(const bq_paged_append_desc* desc, void* stream);
 /* out = softmax(scale * q k^T) v over each sequence's paged cache, the new
  * tokens included (append them first): row i of the n new rows of sequence b
  * sees positions [0, seq_lens[b] - n + i + 1), or all seq_lens[b] with
- * BQ_PAGED_FULL. A row that sees none gets zeros (lse -inf). Query head h reads
+ * BQ_PAGED_FULL. A row that sees none gets zeros (lse -inf), one that sees only
+ * scores of -inf gets NaN (lse -inf). Query head h reads
  * kv head h / (HQ / HKV). fp32 softmax statistics and accumulation; lse, when
  * given, is the natural logarithm of each row's sum of exponentials.
  * prefix_len > 0: the first prefix_len positions (a multiple of page_size) are

@@ -8,7 +8,7 @@ import torch
 
 from oracle import paged as op
 from tests import paged_cases as pc
-from tests.test_paged_gpu import _clean_status, _status, compare, run  # noqa: F401 - fixtures
+from tests.test_paged_gpu import _clean_status, _status, compare, run, table_room  # noqa: F401 - fixtures
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -72,3 +72,48 @@ def test_unused_slots_need_no_prefix_pages(lens, new, prefix, hq, hkv, dim, page
         assert _status() == _lib.BQ_DEVERR_POSITION
     compare(c, out, lse)
     compare(c, *run(dict(c, lens=c["lens"].clamp(max=c["table"].shape[1] * page)), always=False))
+
+
+MINUS = [
+    # lens, new, prefix, hq, hkv, dim, page, dtype
+    ([300, 90], None, 0, 4, 2, 128, 32, BF),
+    ([2000, 5], None, 0, 2, 1, 64, 16, F16),
+    ([900, 333], [40, 30], 0, 4, 2, 128, 32, BF),
+    ([4000], [300], 0, 2, 1, 64, 64, F16),
+    ([300, 280], [4, 9], 256, 4, 2, 128, 16, BF),
+    ([700, 600], [150, 33], 448, 4, 2, 64, 64, F16),
+    ([700, 690], None, 640, 2, 2, 128, 64, BF),
+]
+
+
+@pytest.mark.parametrize("lens,new,prefix,hq,hkv,dim,page,dtype", MINUS)
+@pytest.mark.parametrize("single", [True, False])
+def test_scores_of_minus_infinity(lens, new, prefix, hq, hkv, dim, page, dtype, single, table_room):  # noqa: F811
+    """All of a row's scores -inf: the softmax is 0 / 0, the row NaN, its lse -inf
+    (the logarithm of 0). With one finite score among them (``single``: the rows
+    that see position lens[0] / 2 of sequence 0) the row is that v."""
+    c = table_room(pc.batch(lens, new, hq, hkv, dim, page, dtype, seed=53, prefix=prefix))
+    table, ls, starts = pc.lists(c)
+    c["k"][..., 7] = -INF  # everywhere, but at one position
+    alone = lens[0] // 2
+    if single:
+        c["k"][table[0][alone // page], :, alone % page] = 0.5
+    c["q"].view(-1, hq, dim)[..., 7] = 1.0
+    q = c["q"].view(-1, hq, dim)
+    q[0, 0, 7] = 0.0  # 0 * -inf: NaN scores
+    ref = op.attention(c["q"], c["k"], c["v"], table, ls, starts)
+    out, lse = run(c)
+    o = out.double().reshape(c["rows"], hq, dim)
+    first = torch.zeros(c["rows"], hq, dtype=torch.bool)
+    first[0, 0] = True
+    assert torch.equal(torch.isnan(o), torch.isnan(ref["out"]))
+    assert torch.equal(torch.isnan(lse), first)
+    none = torch.isinf(ref["lse"])
+    assert (none.any() or single) and torch.equal(lse[none], ref["lse"][none].float())
+    rest = torch.isfinite(ref["lse"])
+    if rest.any():  # one position takes all: v itself, within the output's rounding
+        u = torch.finfo(dtype).eps / 2
+        assert ((o - ref["out"]).abs() <= u * ref["out"].abs() + 2.0 ** -22)[rest].all()
+        # |score| <= sum |q k| terms of which each of D + 8 roundings takes 2^-23
+        bound = (dim + 8) * 2.0 ** -23 * (c["q"].double().abs().sum(-1).max() / 2 + 1)
+        assert ((lse.double() - ref["lse"]).abs()[rest] <= bound).all()
