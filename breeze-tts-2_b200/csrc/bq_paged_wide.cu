@@ -478,6 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_wide_kernel(const __grid_co
                     const bool move = m > mref + 8.f;  // also the first finite maximum
                     again = __any_sync(0xffffffffu, move);
                     if (again) {
+                        tmem_wait_st();  // the probabilities are about to be written again, and stores have no order of their own
                         const float f = move ? ex2(mref - m) : 1.f;
                         mref = move ? m : mref;
                         l *= f;

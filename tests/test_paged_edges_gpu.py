@@ -117,3 +117,16 @@ def test_scores_of_minus_infinity(lens, new, prefix, hq, hkv, dim, page, dtype, 
         # |score| <= sum |q k| terms of which each of D + 8 roundings takes 2^-23
         bound = (dim + 8) * 2.0 ** -23 * (c["q"].double().abs().sum(-1).max() / 2 + 1)
         assert ((lse.double() - ref["lse"]).abs()[rest] <= bound).all()
+
+
+def test_a_maximum_that_moves_at_every_unit():
+    """In the kernel for many rows each unit's probabilities are then written twice; repeated."""
+    c = pc.batch([1900], [260], 2, 1, 128, 64, BF, seed=9)
+    c["q"][:] = 1.0
+    for p in range(1900):
+        c["k"][c["table"][0, p // 64], :, p % 64] = p / 64
+    first = run(c)
+    compare(c, *first)
+    for _ in range(50):
+        again = run(c)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
