@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_cluster_kernel(const __grid
             *reinterpret_cast<float4*>(out + r * D + d) = a;
             if (d == 0) s_row[r] = make_float2(mm, ll);
         });
+        __syncwarp();        // (the barriers below want whole warps)
         cluster_sync_all();  // every rank's rows are in its shared memory
         for (int idx = rank * kThreads + threadIdx.x; idx < t.nrows * (D / 4); idx += ranks * kThreads) {
             const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
@@ -431,8 +432,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_cluster_kernel(const __grid
                 pack4<E>(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
             if (p.lse && d == 0) p.lse[row * p.ldl + head] = ll != 0.f ? (mm + log2f(ll)) * kLn2 : -INFINITY;
         }
-        cluster_sync_relaxed();  // rows are not written over, nor does a rank leave, while another reads them (the reads
-                                 // were consumed by the stores)
+        __syncwarp();
+        if ((i + 1) * kNarrowRows < t.s.rows)
+            cluster_sync_all();  // the next tile's rows are written after every rank has read these
+        else
+            cluster_sync_relaxed();  // no rank leaves while another reads its rows (the reads were consumed by the stores)
     }
 }
 

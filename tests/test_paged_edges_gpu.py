@@ -119,6 +119,18 @@ def test_scores_of_minus_infinity(lens, new, prefix, hq, hkv, dim, page, dtype, 
         assert ((lse.double() - ref["lse"]).abs()[rest] <= bound).all()
 
 
+@pytest.mark.parametrize("dim,hq", [(64, 3), (64, 5), (128, 7)])
+def test_several_tiles_of_a_cluster(dim, hq):
+    """max_q told too low: a cluster walks many tiles of odd heights; repeated, since
+    a tile written too early is a matter of time."""
+    c = pc.batch([300, 77], [61, 33], hq, 1, dim, 32, BF, seed=33, spare_cols=0)
+    first = run(c, max_q=1)
+    compare(c, *first)
+    for _ in range(50):
+        again = run(c, max_q=1)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 def test_a_maximum_that_moves_at_every_unit():
     """In the kernel for many rows each unit's probabilities are then written twice; repeated."""
     c = pc.batch([1900], [260], 2, 1, 128, 64, BF, seed=9)
