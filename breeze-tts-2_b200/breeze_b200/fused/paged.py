@@ -71,9 +71,9 @@ def _native():
 
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
-    """Row stride of a 2-D tensor with contiguous rows."""
+    """Row stride of a 2-D tensor with contiguous rows (a dimension of size one has no stride)."""
     st = t.stride()
-    if len(st) != 2 or st[1] != 1:
+    if len(st) != 2 or (st[1] != 1 and t.shape[1] != 1):
         raise ValueError(f"{name} must be a 2-D tensor with unit stride in the last dimension")
     return st[0] if t.shape[0] > 1 else t.shape[1]
 
@@ -97,10 +97,10 @@ def _cache_fields(dev: int, dtype: torch.dtype, rows: int, k_pages, v_pages, pag
     ts = page_table.stride()
     if k3 != 1 or v3 != 1:
         raise ValueError("the last dimension of the pages must be contiguous")
-    if page_table.dtype != _I32 or len(ts) != 2 or ts[1] != 1:
+    if page_table.dtype != _I32 or len(ts) != 2 or (ts[1] != 1 and page_table.shape[1] != 1):
         raise ValueError("page_table must be int32 (B, columns) with contiguous rows")
     batch, columns = page_table.shape
-    if seq_lens.dtype != _I32 or seq_lens.shape != (batch,) or seq_lens.stride() != _UNIT:
+    if seq_lens.dtype != _I32 or seq_lens.shape != (batch,) or (seq_lens.stride() != _UNIT and batch != 1):
         raise ValueError("seq_lens must be a contiguous int32 (B,)")
     if q_starts is None:
         if rows != batch:

@@ -54,13 +54,13 @@ float real(PyObject* o) {
     return float(v);
 }
 bool on(const at::Tensor& t, int dev) { return t.is_cuda() && t.get_device() == dev; }
-// Row stride of a 2-D tensor with contiguous rows.
+// Row stride of a 2-D tensor with contiguous rows (a dimension of size one has no stride).
 int64_t row_stride(const at::Tensor& t) {
-    need(t.dim() == 2 && t.stride(1) == 1);
+    need(t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1));
     return t.size(0) > 1 ? t.stride(0) : t.size(1);
 }
 bool vector(const at::Tensor& t, at::ScalarType type, int64_t n, int dev) {
-    return t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.stride(0) == 1 && on(t, dev);
+    return t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && (t.stride(0) == 1 || n == 1) && on(t, dev);
 }
 
 // The cache part of both descriptors. rows: new tokens, of dtype `type`.
@@ -73,7 +73,7 @@ int fill(bq_paged_kv* kv, const at::Tensor& rows, PyObject* k_, PyObject* v_, Py
     need(type == at::kBFloat16 || type == at::kHalf);
     need(on(k, dev) && on(v, dev) && on(table, dev) && k.scalar_type() == type && v.scalar_type() == type);
     need(k.dim() == 4 && v.sizes() == k.sizes() && k.stride(3) == 1 && v.stride(3) == 1 && k.numel() > 0);
-    need(table.scalar_type() == at::kInt && table.dim() == 2 && table.stride(1) == 1 && table.numel() > 0);
+    need(table.scalar_type() == at::kInt && table.dim() == 2 && (table.stride(1) == 1 || table.size(1) == 1) && table.numel() > 0);
     const int64_t batch = table.size(0);
     need(vector(lens, at::kInt, batch, dev));
     kv->B = i32(batch);

@@ -31,7 +31,9 @@ int paged_validate(const bq_paged_kv* kv, int T, int HQ) {
         return set_error(BQ_ERR_SHAPE, "%d rows for %d sequences: ragged rows need q_starts", T, kv->B);
     if (kv->ld_table < kv->max_pages)
         return set_error(BQ_ERR_SHAPE, "page table stride %lld < %d columns", (long long)kv->ld_table, kv->max_pages);
+    const int size[3] = {kv->num_pages, kv->HKV, kv->page_size};
     for (int i = 0; i < 3; ++i) {
+        if (size[i] == 1) continue;  // its stride is never taken
         if (kv->k_stride[i] < kv->D || kv->v_stride[i] < kv->D)
             return set_error(BQ_ERR_SHAPE, "page strides must be at least the head dim");
         if (kv->k_stride[i] % 8 || kv->v_stride[i] % 8) return set_error(BQ_ERR_ALIGN, "page strides must be multiples of 8");

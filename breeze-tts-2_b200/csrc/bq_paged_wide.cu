@@ -789,7 +789,7 @@ int encode_pages(const bq_paged_kv* kv, const void* base, const int64_t* st, int
     const cuuint32_t es[4] = {1, 1, 1, 1};
     for (int i = 0; i < 3; ++i) {
         dims[i + 1] = cuuint64_t(d[i].size);
-        strides[i] = cuuint64_t(d[i].stride) * 2;
+        strides[i] = cuuint64_t(d[i].size == 1 ? kv->D : d[i].stride) * 2;  // of one element: any that the encoder takes
         boxes[i + 1] = d[i].what == 2 ? cuuint32_t(box) : 1u;
         if (d[i].what == 2) *slot = i + 1;
         if (d[i].what == 1) *head = i + 1;

@@ -299,7 +299,8 @@ typedef struct bq_paged_kv {
     int32_t dtype;         /* BQ_DT_BF16 or BQ_DT_F16: pages, q / k / v rows, outputs */
     int32_t reserved;
     void* k_pages;         /* element strides of a page, a kv head and a slot; the D elements of a */
-    int64_t k_stride[3];   /* slot are contiguous; bases 16-byte aligned, strides multiples of 8   */
+    int64_t k_stride[3];   /* slot are contiguous; bases 16-byte aligned, strides multiples of 8 (of
+                              one page or one kv head: any) */
     void* v_pages;
     int64_t v_stride[3];
     const int32_t* page_table; /* [B, ld_table] */

@@ -119,6 +119,31 @@ def test_scores_of_minus_infinity(lens, new, prefix, hq, hkv, dim, page, dtype, 
         assert ((lse.double() - ref["lse"]).abs()[rest] <= bound).all()
 
 
+@pytest.mark.parametrize("new", [None, [70, 3]])
+@pytest.mark.parametrize("stride", [0, 1, 4, 2 ** 41])
+def test_strides_of_dimensions_of_size_one(new, stride):
+    """One kv head, one page, one sequence, one query head: what their strides say does not matter."""
+    from breeze_b200.fused import paged
+
+    c = pc.batch([200, 131], new, 4, 1, 128, 64, BF, seed=2)
+    same = lambda t, dims: t.as_strided(t.shape, [stride if i in dims else s for i, s in enumerate(t.stride())])  # noqa: E731
+    d = pc.to(c, DEV)
+    lse = torch.empty(c["rows"], 4, device=DEV)
+    out = paged.paged_attention(d["q"], same(d["k"], [1]), same(d["v"], [1]), d["table"], d["lens"], q_starts=d["starts"], lse=lse)
+    torch.cuda.synchronize()
+    compare(c, out.cpu(), lse.cpu())
+    rows = 1 if new is None else 70
+    c = pc.batch([50], None if new is None else [50], 1, 1, 64, 64, BF, seed=2, spare_cols=0)
+    c["k"], c["v"], c["table"] = c["k"][int(c["table"][0, 0])][None], c["v"][int(c["table"][0, 0])][None], torch.zeros(1, 1, dtype=torch.int32)
+    d = pc.to(c, DEV)
+    rows = c["rows"]
+    lse = torch.empty(rows, 1, device=DEV)
+    out = paged.paged_attention(same(d["q"], [0] if rows == 1 else []), same(d["k"], [0, 1]), same(d["v"], [0, 1]), same(d["table"], [0, 1]),
+                                same(d["lens"], [0]), q_starts=d["starts"], lse=same(lse, [1] if rows > 1 else [0, 1]))
+    torch.cuda.synchronize()
+    compare(c, out.cpu(), lse.cpu())
+
+
 @pytest.mark.parametrize("dim,hq", [(64, 3), (64, 5), (128, 7)])
 def test_several_tiles_of_a_cluster(dim, hq):
     """max_q told too low: a cluster walks many tiles of odd heights; repeated, since
