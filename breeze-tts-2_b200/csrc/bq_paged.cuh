@@ -156,7 +156,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedWork& p, const PagedPre
     } else {
         paged_rows(p.kv, b, s.begin, s.count);
         s.len = max(paged_len(p.kv, b, cut), 0);
-        s.off = p.kv.lens[b] - s.count;
+        s.off = max(p.kv.lens[b], 0) - s.count;
     }
     s.rows = s.count * p.G;
     return s;
@@ -391,7 +391,7 @@ __device__ __forceinline__ int paged_row_limit(const PagedWork& p, const PagedSe
     paged_rows(p.kv, b, begin, count);
     bool cut;
     const int len = max(paged_len(p.kv, b, cut), 0);
-    const int lim = p.causal ? min(len, p.kv.lens[b] - count + (tok - begin) + 1) : len;
+    const int lim = p.causal ? min(len, max(p.kv.lens[b], 0) - count + (tok - begin) + 1) : len;
     return max(0, min(lim, p.prefix_len));
 }
 

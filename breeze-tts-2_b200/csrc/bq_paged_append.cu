@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
         if (threadIdx.x == 0) s_seq = -1;
         __syncthreads();
         for (int i = threadIdx.x; i < kv.B; i += kAppendThreads) {
-            const int begin = kv.starts[i], end = kv.starts[i + 1], len = kv.lens[i];
+            const int begin = kv.starts[i], end = kv.starts[i + 1], len = max(kv.lens[i], 0);
             if (t >= begin && t < end) {
                 s_seq = i;
                 s_pos = len - (min(end, kv.T) - max(begin, 0)) + (t - max(begin, 0));
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
         if (b < 0) return;  // a row of no sequence
         pos = s_pos;
     } else {
-        pos = kv.lens[b] - 1;
+        pos = max(kv.lens[b], 0) - 1;
     }
     if (pos < 0) return;  // an unused batch slot
     bool ok = pos < p.rope_rows && (pos >> kv.page_shift) < kv.max_pages;

@@ -144,6 +144,23 @@ def test_strides_of_dimensions_of_size_one(new, stride):
     compare(c, out.cpu(), lse.cpu())
 
 
+def test_a_length_far_below_zero_is_an_unused_slot():
+    from breeze_b200.fused import paged
+
+    for new in (None, [3, 2]):
+        c = pc.batch([5, 20], new, 2, 1, 64, 16, BF, seed=1)
+        c["lens"][0] = -2 ** 31
+        d = pc.to(c, DEV)
+        rows = c["rows"]
+        qkv = torch.randn(rows, 4 * 64, generator=torch.Generator().manual_seed(12)).to(BF).to(DEV)
+        table = torch.ones(64, 64, device=DEV)
+        out = torch.full((rows, 128), 300.0, dtype=BF, device=DEV)
+        paged.paged_append(qkv, table, table, d["k"], d["v"], d["table"], d["lens"], q_starts=d["starts"], out=out)
+        torch.cuda.synchronize()
+        dead = rows - (1 if new is None else 2)
+        assert (out[:dead] == 300.0).all() and not (out[dead:] == 300.0).any(-1).any()
+
+
 @pytest.mark.parametrize("dim,hq", [(64, 3), (64, 5), (128, 7)])
 def test_several_tiles_of_a_cluster(dim, hq):
     """max_q told too low: a cluster walks many tiles of odd heights; repeated, since
