@@ -2,6 +2,7 @@
 // bq_paged_attention (attention of the new tokens of a ragged batch over
 // their paged caches).
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 
 #include "bq_host.h"
@@ -104,6 +105,7 @@ int paged_launch(const void* fn, dim3 grid, dim3 block, uint32_t smem, void** ar
 namespace {
 
 constexpr int kJoinWarps = 8;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // One pass's parts, as the joining kernel reads them.
 struct PagedParts {
@@ -442,7 +444,8 @@ int validate_attention(const bq_paged_attn_desc* d) {
     if (d->lse && d->ldl < d->HQ) return set_error(BQ_ERR_SHAPE, "lse row stride %lld < %d", (long long)d->ldl, d->HQ);
     if (!paged_aligned(d->q, d->ldq, 2) || !paged_aligned(d->out, d->ldo, 2))
         return set_error(BQ_ERR_ALIGN, "q and out rows must be 16-byte aligned");
-    if (!(d->scale > 0.f) || d->scale > 3.0e38f) return set_error(BQ_ERR_INVALID_ARG, "scale must be positive and finite");
+    if (!(d->scale > 0.f) || !std::isfinite(d->scale * kLog2e))  // the kernels' factor: scores are kept in base 2
+        return set_error(BQ_ERR_INVALID_ARG, "scale must be positive and finite (times log2(e), too)");
     if (d->prefix_len < 0 || d->prefix_len % d->kv.page_size)
         return set_error(BQ_ERR_SHAPE, "prefix_len=%d must be a multiple of the page size %d", d->prefix_len,
                          d->kv.page_size);
@@ -490,7 +493,7 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
     w.by_G.set(uint32_t(w.G));
     w.causal = (d->flags & BQ_PAGED_FULL) ? 0 : 1;
     w.prefix_len = pl.prefix;
-    w.scale_log2 = d->scale * 1.4426950408889634f;
+    w.scale_log2 = d->scale * kLog2e;
     w.q = d->q;
     w.ldq = d->ldq;
     w.out = d->out;

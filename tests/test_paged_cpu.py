@@ -183,3 +183,10 @@ def test_registers_move_by_one_instruction_per_warpgroup():
         text = src.read_text()
         for kind in ("inc", "dec"):
             assert len(re.findall(rf'"setmaxnreg\.{kind}\.', text)) <= 1, (src.name, kind)
+
+
+def test_a_scale_that_is_infinite_in_base_2_is_refused(lib):
+    n = ctypes.c_size_t(0)
+    for scale in (2.4e38, 2.9e38, 3.4e38):  # finite, but not times log2(e) = 1.44
+        assert lib.bq_paged_attention_workspace_bytes(ctypes.byref(attn(scale=scale)), ctypes.byref(n)) == L.BQ_ERR_INVALID_ARG
+        assert "scale" in L.last_error()
