@@ -38,6 +38,8 @@ captured from them, share none.
 from __future__ import annotations
 
 import ctypes
+import math
+import operator
 
 import torch
 
@@ -68,6 +70,21 @@ def _native():
             lib.bq_paged_append, lib.bq_paged_attention, lib.bq_paged_attention_workspace_bytes)))
         _bound = _paged_bind
     return _bound
+
+
+def _count(value, name: str) -> int:
+    """A number of positions or rows, as the descriptors hold it."""
+    n = operator.index(value)
+    if not 0 <= n < 2 ** 31:
+        raise ValueError(f"{name} must be from 0 to 2^31 - 1 (got {n})")
+    return n
+
+
+def _real(value, name: str) -> float:
+    """A number that fp32 can hold."""
+    if not math.isfinite(value) or abs(value) >= 3.4e38:
+        raise ValueError(f"{name} must be finite in fp32 (got {value})")
+    return value
 
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
@@ -176,7 +193,7 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_page
         raise ValueError("out must be (T, HQ D) of the cache's dtype and device")
     else:
         ldq = _row_stride(out, "out")
-    desc = _pack_append(*fields, rows, hq, _lib._DT[cs_dtype], cs_shape[0], eps, _lib.default_flags(), qkv.data_ptr(), ldqkv,
+    desc = _pack_append(*fields, rows, hq, _lib._DT[cs_dtype], cs_shape[0], _real(eps, "eps"), _lib.default_flags(), qkv.data_ptr(), ldqkv,
                         cos.data_ptr(), sin.data_ptr(), ldcs, qn, kn, out.data_ptr(), ldq)
     _launch(dev, "bq_paged_append", _lib.load().bq_paged_append, desc)
     return out
@@ -214,9 +231,10 @@ def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, 
         if lse.shape != (rows, hq) or lse.dtype != _F32 or lse.get_device() != dev:
             raise ValueError("lse must be fp32 (T, HQ) on q's device")
         lse_ptr, ldl = lse.data_ptr(), _row_stride(lse, "lse")
-    max_q = 0 if max_q is None else max_q
-    desc = _pack_attn(*fields, rows, hq, prefix_len, max_q, dim ** -0.5 if scale is None else scale,
-                      flags, q.data_ptr(), ldq, out.data_ptr(), ldo, lse_ptr, ldl)
+    max_q = 0 if max_q is None else _count(max_q, "max_q")
+    scale = dim ** -0.5 if scale is None else _real(scale, "scale")
+    desc = _pack_attn(*fields, rows, hq, _count(prefix_len, "prefix_len"), max_q, scale, flags, q.data_ptr(),
+                      ldq, out.data_ptr(), ldo, lse_ptr, ldl)
     size = ctypes.c_size_t(0)
     _launch(dev, "bq_paged_attention_workspace_bytes", _workspace_bytes, desc, ctypes.byref(size))
     need = size.value

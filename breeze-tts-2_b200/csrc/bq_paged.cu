@@ -446,6 +446,7 @@ int validate_attention(const bq_paged_attn_desc* d) {
         return set_error(BQ_ERR_ALIGN, "q and out rows must be 16-byte aligned");
     if (!(d->scale > 0.f) || !std::isfinite(d->scale * kLog2e))  // the kernels' factor: scores are kept in base 2
         return set_error(BQ_ERR_INVALID_ARG, "scale must be positive and finite (times log2(e), too)");
+    if (d->max_q < 0) return set_error(BQ_ERR_INVALID_ARG, "max_q=%d is negative", d->max_q);
     if (d->prefix_len < 0 || d->prefix_len % d->kv.page_size)
         return set_error(BQ_ERR_SHAPE, "prefix_len=%d must be a multiple of the page size %d", d->prefix_len,
                          d->kv.page_size);

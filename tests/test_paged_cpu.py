@@ -190,3 +190,9 @@ def test_a_scale_that_is_infinite_in_base_2_is_refused(lib):
     for scale in (2.4e38, 2.9e38, 3.4e38):  # finite, but not times log2(e) = 1.44
         assert lib.bq_paged_attention_workspace_bytes(ctypes.byref(attn(scale=scale)), ctypes.byref(n)) == L.BQ_ERR_INVALID_ARG
         assert "scale" in L.last_error()
+
+
+def test_a_negative_hint_is_refused(lib):
+    n = ctypes.c_size_t(0)
+    assert lib.bq_paged_attention_workspace_bytes(ctypes.byref(attn(max_q=-1)), ctypes.byref(n)) == L.BQ_ERR_INVALID_ARG
+    assert "max_q" in L.last_error()

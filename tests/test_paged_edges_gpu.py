@@ -184,3 +184,74 @@ def test_a_maximum_that_moves_at_every_unit():
     for _ in range(50):
         again = run(c)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+class _Aside:
+    """Stands in for the compiled calls: leaves every call to Python."""
+
+    @staticmethod
+    def append(*args):
+        return None
+
+    attention = append
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_compiled_calls_and_python_refuse_the_same(compiled, monkeypatch):
+    """Whichever checks a call, what may not run is refused, by the same kind of error."""
+    from breeze_b200.fused import paged
+
+    paged._native()
+    if not compiled:
+        monkeypatch.setattr(paged, "_bound", _Aside)
+    c = pc.to(pc.batch([40, 20], None, 4, 2, 64, 16, BF, seed=1), DEV)
+    q, k, v, table, lens = (c[n] for n in ("q", "k", "v", "table", "lens"))
+    cs = torch.ones(64, 64, dtype=BF, device=DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    rows = torch.zeros(2, 8 * 64, dtype=BF, device=DEV)
+    shared = [
+        (dict(k_pages=k.half()), ValueError), (dict(v_pages=v.float()), ValueError), (dict(k_pages=k[0]), ValueError),
+        (dict(v_pages=v[:, :1]), ValueError), (dict(k_pages=k.transpose(2, 3)), ValueError),
+        (dict(k_pages=k[..., :32], v_pages=v[..., :32]), ValueError), (dict(k_pages=k[:, :, :8], v_pages=v[:, :, :8]), ValueError),
+        (dict(k_pages=k[:0], v_pages=v[:0]), ValueError), (dict(k_pages=k.expand(2, *k.shape)[0][:1].expand(k.shape)), ValueError),
+        (dict(k_pages=k.view(-1)[4:][:k[1:].numel()].view_as(k[1:]), v_pages=v[1:]), ValueError),  # 8-byte aligned
+        (dict(page_table=table.long()), ValueError), (dict(page_table=table[0]), ValueError),
+        (dict(page_table=table.repeat(1, 2)[:, ::2]), ValueError), (dict(page_table=table[:, :0]), ValueError),
+        (dict(page_table=table[:1].expand(2, -1)), ValueError), (dict(seq_lens=lens.long()), ValueError),
+        (dict(seq_lens=lens[:1]), ValueError), (dict(seq_lens=lens.repeat(2)[::2]), ValueError),
+        (dict(seq_lens=lens.cpu()), RuntimeError), (dict(page_table=table.cpu()), RuntimeError),
+        (dict(k_pages=k.cpu(), v_pages=v.cpu()), RuntimeError), (dict(q_starts=torch.zeros(2, **i32)), ValueError),
+        (dict(q_starts=torch.zeros(3, device=DEV)), ValueError), (dict(q_starts=torch.zeros(3, dtype=torch.int32)), RuntimeError),
+    ]
+    attention = shared + [
+        (dict(q=q.float()), ValueError), (dict(q=q[0]), ValueError), (dict(q=q[:, ::2]), ValueError), (dict(q=q[:1]), ValueError),
+        (dict(q=q[:, :192]), ValueError), (dict(q=q[:, :100]), ValueError), (dict(q=q.cpu()), RuntimeError),
+        (dict(q=q[:1].expand(2, -1)), ValueError), (dict(out=q.float()), ValueError), (dict(out=q[:, :128]), ValueError),
+        (dict(out=q.cpu()), ValueError), (dict(out=torch.empty_like(q[:1]).expand(2, -1)), ValueError),
+        (dict(lse=torch.empty(2, 4, dtype=BF, device=DEV)), ValueError), (dict(lse=torch.empty(2, 4)), ValueError),
+        (dict(lse=torch.empty(4, 2, device=DEV).t()), ValueError), (dict(lse=torch.empty(2, 3, device=DEV)), ValueError),
+        (dict(scale=0.0), ValueError), (dict(scale=-1.0), ValueError), (dict(scale=float("nan")), ValueError),
+        (dict(scale=float("inf")), ValueError), (dict(scale=1e39), ValueError), (dict(scale=3e38), ValueError),
+        (dict(scale="1"), TypeError), (dict(max_q=-1), ValueError), (dict(max_q=2 ** 31), ValueError),
+        (dict(max_q=2 ** 70), ValueError), (dict(max_q=1.5), TypeError), (dict(prefix_len=17), ValueError),
+        (dict(prefix_len=-16), ValueError), (dict(prefix_len=2 ** 31), ValueError), (dict(prefix_len=2 ** 70), ValueError),
+        (dict(prefix_len=16.0), TypeError), (dict(prefix_len=16 * 100), ValueError),
+    ]
+    append = shared + [
+        (dict(qkv=rows.float()), ValueError), (dict(qkv=rows[:, :4 * 64]), ValueError), (dict(qkv=rows[:, :500]), ValueError),
+        (dict(qkv=rows.cpu()), RuntimeError), (dict(qkv=rows[:1]), ValueError), (dict(cos=cs.half()), ValueError),
+        (dict(cos=cs.half(), sin=cs.half()), ValueError), (dict(cos=cs[:, :32], sin=cs[:, :32]), ValueError),
+        (dict(cos=cs[:0], sin=cs[:0]), ValueError), (dict(cos=cs[:32]), ValueError), (dict(sin=cs.cpu()), RuntimeError),
+        (dict(cos=cs[:1].expand(64, -1), sin=cs[:1].expand(64, -1)), ValueError), (dict(q_norm_w=cs[0]), ValueError),
+        (dict(q_norm_w=cs[0], k_norm_w=cs[0].float()), ValueError), (dict(q_norm_w=cs[0], k_norm_w=cs[:, 0]), ValueError),
+        (dict(q_norm_w=cs[0].cpu(), k_norm_w=cs[0].cpu()), ValueError), (dict(out=rows), ValueError),
+        (dict(out=rows[:, :256].float()), ValueError), (dict(eps=1e39), ValueError), (dict(eps=float("nan")), ValueError),
+        (dict(eps=float("inf")), ValueError), (dict(eps="0"), TypeError),
+    ]
+    where = dict(k_pages=k, v_pages=v, page_table=table, seq_lens=lens)
+    for call, good, bad in ((paged.prefix_attention, dict(where, q=q, prefix_len=16), attention),
+                            (paged.paged_append, dict(where, qkv=rows, cos=cs, sin=cs), append)):
+        for change, error in bad:
+            with pytest.raises(error):
+                call(**{**good, **change})
+                pytest.fail(f"{call.__name__} took {sorted(change)}: {bad.index((change, error))}")
