@@ -8,7 +8,8 @@ the CUDA runtime linked statically, into breeze_b200/libbreeze_b200.so next to
 the Python package that loads it. Objects go to _build/ (git-ignored). The
 library depends on nothing from PyTorch; breeze_b200/_paged_bind.so, the Python
 side of the paged operators (csrc/bind_paged.cpp, host code), is compiled
-against torch's headers.
+against Python's and torch's headers. Where that fails there is a warning and no
+such file, and the operators are called from Python alone.
 """
 
 from __future__ import annotations
@@ -20,6 +21,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -51,18 +53,26 @@ def _stale(obj: Path, src: Path) -> bool:
     return any(d.stat().st_mtime > obj.stat().st_mtime for d in deps)
 
 
-def build_bind() -> Path:
-    """The Python side of the paged operators, against the installed torch."""
-    torch = Path(importlib.util.find_spec("torch").origin).parent
+def build_bind() -> str | None:
+    """The Python side of the paged operators, against the installed torch. What went wrong, if anything did."""
+    BIND_OUT.unlink(missing_ok=True)  # an old one might not fit the library
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return "torch is not installed"
+    torch = Path(spec.origin).parent
     cuda = Path(nvcc()).resolve().parents[1]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-I{sysconfig.get_paths()['include']}", f"-I{torch / 'include'}", f"-I{torch / 'include/torch/csrc/api/include'}",
            f"-I{cuda / 'include'}", f"-I{INCLUDE}", str(BIND_SRC), "-o", str(BIND_OUT), f"-L{torch / 'lib'}",
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{torch / 'lib'}"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        return str(e)
     if r.returncode != 0:
-        raise RuntimeError(f"{cmd[0]} failed on {BIND_SRC.name}:\n{r.stdout}\n{r.stderr}")
-    return BIND_OUT
+        BIND_OUT.unlink(missing_ok=True)
+        return f"{cmd[0]} failed on {BIND_SRC.name}:\n{r.stdout}\n{r.stderr}"
+    return None
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -> Path:
@@ -87,14 +97,15 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         for log in ex.map(compile_one, todo):
             if verbose and log:
                 print(log)
-        if bind is not None:
-            bind.result()
     if todo or force or not OUT.exists():
         cmd = [nvcc(), *ARCH, "-shared", "-rdc=true", "-Xcompiler", "-fPIC", "-cudart", "static",
                *map(str, objs), "-o", str(OUT)]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    why = None if bind is None else bind.result()
+    if why is not None:
+        warnings.warn(f"no {BIND_OUT.name} (the paged operators' calls then cost a few microseconds more): {why}", stacklevel=2)
     return OUT
 
 
