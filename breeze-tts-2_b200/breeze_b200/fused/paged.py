@@ -40,6 +40,7 @@ from __future__ import annotations
 import ctypes
 import math
 import operator
+import warnings
 
 import torch
 
@@ -53,6 +54,16 @@ _pack_attn = _lib.packer(_lib.PagedAttnDesc)
 _bound = None
 
 
+class _Python:
+    """Stands in for compiled calls that do not load: the functions below check and launch every call themselves."""
+
+    @staticmethod
+    def append(*args):
+        return None
+
+    attention = append
+
+
 def _native():
     """The compiled calls (csrc/bind_paged.cpp), bound to the loaded library:
     plain calls in a few microseconds of host time. They answer None where
@@ -63,9 +74,15 @@ def _native():
         lib = _lib.load()
         try:
             from .. import _paged_bind
+
+            built_for = _paged_bind.torch_version
+            if built_for != torch.__version__:
+                raise ImportError(f"built for torch {built_for}, not {torch.__version__}")
         except ImportError as e:
-            raise RuntimeError(f"breeze_b200/_paged_bind.so does not load ({e}): build it with "
-                               "`python breeze-tts-2_b200/build.py`") from e
+            warnings.warn(f"breeze_b200/_paged_bind.so does not load ({e}): calls of the paged operators take 6 us more. "
+                          "Build it with `python breeze-tts-2_b200/build.py`", RuntimeWarning, stacklevel=2)
+            _bound = _Python
+            return _bound
         _paged_bind.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
             lib.bq_paged_append, lib.bq_paged_attention, lib.bq_paged_attention_workspace_bytes)))
         _bound = _paged_bind

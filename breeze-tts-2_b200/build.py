@@ -17,6 +17,7 @@ from __future__ import annotations
 import argparse
 import importlib.util
 import os
+import runpy
 import shutil
 import subprocess
 import sys
@@ -53,6 +54,22 @@ def _stale(obj: Path, src: Path) -> bool:
     return any(d.stat().st_mtime > obj.stat().st_mtime for d in deps)
 
 
+def torch_version() -> str | None:
+    """Version of the installed torch, read without importing it."""
+    spec = importlib.util.find_spec("torch")
+    return None if spec is None else str(runpy.run_path(str(Path(spec.origin).parent / "version.py"))["__version__"])
+
+
+def _bind_for() -> str:
+    """What the bindings fit: the versions they were compiled against."""
+    return f"{torch_version()} {sysconfig.get_config_var('SOABI')}"
+
+
+def _bind_stale() -> bool:
+    made = BUILD / "bind_for.txt"
+    return _stale(BIND_OUT, BIND_SRC) or not made.exists() or made.read_text() != _bind_for()
+
+
 def build_bind() -> str | None:
     """The Python side of the paged operators, against the installed torch. What went wrong, if anything did."""
     BIND_OUT.unlink(missing_ok=True)  # an old one might not fit the library
@@ -63,7 +80,7 @@ def build_bind() -> str | None:
     cuda = Path(nvcc()).resolve().parents[1]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-I{sysconfig.get_paths()['include']}", f"-I{torch / 'include'}", f"-I{torch / 'include/torch/csrc/api/include'}",
-           f"-I{cuda / 'include'}", f"-I{INCLUDE}", str(BIND_SRC), "-o", str(BIND_OUT), f"-L{torch / 'lib'}",
+           f"-I{cuda / 'include'}", f"-I{INCLUDE}", f'-DBREEZE_TORCH_VERSION="{torch_version()}"', str(BIND_SRC), "-o", str(BIND_OUT), f"-L{torch / 'lib'}",
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{torch / 'lib'}"]
     try:
         r = subprocess.run(cmd, capture_output=True, text=True)
@@ -72,6 +89,7 @@ def build_bind() -> str | None:
     if r.returncode != 0:
         BIND_OUT.unlink(missing_ok=True)
         return f"{cmd[0]} failed on {BIND_SRC.name}:\n{r.stdout}\n{r.stderr}"
+    (BUILD / "bind_for.txt").write_text(_bind_for())
     return None
 
 
@@ -93,7 +111,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         return r.stderr
 
     with ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 1)) as ex:
-        bind = ex.submit(build_bind) if force or _stale(BIND_OUT, BIND_SRC) else None
+        bind = ex.submit(build_bind) if force or _bind_stale() else None
         for log in ex.map(compile_one, todo):
             if verbose and log:
                 print(log)

@@ -249,4 +249,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_bind", "Calls of the paged-
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__paged_bind() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__paged_bind() {
+    PyObject* m = PyModule_Create(&module);
+    // the torch whose classes this file was compiled for; no other may use it
+    if (m && PyModule_AddStringConstant(m, "torch_version", BREEZE_TORCH_VERSION) < 0) Py_CLEAR(m);
+    return m;
+}
