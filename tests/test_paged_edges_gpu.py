@@ -119,6 +119,25 @@ def test_scores_of_minus_infinity(lens, new, prefix, hq, hkv, dim, page, dtype, 
         assert ((lse.double() - ref["lse"]).abs()[rest] <= bound).all()
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("new,prefix,dim", [(None, 0, 64), ([1, 20], 0, 64), ([1, 100], 0, 128), ([70, 100], 0, 64),
+                                            ([1, 20], 64, 64), ([1, 100], 64, 128), (None, 64, 128)])
+def test_a_cut_length_reads_what_the_table_holds(causal, new, prefix, dim):
+    from breeze_b200 import _lib
+
+    c = pc.batch([200, 256], new, 4, 2, dim, 64, BF, seed=5, spare_cols=0, prefix=prefix)
+    ref = op.attention(c["q"], c["k"], c["v"], *pc.lists(c), None, causal)
+    full = op.attention(c["q"], c["k"], c["v"], *pc.lists(c), None, False)  # its rows all lie behind the table
+    cut = 1 if new is None else new[0]
+    want = {k: torch.cat([ref[k][:cut], full[k][cut:]]) for k in ("out", "lse", "weight", "terms", "seen")}
+    tol, ltol = op.attention_bounds(dict(want, vmax=full["vmax"]), dim, BF)
+    c["lens"][1] = 10 ** 6
+    out, lse = run(c, causal=causal)
+    assert _status() == _lib.BQ_DEVERR_POSITION
+    assert ((out.double().reshape(want["out"].shape) - want["out"]).abs() <= tol).all()
+    assert ((lse.double() - want["lse"]).abs() <= ltol).all()
+
+
 @pytest.mark.parametrize("new", [None, [70, 3]])
 @pytest.mark.parametrize("stride", [0, 1, 4, 2 ** 41])
 def test_strides_of_dimensions_of_size_one(new, stride):
@@ -159,6 +178,36 @@ def test_a_length_far_below_zero_is_an_unused_slot():
         torch.cuda.synchronize()
         dead = rows - (1 if new is None else 2)
         assert (out[:dead] == 300.0).all() and not (out[dead:] == 300.0).any(-1).any()
+
+
+@pytest.mark.parametrize("prefix", [0, 64])
+@pytest.mark.parametrize("hq,dim", [(2, 128), (8, 64)])
+def test_rows_before_the_first_sequence_are_left(prefix, hq, dim, table_room):  # noqa: F811
+    """q_starts[0] > 0: the rows before it belong to nobody, as those behind the last."""
+    c = table_room(pc.batch([130, 90, 300], [20, 1, 40], hq, 2, dim, 32, BF, seed=6, prefix=prefix, spare_rows=9))
+    lead = 5
+    moved = dict(c, starts=c["starts"] + lead)
+    out, lse = run(moved)
+    assert (out[:lead] == 3.0).all() and (lse[:lead] == 7.0).all()
+    table, lens, starts = pc.lists(moved)
+    ref = op.attention(c["q"], c["k"], c["v"], table, lens, starts)
+    tol, ltol = op.attention_bounds(ref, dim, BF)
+    rows = slice(lead, starts[-1])
+    assert ((out.double().reshape(c["rows"], hq, dim) - ref["out"]).abs() <= tol)[rows].all()
+    assert ((lse.double() - ref["lse"]).abs() <= ltol)[rows].all()
+    assert (out[starts[-1]:] == 3.0).all()
+
+
+@pytest.mark.parametrize("lens,new,prefix,hq,hkv,dim,page,dtype", [
+    ([32000, 24001], None, 0, 4, 1, 128, 128, BF),
+    ([31999, 7], [3, 2], 0, 2, 1, 64, 16, F16),
+    ([5003], [5003], 0, 1, 1, 128, 64, BF),
+    ([12300, 12401, 12288], [1, 5, 2], 12288, 4, 1, 128, 64, BF),
+    ([20000], [300], 0, 1, 1, 64, 256, BF),
+])
+def test_long_caches(lens, new, prefix, hq, hkv, dim, page, dtype):
+    c = pc.batch(lens, new, hq, hkv, dim, page, dtype, seed=71, prefix=prefix)
+    compare(c, *run(c))
 
 
 @pytest.mark.parametrize("dim,hq", [(64, 3), (64, 5), (128, 7)])
