@@ -162,7 +162,8 @@ class DecodeStack:
         page_size) int32 its pages out of ``num_pages`` per layer, ``cos`` /
         ``sin`` (kv_len, head_dim) the rotary table by position (1 and 0 until
         filled). ``prefix_len``: the first so many positions are the same pages
-        in every row and are read once for all. Initially all rows are full and
+        in every row that is in use, read once for all where that pays
+        (breeze_b200.fused.paged.prefix_attention). Initially all rows are full and
         take consecutive pages, the prefix's first; with fewer pages than that
         takes, the rows start unused and without pages (-1) of their own.
 
@@ -287,7 +288,10 @@ class DecodeStack:
 
     @property
     def kv_bytes(self) -> int:
-        """KV-cache bytes the attention steps read per decode step."""
+        """KV-cache bytes that the attention steps of one decode step cover,
+        each byte once: a shared prefix counts for one row, also where it is too
+        short to pay for a pass of its own and every row reads it (then the rows
+        after the first find most of it in L2)."""
         if not self.attention:
             return 0
         if self.page_size is not None:
