@@ -304,3 +304,55 @@ def test_compiled_calls_and_python_refuse_the_same(compiled, monkeypatch):
             with pytest.raises(error):
                 call(**{**good, **change})
                 pytest.fail(f"{call.__name__} took {sorted(change)}: {bad.index((change, error))}")
+
+
+@pytest.mark.parametrize("lens,new,prefix,hq,dim", [
+    ([90, 300], None, 0, 128, 128), ([300, 33], [1, 9], 0, 128, 64),    # a token is a box of queries
+    ([90, 300], None, 0, 256, 64), ([130, 140], [3, 2], 128, 256, 64),  # a tile is one token
+    ([70], [5], 0, 300, 64), ([200, 190], None, 128, 300, 128),         # a token goes on in the next tile
+    ([700], [40], 0, 96, 64),
+])
+def test_many_query_heads_on_one_kv_head(lens, new, prefix, hq, dim, table_room):  # noqa: F811
+    c = table_room(pc.batch(lens, new, hq, 1, dim, 32, BF, seed=81, prefix=prefix))
+    compare(c, *run(c))
+
+
+@pytest.mark.parametrize("what", ["append", "cluster", "narrow", "wide", "prefix"])
+def test_a_first_call_inside_a_capture(what):
+    """A process whose first paged call is captured: nothing that a capture forbids is left to the first call."""
+    code = f"""
+import torch
+from breeze_b200 import _lib
+from breeze_b200.fused import paged
+from tests import paged_cases as pc
+what = {what!r}
+new = None if what in ("append", "cluster", "narrow") else [100, 60]
+c = pc.batch([300, 200], new, 4, 2, 128, 64, torch.bfloat16, seed=1, prefix=128 if what == "prefix" else 0)
+if what == "narrow":
+    c["table"] = torch.nn.functional.pad(c["table"], (0, 1000), value=-1)
+d = pc.to(c, "cuda")
+where = (d["k"], d["v"], d["table"], d["lens"])
+rows = torch.ones(2, 8 * 128, dtype=torch.bfloat16, device="cuda")
+cs = torch.ones(512, 128, device="cuda")
+def call():
+    if what == "append":
+        return paged.paged_append(rows, cs, cs, *where)
+    if what == "prefix":
+        return paged.prefix_attention(d["q"], *where, 128, q_starts=d["starts"], always=True)
+    return paged.paged_attention(d["q"], *where, q_starts=d["starts"])
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = call()
+out.zero_()
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, call()) and out.abs().sum() > 0 and _lib.device_status(0) == 0
+"""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parents[1]
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
