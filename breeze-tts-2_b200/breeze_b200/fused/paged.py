@@ -174,7 +174,7 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_page
     into their pages. ``cos`` / ``sin``: (positions, D) tables (fp32 or the
     cache's dtype), row p for cache position p, both halves given as rotate_half
     takes them. The math is fp32 with one rounding at the end. ``out`` may be
-    ``qkv[:, :HQ * D]`` itself. Tokens of an unused batch slot (seq_lens[b] less
+    ``qkv[:, :HQ * D]`` itself, and else shares no memory with ``qkv``. Tokens of an unused batch slot (seq_lens[b] less
     than its new tokens) are skipped where their position would be negative."""
     done = (_bound or _native()).append(qkv, cos, sin, k_pages, v_pages, page_table, seq_lens, q_starts, q_norm_w, k_norm_w,
                                         eps, out, _lib.default_flags())
@@ -270,7 +270,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     that sees none gets zeros, one whose scores are all -inf gets NaN; infinite or NaN keys and values at positions it does
     not see stay without effect. Query head h reads kv head h // (HQ / HKV).
     ``scale`` defaults to D^-0.5. ``max_q``: most new tokens of one sequence, a
-    hint that picks the kernel (default: T / B rounded up). ``lse`` (T, HQ) fp32
+    hint that picks the kernel (0 or None: T / B rounded up; say it where they differ:
+    a prompt among many running streams is slow in the kernel for few rows). ``lse`` (T, HQ) fp32
     receives log(sum(exp(scores))), -inf for a row that sees nothing."""
     return _attention(q, k_pages, v_pages, page_table, seq_lens, 0, q_starts, scale, causal, max_q, out, lse)
 

@@ -349,9 +349,16 @@ const void* join_kernel(bool prefix, bool many) {
 constexpr int kClusterPositions = 512;
 
 // Bytes of repeated reads that a shared prefix must save for its second pass and
-// the join of every row to pay. Shared against not, 128 dims, prefix of 1024 / 4096
-// positions: 16 sequences of 8 heads (63 / 252 MB saved) 25 / 27 us against 20 / 42
-// us, 48 sequences of 2 heads (49 / 197 MB) 28 / 29 us against 18 / 35 us.
+// the join of every row to pay. Shared against not, 128 dims, 64 positions of their
+// own, prefix of 1024 / 2048 / 4096 (MB saved; us, in a graph):
+//                             one new token, 4 rows per kv head   8 tokens, 32 rows (256-row kernel)
+//   16 sequences of 8 kv heads, 60 / 120 / 240 MB
+//                             23 / 24 / 25 and 16 / 23 / 36       34 / 37 / 40 and 26 / 36 / 56
+//   48 of 2, 47 / 94 / 188    23 / 23 / 24 and 14 / 19 / 29       30 / 34 / 36 and 24 / 31 / 46
+//   96 of 8, 380 / 760 / 1520 32 / 34 / 37 and 55 / 93 / 168      88 / 98 / 119 and 104 / 155 / 265
+// 64 dims break even at 60 to 110 MB. Bytes alone misjudge many rows behind a short
+// prefix, where joining them costs most: 96 sequences of 64 rows per kv head behind 512
+// or 1024 positions (190 / 380 MB) take 116 / 128 us shared, 81 / 105 not.
 constexpr int64_t kSharedBytes = 96ll << 20;
 
 // One pass over positions: its kernel and its CTAs.

@@ -11,8 +11,9 @@
 // lines, the norm is a shuffle reduction inside the group, and the rotation's
 // partner (dim +- D / 2) is the lane half a group away.
 //
-// Measured (B200): 2 rows of 48 heads of 128 in 2.2 us, 200 rows (5 MB) in 3.1 us,
-// 2751 ragged rows of 40 heads of 64 (29 MB) in 10.5 us, 2.8 TB/s. Blocks of 64, 256
+// Measured (B200, in a graph): 2 rows of 48 heads of 128 in 1.9 us, 200 rows (5 MB) in
+// 2.7 us, 2751 ragged rows of 40 heads of 64 (29 MB) in 10.2 us from L2, 12.4 us with
+// other rows each call, 2.3 TB/s. Blocks of 64, 256
 // and 512 threads, several rows per block and several heads per lane group were no
 // faster.
 #include <cstring>

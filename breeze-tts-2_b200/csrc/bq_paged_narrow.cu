@@ -18,11 +18,13 @@
 //
 // Scores, statistics and outputs are fp32; the probabilities are rounded to the
 // element type for the second product (relative error of half a step of that
-// type each, as the values they weight).
+// type each, as the values they weight). Over long caches that is the larger part
+// of what the result is off: 0.0020 of its size in bf16 where probabilities in fp32
+// leave 0.0017, the output's own rounding.
 //
 // Measured, join included (B200, copies run at 6554 GB/s): 8 sequences of 24 to 32
-// thousand positions, 8 kv heads of 128, 881 MB in 145 us (6.1 TB/s); 48 of 17 to
-// 6000, 184 MB in 38 us (4.8 TB/s), where finding the shares (2 us), each tile's
+// thousand positions, 8 kv heads of 128, 881 MB in 145 to 150 us (6.0 TB/s); 48 of 17 to
+// 6000, 184 MB in 39 us (4.7 TB/s), where finding the shares (2 us), each tile's
 // start and end and the join (5 us) show. The shares are equal, the SMs' speeds are
 // not: on average an SM is done after 87 % of the time. Two, four and eight times
 // as many smaller shares, dealt out as CTAs end, cost more in starts than they
@@ -368,8 +370,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_narrow_kernel(const __grid_
 // (rank order, deterministic). No schedule to work out, no partials in memory and
 // no second kernel. A shared prefix is read by each pair, mostly from L2. Bound:
 // latency (length, page, keys, cluster barrier, output). Two sequences of 16 heads
-// of 128, 300 to 700 positions: 6.8 us (equal shares and join: 10.6 us); four that
-// share 512 of 520 to 800 positions: 8.2 us (two passes and join: 16.7 us).
+// of 128, 300 to 700 positions: 6.0 us in a graph (equal shares and join: 10.6 us); four
+// that share 512 of 520 to 800 positions: 7.6 us (two passes and join: 16.7 us).
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads, 2) paged_cluster_kernel(const __grid_constant__ PagedWork p, int ranks) {
     using SM = NarrowSmem<D>;

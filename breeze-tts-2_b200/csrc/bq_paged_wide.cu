@@ -39,9 +39,10 @@
 // are cleared likewise, and added in memory to the outputs of the rows that see
 // them.
 //
-// Measured, join included (B200): 7000 new positions of 16 query and 8 kv heads of
-// 128, causal, 201 GFLOP in 207 us (0.97 PFLOP/s; library products of 8192^3 run at
-// 1.65); 1474 ragged ones of 32 heads over 18 thousand in 112 us. The tensor cores
+// Measured, join included (B200, calls in a row): 7000 new positions of 16 query and 8
+// kv heads of 128, causal, 201 GFLOP in 209 us on the same inputs again, which are then
+// in L2 (0.96 PFLOP/s; library products of 8192^3 run at 1.65), 233 us on others each
+// call; 1474 ragged ones of 32 heads over 18 thousand in 111 and 120 us. The tensor cores
 // and the exponential units are each busy half of the time; without the softmax's
 // arithmetic the same pipeline takes 163 us, and a change of tile 7700 cycles.
 // Dropped: units of 64 positions with a score buffer per half (271 against then 238
