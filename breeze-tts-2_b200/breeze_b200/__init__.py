@@ -9,6 +9,7 @@ decode kernels, backed by hand-written CUDA kernels in libbreeze_b200.so
   breeze_b200.int8_linear   Int8Linear, quantize_module_int8
   breeze_b200.fused.kernels FusedWeight, rms_gemv, rmsnorm, silu_mul
   breeze_b200.fused.paged   paged_append, paged_attention, prefix_attention
+  breeze_b200.fused.paged_fp8  paged_append_fp8, paged_attention_fp8, paged_read_fp8
 
 Put the ``breeze-tts-2_b200`` directory, or the repository's root, on sys.path to import it.
 """

@@ -136,6 +136,45 @@ class PagedAttnDesc(ctypes.Structure):
     ]
 
 
+_PAGED8_KV_FIELDS = [
+    ("B", ctypes.c_int32), ("HKV", ctypes.c_int32), ("D", ctypes.c_int32), ("page_size", ctypes.c_int32),
+    ("num_pages", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("block", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ("k_pages", ctypes.c_void_p), ("k_page_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+    ("k_slot_stride", ctypes.c_int64), ("v_pages", ctypes.c_void_p), ("v_page_stride", ctypes.c_int64),
+    ("v_head_stride", ctypes.c_int64), ("v_slot_stride", ctypes.c_int64),
+    ("k_scales", ctypes.c_void_p), ("k_scale_page_stride", ctypes.c_int64), ("k_scale_head_stride", ctypes.c_int64),
+    ("v_scales", ctypes.c_void_p), ("v_scale_page_stride", ctypes.c_int64), ("v_scale_head_stride", ctypes.c_int64),
+    ("page_table", ctypes.c_void_p), ("ld_table", ctypes.c_int64), ("seq_lens", ctypes.c_void_p),
+    ("q_starts", ctypes.c_void_p),
+]
+
+
+class Paged8AppendDesc(ctypes.Structure):
+    """bq_paged8_append_desc with its bq_paged8_kv laid out in line (include/breeze_b200.h)."""
+
+    _fields_ = _PAGED8_KV_FIELDS + PagedAppendDesc._fields_[len(_PAGED_KV_FIELDS):]
+
+
+class Paged8AttnDesc(ctypes.Structure):
+    """bq_paged8_attn_desc with its bq_paged8_kv laid out in line (include/breeze_b200.h)."""
+
+    _fields_ = _PAGED8_KV_FIELDS + [
+        ("T", ctypes.c_int32), ("HQ", ctypes.c_int32), ("max_q", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("flags", ctypes.c_uint32), ("reserved", ctypes.c_int32), ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64), ("lse", ctypes.c_void_p), ("ldl", ctypes.c_int64),
+    ]
+
+
+class Paged8ReadDesc(ctypes.Structure):
+    """bq_paged8_read_desc with its bq_paged8_kv laid out in line (include/breeze_b200.h)."""
+
+    _fields_ = _PAGED8_KV_FIELDS + [
+        ("T", ctypes.c_int32), ("flags", ctypes.c_uint32), ("k_out", ctypes.c_void_p), ("k_out_row_stride", ctypes.c_int64),
+        ("k_out_head_stride", ctypes.c_int64), ("v_out", ctypes.c_void_p), ("v_out_row_stride", ctypes.c_int64),
+        ("v_out_head_stride", ctypes.c_int64),
+    ]
+
+
 _PACK_CODES = {ctypes.c_int32: "i", ctypes.c_uint32: "I", ctypes.c_float: "f", ctypes.c_int64: "q", ctypes.c_void_p: "Q"}
 
 
@@ -191,6 +230,10 @@ _SIGS = {
     "bq_paged_append": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
     "bq_paged_attention_workspace_bytes": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]),
     "bq_paged_attention": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "bq_paged8_append": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
+    "bq_paged8_attention_workspace_bytes": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "bq_paged8_attention": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "bq_paged8_read": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
     "bq_int4_tinygemm_pack": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
                                                ctypes.c_int32, ctypes.c_void_p]),
     "bq_int4_tinygemm_unpack": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,

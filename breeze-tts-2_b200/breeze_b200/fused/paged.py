@@ -216,8 +216,9 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_page
     return out
 
 
-def _workspace_bytes(desc: bytes, need, stream) -> int:  # noqa: ARG001 - _launch passes the stream
-    return _lib.load().bq_paged_attention_workspace_bytes(desc, need)
+def _workspace_bytes_of(entry):
+    """A *_workspace_bytes entry as _launch calls it, with a stream behind the arguments."""
+    return lambda desc, need, stream: entry(desc, need)
 
 
 def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, scale, causal, max_q, out, lse, extra=0):
@@ -253,7 +254,8 @@ def _attention(q, k_pages, v_pages, page_table, seq_lens, prefix_len, q_starts, 
     desc = _pack_attn(*fields, rows, hq, _count(prefix_len, "prefix_len"), max_q, scale, flags, q.data_ptr(),
                       ldq, out.data_ptr(), ldo, lse_ptr, ldl)
     size = ctypes.c_size_t(0)
-    _launch(dev, "bq_paged_attention_workspace_bytes", _workspace_bytes, desc, ctypes.byref(size))
+    _launch(dev, "bq_paged_attention_workspace_bytes", _workspace_bytes_of(_lib.load().bq_paged_attention_workspace_bytes), desc,
+            ctypes.byref(size))
     need = size.value
     ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
     _launch(dev, "bq_paged_attention", _lib.load().bq_paged_attention, desc, ws.data_ptr() if need else None, need)

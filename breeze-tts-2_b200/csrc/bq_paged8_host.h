@@ -1,0 +1,21 @@
+// Host-side helpers of the 8-bit paged KV cache.
+#pragma once
+
+#include "bq_paged_host.h"
+
+namespace bq {
+
+struct Paged8Scales;
+
+// Checks the cache part of a descriptor with T rows; HQ query heads (0: none).
+int paged8_validate(const bq_paged8_kv* kv, int T, int HQ, bool f32 = false);
+int paged8_fill(PagedKV* out, Paged8Scales* scales, const bq_paged8_kv* kv, int T, int HQ);
+// Rows of a window of the kernels that walk ragged rows: a power of two of at most T / B and `most`, so that
+// a window holds rows of few sequences.
+inline int paged8_window(const bq_paged8_kv* kv, int T, int most) {
+    int w = 1;
+    while (2 * w <= most && int64_t(2 * w) * kv->B <= T) w *= 2;
+    return w;
+}
+
+}  // namespace bq

@@ -1,0 +1,186 @@
+// bq_paged8_read: the last positions of each sequence of an 8-bit paged cache as
+// rows of bf16, fp16 or fp32: code * 2^e, one rounding (none in bf16 and fp32, whose
+// exponents reach further than the cache's).
+//
+// Bound: HBM, 1 byte read and 2 (4) written per element. A CTA takes a window of
+// rows and some heads of k or of v; a thread turns 16 codes at a time (32 bytes out),
+// several of them in flight.
+#include <cstring>
+
+#include "bq_host.h"
+#include "bq_paged8.cuh"
+#include "bq_paged8_host.h"
+
+namespace bq {
+namespace {
+
+constexpr int kThreads = 256, kMostRows = 32, kHeads = 4, kFlight = 4;
+
+struct Read8Params {
+    PagedKV kv;
+    Paged8Scales sc;
+    int32_t window;
+    void* k_out;
+    int64_t ko_row, ko_head;
+    void* v_out;
+    int64_t vo_row, vo_head;
+};
+
+template <typename T>
+__device__ __forceinline__ void store16(T* dst, const float (&v)[16]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+        float a[8], b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = v[i], b[i] = v[8 + i];
+        reinterpret_cast<uint4*>(dst)[0] = pack8<T>(a);
+        reinterpret_cast<uint4*>(dst)[1] = pack8<T>(b);
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__ Read8Params p) {
+    constexpr int CH = D / 16;  // pieces of a head
+    __shared__ int s_page[kMostRows], s_slot[kMostRows];
+    pdl_launch_dependents();
+    pdl_wait();
+    const PagedKV& kv = p.kv;
+    const int w0 = blockIdx.x * p.window, rows = min(p.window, kv.T - w0);
+    const bool is_k = int(blockIdx.y) < (kv.HKV + kHeads - 1) / kHeads;
+    const int h0 = (is_k ? blockIdx.y : blockIdx.y - (kv.HKV + kHeads - 1) / kHeads) * kHeads;
+
+    // page (-1: leave the row) and slot of every row of the window
+    auto place = [&](int r, int b, int pos) {
+        bool ok = (pos >> kv.page_shift) < kv.max_pages;
+        if (pos < 0) {
+            s_page[r] = -1;
+            return;
+        }
+        if (!ok) {
+            if (blockIdx.y == 0) atomicOr(kv.errors, BQ_DEVERR_POSITION_BIT);
+            s_page[r] = -1;
+            return;
+        }
+        const int page = paged_page(kv, b, pos, ok);
+        if (!ok && blockIdx.y == 0) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
+        s_page[r] = ok ? page : -1;
+        s_slot[r] = pos & kv.page_mask;
+    };
+    if (!kv.starts) {
+        if (int(threadIdx.x) < rows) place(threadIdx.x, w0 + threadIdx.x, max(kv.lens[w0 + threadIdx.x], 0) - 1);
+    } else {
+        if (threadIdx.x < kMostRows) s_page[threadIdx.x] = -1;
+        __shared__ int s_begin[kMostRows], s_pos[kMostRows], s_seq[kMostRows];  // of the sequence whose rows reach row r first
+        if (threadIdx.x < kMostRows) s_seq[threadIdx.x] = -1;
+        __syncthreads();
+        for (int b = threadIdx.x; b < kv.B; b += kThreads) {
+            int begin, n;
+            paged_rows(kv, b, begin, n);
+            const int lo = max(begin, w0), hi = min(begin + n, w0 + rows);
+            if (lo >= hi) continue;
+            s_seq[lo - w0] = b;
+            s_begin[lo - w0] = hi - w0;
+            s_pos[lo - w0] = max(kv.lens[b], 0) - n + (lo - begin);
+        }
+        __syncthreads();
+        if (int(threadIdx.x) < rows)
+            for (int r = threadIdx.x; r >= 0; --r)
+                if (s_seq[r] >= 0) {
+                    if (int(threadIdx.x) < s_begin[r]) place(threadIdx.x, s_seq[r], s_pos[r] + (int(threadIdx.x) - r));
+                    break;
+                }
+    }
+    __syncthreads();
+
+    const uint8_t* pages = static_cast<const uint8_t*>(is_k ? kv.k : kv.v);
+    const int64_t st_page = is_k ? kv.ks_page : kv.vs_page, st_head = is_k ? kv.ks_head : kv.vs_head,
+                  st_slot = is_k ? kv.ks_slot : kv.vs_slot;
+    T* out = static_cast<T*>(is_k ? p.k_out : p.v_out);
+    const int64_t o_row = is_k ? p.ko_row : p.vo_row, o_head = is_k ? p.ko_head : p.vo_head;
+    const int total = rows * kHeads * CH;
+    for (int i0 = threadIdx.x; i0 < total; i0 += kThreads * kFlight) {
+        uint4 w[kFlight];
+        uint8_t e[kFlight];
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) {
+            const int i = i0 + f * kThreads, r = i / (kHeads * CH), h = h0 + i / CH % kHeads, c = i % CH;
+            w[f] = make_uint4(0, 0, 0, 0);
+            e[f] = kExpBias;
+            if (i < total && h < kv.HKV && s_page[r] >= 0) {
+                const int page = s_page[r], slot = s_slot[r], blk = slot >> p.sc.block_shift;
+                w[f] = *reinterpret_cast<const uint4*>(pages + page * st_page + h * st_head + slot * st_slot + c * 16);
+                e[f] = is_k ? *k_scale(p.sc, page, h, blk) : *v_scale(p.sc, page, h, blk);
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) {
+            const int i = i0 + f * kThreads, r = i / (kHeads * CH), h = h0 + i / CH % kHeads, c = i % CH;
+            if (i >= total || h >= kv.HKV || s_page[r] < 0) continue;
+            const float s = exp_scale(scale_exp(e[f]));
+            const uint32_t words[4] = {w[f].x, w[f].y, w[f].z, w[f].w};
+            float v[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float x[4];
+                codes_f32(words[q], x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v[4 * q + k] = x[k] * s;
+                    if constexpr (std::is_same_v<T, __half>)  // a finite entry stays finite
+                        v[4 * q + k] = v[4 * q + k] > 65504.f ? 65504.f : v[4 * q + k] < -65504.f ? -65504.f : v[4 * q + k];
+                }
+            }
+            store16<T>(out + (w0 + r) * o_row + h * o_head + c * 16, v);
+        }
+    }
+}
+
+template <int D>
+const void* read_kernel(int dtype) {
+    return dtype == BQ_DT_BF16  ? reinterpret_cast<const void*>(&read8_kernel<__nv_bfloat16, D>)
+           : dtype == BQ_DT_F16 ? reinterpret_cast<const void*>(&read8_kernel<__half, D>)
+                                : reinterpret_cast<const void*>(&read8_kernel<float, D>);
+}
+
+}  // namespace
+}  // namespace bq
+
+using namespace bq;
+
+extern "C" int32_t bq_paged8_read(const bq_paged8_read_desc* d, void* stream) {
+    if (!d) return set_error(BQ_ERR_INVALID_ARG, "desc is NULL");
+    int rc = paged8_validate(&d->kv, d->T, 0, true);
+    if (rc) return rc;
+    if (d->T == 0) return BQ_OK;
+    if (!d->k_out || !d->v_out) return set_error(BQ_ERR_INVALID_ARG, "k_out and v_out must be non-NULL");
+    const int elem = dtype_size(d->kv.dtype), size[2] = {d->T, d->kv.HKV};
+    for (int i = 0; i < 2; ++i) {
+        if (size[i] == 1) continue;  // its stride is never taken
+        if (d->ko_stride[i] < d->kv.D || d->vo_stride[i] < d->kv.D)
+            return set_error(BQ_ERR_SHAPE, "strides of k_out and v_out must be at least the head dim");
+        if (d->ko_stride[i] * elem % 16 || d->vo_stride[i] * elem % 16)
+            return set_error(BQ_ERR_ALIGN, "rows and heads of k_out and v_out must be 16-byte aligned");
+    }
+    if (!paged_aligned(d->k_out, 0, elem) || !paged_aligned(d->v_out, 0, elem))
+        return set_error(BQ_ERR_ALIGN, "k_out and v_out must be 16-byte aligned");
+    rc = paged_check_device();
+    if (rc) return rc;
+    Read8Params p;
+    std::memset(&p, 0, sizeof(p));
+    rc = paged8_fill(&p.kv, &p.sc, &d->kv, d->T, 0);
+    if (rc) return rc;
+    p.window = paged8_window(&d->kv, d->T, kMostRows);
+    p.k_out = d->k_out;
+    p.ko_row = d->ko_stride[0];
+    p.ko_head = d->ko_stride[1];
+    p.v_out = d->v_out;
+    p.vo_row = d->vo_stride[0];
+    p.vo_head = d->vo_stride[1];
+    const void* fn = d->kv.D == 128 ? read_kernel<128>(d->kv.dtype) : read_kernel<64>(d->kv.dtype);
+    void* args[] = {&p};
+    return paged_launch(fn, dim3((d->T + p.window - 1) / p.window, 2 * ((d->kv.HKV + kHeads - 1) / kHeads)), dim3(kThreads), 0, args,
+                        d->flags, stream, "paged read");
+}

@@ -373,6 +373,105 @@ typedef struct bq_paged_attn_desc {
 int32_t bq_paged_attention_workspace_bytes(const bq_paged_attn_desc* desc, size_t* bytes);
 int32_t bq_paged_attention(const bq_paged_attn_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- paged KV cache in 8 bits --------------------------------------------- */
+/* bq_paged_kv's cache held as e4m3 codes with a power-of-two scale for each block
+ * of `block` positions and kv head, for k and v each: an entry's value is its code
+ * times 2^(s - 127), s the block's scale byte (e8m0). No counterpart in the
+ * reference. Pages, rows, lengths, the device data's errors and what slots that hold
+ * no position may hold are bq_paged_kv's; codes are bytes, so strides count bytes.
+ * Scales are written by the append, from 2^-60 to 2^60; a byte outside 67 .. 187 is
+ * read as the nearer of these. */
+typedef struct bq_paged8_kv {
+    int32_t B;             /* sequences, >= 1 */
+    int32_t HKV, D;        /* kv heads, head dim (64 or 128) */
+    int32_t page_size;     /* positions per page: a power of two, 16 .. 1024 */
+    int32_t num_pages;     /* pages in k_pages / v_pages */
+    int32_t max_pages;     /* page-table columns */
+    int32_t block;         /* positions per scale: 16, 32, 64 or 128, at most page_size */
+    int32_t dtype;         /* q / k / v rows and outputs: BQ_DT_BF16 or BQ_DT_F16 (read back: BQ_DT_F32 too) */
+    void* k_pages;         /* e4m3 codes; strides of a page, a kv head and a slot: multiples of 16 (of one */
+    int64_t k_stride[3];   /* page or one kv head: any), the D codes of a slot contiguous; 16-byte aligned */
+    void* v_pages;
+    int64_t v_stride[3];
+    void* k_scales;            /* e8m0 [num_pages, HKV, page_size / block]; strides of a page and a kv */
+    int64_t k_scale_stride[2]; /* head, the scales of a page and head contiguous */
+    void* v_scales;
+    int64_t v_scale_stride[2];
+    const int32_t* page_table; /* [B, ld_table] */
+    int64_t ld_table;
+    const int32_t* seq_lens;   /* [B] */
+    const int32_t* q_starts;   /* [B + 1] ascending, or NULL */
+} bq_paged8_kv;
+
+/* bq_paged_append into such a cache. q rows as there. Of k (normed, rotated, fp32)
+ * and v, per block of positions that gets new tokens, and per head: e is the least
+ * from -60 to 60 with |x| <= 448 * 2^e for every finite new x of the block; where the
+ * block holds positions before the sequence's first new token, e is at least the
+ * block's scale so far, and where it grows those positions' codes are divided by the
+ * power of two (exact, but for codes that become subnormal). New codes are x * 2^-e
+ * rounded to the nearest e4m3 value, ties to even; infinite and NaN x become NaN,
+ * |x| above 448 * 2^60 becomes that. What the block holds behind the new tokens does
+ * not count. A block belongs to one sequence of a call. */
+typedef struct bq_paged8_append_desc {
+    bq_paged8_kv kv;
+    int32_t T, HQ;
+    int32_t cs_dtype;          /* cos / sin: dtype or BQ_DT_F32 */
+    int32_t rope_rows;         /* rows of cos / sin, one per position */
+    float eps;                 /* RMSNorm epsilon */
+    uint32_t flags;            /* BQ_FLAG_PDL */
+    const void* qkv;           /* [T, ldqkv], 16-byte aligned rows (as all rows here) */
+    int64_t ldqkv;
+    const void* cos;           /* [rope_rows, ldcs] */
+    const void* sin;
+    int64_t ldcs;
+    const void* q_norm;        /* [D] in dtype, both or neither */
+    const void* k_norm;
+    void* q_out;               /* [T, ldq]: HQ * D elements a row; may be the q columns of qkv itself */
+    int64_t ldq;
+} bq_paged8_append_desc;
+
+int32_t bq_paged8_append(const bq_paged8_append_desc* desc, void* stream);
+
+/* bq_paged_attention over such a cache: the same rows, masks, empty rows and lse, with
+ * k and v as the values their codes stand for. The codes enter the products as they
+ * are (exact in fp16); the scales are applied in fp32. */
+typedef struct bq_paged8_attn_desc {
+    bq_paged8_kv kv;
+    int32_t T, HQ;
+    int32_t max_q;             /* as in bq_paged_attn_desc */
+    float scale;
+    uint32_t flags;            /* BQ_FLAG_PDL | BQ_PAGED_FULL */
+    int32_t reserved;
+    const void* q;             /* [T, ldq]: HQ * D elements a row */
+    int64_t ldq;
+    void* out;                 /* [T, ldo] */
+    int64_t ldo;
+    float* lse;                /* [T, ldl] or NULL */
+    int64_t ldl;
+} bq_paged8_attn_desc;
+
+/* The workspace (256-byte aligned) needs no initial value and keeps none
+ * between calls; calls that can run at the same time need one each. */
+int32_t bq_paged8_attention_workspace_bytes(const bq_paged8_attn_desc* desc, size_t* bytes);
+int32_t bq_paged8_attention(const bq_paged8_attn_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The last positions of each sequence back: rows q_starts[b] .. q_starts[b + 1] - 1 of
+ * k_out and v_out are the last positions of sequence b (q_starts NULL: T = B, its last
+ * one), as the append's rows are, rounded once to kv.dtype (exact in bf16 and fp32; in
+ * fp16 a finite value stays finite). Rows of no position (of no sequence, before a
+ * sequence's first position, behind the table, of a bad page) are left as they were. */
+typedef struct bq_paged8_read_desc {
+    bq_paged8_kv kv;
+    int32_t T;
+    uint32_t flags;            /* BQ_FLAG_PDL */
+    void* k_out;               /* strides of a row and a head in elements, D contiguous; 16-byte aligned */
+    int64_t ko_stride[2];
+    void* v_out;
+    int64_t vo_stride[2];
+} bq_paged8_read_desc;
+
+int32_t bq_paged8_read(const bq_paged8_read_desc* desc, void* stream);
+
 /* ---- fp32 output heads -------------------------------------------------- */
 /* out[M, N] (fp32) = y @ W, W fp32, where y is x or, when gamma is given, the
  * reference's BreezeRMSNorm of x (models/breeze.py:115-120: xh = bf16(x *
