@@ -341,6 +341,35 @@ const void* join_kernel(bool prefix, bool many) {
                 : reinterpret_cast<const void*>(&paged_join_kernel<E, D, 1>);
 }
 
+// The join of one pass, or of a prefix's and the rows' own: p.pass is filled.
+int launch_join(PagedJoin& p, const PagedWork& w, int dtype, int D, bool wide, int64_t tile_rows, bool prefix, uint32_t flags,
+                void* stream) {
+    p.shared = w.shared;
+    p.starts = w.kv.starts;
+    p.out = w.out;
+    p.ldo = w.ldo;
+    p.lse = w.lse;
+    p.ldl = w.ldl;
+    p.B = w.kv.B;
+    p.T = w.kv.T;
+    p.HQ = w.kv.HQ;
+    p.G = w.G;
+    p.by_G = w.by_G;
+    p.by_HQ.set(uint32_t(w.kv.HQ));
+    // With a prefix, 1024 rows give every SM a row per warp; fewer are shared among a block's warps.
+    const int64_t rows = int64_t(p.T) * p.HQ;
+    const bool many = prefix ? rows >= 1024 : wide;
+    const int per = prefix ? (many ? kJoinWarps : 1) : kJoinWarps * (many ? kJoinRows : 1);
+    const int64_t tile = std::min<int64_t>(p.pass[0].rows, tile_rows);  // (a tile spread over many CTAs: a block per row)
+    const dim3 grid = prefix ? dim3(unsigned(std::min<int64_t>((rows + per - 1) / per, 1 << 20)))
+                             : dim3(p.pass[0].grid, unsigned(std::max((tile + per - 1) / per, std::min<int64_t>(tile, 4))));
+    const bool bf = dtype == BQ_DT_BF16;
+    const void* fn = D == 128 ? (bf ? join_kernel<__nv_bfloat16, 128>(prefix, many) : join_kernel<__half, 128>(prefix, many))
+                              : (bf ? join_kernel<__nv_bfloat16, 64>(prefix, many) : join_kernel<__half, 64>(prefix, many));
+    void* args[] = {&p};
+    return paged_launch(fn, grid, dim3(32 * kJoinWarps), 0, args, flags, stream, "paged attention join");
+}
+
 // Most positions per CTA of a cluster that the page table may hold. Clusters against
 // equal shares, 128 dims, all sequences of the table's length: two sequences of 16
 // heads, 256 / 1024 / 4096 positions 5.4 / 6.4 / 11.8 us and 8.4 / 10.7 / 17.2 us; 9
@@ -463,6 +492,15 @@ int validate_attention(const bq_paged_attn_desc* d) {
 }
 
 }  // namespace
+
+int paged_launch_join(const PagedWork& w, int dtype, int D, int rows, int grid, bool wide, int64_t tile_rows, uint32_t flags,
+                      void* stream) {
+    PagedJoin p;
+    std::memset(&p, 0, sizeof(p));
+    p.pass[0] = PagedParts{w.part_o, w.part_ml, w.row_o, w.row_ml, w.row_at, rows, grid};
+    return launch_join(p, w, dtype, D, wide, tile_rows, false, flags, stream);
+}
+
 }  // namespace bq
 
 using namespace bq;
@@ -527,30 +565,7 @@ int32_t bq_paged_attention(const bq_paged_attn_desc* d, void* workspace, size_t 
         if (rc) return rc;
         p.pass[i] = PagedParts{w.part_o, w.part_ml, w.row_o, w.row_ml, w.row_at, pl.pass[i].rows, pl.pass[i].grid};
     }
-    p.shared = w.shared;
-    p.starts = w.kv.starts;
-    p.out = w.out;
-    p.ldo = w.ldo;
-    p.lse = w.lse;
-    p.ldl = w.ldl;
-    p.B = w.kv.B;
-    p.T = d->T;
-    p.HQ = d->HQ;
-    p.G = w.G;
-    p.by_G = w.by_G;
-    p.by_HQ.set(uint32_t(d->HQ));
-    // With a prefix, 1024 rows give every SM a row per warp; fewer are shared among a block's warps.
-    const int64_t rows = int64_t(d->T) * d->HQ;
-    const bool many = prefix ? rows >= 1024 : pl.pass[0].wide;
-    const int per = prefix ? (many ? kJoinWarps : 1) : kJoinWarps * (many ? kJoinRows : 1);
-    const int64_t tile = std::min<int64_t>(pl.pass[0].rows, pl.tile_rows);  // (a tile spread over many CTAs: a block per row)
-    const dim3 grid = prefix ? dim3(unsigned(std::min<int64_t>((rows + per - 1) / per, 1 << 20)))
-                             : dim3(pl.pass[0].grid, unsigned(std::max((tile + per - 1) / per, std::min<int64_t>(tile, 4))));
-    const bool bf = d->kv.dtype == BQ_DT_BF16;
-    const void* fn = d->kv.D == 128 ? (bf ? join_kernel<__nv_bfloat16, 128>(prefix, many) : join_kernel<__half, 128>(prefix, many))
-                                    : (bf ? join_kernel<__nv_bfloat16, 64>(prefix, many) : join_kernel<__half, 64>(prefix, many));
-    void* args[] = {&p};
-    return paged_launch(fn, grid, dim3(32 * kJoinWarps), 0, args, d->flags, stream, "paged attention join");
+    return launch_join(p, w, d->kv.dtype, d->kv.D, pl.pass[0].wide, pl.tile_rows, prefix, d->flags, stream);
 }
 
 }  // extern "C"

@@ -82,81 +82,47 @@ int paged8_fill(PagedKV* o, Paged8Scales* sc, const bq_paged8_kv* kv, int T, int
 
 namespace {
 
-constexpr int kWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct Attn8Params {
-    PagedKV kv;
-    Paged8Scales sc;
-    int32_t G, causal;
-    float scale_log2;
-    const void* q;
-    int64_t ldq;
-    void* out;
-    int64_t ldo;
-    float* lse;
-    int64_t ldl;
+// Most positions per CTA of a cluster that the page table may hold.
+constexpr int kClusterPositions = 512;
+
+// How a call is divided: clusters of `ranks` CTAs per (sequence, kv head), or equal shares of all positions for
+// `grid` CTAs with scratch for the tiles that they share.
+struct Plan8 {
+    int ranks, grid;
+    int64_t tile_rows;  // rows of a tile as far as is known
+    size_t part_o, part_ml, shared, total;
 };
 
-// One warp per row and query head, position by position with a running maximum.
-template <typename E, int D>
-__global__ void __launch_bounds__(32 * kWarps) attend8_kernel(const __grid_constant__ Attn8Params p) {
-    constexpr int DPL = D / 32;
-    pdl_launch_dependents();
-    pdl_wait();
-    const PagedKV& kv = p.kv;
-    const int lane = threadIdx.x & 31, h = blockIdx.y * kWarps + (threadIdx.x >> 5), t = blockIdx.x, j = h / p.G;
-    if (h >= kv.HQ) return;
-    int b = t;
-    if (kv.starts) {
-        if (t < kv.starts[0] || t >= kv.starts[kv.B]) return;
-        int lo = 0, hi = kv.B;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (kv.starts[mid] <= t) lo = mid; else hi = mid;
+int plan8(const bq_paged8_attn_desc* d, Plan8* pl) {
+    const DeviceInfo* di = device_info();
+    if (!di) return BQ_ERR_CUDA;
+    *pl = Plan8{};
+    const int64_t most = !d->kv.q_starts ? 1 : d->max_q > 0 ? d->max_q : (int64_t(d->T) + d->kv.B - 1) / d->kv.B;
+    pl->tile_rows = most * (d->HQ / d->kv.HKV);
+    if (pl->tile_rows <= kNarrowRows) {
+        const int64_t pairs = int64_t(d->kv.B) * d->kv.HKV, room = int64_t(d->kv.max_pages) * d->kv.page_size;
+        int ranks = kNarrowRanks;
+        while (ranks > 1 && pairs * ranks > 2 * di->sm_count) ranks >>= 1;
+        if (ranks > 1 && room <= int64_t(kClusterPositions) * ranks) {
+            pl->ranks = ranks;
+            return BQ_OK;
         }
-        b = lo;
     }
-    int begin, count;
-    paged_rows(kv, b, begin, count);
-    bool cut;
-    const int len = max(paged_len(kv, b, cut), 0);
-    const int limit = p.causal ? max(0, min(len, max(kv.lens[b], 0) - count + (t - begin) + 1)) : len;
-    if (cut && lane == 0) atomicOr(kv.errors, BQ_DEVERR_POSITION_BIT);
-    float q[DPL], o[DPL] = {}, m = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int i = 0; i < DPL; ++i) {
-        const E x = static_cast<const E*>(p.q)[int64_t(t) * p.ldq + h * D + lane * DPL + i];
-        q[i] = float(x);
-    }
-    for (int pos = 0; pos < limit; ++pos) {
-        const int page = paged_page(kv, b, pos, ok), slot = pos & kv.page_mask, blk = slot >> p.sc.block_shift;
-        const uint8_t* kc = static_cast<const uint8_t*>(kv.k) + page * kv.ks_page + j * kv.ks_head + slot * kv.ks_slot + lane * DPL;
-        const uint8_t* vc = static_cast<const uint8_t*>(kv.v) + page * kv.vs_page + j * kv.vs_head + slot * kv.vs_slot + lane * DPL;
-        uint32_t kw, vw;
-        if (DPL == 4) {
-            kw = *reinterpret_cast<const uint32_t*>(kc);
-            vw = *reinterpret_cast<const uint32_t*>(vc);
-        } else {
-            kw = *reinterpret_cast<const uint16_t*>(kc);
-            vw = *reinterpret_cast<const uint16_t*>(vc);
-        }
-        float k[4], v[4], s = 0.f;
-        codes_f32(kw, k);
-        codes_f32(vw, v);
-        for (int i = 0; i < DPL; ++i) s = fmaf(q[i], k[i], s);
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= p.scale_log2 * exp_scale(scale_exp(*k_scale(p.sc, page, j, blk)));
-        const float nm = fmaxf(m, s), u = nm == -INFINITY ? 0.f : nm, f = exp2f(m - u), w = exp2f(s - u);
-        const float sv = exp_scale(scale_exp(*v_scale(p.sc, page, j, blk)));
-        m = nm;
-        l = l * f + w;
-        for (int i = 0; i < DPL; ++i) o[i] = o[i] * f + w * (v[i] * sv);
-    }
-    if (!ok && lane == 0) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
-    const float inv = limit ? 1.f / l : 0.f;
-    for (int i = 0; i < DPL; ++i) static_cast<E*>(p.out)[int64_t(t) * p.ldo + h * D + lane * DPL + i] = E(o[i] * inv);
-    if (p.lse && lane == 0) p.lse[int64_t(t) * p.ldl + h] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    pl->grid = 2 * di->sm_count;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) & ~size_t(255);
+        return here;
+    };
+    const size_t slots = size_t(2) * pl->grid * kNarrowRows;
+    pl->part_o = take(slots * d->kv.D * 4);
+    pl->part_ml = take(slots * 8);
+    pl->shared = take(size_t(pl->grid) * sizeof(PagedShared));
+    pl->total = at;
+    return BQ_OK;
 }
 
 int validate_attention(const bq_paged8_attn_desc* d) {
@@ -185,9 +151,12 @@ extern "C" {
 
 int32_t bq_paged8_attention_workspace_bytes(const bq_paged8_attn_desc* d, size_t* bytes) {
     if (!bytes) return set_error(BQ_ERR_INVALID_ARG, "bytes is NULL");
-    const int rc = validate_attention(d);
+    int rc = validate_attention(d);
     if (rc) return rc;
-    *bytes = 0;
+    Plan8 pl;
+    rc = plan8(d, &pl);
+    if (rc) return rc;
+    *bytes = d->T ? pl.total : 0;
     return BQ_OK;
 }
 
@@ -197,27 +166,36 @@ int32_t bq_paged8_attention(const bq_paged8_attn_desc* d, void* workspace, size_
     if (d->T == 0) return BQ_OK;
     rc = paged_check_device();
     if (rc) return rc;
-    Attn8Params p;
-    std::memset(&p, 0, sizeof(p));
-    rc = paged8_fill(&p.kv, &p.sc, &d->kv, d->T, d->HQ);
+    Plan8 pl;
+    rc = plan8(d, &pl);
     if (rc) return rc;
-    p.G = d->HQ / d->kv.HKV;
-    p.causal = (d->flags & BQ_PAGED_FULL) ? 0 : 1;
-    p.scale_log2 = d->scale * kLog2e;
-    p.q = d->q;
-    p.ldq = d->ldq;
-    p.out = d->out;
-    p.ldo = d->ldo;
-    p.lse = d->lse;
-    p.ldl = d->ldl;
-    (void)workspace, (void)workspace_bytes;
-    const bool bf = d->kv.dtype == BQ_DT_BF16;
-    const void* fn = d->kv.D == 128 ? (bf ? reinterpret_cast<const void*>(&attend8_kernel<__nv_bfloat16, 128>)
-                                          : reinterpret_cast<const void*>(&attend8_kernel<__half, 128>))
-                                    : (bf ? reinterpret_cast<const void*>(&attend8_kernel<__nv_bfloat16, 64>)
-                                          : reinterpret_cast<const void*>(&attend8_kernel<__half, 64>));
-    void* args[] = {&p};
-    return paged_launch(fn, dim3(d->T, (d->HQ + kWarps - 1) / kWarps), dim3(32 * kWarps), 0, args, d->flags, stream, "paged attention");
+    if (pl.total && (!workspace || workspace_bytes < pl.total))
+        return set_error(BQ_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", workspace_bytes, pl.total);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255) return set_error(BQ_ERR_ALIGN, "workspace must be 256-byte aligned");
+    char* ws = static_cast<char*>(workspace);
+    PagedWork w;
+    Paged8Scales sc;
+    std::memset(&w, 0, sizeof(w));
+    std::memset(&sc, 0, sizeof(sc));
+    rc = paged8_fill(&w.kv, &sc, &d->kv, d->T, d->HQ);
+    if (rc) return rc;
+    w.G = d->HQ / d->kv.HKV;
+    w.by_G.set(uint32_t(w.G));
+    w.causal = (d->flags & BQ_PAGED_FULL) ? 0 : 1;
+    w.scale_log2 = d->scale * kLog2e;
+    w.q = d->q;
+    w.ldq = d->ldq;
+    w.out = d->out;
+    w.ldo = d->ldo;
+    w.lse = d->lse;
+    w.ldl = d->ldl;
+    if (pl.ranks) return paged8_launch_cluster(w, sc, d->kv.dtype, d->kv.D, pl.ranks, d->flags, stream);
+    w.part_o = reinterpret_cast<float*>(ws + pl.part_o);
+    w.part_ml = reinterpret_cast<float2*>(ws + pl.part_ml);
+    w.shared = reinterpret_cast<PagedShared*>(ws + pl.shared);
+    rc = paged8_launch_narrow(w, sc, d->kv.dtype, d->kv.D, pl.grid, d->flags, stream);
+    if (rc) return rc;
+    return paged_launch_join(w, d->kv.dtype, d->kv.D, kNarrowRows, pl.grid, false, pl.tile_rows, d->flags, stream);
 }
 
 }  // extern "C"

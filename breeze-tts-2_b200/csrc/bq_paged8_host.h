@@ -7,6 +7,13 @@ namespace bq {
 
 struct Paged8Scales;
 
+// What a tile's start and end cost in units in the kernel for few rows (bq_paged8_narrow.cu), whose tile, unit and
+// warps are those of its 16-bit counterpart.
+constexpr int kNarrow8Overhead = 2;
+int paged8_launch_narrow(const PagedWork& w, const Paged8Scales& sc, int dtype, int D, int grid, uint32_t flags, void* stream);
+// Its form with a cluster of `ranks` CTAs per (sequence, kv head).
+int paged8_launch_cluster(const PagedWork& w, const Paged8Scales& sc, int dtype, int D, int ranks, uint32_t flags, void* stream);
+
 // Checks the cache part of a descriptor with T rows; HQ query heads (0: none).
 int paged8_validate(const bq_paged8_kv* kv, int T, int HQ, bool f32 = false);
 int paged8_fill(PagedKV* out, Paged8Scales* scales, const bq_paged8_kv* kv, int T, int HQ);

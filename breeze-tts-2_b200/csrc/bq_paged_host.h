@@ -23,6 +23,11 @@ int paged_launch_narrow(const PagedWork& w, int dtype, int D, int grid, uint32_t
 constexpr int kNarrowRanks = 8;
 int paged_launch_cluster(const PagedWork& w, int dtype, int D, int ranks, uint32_t flags, void* stream);
 
+// Joins what the CTAs of a schedule over all positions (no prefix) left of the tiles that they share: `grid` CTAs,
+// tiles of `rows` rows of which tile_rows are used as far as is known; wide: the kernel for many rows left them.
+int paged_launch_join(const PagedWork& w, int dtype, int D, int rows, int grid, bool wide, int64_t tile_rows, uint32_t flags,
+                      void* stream);
+
 // Checks the cache part of a descriptor with T new rows of HQ query heads.
 int paged_validate(const bq_paged_kv* kv, int T, int HQ);
 // BQ_OK when the current device is the one this library is built for.
