@@ -61,7 +61,7 @@ class _Python:
     def append(*args):
         return None
 
-    attention = append
+    attention = append8 = attention8 = read8 = append
 
 
 def _native():
@@ -85,6 +85,8 @@ def _native():
             return _bound
         _paged_bind.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
             lib.bq_paged_append, lib.bq_paged_attention, lib.bq_paged_attention_workspace_bytes)))
+        _paged_bind.bind8(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.bq_paged8_append, lib.bq_paged8_attention, lib.bq_paged8_attention_workspace_bytes, lib.bq_paged8_read)))
         _bound = _paged_bind
     return _bound
 

@@ -36,6 +36,7 @@ import ctypes
 import torch
 
 from .. import _lib
+from . import paged
 from .paged import _CACHE_DT, _F32, _I32, _UNIT, _count, _launch, _real, _row_stride, _workspace_bytes_of
 
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -114,6 +115,10 @@ def paged_append_fp8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_
     ``qkv[:, :HQ * D]`` itself, and else shares no memory with ``qkv``. Tokens of
     an unused batch slot (seq_lens[b] less than its new tokens) are skipped where
     their position would be negative. The same call again changes nothing."""
+    done = (paged._bound or paged._native()).append8(qkv, cos, sin, k_pages, v_pages, k_scales, v_scales, page_table, seq_lens,
+                                                     q_starts, q_norm_w, k_norm_w, eps, out, _lib.default_flags())
+    if done is not None:
+        return done if done.__class__ is not int else _lib.check(done, "bq_paged8_append")
     ldqkv = _row_stride(qkv, "qkv")
     rows, width = qkv.shape
     dev, dtype = qkv.get_device(), qkv.dtype
@@ -164,6 +169,11 @@ def paged_attention_fp8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     D^-0.5. ``max_q``: most new tokens of one sequence, a hint that picks the kernel
     (0 or None: T / B rounded up; say it where they differ). ``lse`` (T, HQ) fp32
     receives log(sum(exp(scores))), -inf for a row that sees nothing."""
+    flags = _lib.default_flags() | (0 if causal else _lib.PAGED_FULL)
+    done = (paged._bound or paged._native()).attention8(q, k_pages, v_pages, k_scales, v_scales, page_table, seq_lens, q_starts,
+                                                        scale, max_q, out, lse, flags)
+    if done is not None:
+        return done if done.__class__ is not int else _lib.check(done, "bq_paged8_attention")
     ldq = _row_stride(q, "q")
     rows, width = q.shape
     dev, dtype = q.get_device(), q.dtype
@@ -186,7 +196,6 @@ def paged_attention_fp8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
         lse_ptr, ldl = lse.data_ptr(), _row_stride(lse, "lse")
     max_q = 0 if max_q is None else _count(max_q, "max_q")
     scale = dim ** -0.5 if scale is None else _real(scale, "scale")
-    flags = _lib.default_flags() | (0 if causal else _lib.PAGED_FULL)
     desc = _pack_attn(*fields, rows, hq, max_q, scale, flags, 0, q.data_ptr(), ldq, out.data_ptr(), ldo, lse_ptr, ldl)
     lib = _lib.load()
     size = ctypes.c_size_t(0)
@@ -231,6 +240,10 @@ def paged_read_fp8(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch
         rows = page_table.shape[0]
     else:
         raise ValueError("ragged rows need `rows` or k_out: their number is on the device")
+    done = (paged._bound or paged._native()).read8(k_pages, v_pages, k_scales, v_scales, page_table, seq_lens, q_starts, rows,
+                                                   code, k_out, v_out, _lib.default_flags())
+    if done is not None:
+        return done if done.__class__ is not int else _lib.check(done, "bq_paged8_read")
     dev = k_pages.get_device()
     fields = _cache_fields(dev, rows, code, k_pages, v_pages, k_scales, v_scales, page_table, seq_lens, q_starts)
     hkv, dim = fields[1], fields[2]

@@ -187,6 +187,24 @@ def test_cpu_tensors_are_refused():
         P.paged_read_fp8(*where)
 
 
+def test_the_compiled_calls_leave_what_is_not_plain_to_python():
+    from breeze_b200.fused import paged
+
+    native = paged._native()
+    c = pc.batch([5, 9], None, 2, 1, 64, 16, 16)
+    where = (c["k"], c["v"], c["ks"], c["vs"], c["table"], c["lens"])
+    assert native.attention8(c["q"], *where, None, None, None, None, None, 0) is None  # no GPU
+    assert native.append8(torch.zeros(2, 256, dtype=torch.bfloat16), torch.ones(9, 64), torch.zeros(9, 64), *where, None, None,
+                          None, 1e-6, None, 0) is None
+    assert native.read8(*where, None, 2, L.DT_BF16, None, None, 0) is None
+    for call, n in ((native.attention8, 13), (native.append8, 15), (native.read8, 12)):
+        assert call() is None and call(*[None] * n) is None and call(*["x"] * n) is None
+    with pytest.raises(TypeError, match="four addresses"):
+        native.bind8(1)
+    with pytest.raises(ValueError, match="address 0"):
+        native.bind8(1, 0, 1, 1)
+
+
 class _OnGpu(torch.Tensor):
     """A CPU tensor that says it is on a GPU: reaches the checks behind the first one, never a kernel."""
 
