@@ -35,7 +35,7 @@ BUILD = HERE / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # compiled as whole programs: relocatable code ignores register reallocation (setmaxnreg)
-WHOLE = {"bq_paged_wide"}
+WHOLE = {"bq_paged_wide", "bq_paged8_wide"}
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-rdc=true", "--expt-relaxed-constexpr",
           f"-I{INCLUDE}", f"-I{CSRC}"]
 

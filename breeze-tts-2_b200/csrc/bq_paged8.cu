@@ -88,9 +88,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kClusterPositions = 512;
 
 // How a call is divided: clusters of `ranks` CTAs per (sequence, kv head), or equal shares of all positions for
-// `grid` CTAs with scratch for the tiles that they share.
+// `grid` CTAs with scratch for the tiles (of `rows` rows) that they share.
 struct Plan8 {
-    int ranks, grid;
+    int ranks, grid, rows;
+    bool wide;
     int64_t tile_rows;  // rows of a tile as far as is known
     size_t part_o, part_ml, shared, total;
 };
@@ -110,14 +111,16 @@ int plan8(const bq_paged8_attn_desc* d, Plan8* pl) {
             return BQ_OK;
         }
     }
-    pl->grid = 2 * di->sm_count;
+    pl->wide = pl->tile_rows > kNarrowRows;
+    pl->rows = pl->wide ? kWideRows : kNarrowRows;
+    pl->grid = (pl->wide ? 1 : 2) * di->sm_count;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += (bytes + 255) & ~size_t(255);
         return here;
     };
-    const size_t slots = size_t(2) * pl->grid * kNarrowRows;
+    const size_t slots = size_t(2) * pl->grid * pl->rows;
     pl->part_o = take(slots * d->kv.D * 4);
     pl->part_ml = take(slots * 8);
     pl->shared = take(size_t(pl->grid) * sizeof(PagedShared));
@@ -193,9 +196,9 @@ int32_t bq_paged8_attention(const bq_paged8_attn_desc* d, void* workspace, size_
     w.part_o = reinterpret_cast<float*>(ws + pl.part_o);
     w.part_ml = reinterpret_cast<float2*>(ws + pl.part_ml);
     w.shared = reinterpret_cast<PagedShared*>(ws + pl.shared);
-    rc = paged8_launch_narrow(w, sc, d->kv.dtype, d->kv.D, pl.grid, d->flags, stream);
+    rc = (pl.wide ? paged8_launch_wide : paged8_launch_narrow)(w, sc, d->kv.dtype, d->kv.D, pl.grid, d->flags, stream);
     if (rc) return rc;
-    return paged_launch_join(w, d->kv.dtype, d->kv.D, kNarrowRows, pl.grid, false, pl.tile_rows, d->flags, stream);
+    return paged_launch_join(w, d->kv.dtype, d->kv.D, pl.rows, pl.grid, pl.wide, pl.tile_rows, d->flags, stream);
 }
 
 }  // extern "C"

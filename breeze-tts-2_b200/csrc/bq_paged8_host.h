@@ -9,9 +9,12 @@ struct Paged8Scales;
 
 // What a tile's start and end cost in units in the kernel for few rows (bq_paged8_narrow.cu), whose tile, unit and
 // warps are those of its 16-bit counterpart.
-constexpr int kNarrow8Overhead = 2;
+constexpr int kNarrow8Overhead = 5;
 int paged8_launch_narrow(const PagedWork& w, const Paged8Scales& sc, int dtype, int D, int grid, uint32_t flags, void* stream);
-// Its form with a cluster of `ranks` CTAs per (sequence, kv head).
+// The kernel for many rows (bq_paged8_wide.cu), with the tile and unit of its 16-bit counterpart.
+constexpr int kWide8Overhead = 3;
+int paged8_launch_wide(const PagedWork& w, const Paged8Scales& sc, int dtype, int D, int grid, uint32_t flags, void* stream);
+// The form for few rows with a cluster of `ranks` CTAs per (sequence, kv head).
 int paged8_launch_cluster(const PagedWork& w, const Paged8Scales& sc, int dtype, int D, int ranks, uint32_t flags, void* stream);
 
 // Checks the cache part of a descriptor with T rows; HQ query heads (0: none).
