@@ -87,6 +87,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Most positions per CTA of a cluster that the page table may hold.
 constexpr int kClusterPositions = 512;
 
+// Rows that share a kv head up to which they go to the kernel for few rows, in tiles of 16 of which all but the first find
+// the codes in L2 mostly. Against the 256-row kernel, 4 kv heads of 128 dims: XXX
+constexpr int kFewRows = 96;
+
 // How a call is divided: clusters of `ranks` CTAs per (sequence, kv head), or equal shares of all positions for
 // `grid` CTAs with scratch for the tiles (of `rows` rows) that they share.
 struct Plan8 {
@@ -111,7 +115,7 @@ int plan8(const bq_paged8_attn_desc* d, Plan8* pl) {
             return BQ_OK;
         }
     }
-    pl->wide = pl->tile_rows > kNarrowRows;
+    pl->wide = pl->tile_rows > kFewRows;
     pl->rows = pl->wide ? kWideRows : kNarrowRows;
     pl->grid = (pl->wide ? 1 : 2) * di->sm_count;
     size_t at = 0;
@@ -196,7 +200,8 @@ int32_t bq_paged8_attention(const bq_paged8_attn_desc* d, void* workspace, size_
     w.part_o = reinterpret_cast<float*>(ws + pl.part_o);
     w.part_ml = reinterpret_cast<float2*>(ws + pl.part_ml);
     w.shared = reinterpret_cast<PagedShared*>(ws + pl.shared);
-    rc = (pl.wide ? paged8_launch_wide : paged8_launch_narrow)(w, sc, d->kv.dtype, d->kv.D, pl.grid, d->flags, stream);
+    rc = pl.wide ? paged8_launch_wide(w, sc, &d->kv, pl.grid, d->flags, stream)
+                 : paged8_launch_narrow(w, sc, d->kv.dtype, d->kv.D, pl.grid, d->flags, stream);
     if (rc) return rc;
     return paged_launch_join(w, d->kv.dtype, d->kv.D, pl.rows, pl.grid, pl.wide, pl.tile_rows, d->flags, stream);
 }

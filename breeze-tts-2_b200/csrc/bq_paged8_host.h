@@ -13,7 +13,7 @@ constexpr int kNarrow8Overhead = 5;
 int paged8_launch_narrow(const PagedWork& w, const Paged8Scales& sc, int dtype, int D, int grid, uint32_t flags, void* stream);
 // The kernel for many rows (bq_paged8_wide.cu), with the tile and unit of its 16-bit counterpart.
 constexpr int kWide8Overhead = 3;
-int paged8_launch_wide(const PagedWork& w, const Paged8Scales& sc, int dtype, int D, int grid, uint32_t flags, void* stream);
+int paged8_launch_wide(const PagedWork& w, const Paged8Scales& sc, const bq_paged8_kv* kv, int grid, uint32_t flags, void* stream);
 // The form for few rows with a cluster of `ranks` CTAs per (sequence, kv head).
 int paged8_launch_cluster(const PagedWork& w, const Paged8Scales& sc, int dtype, int D, int ranks, uint32_t flags, void* stream);
 

@@ -19,25 +19,39 @@ constexpr int kThreads = 256, kMostRows = 32, kHeads = 4, kFlight = 4;
 struct Read8Params {
     PagedKV kv;
     Paged8Scales sc;
-    int32_t window;
+    int32_t window, aligned;  // rows of a CTA; outputs 32-byte aligned
     void* k_out;
     int64_t ko_row, ko_head;
     void* v_out;
     int64_t vo_row, vo_head;
 };
 
+// 32 bytes by one instruction where they are aligned: a warp then writes whole sectors.
+__device__ __forceinline__ void store32(void* dst, const uint4& a, const uint4& b, bool aligned) {
+    if (aligned) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x),
+                     "r"(b.y), "r"(b.z), "r"(b.w)
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4*>(dst)[0] = a;
+        reinterpret_cast<uint4*>(dst)[1] = b;
+    }
+}
 template <typename T>
-__device__ __forceinline__ void store16(T* dst, const float (&v)[16]) {
+__device__ __forceinline__ void store16(T* dst, const float (&v)[16], bool aligned) {
     if constexpr (sizeof(T) == 4) {
+        uint4 x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            x[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                              __float_as_uint(v[4 * i + 3]));
+        store32(dst, x[0], x[1], aligned);
+        store32(dst + 8, x[2], x[3], aligned);
     } else {
         float a[8], b[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = v[i], b[i] = v[8 + i];
-        reinterpret_cast<uint4*>(dst)[0] = pack8<T>(a);
-        reinterpret_cast<uint4*>(dst)[1] = pack8<T>(b);
+        store32(dst, pack8<T>(a), pack8<T>(b), aligned);
     }
 }
 
@@ -133,7 +147,7 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
                         v[4 * q + k] = v[4 * q + k] > 65504.f ? 65504.f : v[4 * q + k] < -65504.f ? -65504.f : v[4 * q + k];
                 }
             }
-            store16<T>(out + (w0 + r) * o_row + h * o_head + c * 16, v);
+            store16<T>(out + (w0 + r) * o_row + h * o_head + c * 16, v, p.aligned);
         }
     }
 }
@@ -179,6 +193,9 @@ extern "C" int32_t bq_paged8_read(const bq_paged8_read_desc* d, void* stream) {
     p.v_out = d->v_out;
     p.vo_row = d->vo_stride[0];
     p.vo_head = d->vo_stride[1];
+    p.aligned = ((reinterpret_cast<uintptr_t>(d->k_out) | reinterpret_cast<uintptr_t>(d->v_out)) & 31) == 0;
+    for (int i = 0; i < 2; ++i)
+        if (size[i] > 1 && (d->ko_stride[i] * elem % 32 || d->vo_stride[i] * elem % 32)) p.aligned = 0;
     const void* fn = d->kv.D == 128 ? read_kernel<128>(d->kv.dtype) : read_kernel<64>(d->kv.dtype);
     void* args[] = {&p};
     return paged_launch(fn, dim3((d->T + p.window - 1) / p.window, 2 * ((d->kv.HKV + kHeads - 1) / kHeads)), dim3(kThreads), 0, args,

@@ -4,23 +4,23 @@
 // in one score buffer, probabilities and outputs stay in tensor memory, roles walk
 // ahead. What differs is how k and v come in, and the scales.
 //
-// The tensor cores take both operands in one type, so codes are converted: four warps
-// copy them (cp.async, one unit ahead, each lane what it will convert itself) and write
-// them as 16-bit tiles in the swizzled layout of the products, once for the 256 rows.
-// Keys become the queries' type, values fp16; either holds every code exactly. Queries
-// split into e4m3 terms would leave the keys as they are, but probabilities need more
-// range than e4m3 has, so values have to be converted all the same.
+// The tensor cores take both operands in one type, so codes are converted: a warp
+// fetches them by TMA, a unit ahead, four others write them as 16-bit tiles in the
+// swizzled layout of the products, once for the 256 rows. Keys become the queries' type,
+// values fp16; either holds every code exactly. Queries split into e4m3 terms would leave
+// the keys as they are, but probabilities need more range than e4m3 has, so values have
+// to be converted all the same.
 //
 // Scales: 2^ek multiplies the scores of a block, 2^ev goes into the exponent of its
 // probabilities, as in the kernel for few rows: the weights are 2^(s + ev - M + 7), M a
 // reference that may lag behind the largest s + ev by up to 8, so at most 2^15 in fp16.
-// The converting warps leave each unit's eight pairs of factors in shared memory. Where
+// The fetching warp leaves each unit's eight sets of factors in shared memory. Where
 // the ev of a unit lie more than 100 below one of the tile so far, weights that fp32
 // flushes might still count in the sum of exponentials, which is then computed on its own.
 //
 // Roles (one CTA per SM, all 512 tensor-memory columns): warps 0-3, 4-7 softmax of half
 // 0 / 1; 8 issues the scores' products, 9 the outputs'; 10 walks the tiles and fetches
-// their queries; 12-15 convert.
+// their queries; 11 fetches codes and scales; 12-15 convert.
 #include "bq_paged8.cuh"
 #include "bq_paged8_host.h"
 #include "bq_paged_wide.cuh"
@@ -28,10 +28,13 @@
 namespace bq {
 
 struct Wide8Params {
-    CUtensorMap qmap;  // (D, heads, rows), boxes of 64 dims x 128 rows
+    CUtensorMap qmap, kmap, vmap;  // queries: (D, heads, rows), boxes of 64 dims x 128 rows; codes: (D, then slot, head and
+                                   // page in order of stride), boxes of positions of one page
     PagedWork w;
     Paged8Scales sc;
-    int32_t q_tma;     // the queries come by TMA
+    int32_t q_tma;                           // the queries come by TMA
+    int32_t box;                             // positions per box: min(page size, 128)
+    int32_t k_slot, k_head, v_slot, v_head;  // which of coordinates 1 .. 3 is the slot, the head (the third is the page)
     uint32_t idesc_qk, idesc_pv;
     long long wait_cycles;
 };
@@ -40,11 +43,11 @@ namespace {
 
 constexpr int kThreads = 512;
 // Registers: the CTA starts with 512 x 128; the third and fourth warpgroup give up what the softmax warps, a row of
-// 128 scores per thread, need more (256 x 208 + 256 x 48). The file is compiled as a whole program, since relocatable
+// 128 scores per thread, need more (256 x 200 + 256 x 56). The file is compiled as a whole program, since relocatable
 // code may not move registers.
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 48;
-constexpr int kScores = 8, kOutputs = 9, kWalker = 10, kConvert = 12;  // warps of the roles behind the softmax
-constexpr int kReaders = 14;      // warps that read a tile of the walker's
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 56;
+constexpr int kScores = 8, kOutputs = 9, kWalker = 10, kFetch = 11, kConvert = 12;  // warps of the roles behind the softmax
+constexpr int kReaders = 15;      // warps that read a tile of the walker's
 constexpr int kBlocks = kUnit / 16;
 constexpr int kLift = 7, kFarLift = 64;  // weights are kept times 2^7; where that is not enough, their sum is of 2^64 times
 constexpr int kSpread = 100;
@@ -53,10 +56,10 @@ template <int D>
 struct Wide8Smem {
     static constexpr uint32_t kTile = 128 * D * 2;                   // one k or v tile, one half of the queries
     static constexpr int kStages = D == 128 ? 4 : 8;
-    // Units whose factors are kept. When those of unit U are written, its keys' stage is free: the scores of unit
-    // U - kStages / 2 have been multiplied, so that both halves have read those of the unit before and are done with
-    // all before that.
-    static constexpr int kTables = kStages / 2 + 2;
+    // Units whose factors are kept. When those of unit U are written, the keys of U - 1 have been converted, so their
+    // stage was free: the scores of U - 1 - kStages / 2 have been multiplied, both halves have read those of the unit
+    // before, and are done with all before that.
+    static constexpr int kTables = kStages / 2 + 3;
     static constexpr uint32_t kRing = 2 * kTile;
     static constexpr uint32_t kCodes = kRing + kStages * kTile;      // the codes of a k and a v tile on their way
     static constexpr uint32_t kBars = kCodes + kTile;
@@ -65,6 +68,13 @@ struct Wide8Smem {
 
 // NaN among four codes: 0xff in its byte.
 __device__ __forceinline__ uint32_t nan4(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
+
+__device__ __forceinline__ void lds128(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t t) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(t) : "memory");
+}
 
 // Four codes -> four elements (exact).
 template <typename E>
@@ -81,34 +91,47 @@ __device__ __forceinline__ uint2 codes_to(uint32_t w) {
     }
 }
 
-// A lane's 16-byte pieces of a 128-position tile: rows row(k), codes 16 c .. 16 c + 15. Eight neighbouring lanes have
-// two rows that differ in bit 0, so that their swizzled chunks fall on different banks.
+// A lane's 16-byte pieces of a 128-position tile: codes 16 c .. 16 c + 15 of rows row(k). Eight neighbouring lanes have
+// two rows that differ in bit 0, so that their chunks of the converted tile fall on different banks, and, with rows of
+// 128 bytes, in bit 2, so that those of the codes (128-byte swizzle, too) do.
 template <int D>
 struct Piece {
-    static constexpr int kRowsPerWarp = D == 128 ? 4 : 8, kCount = 128 / (4 * kRowsPerWarp);
-    int warp, first, c;
-    __device__ __forceinline__ Piece(int warp_, int lane)
-        : warp(warp_), first(kRowsPerWarp * warp_ + (lane >> 2) % kRowsPerWarp), c((lane & 3) + (D == 128 ? (lane >> 4) * 4 : 0)) {}
-    __device__ __forceinline__ int row(int k) const { return 4 * kRowsPerWarp * k + first; }
-    __device__ __forceinline__ int block(int k) const { return D == 128 ? k : 2 * k + (warp >> 1); }  // of 16 positions
-    // of the first of its two chunks in a tile; the second is at ^ 16
-    __device__ __forceinline__ uint32_t at(int k) const {
+    static constexpr int kCount = D == 128 ? 8 : 4, kStep = D == 128 ? 2 : 1;  // rows k and k + kStep are 32 apart
+    int first, c;
+    __device__ __forceinline__ Piece(int warp, int lane) {
+        const int sub = lane >> 2;
+        first = 8 * warp + (D == 128 ? (sub & 2) | (sub & 1) * 5 : sub);
+        c = (lane & 3) + (D == 128 ? (lane >> 4) * 4 : 0);
+    }
+    __device__ __forceinline__ int row(int k) const { return 32 * (k / kStep) + (first ^ (k % kStep)); }
+    __device__ __forceinline__ uint32_t from(int k) const {  // in the codes
+        const int r = row(k);
+        return r * D + ((D == 128 ? c ^ (r & 7) : c) << 4);
+    }
+    __device__ __forceinline__ uint32_t to(int k) const {  // of its first chunk in the tile; the second is at ^ 16
         const int r = row(k);
         return (c >> 2) * (128 * 128) + r * 128 + ((((c & 3) * 2) ^ (r & 7)) << 4);
     }
 };
 
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+        : "memory");
+}
+
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_constant__ Wide8Params p) {
     using SM = Wide8Smem<D>;
     constexpr int ST = SM::kStages, kTables = SM::kTables;
-    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    extern __shared__ __align__(128) unsigned char smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ PagedPrefix s_prefix;  // (none: the shared pieces want one)
     __shared__ WideTile s_tile[kTiles];
     __shared__ volatile int s_bad[kTiles];   // n + 1: NaN entries of v were cleared from tile n
-    __shared__ float2 s_factor[kTables][kBlocks];  // per block: scores times x, plus y, in base 2
+    __shared__ float4 s_factor[kTables][kBlocks];  // per block: scores times x, plus y, in base 2; sums times z
     __shared__ int s_far[kTables];           // the unit's sum of exponentials needs the longer way
     const uint32_t sraw = smem_u32(smem_raw), sb = (sraw + 1023u) & ~1023u;
     const PagedWork& w = p.w;
@@ -117,10 +140,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
     volatile int* abort = &s_abort;
     const long long lim = p.wait_cycles;
     // full / empty per ring stage; per half: queries staged, scores ready, probabilities written, second product
-    // complete, queries used; scores read; per tile in s_tile: written, read by all its readers
+    // complete, queries used; scores read; per tile in s_tile: written, read by all its readers; codes of keys / values
+    // there, converted
     const uint32_t bar_full = sb + SM::kBars, bar_empty = bar_full + 64, bar_q = bar_full + 128, bar_s = bar_full + 144,
                    bar_p = bar_full + 160, bar_pv = bar_full + 176, bar_read = bar_full + 192, bar_done = bar_full + 200,
-                   bar_used = bar_full + 216, bar_tile = bar_full + 232, bar_free = bar_full + 264;
+                   bar_used = bar_full + 216, bar_tile = bar_full + 232, bar_free = bar_full + 264, bar_codes = bar_full + 296,
+                   bar_taken = bar_full + 312;
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) {
             mbar_init(bar_full + 8 * i, 4);  // an arrival per converting warp
@@ -132,6 +157,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
             mbar_init(bar_s + 8 * h, 1);
             mbar_init(bar_p + 8 * h, 4);  // an arrival per warp
             mbar_init(bar_pv + 8 * h, 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(bar_codes + 8 * x, 1);
+            mbar_init(bar_taken + 8 * x, 4);
         }
         mbar_init(bar_read, 4);
         mbar_init(bar_done, 1);
@@ -184,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                 release(n);
                 continue;
             }
-            const int myrow = t.r0 + 128 * h + row, units = t.nu, p0 = t.p0, p1 = t.p1, table = t.ring >> 1;
+            const int myrow = t.r0 + 128 * h + row, units = t.nu, p0 = t.p0, p1 = t.p1, table = t.ring >> 1, seen = t.seen;
             const bool idle = (warp & 3) * 32 >= hrows;  // no row of this warp exists
             const int limit = row < hrows ? paged_row_limit<false>(w, t.s, myrow) : 0;
             float mref = -INFINITY, l = 0.f;
@@ -194,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                 if (!ok) break;
                 tc_fence_after();
                 const int base = p0 + u * kUnit;
-                const float2* factor = s_factor[(table + u) % kTables];
+                const float4* factor = s_factor[(table + u) % kTables];
                 float s[128];
                 if (!idle) {
 #pragma unroll
@@ -204,32 +233,58 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_read);  // the score buffer may be written again
-                if (!idle && base + kUnit > limit) {
+                if (__builtin_expect(!idle && base + kUnit > seen, 0)) {  // some row of the tile does not see all
                     const int sees = limit - base;
 #pragma unroll
                     for (int i = 0; i < 128; ++i) s[i] = i < sees ? s[i] : -INFINITY;
                 }
-                if (!idle && u == 0) {  // the tile's first reference
-                    mref = -INFINITY;
+                __syncwarp();
+                if (!idle) {
+                    // The largest s + ev, and a new reference where it is more than 8 above: for most data a unit's weights
+                    // would else be computed twice (6500 positions of keys with uneven channels and levels: XXX us, YYY here).
+                    float m = -INFINITY;
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b) {
-                        float mx = s[16 * b];
+                        const float4 fb = factor[b];
+                        float mx[2] = {s[16 * b], s[16 * b + 1]};
 #pragma unroll
-                        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[16 * b + i]);
-                        mref = fmaxf(mref, fmaf(mx, factor[b].x, factor[b].y));
+                        for (int i = 1; i < 8; ++i) mx[i & 1] = max3(mx[i & 1], s[16 * b + 2 * i], s[16 * b + 2 * i + 1]);
+                        m = fmaxf(m, fmaf(fmaxf(mx[0], mx[1]), fb.x, fb.y));
                     }
-                }
-                __syncwarp();
-                // A warp without rows arrives with the others all the same, and never a unit ahead of them: it, too, waits
-                // for the product before (its early arrival would count as another warp's).
-                if (idle && u > 0) ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
-                if (!ok) break;
-                // Weights against the reference as it stands, and the maximum beside them; only where a
-                // maximum turns out to have moved by more than the allowance are they computed once more.
-                bool again = !idle, first = u > 0;
-                while (again) {
+                    const bool move = u == 0 || m > mref + 8.f;
+                    if (__builtin_expect(u > 0 && __any_sync(0xffffffffu, move), 0)) {
+                        ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const float f = move ? ex2(0.5f * (mref - m)) : 1.f;  // in two steps: l may be as far from 1
+                        l = l * f * f;
+#pragma unroll 1
+                        for (int q = 0; q < D / 16; ++q) {
+                            float o[16];
+                            tmem_ld16(t_o + 16 * q, o);
+                            uint32_t o2[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o2[i] = __float_as_uint(o[i] * f * f);
+                            tmem_st16(t_o + 16 * q, o2);
+                        }
+                    }
+                    if (move) mref = m;
                     const float off = (mref == -INFINITY ? 0.f : -mref) + kLift;
-                    float m = -INFINITY, sum = 0.f;
+                    const bool far = s_far[(table + u) % kTables];
+                    if (__builtin_expect(far, 0)) {  // (before the weights, which let go of the scores)
+                        const float up = off + (kFarLift - kLift);
+                        float all = 0.f;
+#pragma unroll
+                        for (int b = 0; b < kBlocks; ++b) {
+                            const float4 fb = factor[b];
+                            float part = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) part += ex2(fmaf(s[16 * b + i], fb.x, fb.y + up));
+                            all = fmaf(part, fb.z * exp_scale(kLift - kFarLift), all);
+                        }
+                        l += all;
+                    }
+                    float sum = 0.f;
                     // The first kHeld quarters wait in registers for the product before, which still reads its weights.
                     constexpr int kHeld = 2;
                     uint32_t held[kHeld][16], now[16];
@@ -238,14 +293,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                         uint32_t(&pk)[16] = q < kHeld ? held[q < kHeld ? q : 0] : now;
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
-                            const float2 fb = factor[2 * q + b];
+                            const float4 fb = factor[2 * q + b];
                             const uint64_t sc2 = f2(fb.x, fb.x), off2 = f2(fb.y + off, fb.y + off);
                             uint64_t part = 0;
-                            float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 const float x = s[32 * q + 16 * b + 2 * i], y = s[32 * q + 16 * b + 2 * i + 1];
-                                mx[i & 1] = max3(mx[i & 1], x, y);
                                 float a, d;
                                 unf2(fma2(f2(x, y), sc2, off2), a, d);
                                 a = ex2(a);
@@ -255,14 +308,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                             }
                             float a, d;
                             unf2(part, a, d);
-                            sum = fmaf(a + d, exp_scale(-int(fb.y) - kLift), sum);
-                            m = fmaxf(m, fmaf(fmaxf(mx[0], mx[1]), fb.x, fb.y));
+                            sum = fmaf(a + d, fb.z, sum);
                         }
-                        if (q == kHeld - 1 && first) {  // it has read its weights and written its outputs
+                        if (q == kHeld - 1 && u > 0) {  // it has read its weights and written its outputs
                             ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
                             if (!ok) break;
                             tc_fence_after();
-                            first = false;
                         }
                         if (q == kHeld - 1) {
 #pragma unroll
@@ -272,40 +323,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                         }
                     }
                     if (!ok) break;
-                    const bool move = m > mref + 8.f;  // also the first finite maximum
-                    again = __any_sync(0xffffffffu, move);
-                    if (again) {
-                        tmem_wait_st();  // the weights are about to be written again, and stores have no order of their own
-                        const float f = move ? ex2(0.5f * (mref - m)) : 1.f;  // in two steps: l may be as far from 1
-                        mref = move ? m : mref;
-                        l = l * f * f;
-                        if (u > 0) {
-#pragma unroll 1
-                            for (int q = 0; q < D / 16; ++q) {
-                                float o[16];
-                                tmem_ld16(t_o + 16 * q, o);
-                                uint32_t o2[16];
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) o2[i] = __float_as_uint(o[i] * f * f);
-                                tmem_st16(t_o + 16 * q, o2);
-                            }
-                        }
-                    } else {
-                        if (s_far[(table + u) % kTables]) {
-                            sum = 0.f;
-                            const float far = (mref == -INFINITY ? 0.f : -mref) + kFarLift;
-#pragma unroll
-                            for (int b = 0; b < kBlocks; ++b) {
-                                const float2 fb = factor[b];
-                                float part = 0.f;
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) part += ex2(fmaf(s[16 * b + i], fb.x, fb.y + far));
-                                sum = fmaf(part, exp_scale(-int(fb.y) - kFarLift), sum);
-                            }
-                        }
-                        l += sum;
-                        tmem_wait_st();
-                    }
+                    if (!far) l += sum;
+                    tmem_wait_st();
+                } else if (u > 0) {
+                    // A warp without rows arrives with the others all the same, and never a unit ahead of them: it, too, waits
+                    // for the product before (its early arrival would count as another warp's).
+                    ok = __all_sync(0xffffffffu, tc_wait(bar_pv + 8 * h, (done_units - 1) & 1, abort, lim, kv.errors));
                 }
                 if (!ok) break;
                 ++done_units;
@@ -386,112 +409,63 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
         if (warp >= kConvert) {
             // -------------------------------------------------------- codes -> tiles
             const Piece<D> piece(warp - kConvert, lane);
-            const uint32_t codes = sb + SM::kCodes + (threadIdx.x & 127) * 16;
-            bool pages_ok = true;
-            int next = 0, nu = 0, np0 = 0, np1 = 0, u_next = 0, page = 0, nj = 0;  // the unit to be copied: tile, units, ...
-            auto open = [&]() {  // the tile `next`; without one, nu = 0
-                wait(bar_tile + 8 * (next % kTiles), next / kTiles);
-                nu = 0;
-                u_next = 0;
-                if (!ok) return;
-                const WideTile& t = tile(next);
-                if (!t.valid) return;
-                nu = t.nu, np0 = t.p0, np1 = t.p1, nj = t.j;
-            };
-            auto look = [&]() {  // the pages of its blocks of 16 positions, a lane each
-                const int pos = np0 + u_next * kUnit + 16 * lane;
-                page = 0;
-                if (nu > 0 && lane < kBlocks && pos < np1) page = paged_page(kv, tile(next).s.table, pos, pages_ok);
-            };
-            auto copy = [&](int x) {  // its keys (0) or values (1)
-                if (nu > 0) {
-                    const int base = np0 + u_next * kUnit;
-                    const uint8_t* from = static_cast<const uint8_t*>(x ? kv.v : kv.k) + nj * (x ? kv.vs_head : kv.ks_head) + piece.c * 16;
-                    const int64_t st_page = x ? kv.vs_page : kv.ks_page, st_slot = x ? kv.vs_slot : kv.ks_slot;
-#pragma unroll
-                    for (int k = 0; k < Piece<D>::kCount; ++k) {
-                        const int pos = base + piece.row(k), pg = __shfl_sync(0xffffffffu, page, piece.block(k));
-                        cp_async16_zfill(codes + x * (SM::kTile / 2) + k * 2048, from + pg * st_page + (pos & kv.page_mask) * st_slot,
-                                         pos < np1);
-                    }
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            open();
-            look();
-            int here = page;  // pages of the unit to be converted
-            copy(0);
-            copy(1);
-            int it = 0, top = 0;
-            for (int n = 0; ok && nu > 0;) {
-                const int u = u_next, units = nu, p0 = np0, p1 = np1, j = nj, base = p0 + u * kUnit;
-                const int seen = tile(n).seen;
-                if (++u_next == nu) {
-                    ++next;
-                    open();
-                    if (!ok) break;
-                }
-                look();
-                uint32_t byte = kExpBias;  // lanes 0 .. 7: of k, 8 .. 15: of v
-                if (piece.warp == 0) {
-                    const int b = lane & 7, pg = __shfl_sync(0xffffffffu, here, b), pos = base + 16 * b,
-                              blk = (pos & kv.page_mask) >> p.sc.block_shift;
-                    if (lane < 16 && pos < p1) byte = lane < 8 ? *k_scale(p.sc, pg, j, blk) : *v_scale(p.sc, pg, j, blk);
-                }
+            int it = 0;
+            for (int n = 0;; ++n) {
+                wait(bar_tile + 8 * (n % kTiles), n / kTiles);
+                if (!ok || !tile(n).valid) break;
+                const int units = tile(n).nu, p0 = tile(n).p0, p1 = tile(n).p1, seen = min(p1, tile(n).seen);
+                release(n);
+                for (int u = 0; ok && u < units; ++u) {
+                    const int base = p0 + u * kUnit;
+                    auto convert = [&](auto type, int x) {
+                        using T = decltype(type);
+                        const int st = it % ST;
+                        wait(bar_codes + 8 * x, it >> 1);
+                        if (ok && it >= ST) wait(bar_empty + 8 * st, it / ST + 1);
+                        if (!ok) return;
+                        const uint32_t src = sb + SM::kCodes + x * (SM::kTile / 2), dst = sb + SM::kRing + st * SM::kTile;
+                        if (x == 1 && base + kUnit > seen) {  // rows of v that no position owns, or, where they are NaN, not every row sees
 #pragma unroll 1
-                for (int x = 0; ok && x < 2; ++x, ++it) {
-                    const int st = it % ST;
-                    if (it >= ST) wait(bar_empty + 8 * st, it / ST + 1);
-                    if (!ok) break;
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    const uint32_t dst = sb + SM::kRing + st * SM::kTile;
+                            for (int k = 0; k < Piece<D>::kCount; ++k) {
+                                const int pos = base + piece.row(k);
+                                if (pos < seen) continue;
+                                uint32_t q[4], bad = 0;
+                                lds128(q, src + piece.from(k));
 #pragma unroll
-                    for (int k = 0; k < Piece<D>::kCount; ++k) {
-                        uint32_t q[4];
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
-                                     : "r"(codes + x * (SM::kTile / 2) + k * 2048) : "memory");
-                        if (x == 1 && base + piece.row(k) >= seen) {  // a value that not every row sees
-                            uint32_t bad = 0;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t nan = nan4(q[e]);
-                                bad |= nan;
-                                q[e] &= ~nan;
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint32_t out = pos < p1 ? nan4(q[e]) : 0xffffffffu;
+                                    bad |= out;
+                                    q[e] &= ~out;
+                                }
+                                if (bad) sts128(src + piece.from(k), q[0], q[1], q[2], q[3]);
+                                if (bad && pos < p1) s_bad[n % kTiles] = n + 1;
                             }
-                            if (bad) s_bad[n % kTiles] = n + 1;
                         }
-                        const uint32_t a = dst + piece.at(k);
+                        // Rolled: with the pieces unrolled the roles' loops exceed the instruction cache, and every phase behind
+                        // a wait begins with its misses (prompt of 6500 positions: all unrolled 314 us, pairs 260, so 251).
+#pragma unroll 1
+                        for (int k = 0; k < Piece<D>::kCount; ++k) {
+                            uint32_t q[4];
+                            lds128(q, src + piece.from(k));
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const uint2 lo = x ? codes_to<__half>(q[2 * half]) : codes_to<E>(q[2 * half]),
-                                        hi = x ? codes_to<__half>(q[2 * half + 1]) : codes_to<E>(q[2 * half + 1]);
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a ^ (half << 4)), "r"(lo.x), "r"(lo.y), "r"(hi.x),
-                                         "r"(hi.y) : "memory");
+                            for (int half = 0; half < 2; ++half) {
+                                const uint2 lo = codes_to<T>(q[2 * half]), hi = codes_to<T>(q[2 * half + 1]);
+                                sts128(dst + (piece.to(k) ^ (half << 4)), lo.x, lo.y, hi.x, hi.y);
+                            }
                         }
-                    }
-                    if (x == 0 && piece.warp == 0) {  // the unit's factors
-                        const int e = scale_exp(byte), ev = __shfl_down_sync(0xffffffffu, e, 8);
-                        const bool live = lane < kBlocks && base + 16 * lane < p1;
-                        if (u == 0) top = -kExpMost;
-                        top = max(top, __reduce_max_sync(0xffffffffu, live ? ev : -kExpMost));
-                        const int least = __reduce_min_sync(0xffffffffu, live ? ev : kExpMost), slot = (it >> 1) % kTables;
-                        if (lane < kBlocks) s_factor[slot][lane] = make_float2(fmaxf(w.scale_log2 * exp_scale(e), 1e-37f), live ? float(ev) : 0.f);
-                        if (lane == 0) s_far[slot] = top - least > kSpread;
-                    }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar_full + 8 * st);
-                    copy(x);
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(bar_full + 8 * st);
+                            mbar_arrive(bar_taken + 8 * x);
+                        }
+                        ++it;
+                    };
+                    convert(E(), 0);
+                    if (ok) convert(__half(), 1);
                 }
                 if (!ok) break;
-                here = page;
-                if (u + 1 == units) {
-                    release(n);
-                    ++n;
-                }
             }
-            if (!pages_ok) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
-            asm volatile("cp.async.wait_all;" ::: "memory");
         } else {
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             if (warp == kScores) {
@@ -601,6 +575,84 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                 if (used0 > 0) tc_wait(bar_q, (used0 - 1) & 1, nullptr, lim, kv.errors);
                 if (used1 > 0) tc_wait(bar_q + 8, (used1 - 1) & 1, nullptr, lim, kv.errors);
                 __syncwarp();
+            } else if (warp == kFetch) {
+                // ---------------------------------------------------- codes and factors
+                int unit = 0, values = 0, next = 0, nu = 0, u = 0, p0 = 0, p1 = 0, j = 0, page = 0, top = 0;
+                uint32_t byte = 0;
+                bool pages_ok = true;
+                auto open = [&]() {  // the tile `next`; without one, nu = 0
+                    nu = u = 0;
+                    wait(bar_tile + 8 * (next % kTiles), next / kTiles);
+                    if (!ok) return;
+                    const WideTile& t = tile(next);
+                    if (t.valid) nu = t.nu, p0 = t.p0, p1 = t.p1, j = t.j;
+                };
+                // Of its unit u: pages of the boxes, a lane each; then scales of its blocks, of k in lanes 0 .. 7, of v in
+                // 8 .. 15. Asked for a unit ahead, between the waits for the converting warps.
+                auto pages = [&]() {
+                    const int at = p0 + u * kUnit + lane * p.box;
+                    page = 0;
+                    if (lane * p.box < kUnit && at < p1) page = paged_page(kv, tile(next).s.table, at, pages_ok);
+                };
+                auto scales = [&]() {
+                    const int b = lane & 7, pos = p0 + u * kUnit + 16 * b, blk = (pos & kv.page_mask) >> p.sc.block_shift;
+                    const int pg = __shfl_sync(0xffffffffu, page, 16 * b / p.box);
+                    byte = kExpBias;
+                    if (lane < 16 && pos < p1) byte = lane < 8 ? *k_scale(p.sc, pg, j, blk) : *v_scale(p.sc, pg, j, blk);
+                };
+                open();
+                if (ok && nu > 0) {
+                    pages();
+                    scales();
+                }
+                while (ok && nu > 0) {
+                    const int base = p0 + u * kUnit, slot = (base + lane * p.box) & kv.page_mask, here = page, end = p1, head = j;
+                    const int nb = max(0, (min(kUnit, end - base) + p.box - 1) / p.box);  // boxes that hold positions
+                    auto fetch = [&](int x) {
+                        const uint32_t bar = bar_codes + 8 * x;
+                        if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(nb * p.box) * D);
+                        __syncwarp();
+                        if (lane < nb) {
+                            const int ps = x ? p.v_slot : p.k_slot, ph = x ? p.v_head : p.k_head;
+                            const int c1 = ps == 1 ? slot : ph == 1 ? head : here, c2 = ps == 2 ? slot : ph == 2 ? head : here,
+                                      c3 = ps == 3 ? slot : ph == 3 ? head : here;
+                            tma_load_4d(sb + SM::kCodes + x * (SM::kTile / 2) + uint32_t(lane * p.box) * D, x ? &p.vmap : &p.kmap, 0, c1, c2, c3,
+                                        bar);
+                        }
+                    };
+                    if (unit > 0) wait(bar_taken, unit - 1);
+                    if (!ok) break;
+                    // the unit's factors, for which the arrival for its keys speaks, too
+                    const int e = scale_exp(byte), ev = __shfl_down_sync(0xffffffffu, e, 8);
+                    const bool live = lane < kBlocks && base + 16 * lane < end;
+                    if (u == 0) top = -kExpMost;
+                    top = max(top, __reduce_max_sync(0xffffffffu, live ? ev : -kExpMost));
+                    const int least = __reduce_min_sync(0xffffffffu, live ? ev : kExpMost), y = live ? ev : 0;
+                    if (lane < kBlocks)
+                        s_factor[unit % kTables][lane] =
+                            make_float4(fmaxf(w.scale_log2 * exp_scale(e), 1e-37f), float(y), exp_scale(-y - kLift), 0.f);
+                    if (lane == 0) s_far[unit % kTables] = top - least > kSpread;
+                    __syncwarp();
+                    fetch(0);
+                    if (++u == nu) {
+                        release(next);
+                        ++next;
+                        open();
+                        if (!ok) nu = 0;  // (the keys are on their way: the end below waits for them)
+                    }
+                    if (nu > 0) pages();
+                    ++unit;
+                    if (ok && unit > 1) wait(bar_taken + 8, unit - 2);
+                    if (!ok) break;
+                    fetch(1);
+                    ++values;
+                    if (nu > 0) scales();
+                }
+                if (!pages_ok) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
+                // no codes may still be landing when the CTA leaves
+                if (unit > 0) tc_wait(bar_codes, (unit - 1) & 1, nullptr, lim, kv.errors);
+                if (values > 0) tc_wait(bar_codes + 8, (values - 1) & 1, nullptr, lim, kv.errors);
+                __syncwarp();
             }
             if (warp <= kOutputs) {  // every product issued above has finished once this completes
                 const uint32_t done = bar_done + 8 * (warp - kScores);
@@ -617,9 +669,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
     if (warp == kScores) tmem_dealloc(tmem, kCols);
 }
 
+// Tensor map of pages of codes (strides st: page, head, slot): dims are D, then the other three in order of their
+// strides; `slot` and `head` receive the coordinate (1 .. 3) of each.
+int encode_codes(const bq_paged8_kv* kv, const void* base, const int64_t* st, int box, CUtensorMap* map, int32_t* slot, int32_t* head) {
+    EncodeTiledFn enc = tensor_map_encoder();
+    if (!enc) return set_error(BQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    struct Dim {
+        int64_t stride, size;
+        int what;  // 0 page, 1 head, 2 slot
+    } d[3] = {{st[0], kv->num_pages, 0}, {st[1], kv->HKV, 1}, {st[2], kv->page_size, 2}};
+    std::stable_sort(d, d + 3, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+    cuuint64_t dims[4] = {cuuint64_t(kv->D)}, strides[3];
+    cuuint32_t boxes[4] = {cuuint32_t(kv->D)};
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 3; ++i) {
+        dims[i + 1] = cuuint64_t(d[i].size);
+        strides[i] = cuuint64_t(d[i].size == 1 ? kv->D : d[i].stride);  // of one element: any that the encoder takes
+        boxes[i + 1] = d[i].what == 2 ? cuuint32_t(box) : 1u;
+        if (d[i].what == 2) *slot = i + 1;
+        if (d[i].what == 1) *head = i + 1;
+    }
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, boxes, es,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, kv->D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(BQ_ERR_CUDA, "cuTensorMapEncodeTiled (codes) failed (%d)", int(r));
+    return BQ_OK;
+}
+
 }  // namespace
 
-int paged8_launch_wide(const PagedWork& w, const Paged8Scales& sc, int dtype, int D, int grid, uint32_t flags, void* stream) {
+int paged8_launch_wide(const PagedWork& w, const Paged8Scales& sc, const bq_paged8_kv* kv, int grid, uint32_t flags, void* stream) {
+    const int dtype = kv->dtype, D = kv->D;
     Wide8Params p;
     std::memset(&p, 0, sizeof(p));
     p.w = w;
@@ -630,6 +710,10 @@ int paged8_launch_wide(const PagedWork& w, const Paged8Scales& sc, int dtype, in
         if (rc) return rc;
         p.q_tma = 1;
     }
+    p.box = std::min(kv->page_size, 128);
+    rc = encode_codes(kv, kv->k_pages, kv->k_stride, p.box, &p.kmap, &p.k_slot, &p.k_head);
+    if (!rc) rc = encode_codes(kv, kv->v_pages, kv->v_stride, p.box, &p.vmap, &p.v_slot, &p.v_head);
+    if (rc) return rc;
     // kind::f16, fp32 accumulate; queries and keys of the rows' type, weights and values fp16; M = 128; N = 128 positions
     // / D dims (B dims-contiguous)
     const uint32_t type = dtype == BQ_DT_BF16 ? 1u : 0u, common = (1u << 4) | (uint32_t(128 >> 4) << 24);
