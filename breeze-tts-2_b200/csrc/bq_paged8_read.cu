@@ -14,12 +14,13 @@
 namespace bq {
 namespace {
 
-constexpr int kThreads = 256, kMostRows = 32, kHeads = 4, kFlight = 4;
+constexpr int kThreads = 256, kMostRows = 64, kMostHeads = 8, kFlight = 4;
 
 struct Read8Params {
     PagedKV kv;
     Paged8Scales sc;
-    int32_t window, aligned;  // rows of a CTA; outputs 32-byte aligned
+    int32_t window, head_shift;  // rows and 2^x heads of a CTA
+    int32_t aligned;             // outputs are 32-byte aligned
     void* k_out;
     int64_t ko_row, ko_head;
     void* v_out;
@@ -63,8 +64,10 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
     pdl_wait();
     const PagedKV& kv = p.kv;
     const int w0 = blockIdx.x * p.window, rows = min(p.window, kv.T - w0);
-    const bool is_k = int(blockIdx.y) < (kv.HKV + kHeads - 1) / kHeads;
-    const int h0 = (is_k ? blockIdx.y : blockIdx.y - (kv.HKV + kHeads - 1) / kHeads) * kHeads;
+    const int half = gridDim.y / 2, h0 = int(blockIdx.y) % half << p.head_shift;
+    const bool is_k = int(blockIdx.y) < half;
+    const int CHH = CH << p.head_shift;  // pieces of a row
+    const int row_shift = p.head_shift + (D == 128 ? 3 : 2);
 
     // page (-1: leave the row) and slot of every row of the window
     auto place = [&](int r, int b, int pos) {
@@ -114,13 +117,13 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
                   st_slot = is_k ? kv.ks_slot : kv.vs_slot;
     T* out = static_cast<T*>(is_k ? p.k_out : p.v_out);
     const int64_t o_row = is_k ? p.ko_row : p.vo_row, o_head = is_k ? p.ko_head : p.vo_head;
-    const int total = rows * kHeads * CH;
+    const int total = rows * CHH;
     for (int i0 = threadIdx.x; i0 < total; i0 += kThreads * kFlight) {
         uint4 w[kFlight];
         uint8_t e[kFlight];
 #pragma unroll
         for (int f = 0; f < kFlight; ++f) {
-            const int i = i0 + f * kThreads, r = i / (kHeads * CH), h = h0 + i / CH % kHeads, c = i % CH;
+            const int i = i0 + f * kThreads, r = i >> row_shift, h = h0 + (i & (CHH - 1)) / CH, c = i % CH;
             w[f] = make_uint4(0, 0, 0, 0);
             e[f] = kExpBias;
             if (i < total && h < kv.HKV && s_page[r] >= 0) {
@@ -131,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
         }
 #pragma unroll
         for (int f = 0; f < kFlight; ++f) {
-            const int i = i0 + f * kThreads, r = i / (kHeads * CH), h = h0 + i / CH % kHeads, c = i % CH;
+            const int i = i0 + f * kThreads, r = i >> row_shift, h = h0 + (i & (CHH - 1)) / CH, c = i % CH;
             if (i >= total || h >= kv.HKV || s_page[r] < 0) continue;
             const float s = exp_scale(scale_exp(e[f]));
             const uint32_t words[4] = {w[f].x, w[f].y, w[f].z, w[f].w};
@@ -186,7 +189,23 @@ extern "C" int32_t bq_paged8_read(const bq_paged8_read_desc* d, void* stream) {
     std::memset(&p, 0, sizeof(p));
     rc = paged8_fill(&p.kv, &p.sc, &d->kv, d->T, 0);
     if (rc) return rc;
+    // A CTA's start (its rows' sequences, lengths and pages) takes as long as some 16 KB of codes do: large pieces, as far
+    // as there is a CTA for every SM (96925 rows of 8 heads of 128: 32 rows of 2 / 4 / 8 heads 253 / 162 / 124 us, 64 of
+    // 8 122 us; 410 rows of 16 heads: 32 rows of 2 / 4 / 8 heads 4.9 / 5.6 / 6.2 us, 16 of 4 4.4 us).
+    const DeviceInfo* di = device_info();
+    if (!di) return BQ_ERR_CUDA;
+    int heads = 1;
+    while (heads < d->kv.HKV && heads < kMostHeads) heads *= 2;
     p.window = paged8_window(&d->kv, d->T, kMostRows);
+    while (int64_t((d->T + p.window - 1) / p.window) * 2 * ((d->kv.HKV + heads - 1) / heads) < di->sm_count) {
+        if (p.window > 16 || (heads == 1 && p.window > 4))
+            p.window /= 2;
+        else if (heads > 1)
+            heads /= 2;
+        else
+            break;
+    }
+    p.head_shift = __builtin_ctz(unsigned(heads));
     p.k_out = d->k_out;
     p.ko_row = d->ko_stride[0];
     p.ko_head = d->ko_stride[1];
@@ -198,6 +217,6 @@ extern "C" int32_t bq_paged8_read(const bq_paged8_read_desc* d, void* stream) {
         if (size[i] > 1 && (d->ko_stride[i] * elem % 32 || d->vo_stride[i] * elem % 32)) p.aligned = 0;
     const void* fn = d->kv.D == 128 ? read_kernel<128>(d->kv.dtype) : read_kernel<64>(d->kv.dtype);
     void* args[] = {&p};
-    return paged_launch(fn, dim3((d->T + p.window - 1) / p.window, 2 * ((d->kv.HKV + kHeads - 1) / kHeads)), dim3(kThreads), 0, args,
+    return paged_launch(fn, dim3((d->T + p.window - 1) / p.window, 2 * ((d->kv.HKV + heads - 1) / heads)), dim3(kThreads), 0, args,
                         d->flags, stream, "paged read");
 }
