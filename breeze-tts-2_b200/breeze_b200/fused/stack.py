@@ -14,7 +14,8 @@ reference keeps its output heads in fp32, cudagraph/backbone_graph.py:70).
 decode attention step (bq_attention_step: q/k RMSNorm, RoPE, KV-cache write,
 flash-decode over the cache) between QKV and O, as FusedDecoderLayer does
 (layer.py:89-90); with ``page_size`` the rows are streams of their own length
-over a paged cache (breeze_b200.fused.paged: append, then attention); otherwise
+over a paged cache (breeze_b200.fused.paged: append, then attention; with
+``kv_dtype`` held in 8 bits, breeze_b200.fused.paged_fp8); otherwise
 the first ``attn_cols`` columns of ``qkv`` (the query block) stand in for it,
 which keeps the QKV -> O data dependency.
 
@@ -31,7 +32,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import _lib
-from . import paged
+from . import paged, paged_fp8
 
 
 @dataclass
@@ -154,7 +155,8 @@ class DecodeStack:
                  eps: float = 1e-6, attn_cols: int | None = None, chain: bool = False, attention: bool = False,
                  head_dim: int = 128, kv_heads: int | None = None, kv_len: int = 256,
                  lm_head: torch.Tensor | None = None, sampling: dict | None = None, page_size: int | None = None,
-                 num_pages: int | None = None, prefix_len: int = 0):
+                 num_pages: int | None = None, prefix_len: int = 0, kv_dtype: torch.dtype | None = None,
+                 kv_block: int | None = None):
         """``page_size`` (needs ``attention``): every row is a stream of its own
         length, up to ``kv_len`` positions, in pages of that size. ``seq_lens``
         (rows,) int32 holds each row's length with this step's token (add 1
@@ -166,6 +168,10 @@ class DecodeStack:
         (breeze_b200.fused.paged.prefix_attention). Initially all rows are full and
         take consecutive pages, the prefix's first; with fewer pages than that
         takes, the rows start unused and without pages (-1) of their own.
+        ``kv_dtype=torch.float8_e4m3fn``: the pages hold e4m3 codes, a power of two
+        for each ``kv_block`` positions (16, 32, 64 or 128; by default 64, or the page
+        size if that is less) and kv head beside them in ``k_scales`` / ``v_scales``;
+        half the cache's bytes. A shared prefix is then read by each row.
 
         ``lm_head``: an fp32 nn.Linear weight (V, hidden) used instead of the
         quantized ``head``, as the backbone graph casts lm_head to fp32
@@ -234,11 +240,21 @@ class DecodeStack:
         self.graph = None
         self.chain = None
         self.attention = attention
-        self.page_size, self.prefix_len = page_size, prefix_len
+        self.page_size, self.prefix_len, self.kv_block = page_size, prefix_len, None
         if page_size is not None and not attention:
             raise ValueError("a paged cache needs attention=True")
         if prefix_len and page_size is None:
             raise ValueError("a shared prefix needs a paged cache (page_size)")
+        if kv_dtype not in (None, torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError(f"the cache is bf16 or float8_e4m3fn (got {kv_dtype})")
+        if kv_dtype == torch.float8_e4m3fn:
+            if page_size is None:
+                raise ValueError("a cache in 8 bits needs pages (page_size)")
+            self.kv_block = min(64, page_size) if kv_block is None else kv_block
+            if self.kv_block not in (16, 32, 64, 128) or page_size % self.kv_block:
+                raise ValueError(f"kv_block={self.kv_block} must be 16, 32, 64 or 128 and divide the page size {page_size}")
+        elif kv_block is not None:
+            raise ValueError("kv_block needs kv_dtype=torch.float8_e4m3fn")
         if attention:
             if chain:
                 raise ValueError("the decode chain runs GEMVs only; attention=True needs chain=False")
@@ -263,8 +279,16 @@ class DecodeStack:
                 if pages <= shared:
                     raise ValueError(f"{pages} pages hold no position behind a prefix of {shared}")
                 shape = (pages, hkv, page_size, head_dim)
-                self.k_pages = [torch.zeros(shape, **bf) for _ in layers]
-                self.v_pages = [torch.zeros(shape, **bf) for _ in layers]
+                if self.kv_block is None:
+                    self.k_pages = [torch.zeros(shape, **bf) for _ in layers]
+                    self.v_pages = [torch.zeros(shape, **bf) for _ in layers]
+                else:
+                    def filled(shape, byte, dtype):
+                        return [torch.full(shape, byte, device=dev, dtype=torch.uint8).view(dtype) for _ in layers]
+
+                    per = (pages, hkv, page_size // self.kv_block)
+                    self.k_pages, self.v_pages = (filled(shape, 0, torch.float8_e4m3fn) for _ in range(2))
+                    self.k_scales, self.v_scales = (filled(per, 127, torch.float8_e8m0fnu) for _ in range(2))  # 2^0
                 enough = pages >= need
                 own = torch.arange(shared, need, dtype=torch.int32) if enough else torch.full((need - shared,), -1, dtype=torch.int32)
                 prefix = torch.arange(shared, dtype=torch.int32).expand(rows, shared)
@@ -297,7 +321,10 @@ class DecodeStack:
         if self.page_size is not None:
             lens = self.seq_lens.clamp(min=0)
             positions = int((lens - self.prefix_len).clamp(min=0).sum()) + min(self.prefix_len, int(lens.max()))
-            return len(self.layers) * 2 * positions * self.hkv * self.head_dim * 2
+            if self.kv_block is None:
+                return len(self.layers) * 2 * positions * self.hkv * self.head_dim * 2
+            blocks = -(-positions // self.kv_block)  # (a few more where several rows end inside one)
+            return len(self.layers) * 2 * self.hkv * (positions * self.head_dim + blocks)
         return len(self.layers) * 2 * self.rows * self.hkv * (int(self.pos.item()) + 1) * self.head_dim * 2
 
     @property
@@ -309,7 +336,7 @@ class DecodeStack:
             return 1
         per_layer = 4
         if self.attention:  # one step; or append, attention (twice with a prefix) and its join
-            per_layer += 1 if self.page_size is None else 4 if self.prefix_len else 3
+            per_layer += 1 if self.page_size is None else 4 if self.prefix_len and self.kv_block is None else 3
         return per_layer * len(self.layers) + 1 + (1 if self.sampling is not None else 0)
 
     def _ops(self):
@@ -334,6 +361,12 @@ class DecodeStack:
     def _paged_attention(self, li: int) -> None:
         """Layer li's attention over the paged caches: qkv -> attn_out."""
         l = self.layers[li]
+        if self.kv_block is not None:
+            where = (self.k_pages[li], self.v_pages[li], self.k_scales[li], self.v_scales[li], self.page_table, self.seq_lens)
+            paged_fp8.paged_append_fp8(self.qkv[:, : l.wqkv.N], self.cos, self.sin, *where, q_norm_w=l.q_norm,
+                                       k_norm_w=l.k_norm, eps=self.eps, out=self.q)
+            paged_fp8.paged_attention_fp8(self.q, *where, out=self.attn_out)
+            return
         where = (self.k_pages[li], self.v_pages[li], self.page_table, self.seq_lens)
         paged.paged_append(self.qkv[:, : l.wqkv.N], self.cos, self.sin, *where, q_norm_w=l.q_norm, k_norm_w=l.k_norm,
                            eps=self.eps, out=self.q)
