@@ -32,8 +32,9 @@ constexpr int kWarps = kNarrowWarps, kThreads = 32 * kWarps;
 constexpr int kRows = kNarrowRows, kUnit = kNarrowUnit, kOverhead = kNarrow8Overhead;
 constexpr int kStep = 32;              // positions of a warp's step
 constexpr int kBatch = 32 * 16 / kStep;  // steps whose pages the lanes hold, one block of 16 positions each
-constexpr int kLift = 64;              // weights are kept times 2^64: 2^-190 of the largest is not lost yet
-constexpr int kHalfLift = 15;          // and enter the product times 2^15
+// Weights are kept times 2^15, as they enter the product. With exponents of v that lie 120 apart (they cannot lie
+// further), what fp32 flushes of them is less than 2^-21 of the largest term of the sum of exponentials each.
+constexpr int kLift = 15;
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool full) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
@@ -217,12 +218,26 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
                 const int slot = (pb + 16 * b) & kv.page_mask;
                 const uint8_t* kp = kh + pages[b] * kv.ks_page + slot * kv.ks_slot;
                 const uint8_t* vp = vh + pages[b] * kv.vs_page + slot * kv.vs_slot;
+                const int r0 = lane / CH, c = lane % CH;  // rows r0 + 32 / CH i
+                kp += r0 * kv.ks_slot + c * 16;
+                vp += r0 * kv.vs_slot + c * 16;
+                constexpr int RS = 32 / CH;
+                if (pb + 16 * b + 16 <= p1) {
 #pragma unroll
-                for (int i = 0; i < 16 * CH / 32; ++i) {
-                    const int idx = lane + 32 * i, r = idx / CH, c = idx % CH, rr = 16 * b + r;
-                    const uint32_t at = rr * D + (chunk_at<D>(rr, c) << 4);
-                    cp_async16_zfill(dst + at, kp + r * kv.ks_slot + c * 16, pb + rr < p1);
-                    cp_async16_zfill(dst + SM::kBlock + at, vp + r * kv.vs_slot + c * 16, pb + rr < p1);
+                    for (int i = 0; i < 16 / RS; ++i) {
+                        const int rr = 16 * b + r0 + RS * i;
+                        const uint32_t at = rr * D + (chunk_at<D>(rr, c) << 4);
+                        cp_async16(dst + at, kp + i * (RS * kv.ks_slot));
+                        cp_async16(dst + SM::kBlock + at, vp + i * (RS * kv.vs_slot));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16 / RS; ++i) {
+                        const int rr = 16 * b + r0 + RS * i;
+                        const uint32_t at = rr * D + (chunk_at<D>(rr, c) << 4);
+                        cp_async16_zfill(dst + at, kp + i * (RS * kv.ks_slot), pb + rr < p1);
+                        cp_async16_zfill(dst + SM::kBlock + at, vp + i * (RS * kv.vs_slot), pb + rr < p1);
+                    }
                 }
             }
         }
@@ -251,6 +266,9 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
 
+    // TWO: the tile has more than 8 rows; else rows g + 8 are left out of the softmax.
+    auto stream = [&](auto two) {
+    constexpr bool TWO = decltype(two)::value;
     for (int st = 0; st < steps; ++st) {
         cp_wait<ST - 2>();
         __syncwarp();  // every lane's copies of this stage have landed, and every lane is done with the one before
@@ -271,42 +289,54 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
                 mma_f16(x[n], qf[i][0], qf[i][1], qf[i][2], qf[i][3], lo, hi);
             }
         }
-        float n0 = m0, n1 = m1, back[2], lift[2];
+        float n0 = m0, n1 = m1, back[2];
+        const bool cut = min(blk + kStep, p1) > seen || blk + kStep > p1;  // some row does not see all of it
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const uint32_t ee = __shfl_sync(0xffffffffu, exp_now, 2 * st % 32 + b);
             const int ev = scale_exp(ee >> 8);
-            const float ks = exp_scale(scale_exp(ee & 255)), a0 = f0 * ks, a1 = f1 * ks;
-            lift[b] = float(ev);
+            const float ks = exp_scale(scale_exp(ee & 255)), a0 = f0 * ks, a1 = f1 * ks, y = float(ev);
             back[b] = exp_scale(-ev - kLift);
 #pragma unroll
             for (int n = 2 * b; n < 2 * b + 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int pos = pb + 8 * n + e;
-                    x[n][e] = pos < lim0 ? fmaf(x[n][e], a0, lift[b]) : -INFINITY;
-                    x[n][2 + e] = pos < lim1 ? fmaf(x[n][2 + e], a1, lift[b]) : -INFINITY;
-                    n0 = fmaxf(n0, x[n][e]);
-                    n1 = fmaxf(n1, x[n][2 + e]);
+                    x[n][e] = fmaf(x[n][e], a0, y);
+                    if constexpr (TWO) x[n][2 + e] = fmaf(x[n][2 + e], a1, y);
                 }
         }
-        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
-        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
-        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
-        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
-        if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {  // a maximum moved: rescale what was summed
-            const float a0 = n0 == m0 ? 1.f : ex2(m0 - n0), a1 = n1 == m1 ? 1.f : ex2(m1 - n1);
-            l0 *= a0;
-            l1 *= a1;
+        if (cut) {
 #pragma unroll
-            for (int n = 0; n < T; ++n) {
-                o[n][0] *= a0;
-                o[n][1] *= a0;
-                o[n][2] *= a1;
-                o[n][3] *= a1;
-            }
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (pb + 8 * n + e >= lim0) x[n][e] = -INFINITY;
+                    if constexpr (TWO)
+                        if (pb + 8 * n + e >= lim1) x[n][2 + e] = -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            n0 = fmaxf(n0, fmaxf(x[n][0], x[n][1]));
+            if constexpr (TWO) n1 = fmaxf(n1, fmaxf(x[n][2], x[n][3]));
+        }
+        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
+        if constexpr (TWO) n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
+        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
+        if constexpr (TWO) n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
+        if (__any_sync(0xffffffffu, n0 != m0 || (TWO && n1 != m1))) {  // a maximum moved: rescale what was summed
+            const float a0 = n0 == m0 ? 1.f : ex2(0.5f * (m0 - n0));  // in two steps: l may be as far from 1
+            l0 = l0 * a0 * a0;
+#pragma unroll
+            for (int n = 0; n < T; ++n) o[n][0] *= a0 * a0, o[n][1] *= a0 * a0;
             m0 = n0;
-            m1 = n1;
+            if constexpr (TWO) {
+                const float a1 = n1 == m1 ? 1.f : ex2(0.5f * (m1 - n1));
+                l1 = l1 * a1 * a1;
+#pragma unroll
+                for (int n = 0; n < T; ++n) o[n][2] *= a1 * a1, o[n][3] *= a1 * a1;
+                m1 = n1;
+            }
         }
         const float u0 = (m0 == -INFINITY ? 0.f : m0) - kLift, u1 = (m1 == -INFINITY ? 0.f : m1) - kLift;  // (rows that see nothing yet)
 #pragma unroll
@@ -316,15 +346,18 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     x[n][e] = ex2(x[n][e] - u0);
-                    x[n][2 + e] = ex2(x[n][2 + e] - u1);
                     l0 = fmaf(x[n][e], back[b], l0);
-                    l1 = fmaf(x[n][2 + e], back[b], l1);
+                    if constexpr (TWO) {
+                        x[n][2 + e] = ex2(x[n][2 + e] - u1);
+                        l1 = fmaf(x[n][2 + e], back[b], l1);
+                    }
                 }
-            if (min(blk + 16 * b + 16, p1) > seen) clear_nan<D>(vb, 16 * b, blk + 16 * b, lim0, lim1, o);
-            const float down = 1.f / (1ull << (kLift - kHalfLift));
-            const uint32_t pf[4] = {pack_half2(x[2 * b][0] * down, x[2 * b][1] * down), pack_half2(x[2 * b][2] * down, x[2 * b][3] * down),
-                                    pack_half2(x[2 * b + 1][0] * down, x[2 * b + 1][1] * down),
-                                    pack_half2(x[2 * b + 1][2] * down, x[2 * b + 1][3] * down)};
+            if (cut && min(blk + 16 * b + 16, p1) > seen) clear_nan<D>(vb, 16 * b, blk + 16 * b, lim0, lim1, o);
+            uint32_t pf[4] = {pack_half2(x[2 * b][0], x[2 * b][1]), 0, pack_half2(x[2 * b + 1][0], x[2 * b + 1][1]), 0};
+            if constexpr (TWO) {
+                pf[1] = pack_half2(x[2 * b][2], x[2 * b][3]);
+                pf[3] = pack_half2(x[2 * b + 1][2], x[2 * b + 1][3]);
+            }
             // the lane's positions 2 tq, 2 tq + 1, 8 + 2 tq, 9 + 2 tq; its D / 8 dims from g D / 8 on
             constexpr int W = D / 32;
             uint32_t v[4][W];
@@ -349,6 +382,11 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
             }
         }
     }
+    };
+    if (t.nrows > 8)
+        stream(std::true_type());
+    else
+        stream(std::false_type());
     cp_wait<0>();
     if (!pages_ok) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
@@ -361,7 +399,7 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
         const int k = l > 0.f && l < INFINITY ? int(__float_as_uint(l) >> 23) - 127 : 0;
         m += float(k);
         l *= exp_scale(-k);
-        return exp_scale(-k - kHalfLift);
+        return exp_scale(-k - kLift);
     };
     const float z0 = settle(m0, l0), z1 = settle(m1, l1);
     __syncthreads();  // every warp is done with its ring: it now takes the warps' outputs
