@@ -15,8 +15,9 @@
 //
 // Two forms. One new token per sequence: a group per head, its block's older codes
 // (rarely) rescaled by the same group. Ragged rows: the tokens of a block share a
-// scale, so one CTA takes all new tokens of a block of one head, and keeps them in
+// scale, so a CTA takes all new tokens of a block of as many heads as its lanes hold in
 // registers between the maximum and the codes; queries go to CTAs of their own.
+#include <algorithm>
 #include <cstring>
 
 #include "bq_host.h"
@@ -34,7 +35,8 @@ constexpr int kQueryHeads = 4;      // of a CTA of queries
 struct Append8Params {
     PagedKV kv;
     Paged8Scales sc;
-    int32_t rope_rows, has_norm, window;
+    int32_t rope_rows, has_norm;
+    int32_t window, kv_ctas, q_parts;  // rows of a CTA; CTAs along y of the k and v heads; CTAs among which a window's queries are divided
     float eps;
     const void* qkv;
     int64_t ldqkv;
@@ -231,7 +233,7 @@ __device__ __forceinline__ int find_segments(const PagedKV& kv, int w0, int w1, 
     return min(*count, kMostBlock);  // (more only where starts are out of order)
 }
 
-// R: rows of a block that each group of lanes holds.
+// R: rows of a block that each group of lanes holds. block / R groups take a head's block, GROUPS R / block heads the CTA.
 template <typename E, typename C, int D, int R>
 __global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __grid_constant__ Append8Params p) {
     constexpr int LG = D / 8, GROUPS = kBlockThreads / LG;
@@ -242,12 +244,19 @@ __global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __g
     pdl_wait();
     const PagedKV& kv = p.kv;
     const int l = threadIdx.x % LG, g = threadIdx.x / LG;
-    const int w0 = blockIdx.x * p.window, w1 = min(w0 + p.window, kv.T);
+    int w0 = blockIdx.x * p.window, w1 = min(w0 + p.window, kv.T), h0 = 0;
+    const bool queries = int(blockIdx.y) >= p.kv_ctas;
+    if (queries) {  // of some heads and a part of the window
+        const int y = blockIdx.y - p.kv_ctas, part = y % p.q_parts;
+        h0 = y / p.q_parts * kQueryHeads;
+        w0 += part * (p.window / p.q_parts);
+        w1 = min(w1, w0 + p.window / p.q_parts);
+        if (w0 >= w1) return;
+    }
     const int n_seg = find_segments(kv, w0, w1, seg, &s_count);
     const int block = 1 << p.sc.block_shift;
 
-    if (int(blockIdx.y) >= 2 * kv.HKV) {  // queries of some heads
-        const int h0 = (blockIdx.y - 2 * kv.HKV) * kQueryHeads;
+    if (queries) {
         for (int r = threadIdx.x; r < w1 - w0; r += kBlockThreads) {
             int pos = -1;
             for (int i = 0; i < n_seg; ++i)
@@ -261,19 +270,35 @@ __global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __g
         }
         __syncthreads();
         const int total = (w1 - w0) * kQueryHeads;
-        for (int i0 = 0; i0 < total; i0 += GROUPS) {  // all lanes of a warp stay for the shuffles
-            const int i = min(i0 + g, total - 1), r = i / kQueryHeads, h = min(h0 + i % kQueryHeads, kv.HQ - 1), pos = s_pos[r];
-            float v[8];
-            unpack8<E>(*reinterpret_cast<const uint4*>(static_cast<const E*>(p.qkv) + int64_t(w0 + r) * p.ldqkv + h * D + l * 8), v);
-            turn<E, C, D>(p, max(pos, 0), l, p.qn, v);
-            if (i0 + g < total && h0 + i % kQueryHeads < kv.HQ && pos >= 0)
-                *reinterpret_cast<uint4*>(static_cast<E*>(p.q_out) + int64_t(w0 + r) * p.ldq + h * D + l * 8) = pack8<E>(v);
+        uint4 raw[2];
+        auto row_of = [&](int i) { return min(i, total - 1) / kQueryHeads; };
+        auto head_of = [&](int i) { return min(h0 + min(i, total - 1) % kQueryHeads, kv.HQ - 1); };
+        auto load = [&](int i) {
+            return *reinterpret_cast<const uint4*>(static_cast<const E*>(p.qkv) + int64_t(w0 + row_of(i)) * p.ldqkv + head_of(i) * D + l * 8);
+        };
+#pragma unroll
+        for (int q = 0; q < 2; ++q) raw[q] = load(q * GROUPS + g);
+        for (int i0 = 0; i0 < total; i0 += 2 * GROUPS) {  // all lanes of a warp stay for the shuffles
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int i = i0 + q * GROUPS + g, r = row_of(i), pos = s_pos[r];
+                float v[8];
+                unpack8<E>(raw[q], v);
+                const bool here = i < total && h0 + i % kQueryHeads < kv.HQ && pos >= 0;
+                const int head = head_of(i);
+                // (q may be written where qkv is read: the next rows are other ones)
+                raw[q] = load(i + 2 * GROUPS);
+                turn<E, C, D>(p, max(pos, 0), l, p.qn, v);
+                if (here) *reinterpret_cast<uint4*>(static_cast<E*>(p.q_out) + int64_t(w0 + r) * p.ldq + head * D + l * 8) = pack8<E>(v);
+            }
         }
         return;
     }
 
-    const int h = blockIdx.y;  // k heads, then v heads
-    const bool is_k = h < kv.HKV;
+    const int mine = block / R, item = g / mine, gi = g - item * mine;  // groups of a head; its index and the group's in it
+    const int h = min(int(blockIdx.y) * (GROUPS / mine) + item, 2 * kv.HKV - 1);  // k heads, then v heads
+    const bool live = int(blockIdx.y) * (GROUPS / mine) + item < 2 * kv.HKV, is_k = h < kv.HKV;
+    const int warp0 = item * mine * LG / 32, warps = mine * LG / 32;  // the head's warps
     int turnover = 0;
     for (int i = 0; i < n_seg; ++i) {
         const Segment s = seg[i];
@@ -307,36 +332,37 @@ __global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __g
 #pragma unroll
                 for (int q = 0; q < R; ++q) {
                     raw[q] = make_uint4(0, 0, 0, 0);
-                    if (g + q * GROUPS < n) raw[q] = *reinterpret_cast<const uint4*>(src + int64_t(g + q * GROUPS) * p.ldqkv);
+                    if (gi + q * mine < n) raw[q] = *reinterpret_cast<const uint4*>(src + int64_t(gi + q * mine) * p.ldqkv);
                 }
                 float v[R][8];
                 uint32_t top = 0;
 #pragma unroll
                 for (int q = 0; q < R; ++q) {
                     unpack8<E>(raw[q], v[q]);
-                    if (is_k) turn<E, C, D>(p, p0 + min(g + q * GROUPS, n - 1), l, p.kn, v[q]);
-                    if (g + q * GROUPS < n) top = max(top, top_of(v[q]));
+                    if (is_k) turn<E, C, D>(p, p0 + min(gi + q * mine, n - 1), l, p.kn, v[q]);  // (the same for a warp)
+                    if (gi + q * mine < n) top = max(top, top_of(v[q]));
                 }
                 top = __reduce_max_sync(0xffffffffu, top);
                 if ((threadIdx.x & 31) == 0) s_top[turnover][threadIdx.x >> 5] = top;
                 __syncthreads();
-#pragma unroll
-                for (int w = 0; w < kBlockThreads / 32; ++w) top = max(top, s_top[turnover][w]);
+                for (int w = 0; w < warps; ++w) top = max(top, s_top[turnover][warp0 + w]);
                 turnover ^= 1;  // the next block's maxima go elsewhere: one barrier per block is enough
                 const int need = need_exp(top), e = kept ? max(was, need) : need;
-                if (kept && e > was) {  // the block's older codes follow
+                if (live && kept && e > was) {  // the block's older codes follow
                     const float r = exp_scale(was - e);
-                    for (int q = g; q < kept; q += GROUPS) {
+                    for (int q = gi; q < kept; q += mine) {
                         uint2* c = reinterpret_cast<uint2*>(at.codes + q * at.slot + l * 8);
                         const uint2 w = *c;
                         *c = make_uint2(rescale4(w.x, r), rescale4(w.y, r));
                     }
                 }
+                if (live) {
 #pragma unroll
-                for (int q = 0; q < R; ++q)
-                    if (g + q * GROUPS < n)
-                        *reinterpret_cast<uint2*>(at.codes + (kept + g + q * GROUPS) * at.slot + l * 8) = encode8(v[q], e);
-                if (threadIdx.x == 0) *at.scale = uint8_t(e + kExpBias);
+                    for (int q = 0; q < R; ++q)
+                        if (gi + q * mine < n)
+                            *reinterpret_cast<uint2*>(at.codes + (kept + gi + q * mine) * at.slot + l * 8) = encode8(v[q], e);
+                    if (gi == 0 && l == 0) *at.scale = uint8_t(e + kExpBias);
+                }
             }
             r0 += rows;
             p0 += rows;
@@ -346,10 +372,8 @@ __global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __g
 
 template <typename E, typename C, int D>
 const void* blocks_kernel(int r) {
-    return r >= 8   ? reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 8>)
-           : r == 4 ? reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 4>)
-           : r == 2 ? reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 2>)
-                    : reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 1>);
+    return r == 8 ? reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 8>)
+                  : reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 4>);
 }
 template <typename E, typename C>
 const void* append_kernel(int D, bool rows, int r) {
@@ -385,7 +409,7 @@ extern "C" int32_t bq_paged8_append(const bq_paged8_append_desc* d, void* stream
     if (!paged_aligned(d->qkv, d->ldqkv, 2) || !paged_aligned(d->q_out, d->ldq, 2) || !paged_aligned(d->cos, d->ldcs, cs) ||
         !paged_aligned(d->sin, d->ldcs, cs) || !paged_aligned(d->q_norm, 0, 2) || !paged_aligned(d->k_norm, 0, 2))
         return set_error(BQ_ERR_ALIGN, "qkv, cos, sin, q_out and norm rows must be 16-byte aligned");
-    if (2 * d->kv.HKV + (d->HQ + kQueryHeads - 1) / kQueryHeads > 65535)
+    if (2 * d->kv.HKV + (d->HQ + kQueryHeads - 1) / kQueryHeads * 8 > 65535)
         return set_error(BQ_ERR_SHAPE, "%d query and %d kv heads are too many", d->HQ, d->kv.HKV);
     rc = paged_check_device();
     if (rc) return rc;
@@ -406,7 +430,7 @@ extern "C" int32_t bq_paged8_append(const bq_paged8_append_desc* d, void* stream
     p.q_out = d->q_out;
     p.ldq = d->ldq;
     const bool f32 = d->cs_dtype == BQ_DT_F32, bf = d->kv.dtype == BQ_DT_BF16, rows = !d->kv.q_starts;
-    const int lanes = d->kv.D / 8, r = d->kv.block * lanes / kBlockThreads;
+    const int lanes = d->kv.D / 8, r = d->kv.block * lanes > 4 * kBlockThreads ? 8 : 4;
     const void* fn = bf ? (f32 ? append_kernel<__nv_bfloat16, float>(d->kv.D, rows, r)
                                : append_kernel<__nv_bfloat16, __nv_bfloat16>(d->kv.D, rows, r))
                         : (f32 ? append_kernel<__half, float>(d->kv.D, rows, r) : append_kernel<__half, __half>(d->kv.D, rows, r));
@@ -416,6 +440,15 @@ extern "C" int32_t bq_paged8_append(const bq_paged8_append_desc* d, void* stream
         return paged_launch(fn, dim3(d->T, (heads + per - 1) / per), dim3(kRowThreads), 0, args, d->flags, stream, "paged append");
     }
     p.window = paged8_window(&d->kv, d->T, d->kv.block);
-    return paged_launch(fn, dim3((d->T + p.window - 1) / p.window, 2 * d->kv.HKV + (d->HQ + kQueryHeads - 1) / kQueryHeads),
+    const int heads = kBlockThreads / lanes * r / d->kv.block;  // of a CTA
+    p.kv_ctas = (2 * d->kv.HKV + heads - 1) / heads;
+    // Queries: a window's are divided among CTAs, down to two rounds each, until there are eight CTAs for every SM (400 rows
+    // of 16 heads: 8 rounds 10.7 us, 2 rounds 7.7; 16000 of 32: 84 and 92 us).
+    const DeviceInfo* di = device_info();
+    if (!di) return BQ_ERR_CUDA;
+    const int windows = (d->T + p.window - 1) / p.window, q_heads = (d->HQ + kQueryHeads - 1) / kQueryHeads;
+    p.q_parts = 1;
+    while (2 * p.q_parts * kBlockThreads <= p.window * lanes && int64_t(windows) * q_heads * p.q_parts < 8 * di->sm_count) p.q_parts *= 2;
+    return paged_launch(fn, dim3(windows, p.kv_ctas + q_heads * p.q_parts),
                         dim3(kBlockThreads), 0, args, d->flags, stream, "paged append");
 }
