@@ -84,11 +84,21 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Most positions per CTA of a cluster that the page table may hold.
+// Most positions per CTA of a cluster that the page table may hold, as for 16-bit caches: a cluster costs its longest
+// sequence, so a roomy table, which may hold uneven ones, takes equal shares. Clusters against equal shares, all sequences
+// of the table's length, 128 dims, us:
+//   2 of 16 heads   256 / 1024 / 4096 positions    6.2 / 6.8 / 11.3   and    9.0 / 11.2 / 15.3
+//   9 of 8          128 /  512 / 1024 (2 CTAs)     5.8 / 7.7 / 10.6   and    9.5 / 11.0 / 12.8
+//   18 of 8         512 / 1024        (2 CTAs)     8.2 / 11.2         and   13.5 / 16.7
 constexpr int kClusterPositions = 512;
 
-// Rows that share a kv head up to which they go to the kernel for few rows, in tiles of 16 of which all but the first find
-// the codes in L2 mostly. Against the 256-row kernel, 4 kv heads of 128 dims: XXX
+// Rows that share a kv head up to which they go to the kernel for few rows, in tiles of 16, of which all but the first
+// find the codes in L2 mostly. Against the 256-row kernel (as it was then, about 8 % slower than now), 4 kv heads, us:
+//                             24 rows      32          64          96          128
+//   128 dims, 32 x 6000      49 / 134    60 / 134    70 / 136    84 / 136   123 / 138
+//             4 x 20000      32 / 69     35 / 71     42 / 69     48 / 67     93 / 69
+//   64 dims,  32 x 6000      37 / 106    43 / 106    50 / 106    61 / 106    88 / 107
+//             32 x 700       13 / 26     13 / 26     17 / 27     22 / 27     20 / 27
 constexpr int kFewRows = 96;
 
 // How a call is divided: clusters of `ranks` CTAs per (sequence, kv head), or equal shares of all positions for
@@ -108,9 +118,12 @@ int plan8(const bq_paged8_attn_desc* d, Plan8* pl) {
     pl->tile_rows = most * (d->HQ / d->kv.HKV);
     if (pl->tile_rows <= kNarrowRows) {
         const int64_t pairs = int64_t(d->kv.B) * d->kv.HKV, room = int64_t(d->kv.max_pages) * d->kv.page_size;
+        // Two CTAs per SM. Clusters of more than two do not find places for that many, since a cluster stays within a part
+        // of the GPU: 72 clusters of 4, 128 positions each, take 10.1 us in two waves, 72 of 2 5.8.
+        auto fits = [&](int ranks) { return pairs * ranks * 4 <= (ranks > 2 ? 7 : 8) * di->sm_count; };
         int ranks = kNarrowRanks;
-        while (ranks > 1 && pairs * ranks > 2 * di->sm_count) ranks >>= 1;
-        if (ranks > 1 && room <= int64_t(kClusterPositions) * ranks) {
+        while (ranks > 1 && !fits(ranks)) ranks >>= 1;
+        if (fits(ranks) && room <= int64_t(kClusterPositions) * ranks) {
             pl->ranks = ranks;
             return BQ_OK;
         }

@@ -240,8 +240,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                 }
                 __syncwarp();
                 if (!idle) {
-                    // The largest s + ev, and a new reference where it is more than 8 above: for most data a unit's weights
-                    // would else be computed twice (6500 positions of keys with uneven channels and levels: XXX us, YYY here).
+                    // The largest s + ev, and a new reference where it is more than 8 above. The maximum beside the weights,
+                    // which are then computed twice where it moved, is no faster for even data and slower for keys with
+                    // uneven channels and levels, whose maxima move (6500 positions, at an earlier stage: 255 and 285 us,
+                    // so 257 and 267).
                     float m = -INFINITY;
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b) {
