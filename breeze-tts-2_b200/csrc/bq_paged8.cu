@@ -90,6 +90,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 //   2 of 16 heads   256 / 1024 / 4096 positions    6.2 / 6.8 / 11.3   and    9.0 / 11.2 / 15.3
 //   9 of 8          128 /  512 / 1024 (2 CTAs)     5.8 / 7.7 / 10.6   and    9.5 / 11.0 / 12.8
 //   18 of 8         512 / 1024        (2 CTAs)     8.2 / 11.2         and   13.5 / 16.7
+//   64 of 8         128 /  512        (1 CTA)     10.9 / 19.8         and   14.4 / 24.6   (200 of 8: no difference)
 constexpr int kClusterPositions = 512;
 
 // Rows that share a kv head up to which they go to the kernel for few rows, in tiles of 16, of which all but the first
@@ -123,7 +124,7 @@ int plan8(const bq_paged8_attn_desc* d, Plan8* pl) {
         auto fits = [&](int ranks) { return pairs * ranks * 4 <= (ranks > 2 ? 7 : 8) * di->sm_count; };
         int ranks = kNarrowRanks;
         while (ranks > 1 && !fits(ranks)) ranks >>= 1;
-        if (fits(ranks) && room <= int64_t(kClusterPositions) * ranks) {
+        if ((fits(ranks) || pairs <= 4 * di->sm_count) && room <= int64_t(kClusterPositions) * ranks) {
             pl->ranks = ranks;
             return BQ_OK;
         }
