@@ -565,6 +565,56 @@ def test_append_attend_and_read_together(roomy):
         check_read(c, kk, vv, BF)
 
 
+def test_calls_without_rows():
+    P = _api()
+    c = pc.batch([5, 9], [0, 0], 4, 2, 64, 16, 16, BF, seed=1)
+    d = pc.to({k: c[k] for k in ("q", "k", "v", "ks", "vs", "table", "lens")}, DEV)
+    starts, one = c["starts"].to(DEV), torch.ones(16, 64, device=DEV)
+    before = caches(d)
+    assert P.paged_append_fp8(torch.zeros(0, 8 * 64, dtype=BF, device=DEV), one, one, *where(d), q_starts=starts).shape == (0, 256)
+    assert P.paged_attention_fp8(torch.zeros(0, 256, dtype=BF, device=DEV), *where(d), q_starts=starts).shape == (0, 256)
+    k, v = P.paged_read_fp8(*where(d), q_starts=starts, rows=0)
+    assert k.shape == v.shape == (0, 2, 64)
+    torch.cuda.synchronize()
+    assert all(torch.equal(pc.bits(x), pc.bits(y)) for x, y in zip(before, caches(d)))
+
+
+def test_lengths_below_zero_are_unused_slots():
+    P = _api()
+    c = pc.batch([40, 33, 20], [3, 4, 2], 2, 1, 64, 16, 16, BF, seed=3)
+    d = pc.to({k: c[k] for k in ("q", "k", "v", "ks", "vs", "table", "lens")}, DEV)
+    d["lens"][1] = -2 ** 31
+    starts, one = c["starts"].to(DEV), torch.ones(64, 64, device=DEV)
+    before = caches(d)
+    out = torch.full((9, 128), 3.0, dtype=BF, device=DEV)
+    P.paged_append_fp8(torch.ones(9, 4 * 64, dtype=BF, device=DEV), one, one, *where(d), q_starts=starts, out=out)
+    assert (out[3:7] == 3.0).all() and (out[:3] != 3.0).any() and (out[7:] != 3.0).any()
+    mine = c["table"][1, :3].long()
+    assert all(torch.equal(pc.bits(x)[mine], pc.bits(y)[mine]) for x, y in zip(before, caches(d)))
+    lse = torch.zeros(9, 2, device=DEV)
+    for max_q in (4, 1000):
+        o = P.paged_attention_fp8(d["q"], *where(d), q_starts=starts, max_q=max_q, lse=lse)
+        assert (o[3:7] == 0).all() and (lse[3:7] == -math.inf).all() and torch.isfinite(lse[:3]).all()
+    k, v = (torch.full((9, 1, 64), 3.0, dtype=BF, device=DEV) for _ in range(2))
+    P.paged_read_fp8(*where(d), q_starts=starts, k_out=k, v_out=v)
+    assert (k[3:7] == 3.0).all() and (v[3:7] == 3.0).all() and (v[:3] != 3.0).any()
+
+
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+def test_one_page_or_one_kv_head(layout):
+    """Dimensions of size one, whose strides mean nothing."""
+    for lens, hkv, page in (([40], 1, 64), ([40], 3, 64), ([90, 20, 130], 1, 32)):
+        for new in (None, [7 + b for b in range(len(lens))], [20] * len(lens)):
+            c = pc.batch(lens, new, 8 * hkv, hkv, 64, page, 16, BF, seed=8, layout=layout)
+            if page == 64:
+                p = int(c["table"][0, 0])
+                for n in ("k", "v", "ks", "vs"):
+                    c[n] = c[n][p:p + 1]
+                c["table"][0, 0] = 0
+            compare(c, *run(c))
+            compare(c, *run(c, max_q=1000))
+
+
 # ---------------------------------------------------------------- errors, streams, graphs
 def test_lengths_behind_the_table_and_bad_pages_are_reported():
     from breeze_b200 import _lib
