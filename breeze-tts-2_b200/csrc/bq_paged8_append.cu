@@ -17,6 +17,11 @@
 // (rarely) rescaled by the same group. Ragged rows: the tokens of a block share a
 // scale, so a CTA takes all new tokens of a block of as many heads as its lanes hold in
 // registers between the maximum and the codes; queries go to CTAs of their own.
+//
+// Measured in a graph: 2 rows of 48 heads 2.1 us, 160 rows of 48 heads 3.0 us (both the
+// chain of loads); seven prompts of 28 heads of 64, blocks of 16, 26.9 MB in 15.0 us
+// (1.8 TB/s: waves of short CTAs, each with its search for the sequence, its loads, one
+// barrier and its stores).
 #include <algorithm>
 #include <cstring>
 

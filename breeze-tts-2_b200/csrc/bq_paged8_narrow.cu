@@ -21,6 +21,15 @@
 // largest entry to at least 2^14: exact but for entries under 2^-28 of it), the
 // weights as f16 times 2^15 (half a step, 2^-11, and what is under 2^-29 of the
 // largest loses less than 2^-40 of it). Scores, statistics and outputs are fp32.
+//
+// Measured (bf16, 32 query and 8 kv heads of 128, in a graph, join included): 6 sequences
+// of 40 to 60 thousand positions, 581 MB, 102 us (5.7 TB/s; 115 when run for a second on
+// end, at lower clocks); 64 sequences of 11 to 7000 positions, 168 MB, 44 us (3.9 TB/s:
+// 5 to 7 us of shares and join, and each tile's start and end). The schedulers issue in
+// 46 % of cycles, the ALU pipe (conversion, masks, exponents) is busy in 45 %: between
+// the 16-bit form's balance and HBM. Not kept: a share per warp instead of per CTA (no
+// sum over warps at a tile's end, but four times the parts to join: 47 us for the
+// 64 sequences), finding the next tile's place and pages ahead (44.3 against 43.7).
 #include "bq_host.h"
 #include "bq_paged8.cuh"
 #include "bq_paged8_host.h"
