@@ -111,5 +111,7 @@ class ReplicaGroup:
             while others and time.monotonic() < deadline:
                 others = [r for r in others if not self.store.check([self._key("close", f"left{r}")])]
                 time.sleep(0.001)
+            if self.world > 1:
+                time.sleep(0.5)  # the others' processes end after their mark; a launcher may end what outlives this one
         except (RuntimeError, OSError):
             pass
