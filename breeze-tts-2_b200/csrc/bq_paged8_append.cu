@@ -41,7 +41,8 @@ struct Append8Params {
     PagedKV kv;
     Paged8Scales sc;
     int32_t rope_rows, has_norm;
-    int32_t window, kv_ctas, q_parts;  // rows of a CTA; CTAs along y of the k and v heads; CTAs among which a window's queries are divided
+    int32_t window, kv_ctas;  // rows of a CTA; CTAs along y of the k and v heads
+    int32_t q_parts, q_sets;  // CTAs among which a window's queries are divided; a CTA's query heads / kQueryHeads
     float eps;
     const void* qkv;
     int64_t ldqkv;
@@ -54,28 +55,42 @@ struct Append8Params {
     int64_t ldq;
 };
 
+// Eight entries each of a position's cos and sin row, as they are in memory: loaded well
+// before they are needed.
 template <typename C>
-__device__ __forceinline__ void load8(const C* p, float (&v)[8]) {
-    if constexpr (sizeof(C) == 4) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-        unpack8<C>(*reinterpret_cast<const uint4*>(p), v);
+struct Angle {
+    static constexpr int N = sizeof(C) / 2;
+    uint4 c[N], s[N];
+    __device__ __forceinline__ void load(const Append8Params& p, int pos, int l) {
+        const uint4* a = reinterpret_cast<const uint4*>(static_cast<const C*>(p.cos) + int64_t(pos) * p.ldcs + l * 8);
+        const uint4* b = reinterpret_cast<const uint4*>(static_cast<const C*>(p.sin) + int64_t(pos) * p.ldcs + l * 8);
+#pragma unroll
+        for (int i = 0; i < N; ++i) c[i] = a[i], s[i] = b[i];
     }
-}
+    __device__ static __forceinline__ void unpack(const uint4 (&w)[N], float (&v)[8]) {
+        if constexpr (N == 2) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                v[4 * i] = __uint_as_float(w[i].x), v[4 * i + 1] = __uint_as_float(w[i].y);
+                v[4 * i + 2] = __uint_as_float(w[i].z), v[4 * i + 3] = __uint_as_float(w[i].w);
+            }
+        } else {
+            unpack8<C>(w[0], v);
+        }
+    }
+};
 
 // Norm and rotation of one head: lane l of its group holds dims 8 l .. 8 l + 7. Every
 // lane of the warp calls it (the shuffles are the warp's).
 template <typename E, typename C, int D>
-__device__ __forceinline__ void turn(const Append8Params& p, int pos, int l, const void* gain, float (&v)[8]) {
+__device__ __forceinline__ void turn(const Append8Params& p, const Angle<C>& at, int l, const uint4& gain, float (&v)[8]) {
     constexpr int LG = D / 8;
     float c[8], s[8];
-    load8<C>(static_cast<const C*>(p.cos) + int64_t(pos) * p.ldcs + l * 8, c);
-    load8<C>(static_cast<const C*>(p.sin) + int64_t(pos) * p.ldcs + l * 8, s);
+    Angle<C>::unpack(at.c, c);
+    Angle<C>::unpack(at.s, s);
     if (p.has_norm) {
         float g[8], ss = 0.f;
-        load8<E>(static_cast<const E*>(gain) + l * 8, g);
+        unpack8<E>(gain, g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
@@ -89,6 +104,11 @@ __device__ __forceinline__ void turn(const Append8Params& p, int pos, int l, con
         const float other = __shfl_xor_sync(0xffffffffu, v[i], LG / 2);
         v[i] = v[i] * c[i] + (l < LG / 2 ? -other : other) * s[i];
     }
+}
+
+template <typename E>
+__device__ __forceinline__ uint4 gain_of(const Append8Params& p, const void* gain, int l) {
+    return p.has_norm ? *reinterpret_cast<const uint4*>(static_cast<const E*>(gain) + l * 8) : make_uint4(0, 0, 0, 0);
 }
 
 // Largest finite magnitude, as its bits (they order as the values do).
@@ -159,6 +179,7 @@ __global__ void __launch_bounds__(kRowThreads) append8_rows_kernel(const __grid_
     const bool live = h < heads;
     uint4 raw = make_uint4(0, 0, 0, 0);
     if (live) raw = *reinterpret_cast<const uint4*>(static_cast<const E*>(p.qkv) + int64_t(b) * p.ldqkv + h * D + l * 8);
+    const uint4 gain = gain_of<E>(p, h < kv.HQ ? p.qn : p.kn, l);
     const int pos = max(kv.lens[b], 0) - 1;
     if (pos < 0) return;  // an unused batch slot
     bool ok = pos < p.rope_rows && (pos >> kv.page_shift) < kv.max_pages;
@@ -166,6 +187,9 @@ __global__ void __launch_bounds__(kRowThreads) append8_rows_kernel(const __grid_
         if (threadIdx.x == 0) atomicOr(kv.errors, BQ_DEVERR_POSITION_BIT);
         return;
     }
+    const bool turns = blockIdx.y * HEADS < kv.HQ + kv.HKV;  // block-uniform: some head of this block is a q or k head
+    Angle<C> angle;
+    if (turns) angle.load(p, pos, l);
     const int page = paged_page(kv, b, pos, ok);
     if (!ok) {
         if (threadIdx.x == 0) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
@@ -181,11 +205,11 @@ __global__ void __launch_bounds__(kRowThreads) append8_rows_kernel(const __grid_
     }
     float v[8];
     unpack8<E>(raw, v);
-    if (blockIdx.y * HEADS < kv.HQ + kv.HKV) {  // block-uniform: some head of this block is a q or k head
+    if (turns) {
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = v[i];
-        turn<E, C, D>(p, pos, l, h < kv.HQ ? p.qn : p.kn, y);
+        turn<E, C, D>(p, angle, l, gain, y);
         if (h < kv.HQ + kv.HKV) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = y[i];
@@ -240,7 +264,7 @@ __device__ __forceinline__ int find_segments(const PagedKV& kv, int w0, int w1, 
 
 // R: rows of a block that each group of lanes holds. block / R groups take a head's block, GROUPS R / block heads the CTA.
 template <typename E, typename C, int D, int R>
-__global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __grid_constant__ Append8Params p) {
+__global__ void __launch_bounds__(kBlockThreads, R == 2 ? 3 : 2) append8_blocks_kernel(const __grid_constant__ Append8Params p) {
     constexpr int LG = D / 8, GROUPS = kBlockThreads / LG;
     __shared__ Segment seg[kMostBlock];
     __shared__ int s_count, s_pos[kMostBlock];
@@ -253,7 +277,7 @@ __global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __g
     const bool queries = int(blockIdx.y) >= p.kv_ctas;
     if (queries) {  // of some heads and a part of the window
         const int y = blockIdx.y - p.kv_ctas, part = y % p.q_parts;
-        h0 = y / p.q_parts * kQueryHeads;
+        h0 = y / p.q_parts * (p.q_sets * kQueryHeads);
         w0 += part * (p.window / p.q_parts);
         w1 = min(w1, w0 + p.window / p.q_parts);
         if (w0 >= w1) return;
@@ -274,27 +298,33 @@ __global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __g
             s_pos[r] = pos;
         }
         __syncthreads();
-        const int total = (w1 - w0) * kQueryHeads;
-        uint4 raw[2];
-        auto row_of = [&](int i) { return min(i, total - 1) / kQueryHeads; };
-        auto head_of = [&](int i) { return min(h0 + min(i, total - 1) % kQueryHeads, kv.HQ - 1); };
-        auto load = [&](int i) {
-            return *reinterpret_cast<const uint4*>(static_cast<const E*>(p.qkv) + int64_t(w0 + row_of(i)) * p.ldqkv + head_of(i) * D + l * 8);
-        };
+        // A group takes the heads of one row at a time, the next row's on their way meanwhile. (q may be written where qkv
+        // is read: the next row is another one.)
+        const uint4 gain = gain_of<E>(p, p.qn, l);
+        uint4 raw[kQueryHeads];
+        Angle<C> angle;
+        auto row_at = [&](int r) { return static_cast<const E*>(p.qkv) + int64_t(w0 + r) * p.ldqkv + l * 8; };
+        auto load = [&](const E* row, int q) { raw[q] = *reinterpret_cast<const uint4*>(row + min(h0 + q, kv.HQ - 1) * D); };
+        const int per = GROUPS / p.q_sets;  // rows at a time; the sets of heads beside one another
+        h0 += g / per * kQueryHeads;
+        int next = min(g % per, w1 - w0 - 1);
+        angle.load(p, max(s_pos[next], 0), l);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) raw[q] = load(q * GROUPS + g);
-        for (int i0 = 0; i0 < total; i0 += 2 * GROUPS) {  // all lanes of a warp stay for the shuffles
+        for (int q = 0; q < kQueryHeads; ++q) load(row_at(next), q);
+        for (int r0 = 0; r0 < w1 - w0; r0 += per) {  // all lanes of a warp stay for the shuffles
+            const int r = r0 + g % per;
+            const bool here = r < w1 - w0 && s_pos[r] >= 0;
+            const Angle<C> at = angle;
+            next = min(r + per, w1 - w0 - 1);
+            angle.load(p, max(s_pos[next], 0), l);
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int i = i0 + q * GROUPS + g, r = row_of(i), pos = s_pos[r];
+            for (int q = 0; q < kQueryHeads; ++q) {
                 float v[8];
                 unpack8<E>(raw[q], v);
-                const bool here = i < total && h0 + i % kQueryHeads < kv.HQ && pos >= 0;
-                const int head = head_of(i);
-                // (q may be written where qkv is read: the next rows are other ones)
-                raw[q] = load(i + 2 * GROUPS);
-                turn<E, C, D>(p, max(pos, 0), l, p.qn, v);
-                if (here) *reinterpret_cast<uint4*>(static_cast<E*>(p.q_out) + int64_t(w0 + r) * p.ldq + head * D + l * 8) = pack8<E>(v);
+                load(row_at(next), q);
+                turn<E, C, D>(p, at, l, gain, v);
+                if (here && h0 + q < kv.HQ)
+                    *reinterpret_cast<uint4*>(static_cast<E*>(p.q_out) + int64_t(w0 + r) * p.ldq + (h0 + q) * D + l * 8) = pack8<E>(v);
             }
         }
         return;
@@ -304,6 +334,7 @@ __global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __g
     const int h = min(int(blockIdx.y) * (GROUPS / mine) + item, 2 * kv.HKV - 1);  // k heads, then v heads
     const bool live = int(blockIdx.y) * (GROUPS / mine) + item < 2 * kv.HKV, is_k = h < kv.HKV;
     const int warp0 = item * mine * LG / 32, warps = mine * LG / 32;  // the head's warps
+    const uint4 gain = gain_of<E>(p, p.kn, l);
     int turnover = 0;
     for (int i = 0; i < n_seg; ++i) {
         const Segment s = seg[i];
@@ -323,28 +354,36 @@ __global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __g
             const int n = min(rows, max(0, p.rope_rows - p0));
             bool ok = (p0 >> kv.page_shift) < kv.max_pages;
             if ((!ok || n < rows) && threadIdx.x == 0) atomicOr(kv.errors, BQ_DEVERR_POSITION_BIT);
+            ok = ok && n > 0;
             int page = 0;
-            if (ok && n > 0) {
-                page = paged_page(kv, s.b, p0, ok);
-                if (!ok && threadIdx.x == 0) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
-            }
-            if (ok && n > 0) {  // (the same for all threads)
-                const int slot = p0 & kv.page_mask;
-                const BlockAt at = block_at(p, h, page, slot - kept);
-                const int was = kept ? scale_exp(*at.scale) : -kExpMost;
+            uint4 raw[R];
+            Angle<C> angle;  // of the group's next row
+            if (ok) {
                 const E* src = static_cast<const E*>(p.qkv) + int64_t(r0) * p.ldqkv + (kv.HQ + h) * D + l * 8;
-                uint4 raw[R];
 #pragma unroll
                 for (int q = 0; q < R; ++q) {
                     raw[q] = make_uint4(0, 0, 0, 0);
                     if (gi + q * mine < n) raw[q] = *reinterpret_cast<const uint4*>(src + int64_t(gi + q * mine) * p.ldqkv);
                 }
+                if (is_k) angle.load(p, p0 + min(gi, n - 1), l);  // (the same for a warp)
+                page = paged_page(kv, s.b, p0, ok);
+                if (!ok && threadIdx.x == 0) atomicOr(kv.errors, BQ_DEVERR_PAGE_BIT);
+            }
+            if (ok) {  // (the same for all threads)
+                const int slot = p0 & kv.page_mask;
+                const BlockAt at = block_at(p, h, page, slot - kept);
+                const int was = kept ? scale_exp(*at.scale) : -kExpMost;
                 float v[R][8];
                 uint32_t top = 0;
 #pragma unroll
                 for (int q = 0; q < R; ++q) {
+                    if (q * mine >= n) continue;  // (the same for all threads)
                     unpack8<E>(raw[q], v[q]);
-                    if (is_k) turn<E, C, D>(p, p0 + min(gi + q * mine, n - 1), l, p.kn, v[q]);  // (the same for a warp)
+                    if (is_k) {
+                        const Angle<C> now = angle;
+                        if (q + 1 < R) angle.load(p, p0 + min(gi + (q + 1) * mine, n - 1), l);
+                        turn<E, C, D>(p, now, l, gain, v[q]);
+                    }
                     if (gi + q * mine < n) top = max(top, top_of(v[q]));
                 }
                 top = __reduce_max_sync(0xffffffffu, top);
@@ -377,7 +416,8 @@ __global__ void __launch_bounds__(kBlockThreads) append8_blocks_kernel(const __g
 
 template <typename E, typename C, int D>
 const void* blocks_kernel(int r) {
-    return r == 8 ? reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 8>)
+    return r == 2   ? reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 2>)
+           : r == 8 ? reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 8>)
                   : reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 4>);
 }
 template <typename E, typename C>
@@ -435,7 +475,7 @@ extern "C" int32_t bq_paged8_append(const bq_paged8_append_desc* d, void* stream
     p.q_out = d->q_out;
     p.ldq = d->ldq;
     const bool f32 = d->cs_dtype == BQ_DT_F32, bf = d->kv.dtype == BQ_DT_BF16, rows = !d->kv.q_starts;
-    const int lanes = d->kv.D / 8, r = d->kv.block * lanes > 4 * kBlockThreads ? 8 : 4;
+    const int lanes = d->kv.D / 8, r = std::max(2, d->kv.block * lanes / kBlockThreads);
     const void* fn = bf ? (f32 ? append_kernel<__nv_bfloat16, float>(d->kv.D, rows, r)
                                : append_kernel<__nv_bfloat16, __nv_bfloat16>(d->kv.D, rows, r))
                         : (f32 ? append_kernel<__half, float>(d->kv.D, rows, r) : append_kernel<__half, __half>(d->kv.D, rows, r));
@@ -451,8 +491,9 @@ extern "C" int32_t bq_paged8_append(const bq_paged8_append_desc* d, void* stream
     // of 16 heads: 8 rounds 10.7 us, 2 rounds 7.7; 16000 of 32: 84 and 92 us).
     const DeviceInfo* di = device_info();
     if (!di) return BQ_ERR_CUDA;
-    const int windows = (d->T + p.window - 1) / p.window, q_heads = (d->HQ + kQueryHeads - 1) / kQueryHeads;
-    p.q_parts = 1;
+    p.q_parts = p.q_sets = 1;
+    while (2 * p.q_sets * p.window * lanes <= kBlockThreads) p.q_sets *= 2;
+    const int windows = (d->T + p.window - 1) / p.window, q_heads = (d->HQ + p.q_sets * kQueryHeads - 1) / (p.q_sets * kQueryHeads);
     while (2 * p.q_parts * kBlockThreads <= p.window * lanes && int64_t(windows) * q_heads * p.q_parts < 8 * di->sm_count) p.q_parts *= 2;
     return paged_launch(fn, dim3(windows, p.kv_ctas + q_heads * p.q_parts),
                         dim3(kBlockThreads), 0, args, d->flags, stream, "paged append");
