@@ -18,10 +18,11 @@
 // scale, so a CTA takes all new tokens of a block of as many heads as its lanes hold in
 // registers between the maximum and the codes; queries go to CTAs of their own.
 //
-// Measured in a graph: 2 rows of 48 heads 2.1 us, 160 rows of 48 heads 3.0 us (both the
-// chain of loads); seven prompts of 28 heads of 64, blocks of 16, 26.9 MB in 15.0 us
-// (1.8 TB/s: waves of short CTAs, each with its search for the sequence, its loads, one
-// barrier and its stores).
+// Measured in a graph: 2 rows of 48 heads 2.0 us, 160 rows of 48 heads 3.0 us (both the
+// chain of loads); eight drafted rows of 48 heads 4.8 us; seven prompts of 28 heads of
+// 64, blocks of 16, 26.9 MB in 11.5 us (2.3 TB/s: waves of short CTAs, each with its search
+// for the sequence, its loads, one barrier and its stores). cos and sin are loaded a row
+// ahead: loaded where they are used, each row waited for its own (prompts 15.0 us).
 #include <algorithm>
 #include <cstring>
 
@@ -262,7 +263,9 @@ __device__ __forceinline__ int find_segments(const PagedKV& kv, int w0, int w1, 
     return min(*count, kMostBlock);  // (more only where starts are out of order)
 }
 
-// R: rows of a block that each group of lanes holds. block / R groups take a head's block, GROUPS R / block heads the CTA.
+// R: rows of a block that each group of lanes holds: as few as give each CTA one head, but for short blocks, of which a
+// CTA takes several heads (blocks of 16 rows of 64 dims: 1 row 13.1 us, 2 rows 11.5, 4 rows 12.9). With two rows three CTAs
+// fit an SM, with more two (three, spilling: 400 rows 11.0 against 7.0 us). block / R groups take a head's block, GROUPS R / block heads the CTA.
 template <typename E, typename C, int D, int R>
 __global__ void __launch_bounds__(kBlockThreads, R == 2 ? 3 : 2) append8_blocks_kernel(const __grid_constant__ Append8Params p) {
     constexpr int LG = D / 8, GROUPS = kBlockThreads / LG;
@@ -487,14 +490,15 @@ extern "C" int32_t bq_paged8_append(const bq_paged8_append_desc* d, void* stream
     p.window = paged8_window(&d->kv, d->T, d->kv.block);
     const int heads = kBlockThreads / lanes * r / d->kv.block;  // of a CTA
     p.kv_ctas = (2 * d->kv.HKV + heads - 1) / heads;
-    // Queries: a window's are divided among CTAs, down to two rounds each, until there are eight CTAs for every SM (400 rows
-    // of 16 heads: 8 rounds 10.7 us, 2 rounds 7.7; 16000 of 32: 84 and 92 us).
+    // Queries: a short window's rows do not fill a CTA, which takes several sets of heads then (prompts with blocks of 16:
+    // 14.7 -> 11.5 us). A long one's are divided among CTAs until there are three for every SM (400 rows of 16 heads: undivided
+    // 8.0 us, in four 7.0; 16000 of 32: 60 and 74 us).
     const DeviceInfo* di = device_info();
     if (!di) return BQ_ERR_CUDA;
     p.q_parts = p.q_sets = 1;
     while (2 * p.q_sets * p.window * lanes <= kBlockThreads) p.q_sets *= 2;
     const int windows = (d->T + p.window - 1) / p.window, q_heads = (d->HQ + p.q_sets * kQueryHeads - 1) / (p.q_sets * kQueryHeads);
-    while (2 * p.q_parts * kBlockThreads <= p.window * lanes && int64_t(windows) * q_heads * p.q_parts < 8 * di->sm_count) p.q_parts *= 2;
+    while (2 * p.q_parts * kBlockThreads <= p.window * lanes && int64_t(windows) * q_heads * p.q_parts < 3 * di->sm_count) p.q_parts *= 2;
     return paged_launch(fn, dim3(windows, p.kv_ctas + q_heads * p.q_parts),
                         dim3(kBlockThreads), 0, args, d->flags, stream, "paged append");
 }
