@@ -263,9 +263,10 @@ __device__ __forceinline__ int find_segments(const PagedKV& kv, int w0, int w1, 
     return min(*count, kMostBlock);  // (more only where starts are out of order)
 }
 
-// R: rows of a block that each group of lanes holds: as few as give each CTA one head, but for short blocks, of which a
-// CTA takes several heads (blocks of 16 rows of 64 dims: 1 row 13.1 us, 2 rows 11.5, 4 rows 12.9). With two rows three CTAs
-// fit an SM, with more two (three, spilling: 400 rows 11.0 against 7.0 us). block / R groups take a head's block, GROUPS R / block heads the CTA.
+// R: rows of a block that each group of lanes holds: block / R groups take a head's block, GROUPS R / block heads the CTA.
+// As few as give each CTA one head, but for short blocks, of which it takes several heads (blocks of 16 rows of 64 dims:
+// 1 row 13.1 us, 2 rows 11.5, 4 rows 12.9). With two rows three CTAs fit an SM, with more two (three, spilling: 400 rows
+// 11.0 against 7.0 us).
 template <typename E, typename C, int D, int R>
 __global__ void __launch_bounds__(kBlockThreads, R == 2 ? 3 : 2) append8_blocks_kernel(const __grid_constant__ Append8Params p) {
     constexpr int LG = D / 8, GROUPS = kBlockThreads / LG;

@@ -5,7 +5,7 @@
 // Bound: HBM, 1 byte read and 2 (4) written per element. A CTA takes a window of
 // rows and some heads of k or of v; a thread turns 16 codes at a time (32 bytes out),
 // several of them in flight. Measured: 96925 rows of 8 heads of 128 to bf16, 595 MB in
-// 122 us (4.9 TB/s); 410 rows of 16 heads 4.5 us. Two
+// 105 us (5.7 TB/s); 410 rows of 16 heads 4.4 us. Two
 // stores of 16 bytes instead of one of 32 cost the long case 5 %.
 #include <cstring>
 
@@ -16,7 +16,7 @@
 namespace bq {
 namespace {
 
-constexpr int kThreads = 256, kMostRows = 64, kMostHeads = 8, kFlight = 4;
+constexpr int kThreads = 256, kMostRows = 64, kMostHeads = 8;
 
 struct Read8Params {
     PagedKV kv;
@@ -58,8 +58,11 @@ __device__ __forceinline__ void store16(T* dst, const float (&v)[16], bool align
     }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__ Read8Params p) {
+// FLIGHT: pieces that a thread has on their way. Four where all CTAs run at once (they fit an SM four times); two where
+// more CTAs come after one another, eight on an SM then (96925 rows of 8 heads of 128: 122 us with four, 105 with two;
+// 410 rows of 16 heads: 4.4 and 5.0; 6500 rows of 8: 9.6 and 16).
+template <typename T, int D, int FLIGHT>
+__global__ void __launch_bounds__(kThreads, FLIGHT == 2 ? 8 : 1) read8_kernel(const __grid_constant__ Read8Params p) {
     constexpr int CH = D / 16;  // pieces of a head
     __shared__ int s_page[kMostRows], s_slot[kMostRows];
     pdl_launch_dependents();
@@ -120,11 +123,11 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
     T* out = static_cast<T*>(is_k ? p.k_out : p.v_out);
     const int64_t o_row = is_k ? p.ko_row : p.vo_row, o_head = is_k ? p.ko_head : p.vo_head;
     const int total = rows * CHH;
-    for (int i0 = threadIdx.x; i0 < total; i0 += kThreads * kFlight) {
-        uint4 w[kFlight];
-        uint8_t e[kFlight];
+    for (int i0 = threadIdx.x; i0 < total; i0 += kThreads * FLIGHT) {
+        uint4 w[FLIGHT];
+        uint8_t e[FLIGHT];
 #pragma unroll
-        for (int f = 0; f < kFlight; ++f) {
+        for (int f = 0; f < FLIGHT; ++f) {
             const int i = i0 + f * kThreads, r = i >> row_shift, h = h0 + (i & (CHH - 1)) / CH, c = i % CH;
             w[f] = make_uint4(0, 0, 0, 0);
             e[f] = kExpBias;
@@ -135,7 +138,7 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
             }
         }
 #pragma unroll
-        for (int f = 0; f < kFlight; ++f) {
+        for (int f = 0; f < FLIGHT; ++f) {
             const int i = i0 + f * kThreads, r = i >> row_shift, h = h0 + (i & (CHH - 1)) / CH, c = i % CH;
             if (i >= total || h >= kv.HKV || s_page[r] < 0) continue;
             const float s = exp_scale(scale_exp(e[f]));
@@ -157,11 +160,11 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
     }
 }
 
-template <int D>
+template <int D, int FLIGHT>
 const void* read_kernel(int dtype) {
-    return dtype == BQ_DT_BF16  ? reinterpret_cast<const void*>(&read8_kernel<__nv_bfloat16, D>)
-           : dtype == BQ_DT_F16 ? reinterpret_cast<const void*>(&read8_kernel<__half, D>)
-                                : reinterpret_cast<const void*>(&read8_kernel<float, D>);
+    return dtype == BQ_DT_BF16  ? reinterpret_cast<const void*>(&read8_kernel<__nv_bfloat16, D, FLIGHT>)
+           : dtype == BQ_DT_F16 ? reinterpret_cast<const void*>(&read8_kernel<__half, D, FLIGHT>)
+                                : reinterpret_cast<const void*>(&read8_kernel<float, D, FLIGHT>);
 }
 
 }  // namespace
@@ -191,15 +194,16 @@ extern "C" int32_t bq_paged8_read(const bq_paged8_read_desc* d, void* stream) {
     std::memset(&p, 0, sizeof(p));
     rc = paged8_fill(&p.kv, &p.sc, &d->kv, d->T, 0);
     if (rc) return rc;
-    // A CTA's start (its rows' sequences, lengths and pages) takes as long as some 16 KB of codes do: large pieces, as far
-    // as there is a CTA for every SM (96925 rows of 8 heads of 128: 32 rows of 2 / 4 / 8 heads 253 / 162 / 124 us, 64 of
-    // 8 122 us; 410 rows of 16 heads: 32 rows of 2 / 4 / 8 heads 4.9 / 5.6 / 6.2 us, 16 of 4 4.4 us).
+    // A CTA's start (its rows' sequences, lengths and pages) takes as long as some 16 KB of codes do: large pieces (96925 rows
+    // of 8 heads of 128: 32 rows of 2 / 4 / 8 heads 253 / 162 / 124 us, 64 of 8 122 us), but two CTAs for every SM, so that
+    // enough is on its way (at least one / two / four for each: 5000 rows of 8 heads 15.7 / 9.6 / 10.8 us, 3000 rows 9.3 /
+    // 6.5 / 7.2, 410 rows of 16 heads 4.5 / 4.4 / 4.5).
     const DeviceInfo* di = device_info();
     if (!di) return BQ_ERR_CUDA;
     int heads = 1;
     while (heads < d->kv.HKV && heads < kMostHeads) heads *= 2;
     p.window = paged8_window(&d->kv, d->T, kMostRows);
-    while (int64_t((d->T + p.window - 1) / p.window) * 2 * ((d->kv.HKV + heads - 1) / heads) < di->sm_count) {
+    while (int64_t((d->T + p.window - 1) / p.window) * 2 * ((d->kv.HKV + heads - 1) / heads) < 2 * di->sm_count) {
         if (p.window > 16 || (heads == 1 && p.window > 4))
             p.window /= 2;
         else if (heads > 1)
@@ -217,8 +221,10 @@ extern "C" int32_t bq_paged8_read(const bq_paged8_read_desc* d, void* stream) {
     p.aligned = ((reinterpret_cast<uintptr_t>(d->k_out) | reinterpret_cast<uintptr_t>(d->v_out)) & 31) == 0;
     for (int i = 0; i < 2; ++i)
         if (size[i] > 1 && (d->ko_stride[i] * elem % 32 || d->vo_stride[i] * elem % 32)) p.aligned = 0;
-    const void* fn = d->kv.D == 128 ? read_kernel<128>(d->kv.dtype) : read_kernel<64>(d->kv.dtype);
+    const dim3 grid((d->T + p.window - 1) / p.window, 2 * ((d->kv.HKV + heads - 1) / heads));
+    const bool many = int64_t(grid.x) * grid.y > 4 * di->sm_count;
+    const void* fn = d->kv.D == 128 ? (many ? read_kernel<128, 2>(d->kv.dtype) : read_kernel<128, 4>(d->kv.dtype))
+                                    : (many ? read_kernel<64, 2>(d->kv.dtype) : read_kernel<64, 4>(d->kv.dtype));
     void* args[] = {&p};
-    return paged_launch(fn, dim3((d->T + p.window - 1) / p.window, 2 * ((d->kv.HKV + heads - 1) / heads)), dim3(kThreads), 0, args,
-                        d->flags, stream, "paged read");
+    return paged_launch(fn, grid, dim3(kThreads), 0, args, d->flags, stream, "paged read");
 }
