@@ -339,6 +339,20 @@ def test_reading_back(lens, new, hkv, dim, page, block, dtype, layout):
     assert (wide[0, :, 0] == 3.0).all() and (wide[0, :, :, :dim] == 3.0).all() and (wide[1, :, -1] == 3.0).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, F16, torch.float32])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_reading_back_with_more_blocks_than_run_at_once(ragged, dtype, dim):
+    """700 sequences of one to three rows: some 1400 thread blocks."""
+    lens = [1 + (7 * i) % 40 for i in range(700)]
+    new = [min(n, 1 + i % 3) for i, n in enumerate(lens)] if ragged else None
+    c = pc.batch(lens, new, 3, 3, dim, 16, 16, BF, seed=33, levels=30)
+    d = pc.to({k: c[k] for k in ("k", "v", "ks", "vs", "table", "lens")}, DEV)
+    k, v = _api().paged_read_fp8(*where(d), q_starts=c["starts"].to(DEV) if ragged else None, rows=c["rows"], dtype=dtype)
+    torch.cuda.synchronize()
+    check_read(c, k, v, dtype)
+
+
 def test_every_code_and_scale_is_read_as_what_it_is():
     codes = torch.arange(256, dtype=torch.uint8).repeat(64).reshape(1, 1, 128, 128)  # 8 blocks of 16 positions
     scales = torch.tensor([[[67, 187, 127, 110, 135, 0, 254, 255]]], dtype=torch.uint8)
