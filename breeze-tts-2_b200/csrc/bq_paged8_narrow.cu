@@ -41,9 +41,13 @@ constexpr int kWarps = kNarrowWarps, kThreads = 32 * kWarps;
 constexpr int kRows = kNarrowRows, kUnit = kNarrowUnit, kOverhead = kNarrow8Overhead;
 constexpr int kStep = 32;              // positions of a warp's step
 constexpr int kBatch = 32 * 16 / kStep;  // steps whose pages the lanes hold, one block of 16 positions each
-// Weights are kept times 2^15, as they enter the product. With exponents of v that lie 120 apart (they cannot lie
-// further), what fp32 flushes of them is less than 2^-21 of the largest term of the sum of exponentials each.
+// Weights are kept times 2^15, as they enter the product: relative to a reference 15 below the largest score. With
+// exponents of v that lie 120 apart (they cannot lie further), what fp32 flushes of them is less than 2^-21 of the
+// largest term of the sum of exponentials each.
 constexpr int kLift = 15;
+// Rounded up, so that no weight passes 2^15 however large the scores are (from 2^24 on fp32 does not hold m - 15, and
+// fp16 ends at 2^16); sums and outputs are relative to what came out, so that nothing else depends on it.
+__device__ __forceinline__ float reference(float m) { return __fadd_ru(m, -float(kLift)); }
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool full) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
@@ -305,7 +309,7 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
             const uint32_t ee = __shfl_sync(0xffffffffu, exp_now, 2 * st % 32 + b);
             const int ev = scale_exp(ee >> 8);
             const float ks = exp_scale(scale_exp(ee & 255)), a0 = f0 * ks, a1 = f1 * ks, y = float(ev);
-            back[b] = exp_scale(-ev - kLift);
+            back[b] = exp_scale(-ev);
 #pragma unroll
             for (int n = 2 * b; n < 2 * b + 2; ++n)
 #pragma unroll
@@ -334,20 +338,20 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
         n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
         if constexpr (TWO) n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
         if (__any_sync(0xffffffffu, n0 != m0 || (TWO && n1 != m1))) {  // a maximum moved: rescale what was summed
-            const float a0 = n0 == m0 ? 1.f : ex2(0.5f * (m0 - n0));  // in two steps: l may be as far from 1
+            const float a0 = n0 == m0 ? 1.f : ex2(0.5f * (reference(m0) - reference(n0)));  // in two steps: l may be as far from 1
             l0 = l0 * a0 * a0;
 #pragma unroll
             for (int n = 0; n < T; ++n) o[n][0] *= a0 * a0, o[n][1] *= a0 * a0;
             m0 = n0;
             if constexpr (TWO) {
-                const float a1 = n1 == m1 ? 1.f : ex2(0.5f * (m1 - n1));
+                const float a1 = n1 == m1 ? 1.f : ex2(0.5f * (reference(m1) - reference(n1)));
                 l1 = l1 * a1 * a1;
 #pragma unroll
                 for (int n = 0; n < T; ++n) o[n][2] *= a1 * a1, o[n][3] *= a1 * a1;
                 m1 = n1;
             }
         }
-        const float u0 = (m0 == -INFINITY ? 0.f : m0) - kLift, u1 = (m1 == -INFINITY ? 0.f : m1) - kLift;  // (rows that see nothing yet)
+        const float u0 = m0 == -INFINITY ? 0.f : reference(m0), u1 = m1 == -INFINITY ? 0.f : reference(m1);  // (rows that see nothing yet)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
 #pragma unroll
@@ -406,9 +410,9 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
     // exponent of l goes into m, and out of l and o.
     auto settle = [&](float& m, float& l) {
         const int k = l > 0.f && l < INFINITY ? int(__float_as_uint(l) >> 23) - 127 : 0;
-        m += float(k);
+        m = reference(m) + float(k);
         l *= exp_scale(-k);
-        return exp_scale(-k - kLift);
+        return exp_scale(-k);
     };
     const float z0 = settle(m0, l0), z1 = settle(m1, l1);
     __syncthreads();  // every warp is done with its ring: it now takes the warps' outputs

@@ -1,0 +1,101 @@
+"""8-bit paged cache, far ends of its ranges: scores so large that fp32 steps over whole units. Tolerances stand beside
+each case."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import paged8 as o8
+from tests import paged_fp8_cases as pc
+from tests.test_paged_fp8_gpu import DEV, _api, _clean_status, oracle, run, table_room, where  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+BF, F16, F8, E8 = pc.BF, pc.F16, pc.F8, pc.E8
+LOG2E = 1.4426950408889634
+
+# one token per sequence, and a few (12 rows per kv head)
+FORMS = [([700, 260], None), ([700, 260], [6, 5])]
+
+
+def fill(c, values):
+    """Keys: the same value in every dim, values(b, p) at position p of sequence b."""
+    k = torch.zeros(c["k"].shape)
+    for b, n in enumerate(c["lens"].tolist()):
+        for p in range(n):
+            k[c["table"][b, p // c["page"]], :, p % c["page"]] = values(b, p)
+    c["k"], c["ks"] = pc.quantise(k, c["used"], c["block"])
+
+
+def visible(c):
+    """Sequence and visible positions of every row."""
+    lens = c["lens"].tolist()
+    starts = list(range(len(lens) + 1)) if c["starts"] is None else c["starts"].tolist()
+    for b, n in enumerate(lens):
+        for r in range(starts[b], starts[b + 1]):
+            yield r, b, n - starts[b + 1] + r + 1
+
+
+def gathered(c, codes, scales, b, n):
+    """(HKV, n, D) in 64 bits."""
+    x = o8.values(codes, scales)[c["table"][b, :-(-n // c["page"])].long()]
+    return x.transpose(0, 1).reshape(c["hkv"], -1, c["dim"])[:, :n]
+
+
+LARGE = [2.0 ** 22, 2.0 ** 24 + 2, 3.1e7, 2.0 ** 25, 1.3e8, 2.0 ** 28, 1e9, 7e9, 1e30, -2.0 ** 24, -3.1e7, -1e9, -7e9]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("lens,new", FORMS)
+@pytest.mark.parametrize("top", LARGE)
+def test_one_large_score_takes_all(top, lens, new, dtype, table_room):
+    """The largest score, `top` in base 2, is a seventh of |top| or more above the others: its probability is 1 whatever
+    the scores' roundings, and the row is that position's value, exactly (four significant bits, sums of zeros)."""
+    dim = 128
+    c = table_room(pc.batch(lens, new, 4, 2, dim, 32, 16, dtype, seed=3, levels=2))
+    best, sign = (1.75, 1.0) if top > 0 else (0.25, -1.0)
+    c["q"][:] = sign
+    at = [5, 130]
+    others = [0.5, 0.75, 1.0, 1.25, 1.5]
+    fill(c, lambda b, p: best if p == at[b] else others[(p * 7) % 5])
+    scale = abs(top) / (best * dim * LOG2E)
+    out, lse = run(c, scale=scale)
+    o = out.double().reshape(c["rows"], 4, dim)
+    for r, b, n in visible(c):
+        want = gathered(c, c["v"], c["vs"], b, n)[:, at[b]].repeat_interleave(2, 0)
+        assert torch.equal(o[r], want), r
+    # a sum of `dim` equal terms, three roundings of the factor, the reference's, its part's and the last steps': 2^-23 each
+    assert ((lse.double() - top / LOG2E).abs() <= (dim + 16) * 2.0 ** -23 * abs(top)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("lens,new", FORMS)
+@pytest.mark.parametrize("base", [2.0 ** 23, 2.0 ** 24, 2.0 ** 25, 2.0 ** 26, -2.0 ** 24])
+def test_large_scores_that_rise_by_a_few_units(base, lens, new, dtype, table_room):
+    """Scores of `base` that rise by 7 or 8 from one piece of 128 positions to the next, which a reference may lag
+    behind: whatever the roundings, a row stays within the values that it sees."""
+    dim = 64
+    c = table_room(pc.batch(lens, new, 4, 2, dim, 32, 16, dtype, seed=5))
+    half = abs(base) / 512  # two dims of keys of 256
+    c["q"][:] = 0.0
+    q = c["q"].view(c["rows"], 4, dim)
+    parts = max(1, int(half // 2 ** 15))  # f16 queries hold 2^15
+    q[:, :, :2 * parts] = math.copysign(half / parts, base)
+    q[:, :, 60:] = 1.0
+    k = torch.zeros(c["k"].shape)
+    for b, n in enumerate(lens):
+        for p in range(n):
+            spot = k[c["table"][b, p // 32], :, p % 32]
+            spot[:, :2 * parts] = 256.0
+            rise = p // 128 * (7 + b)
+            for d in range(60, 64):  # as the sum of four: codes have four bits, and a step of 2^-1 at most here
+                step = min(rise, 15)
+                spot[:, d], rise = step, rise - step
+    c["k"], c["ks"] = pc.quantise(k, c["used"], 16)
+    out, lse = run(c, scale=math.log(2))
+    o = out.double().reshape(c["rows"], 4, dim)
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+    for r, b, n in visible(c):
+        v = gathered(c, c["v"], c["vs"], b, n).repeat_interleave(2, 0)
+        slack = (torch.finfo(dtype).eps / 2 + 2.0 ** -10 + (n + 24) * 2.0 ** -23) * v.abs().amax(1)
+        assert (o[r] <= v.amax(1) + slack).all() and (o[r] >= v.amin(1) - slack).all(), r
