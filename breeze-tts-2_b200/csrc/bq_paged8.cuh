@@ -35,6 +35,17 @@ __device__ __forceinline__ const uint8_t* v_scale(const Paged8Scales& s, int pag
     return static_cast<const uint8_t*>(s.v) + page * s.vs_page + j * s.vs_head + blk;
 }
 
+// The exponent of a part's sum of exponentials l goes into its reference m, as far as fp32 holds the two together (a
+// reference of 2^24 and more does not take every integer: equal parts would be weighed by up to a factor of two each),
+// and out of l; returns what the part's outputs are to be multiplied with.
+__device__ __forceinline__ float settle_part(float& m, float& l) {
+    if (!(l > 0.f && l < INFINITY)) return 1.f;
+    const float to = m + float(int(__float_as_uint(l) >> 23) - 127), f = ex2(m - to);
+    m = to;
+    l *= f;
+    return f;
+}
+
 // Four codes -> two pairs of f16 (exact; NaN stays NaN).
 __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
     lo = e4m3x2_to_f16x2(uint16_t(w));

@@ -406,13 +406,10 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    // From here on a part's reference is near its sum, so that parts are weighed by what they hold of the row: the
-    // exponent of l goes into m, and out of l and o.
+    // From here on a part's reference is near its sum, so that parts are weighed by what they hold of the row.
     auto settle = [&](float& m, float& l) {
-        const int k = l > 0.f && l < INFINITY ? int(__float_as_uint(l) >> 23) - 127 : 0;
-        m = reference(m) + float(k);
-        l *= exp_scale(-k);
-        return exp_scale(-k);
+        m = reference(m);
+        return settle_part(m, l);
     };
     const float z0 = settle(m0, l0), z1 = settle(m1, l1);
     __syncthreads();  // every warp is done with its ring: it now takes the warps' outputs

@@ -70,6 +70,30 @@ def test_one_large_score_takes_all(top, lens, new, dtype, table_room):
 
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("lens,new", FORMS)
+@pytest.mark.parametrize("top", LARGE)
+def test_large_scores_that_are_all_the_same(top, lens, new, dtype, table_room):
+    """Equal scores and equal exponents: the row is the mean of the values that it sees."""
+    dim = 64
+    c = table_room(pc.batch(lens, new, 4, 2, dim, 32, 32, dtype, seed=4))
+    c["q"][:] = 1.0 if top > 0 else -1.0
+    fill(c, lambda b, p: 1.0)
+    g = torch.Generator().manual_seed(1)
+    codes = (torch.randn(c["v"].shape, generator=g) * 100).clamp(-448, 448).masked_fill(~c["used"][:, None, :, None], math.nan)
+    c["v"] = codes.to(F8)
+    pc.bits(c["vs"])[:] = 119  # 2^-8
+    out, _ = run(c, scale=abs(top) / (dim * LOG2E))
+    o = out.double().reshape(c["rows"], 4, dim)
+    u = torch.finfo(dtype).eps / 2
+    for r, b, n in visible(c):
+        v = gathered(c, c["v"], c["vs"], b, n).repeat_interleave(2, 0)
+        want, size = v.mean(1), v.abs().mean(1)
+        # one rounding of the result (at least fp16's smallest), the same weight at each position up to ex2's 2^-22 in
+        # the sum of exponentials, n roundings of the sums and some at their joins
+        assert ((o[r] - want).abs() <= u * want.abs() + 2.0 ** -25 + (n + 24) * 2.0 ** -23 * size).all(), r
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("lens,new", FORMS)
 @pytest.mark.parametrize("base", [2.0 ** 23, 2.0 ** 24, 2.0 ** 25, 2.0 ** 26, -2.0 ** 24])
 def test_large_scores_that_rise_by_a_few_units(base, lens, new, dtype, table_room):
     """Scores of `base` that rise by 7 or 8 from one piece of 128 positions to the next, which a reference may lag
