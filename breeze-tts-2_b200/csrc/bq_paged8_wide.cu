@@ -62,6 +62,12 @@ constexpr int kReaders = 15;      // warps that read a tile of the walker's
 constexpr int kBlocks = kUnit / 16;
 constexpr int kLift = 7, kFarLift = 64;  // weights are kept times 2^7; where that is not enough, their sum is of 2^64 times
 constexpr int kSpread = 100;
+// Rows with maxima of this size and more are computed again at the tile's end (large_row). Below, the exponent of a
+// weight, s x + (y + 7 - M), is at most 15 for a score 8 above the reference M, and its roundings (half a unit of M's last
+// place, three times) are less than 0.1; from 2^23 on they would take it past fp16's range, and further on under it. Taking
+// the score's distance from the reference first, for all scores, costs prompts 257 us instead of 245, under a condition
+// behind the maximum 255 to 262, before it 269, in an instance of the loop of its own 370 (registers spill).
+constexpr float kLargeScore = 1048576.f;  // 2^20
 
 template <int D>
 struct Wide8Smem {
@@ -130,6 +136,69 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
         : "memory");
+}
+
+// Row `row` of a tile over positions [t.p0, end) in fp32, by one thread (slow, and little code: unrolled by two it would
+// cost every prompt 12 us), to where the tile's rows go:
+// `at` of the parts. Not a call: its registers would cost every tile (prompts 254 us instead of 245).
+template <typename E, int D>
+__device__ __forceinline__ void large_row(const PagedWork& w, const Paged8Scales& sc, const WideTile& t, int row, int end, int64_t at) {
+    const PagedKV& kv = w.kv;
+    const int tok = w.by_G(row), head = t.j * w.G + row - tok * w.G;
+    const E* q = static_cast<const E*>(w.q) + int64_t(t.s.begin + tok) * w.ldq + head * D;
+    bool page_ok = true;  // (a bad page has been reported by the warp that fetched it)
+    auto score = [&](int pos) {
+        const int page = paged_page(kv, t.s.table, pos, page_ok), slot = pos & kv.page_mask;
+        const uint8_t* k = static_cast<const uint8_t*>(kv.k) + page * kv.ks_page + t.j * kv.ks_head + int64_t(slot) * kv.ks_slot;
+        float s = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < D; d += 8) {
+            const uint2 codes = *reinterpret_cast<const uint2*>(k + d);
+            float x[8], c[4];
+            unpack8<E>(*reinterpret_cast<const uint4*>(q + d), x);
+            codes_f32(codes.x, c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s = fmaf(x[i], c[i], s);
+            codes_f32(codes.y, c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s = fmaf(x[4 + i], c[i], s);
+        }
+        // (rounded: as part of the difference below the product would not be, and its maximum is)
+        return __fmul_rn(s, w.scale_log2 * exp_scale(scale_exp(*k_scale(sc, page, t.j, slot >> sc.block_shift))));
+    };
+    float top = -INFINITY, sum = 0.f, o[D];
+#pragma unroll 1
+    for (int pos = t.p0; pos < end; ++pos) top = fmaxf(top, score(pos));
+#pragma unroll 1
+    for (int d = 0; d < D; ++d) o[d] = 0.f;
+#pragma unroll 1
+    for (int pos = t.p0; pos < end; ++pos) {
+        const float p = ex2(score(pos) - top);
+        sum += p;
+        const int page = paged_page(kv, t.s.table, pos, page_ok), slot = pos & kv.page_mask;
+        const uint8_t* v = static_cast<const uint8_t*>(kv.v) + page * kv.vs_page + t.j * kv.vs_head + int64_t(slot) * kv.vs_slot;
+        const float f = p * exp_scale(scale_exp(*v_scale(sc, page, t.j, slot >> sc.block_shift)));
+#pragma unroll 1
+        for (int d = 0; d < D; d += 4) {
+            float c[4];
+            codes_f32(*reinterpret_cast<const uint32_t*>(v + d), c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[d + i] = fmaf(f, c[i], o[d + i]);
+        }
+    }
+    const int64_t orow = t.s.begin + tok;
+    const float inv = t.whole ? 1.f / sum : 1.f;
+#pragma unroll 1
+    for (int d = 0; d < D; d += 2) {
+        if (t.whole)
+            *reinterpret_cast<uint32_t*>(static_cast<E*>(w.out) + orow * w.ldo + head * D + d) = pack2<E>(o[d] * inv, o[d + 1] * inv);
+        else
+            *reinterpret_cast<float2*>(w.part_o + at * D + d) = make_float2(o[d], o[d + 1]);
+    }
+    if (!t.whole)
+        w.part_ml[at] = make_float2(top, sum);
+    else if (w.lse)
+        w.lse[orow * w.ldl + head] = (top + log2f(sum)) * kLn2;
 }
 
 template <typename E, int D>
@@ -228,6 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
             const bool idle = (warp & 3) * 32 >= hrows;  // no row of this warp exists
             const int limit = row < hrows ? paged_row_limit<false>(w, t.s, myrow) : 0;
             float mref = -INFINITY, l = 0.f;
+            bool again = false;  // the row is one for large_row
             __syncwarp();  // tensor-memory instructions below are warp-wide
             for (int u = 0; u < units; ++u) {
                 ok = __all_sync(0xffffffffu, tc_wait(bar_s + 8 * h, done_units & 1, abort, lim, kv.errors));
@@ -282,6 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                         }
                     }
                     if (move) mref = m;
+                    again |= fabsf(mref) >= kLargeScore && mref != -INFINITY;
                     const float off = (mref == -INFINITY ? 0.f : -mref) + kLift;
                     const bool far = s_far[(table + u) % kTables];
                     if (__builtin_expect(far, 0)) {  // (before the weights, which let go of the scores)
@@ -392,6 +463,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                         w.lse[orow * w.ldl + head] = l != 0.f ? (mref + log2f(l)) * kLn2 : -INFINITY;
                 }
             }
+            if (__builtin_expect(again && row < hrows, 0))
+                large_row<E, D>(w, p.sc, t, myrow, min(limit, p1), int64_t(2 * blockIdx.x + (t.k0 == 0 ? 1 : 0)) * kRows + 128 * h + row);
             if (s_bad[n % kTiles] == n + 1 && row < hrows) {  // the rows that see a NaN value
                 const int tok = w.by_G(myrow), head = t.j * w.G + myrow - tok * w.G;
                 const int64_t orow = t.s.begin + tok;
