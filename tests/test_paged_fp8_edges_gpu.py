@@ -69,7 +69,7 @@ def test_one_large_score_takes_all(top, lens, new, dtype, table_room):
 
 
 @pytest.mark.parametrize("dtype", [BF, F16])
-@pytest.mark.parametrize("lens,new", FORMS[:2])
+@pytest.mark.parametrize("lens,new", FORMS)
 @pytest.mark.parametrize("top", LARGE)
 def test_large_scores_that_are_all_the_same(top, lens, new, dtype, table_room):
     """Equal scores and equal exponents: the row is the mean of the values that it sees."""
