@@ -714,9 +714,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                     if (u == 0) top = -kExpMost;
                     top = max(top, __reduce_max_sync(0xffffffffu, live ? ev : -kExpMost));
                     const int least = __reduce_min_sync(0xffffffffu, live ? ev : kExpMost), y = live ? ev : 0;
-                    if (lane < kBlocks)
+                    if (lane < kBlocks)  // (a factor of zero would make NaN of a masked score)
                         s_factor[unit % kTables][lane] =
-                            make_float4(fmaxf(w.scale_log2 * exp_scale(e), 1e-37f), float(y), exp_scale(-y - kLift), 0.f);
+                            make_float4(fmaxf(w.scale_log2 * exp_scale(e), 0x1p-149f), float(y), exp_scale(-y - kLift), 0.f);
                     if (lane == 0) s_far[unit % kTables] = top - least > kSpread;
                     __syncwarp();
                     fetch(0);

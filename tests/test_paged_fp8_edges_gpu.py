@@ -1,5 +1,5 @@
-"""8-bit paged cache, far ends of its ranges: scores so large that fp32 steps over whole units. Tolerances stand beside
-each case."""
+"""8-bit paged cache, far ends of its ranges: scores so large that fp32 steps over whole units, factors as small as
+they go. Tolerances stand beside each case."""
 
 import math
 
@@ -123,3 +123,26 @@ def test_large_scores_that_rise_by_a_few_units(base, lens, new, dtype, table_roo
         v = gathered(c, c["v"], c["vs"], b, n).repeat_interleave(2, 0)
         slack = (torch.finfo(dtype).eps / 2 + 2.0 ** -10 + (n + 24) * 2.0 ** -23) * v.abs().amax(1)
         assert (o[r] <= v.amax(1) + slack).all() and (o[r] >= v.amin(1) - slack).all(), r
+
+
+@pytest.mark.parametrize("lens,new", FORMS)
+def test_a_small_factor_over_large_products(lens, new, table_room):
+    """Products of 2^126, blocks of keys of 2^-60 and a scale of 1e-25: scores of 2^-16, so all positions count alike."""
+    dim = 64
+    c = table_room(pc.batch(lens, new, 4, 2, dim, 32, 16, BF, seed=6))
+    c["q"][:] = 0.0
+    c["q"].view(c["rows"], 4, dim)[:, :, 3] = 2.0 ** 118
+    k = torch.zeros(c["k"].shape)
+    k[..., 3] = torch.where(torch.rand(k.shape[:3], generator=torch.Generator().manual_seed(2)) < 0.5, 256.0, -256.0)
+    k = k.masked_fill(~c["used"][:, None, :, None], math.nan)
+    c["k"] = k.to(F8)
+    pc.bits(c["ks"])[:] = 67
+    out, lse = run(c, scale=1e-25)
+    o = out.double().reshape(c["rows"], 4, dim)
+    for r, b, n in visible(c):
+        v = gathered(c, c["v"], c["vs"], b, n).repeat_interleave(2, 0)
+        want, size = v.mean(1), v.abs().mean(1)
+        # weights: 2^-15 for the scores, a factor of fp32's smallest step (2^-149 2^126), half a step of fp16 and the sums'
+        tol = torch.finfo(BF).eps / 2 * want.abs() + (2.0 ** -14 + 2.0 ** -21 + 2.0 ** -11 + (n + 24) * 2.0 ** -23) * size
+        assert ((o[r] - want).abs() <= tol).all(), r
+        assert ((lse[r].double() - math.log(n)).abs() <= 2.0 ** -14 + (n + 24) * 2.0 ** -22).all(), r
