@@ -42,9 +42,10 @@ constexpr int kRows = kNarrowRows, kUnit = kNarrowUnit, kOverhead = kNarrow8Over
 constexpr int kStep = 32;              // positions of a warp's step
 constexpr int kBatch = 32 * 16 / kStep;  // steps whose pages the lanes hold, one block of 16 positions each
 // Weights are kept times 2^15, as they enter the product: relative to a reference 15 below the largest score. With
-// exponents of v that lie 120 apart (they cannot lie further), what fp32 flushes of them is less than 2^-21 of the
-// largest term of the sum of exponentials each.
-constexpr int kLift = 15;
+// exponents of v up to kSpread apart, what fp32 flushes of them is less than 2^-41 of the largest term of the sum of
+// exponentials each. Exponents may lie 120 apart: then the sum takes what is flushed times 2^kFarLift. (Beside the masks,
+// under a condition that both share: one of its own costs 6 sequences of 50 thousand positions 104.8 instead of 102.5 us.)
+constexpr int kLift = 15, kSpread = 100, kFarLift = 64;
 // Rounded up, so that no weight passes 2^15 however large the scores are (from 2^24 on fp32 does not hold m - 15, and
 // fp16 ends at 2^16); sums and outputs are relative to what came out, so that nothing else depends on it.
 __device__ __forceinline__ float reference(float m) { return __fadd_ru(m, -float(kLift)); }
@@ -282,11 +283,18 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
     // TWO: the tile has more than 8 rows; else rows g + 8 are left out of the softmax.
     auto stream = [&](auto two) {
     constexpr bool TWO = decltype(two)::value;
+    int top = -kExpMost;  // largest exponent of v so far
+    bool far = false;
     for (int st = 0; st < steps; ++st) {
         cp_wait<ST - 2>();
         __syncwarp();  // every lane's copies of this stage have landed, and every lane is done with the one before
         issue(st + ST - 1);
-        if (st % kBatch == 0) exp_now = exp_issue;
+        if (st % kBatch == 0) {
+            exp_now = exp_issue;
+            const int ev = scale_exp(exp_now >> 8);  // (0 where there is no block: not far from both ends)
+            top = max(top, __reduce_max_sync(0xffffffffu, ev));
+            far = top - __reduce_min_sync(0xffffffffu, ev) > kSpread;
+        }
         const uint32_t kb = ring + (st % ST) * (2 * SM::kBlock), vb = kb + SM::kBlock;
         const int blk = p0 + kStep * (warp + kWarps * st), pb = blk + 2 * tq;
         float x[4][4] = {};
@@ -304,6 +312,7 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
         }
         float n0 = m0, n1 = m1, back[2];
         const bool cut = min(blk + kStep, p1) > seen || blk + kStep > p1;  // some row does not see all of it
+        const bool unusual = cut || far;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const uint32_t ee = __shfl_sync(0xffffffffu, exp_now, 2 * st % 32 + b);
@@ -354,6 +363,20 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
         const float u0 = m0 == -INFINITY ? 0.f : reference(m0), u1 = m1 == -INFINITY ? 0.f : reference(m1);  // (rows that see nothing yet)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
+            if (unusual) {
+                if (far) {
+                    const float z = back[b] * exp_scale(-kFarLift);
+                    auto flushed = [&](float d) { return d < -126.f ? ex2(d + kFarLift) * z : 0.f; };
+#pragma unroll
+                    for (int n = 2 * b; n < 2 * b + 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            l0 += flushed(x[n][e] - u0);
+                            if constexpr (TWO) l1 += flushed(x[n][2 + e] - u1);
+                        }
+                }
+                if (min(blk + 16 * b + 16, p1) > seen) clear_nan<D>(vb, 16 * b, blk + 16 * b, lim0, lim1, o);
+            }
 #pragma unroll
             for (int n = 2 * b; n < 2 * b + 2; ++n)
 #pragma unroll
@@ -365,7 +388,6 @@ __device__ __forceinline__ void tile8(const PagedWork& p, const Paged8Scales& sc
                         l1 = fmaf(x[n][2 + e], back[b], l1);
                     }
                 }
-            if (cut && min(blk + 16 * b + 16, p1) > seen) clear_nan<D>(vb, 16 * b, blk + 16 * b, lim0, lim1, o);
             uint32_t pf[4] = {pack_half2(x[2 * b][0], x[2 * b][1]), 0, pack_half2(x[2 * b + 1][0], x[2 * b + 1][1]), 0};
             if constexpr (TWO) {
                 pf[1] = pack_half2(x[2 * b][2], x[2 * b][3]);

@@ -68,14 +68,12 @@ def attention(q, codes, scales, table, lens, starts, scale=None, causal=True):
     ref["heaviest"] = torch.zeros(rows, heads, dtype=torch.float64)
     qd = q.double().reshape(rows, hkv, group, dim)
     ev = scales_of(scales[1])
-    ref["apart"] = 0  # exponents of v of one sequence and head: most between two
     for b, a, z, n in op.sequences(rows, lens, starts):
         n = max(n, 0)
         if n == 0:
             continue
         kk = op.gather(k, table[b], n)
         e = torch.stack([ev[table[b][p // size], :, p % size // block] for p in range(0, n, block)], 1)
-        ref["apart"] = max(ref["apart"], int((e.amax(1) - e.amin(1)).max()))
         e = e.repeat_interleave(block, 1)[:, :n].double()
         for t in range(a, z):
             m = int(ref["seen"][t])
@@ -98,14 +96,14 @@ def attention_bounds(ref, dim: int, dtype: torch.dtype):
     two so that a row's largest entry is at least 2^14 in fp16, and lose at most 2^-25
     there: 2^-39 of the largest entry per product, far under the (dim + 8) 2^-23 of the
     sum's own roundings, which count for |q| |k| summed; 2^-23 more covers them where
-    one entry is all there is. The sum of exponentials comes from the same weights: where
-    exponents of v lie x apart, what fp32 flushes of a weight (under 2^-126, at 2^15 times
-    its size) is at most 2^(x - 141) of the sum's largest term; 2^-33 where the weights of
-    up to 100 apart are kept 2^7 times only."""
+    one entry is all there is. The sum of exponentials comes from the same weights: with
+    exponents of v up to 100 apart, what fp32 flushes of a weight (under 2^-126, at 2^7
+    times its size) is at most 2^-33 of the sum's largest term; further apart the sum is of
+    weights 2^64 times as large."""
     u, up = torch.finfo(dtype).eps / 2, 2.0 ** -11
     seen = ref["seen"].double()[:, None]
     score = (dim + 9) * 2.0 ** -23 * (ref["terms"] + 1)
-    spread = (seen + 8) * 2.0 ** -23 + seen * 2.0 ** max(ref["apart"] - 141, -33)
+    spread = (seen + 8) * 2.0 ** -23 + seen * 2.0 ** -33
     out = u * ref["out"].abs() + (up + 2 * score + 2 * spread)[..., None] * ref["weight"]
     out = out + (seen * 2.0 ** -32 * 448.0 * ref["heaviest"])[..., None]
     if dtype == torch.float16:

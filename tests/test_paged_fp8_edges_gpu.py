@@ -1,5 +1,5 @@
-"""8-bit paged cache, far ends of its ranges: scores so large that fp32 steps over whole units, factors as small as
-they go. Tolerances stand beside each case."""
+"""8-bit paged cache, far ends of its ranges: scores so large that fp32 steps over whole units, scales as far apart
+and factors as small as they go. Tolerances stand beside each case."""
 
 import math
 
@@ -146,3 +146,37 @@ def test_a_small_factor_over_large_products(lens, new, table_room):
         tol = torch.finfo(BF).eps / 2 * want.abs() + (2.0 ** -14 + 2.0 ** -21 + 2.0 ** -11 + (n + 24) * 2.0 ** -23) * size
         assert ((o[r] - want).abs() <= tol).all(), r
         assert ((lse[r].double() - math.log(n)).abs() <= 2.0 ** -14 + (n + 24) * 2.0 ** -22).all(), r
+
+
+def test_many_small_terms_beside_a_large_value():
+    """One position whose values are 2^120 times the others', and 40000 others that hold 2^-21.5 of its probability each:
+    together they are 1.3 % of the sum of exponentials, though each weight times 2^exponent is 2^-141.5 of the largest."""
+    dim, page, length, batch = 64, 1024, 40000, 592
+    pages = -(-length // page)
+    k = torch.zeros(pages, 1, page, dim)
+    k[..., 0], k[..., 1] = -20.0, -1.5
+    k[0, :, 7] = 0.0
+    k, ks = pc.quantise(k, torch.ones(pages, page, dtype=torch.bool), 128)
+    v = torch.full((pages, 1, page, dim), 1.0)
+    v[0, :, 7] = torch.arange(dim) % 8 + 8.0  # exact in four bits
+    vs = torch.full((pages, 1, page // 128), 67, dtype=torch.uint8)
+    vs[0, 0, 0] = 187
+    q = torch.zeros(batch, dim, dtype=BF)
+    q[:, :2] = 1.0
+    table = torch.arange(pages, dtype=torch.int32).expand(batch, pages).contiguous()  # pages that all of them read
+    lens = torch.full((batch,), length, dtype=torch.int32)
+    lse = torch.empty(batch, 1, device=DEV)
+    d = [t.to(DEV) for t in (q, pc.bits(k), pc.bits(v.to(F8)), pc.bits(ks), vs, table, lens)]
+    out = _api().paged_attention_fp8(d[0], d[1].view(F8), d[2].view(F8), d[3].view(E8), d[4].view(E8), *d[5:], scale=math.log(2),
+                                     lse=lse)
+    torch.cuda.synchronize()
+    # the other positions of the first block share its exponent, their values are small beside its own
+    total = 1 + (length - 1) * 2.0 ** -21.5
+    near = 127 * 2.0 ** -21.5
+    want = (v[0, 0, 7].double() + near) / total * 2.0 ** 60
+    # scores: (dim + 9) 2^-23 of 21.5; sums of n terms of like size, the largest aside
+    score = (dim + 9) * 2.0 ** -23 * 22.5 * math.log(2)
+    slack = score + (length + 8) * 2.0 ** -23 * (total - 1) + 2.0 ** -20
+    assert ((lse.double().cpu() - math.log(total)).abs() <= slack).all()
+    # one rounding of the result, the weights' in fp16 (here a power of two: none for the largest)
+    assert ((out.double().cpu() - want).abs() <= want * (torch.finfo(BF).eps / 2 + 2.0 ** -11 + 2 * slack)).all()
