@@ -19,8 +19,32 @@ from __future__ import annotations
 
 import json
 import os
+import select
 import time
 from datetime import timedelta
+
+
+def _machine() -> str:
+    """Where a process id means the same process: the running kernel and its namespace of process ids ("-": not known)."""
+    try:
+        with open("/proc/sys/kernel/random/boot_id") as f:
+            return f"{f.read().strip()}/{os.stat('/proc/self/ns/pid').st_ino}"
+    except OSError:
+        return "-"
+
+
+def _wait_for_end(pid: int, deadline: float) -> None:
+    """Until process ``pid`` has ended or the deadline has passed (ended, whether or not its parent has waited for it)."""
+    try:
+        fd = os.pidfd_open(pid)
+    except OSError:  # it has, or the system does not tell
+        return
+    try:
+        ended = select.poll()
+        ended.register(fd, select.POLLIN)
+        ended.poll(max(0.0, deadline - time.monotonic()) * 1e3)
+    finally:
+        os.close(fd)
 
 
 class ReplicaGroup:
@@ -98,20 +122,27 @@ class ReplicaGroup:
             return None
         return {r: json.loads(self.store.get(self._key(name, f"value{r}"))) for r in arrived}
 
-    def close(self, timeout_s: float = 30.0) -> None:
+    def close(self, timeout_s: float = 30.0, linger_s: float = 1.0) -> None:
         """Leave the group. The rank hosting the store waits (up to
         ``timeout_s``) until every rank still counted alive has left, so no
-        rank loses the store while it is still using it."""
+        rank loses the store while it is still using it; and then, up to
+        ``linger_s`` of that time, until the processes of those that left on this
+        machine have ended: a launcher may end what outlives its first rank.
+        Ranks that leave and live on cost the host ``linger_s``."""
         try:
             if not self.hosting:
-                self.store.set(self._key("close", f"left{self.rank}"), "1")
+                self.store.set(self._key("close", f"left{self.rank}"), f"{os.getpid()} {_machine()}")
                 return
             deadline = time.monotonic() + timeout_s
-            others = [r for r in range(self.world) if r != self.rank and r not in self.failed]
+            alive = [r for r in range(self.world) if r != self.rank and r not in self.failed]
+            others = alive
             while others and time.monotonic() < deadline:
                 others = [r for r in others if not self.store.check([self._key("close", f"left{r}")])]
                 time.sleep(0.001)
-            if self.world > 1:
-                time.sleep(0.5)  # the others' processes end after their mark; a launcher may end what outlives this one
+            left = [self.store.get(self._key("close", f"left{r}")).decode().split() for r in alive if r not in others]
+            deadline = min(deadline, time.monotonic() + linger_s)
+            for pid, machine in left:
+                if machine == _machine() != "-":
+                    _wait_for_end(int(pid), deadline)
         except (RuntimeError, OSError):
             pass
