@@ -420,8 +420,9 @@ __global__ void __launch_bounds__(kBlockThreads, R == 2 ? 3 : 2) append8_blocks_
 
 template <typename E, typename C, int D>
 const void* blocks_kernel(int r) {
-    return r == 2   ? reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 2>)
-           : r == 8 ? reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 8>)
+    if constexpr (kMostBlock * (D / 8) == 8 * kBlockThreads)  // blocks of 128 positions of 128 dims
+        if (r == 8) return reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 8>);
+    return r == 2 ? reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 2>)
                   : reinterpret_cast<const void*>(&append8_blocks_kernel<E, C, D, 4>);
 }
 template <typename E, typename C>
