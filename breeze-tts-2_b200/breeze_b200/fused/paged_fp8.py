@@ -9,10 +9,13 @@
 
 Every cache entry is an e4m3 code times a power of two that a block of positions of a
 kv head shares (k and v have their own). A block's scale is 2^e with the least e from
--60 to 60 for which its largest finite magnitude is at most 448 2^e. A block fills up
-over many calls: when a later token needs a larger scale, the codes that are there are
-divided by the power of two in between, which is exact but for the smallest; when it
-would need a smaller one, the scale stays. Infinite and NaN entries are held as NaN.
+-60 to 60 for which the largest finite magnitude that was written to it, since its
+first position was, is at most 448 2^e. A block fills up over many calls: when a later
+token needs a larger scale, the codes that are there are divided by the power of two in
+between, which is exact but for the smallest; when it would need a smaller one, the
+scale stays. So tokens that are taken back (rejected drafts: shorter lengths in the next
+call) leave a block the scale that they needed, with the bits that its codes lost by
+it, until its first position is written again. Infinite and NaN entries are held as NaN.
 
 Arguments as in breeze_b200.fused.paged, but
   k_pages, v_pages    (pages, HKV, page size, D) float8_e4m3fn, any strides that are
@@ -22,7 +25,8 @@ Arguments as in breeze_b200.fused.paged, but
                       size / blocks positions (16, 32, 64 or 128) share a scale.
                       ``pages.float()`` times the block's ``scales.float()`` is the
                       value. Nothing needs to be initialised: what holds no position
-                      may hold anything.
+                      may hold anything. (An append behind positions of a block that
+                      no append wrote finds their codes and scale as they are.)
 page_table, seq_lens and q_starts are the same, and so is what is read on the device, the
 error bits of ``device_status``, the stream, the scratch and what graphs may do. The
 rows' dtype is bf16 or fp16, whatever wrote the cache. A page belongs to one sequence

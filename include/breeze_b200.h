@@ -411,7 +411,10 @@ typedef struct bq_paged8_kv {
  * power of two (exact, but for codes that become subnormal). New codes are x * 2^-e
  * rounded to the nearest e4m3 value, ties to even; infinite and NaN x become NaN,
  * |x| above 448 * 2^60 becomes that. What the block holds behind the new tokens does
- * not count. A block belongs to one sequence of a call. */
+ * not count, but the scale that it took does: a block's scale never falls before its
+ * first position is written again, so tokens that are taken back leave it to the
+ * others. Older positions that no append wrote need codes and a scale of their own. A
+ * block belongs to one sequence of a call. */
 typedef struct bq_paged8_append_desc {
     bq_paged8_kv kv;
     int32_t T, HQ;

@@ -180,3 +180,47 @@ def test_many_small_terms_beside_a_large_value():
     assert ((lse.double().cpu() - math.log(total)).abs() <= slack).all()
     # one rounding of the result, the weights' in fp16 (here a power of two: none for the largest)
     assert ((out.double().cpu() - want).abs() <= want * (torch.finfo(BF).eps / 2 + 2.0 ** -11 + 2 * slack)).all()
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("block", [16, 64])
+def test_a_rejected_draft_leaves_its_blocks_scale(block, ragged):
+    """A drafted token with large entries is taken back: its block keeps the scale that it needed, older and later codes
+    are those of that scale, until the block is written from its first position again."""
+    hkv, dim, page = 2, 64, 64
+    g = torch.Generator().manual_seed(block + ragged)
+    x = torch.randn(14, 3 * hkv, dim, generator=g)
+    x[6] *= 3000.0  # the draft
+    x = x.to(BF)
+    k, v = (torch.full((2, hkv, page, dim), 0x7F, dtype=torch.uint8, device=DEV).view(F8) for _ in range(2))
+    ks, vs = (torch.full((2, hkv, page // block), 255, dtype=torch.uint8, device=DEV).view(E8) for _ in range(2))
+    table, lens = torch.tensor([[1, 0]], dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    one, zero = torch.ones(128, dim, device=DEV), torch.zeros(128, dim, device=DEV)
+
+    def add(rows, at):
+        for r in [rows] if ragged else [[i] for i in rows]:
+            lens.fill_(at + len(r))
+            at += len(r)
+            starts = torch.tensor([0, len(r)], dtype=torch.int32, device=DEV) if ragged else None
+            _api().paged_append_fp8(x[r].reshape(len(r), -1).to(DEV), one, zero, k, v, ks, vs, table, lens, q_starts=starts)
+
+    def check(rows, seen):
+        """Rows in the cache, after a scale that the rows `seen` needed."""
+        starts = torch.tensor([0, len(rows)], dtype=torch.int32, device=DEV)
+        back = _api().paged_read_fp8(k, v, ks, vs, table, lens, q_starts=starts, rows=len(rows), dtype=torch.float32)
+        for got, want, scales in ((back[0], x[:, hkv:2 * hkv], ks), (back[1], x[:, 2 * hkv:], vs)):
+            e = torch.tensor([o8.exponent(float(t)) for t in want[seen].double().abs().amax((0, 2))])
+            assert torch.equal(o8.scales_of(scales.cpu())[1, :, 0].long(), e)
+            # half a step of four significant bits, then, where the code became subnormal, half of 2^(e - 9) at each
+            # rescaling, which at least doubles it: 2^(e - 9) in all
+            tol = want[rows].double().abs() * 2.0 ** -4 + torch.exp2(e.double() - 9)[:, None]
+            assert ((got.cpu().double() - want[rows].double()).abs() <= tol).all()
+
+    add([0, 1, 2, 3, 4, 5, 6], 0)
+    check([0, 1, 2, 3, 4, 5, 6], [0, 1, 2, 3, 4, 5, 6])
+    lens.fill_(6)
+    check([0, 1, 2, 3, 4, 5], [6])
+    add([7, 8], 6)
+    check([0, 1, 2, 3, 4, 5, 7, 8], [6])
+    add([9, 10, 11, 12, 13], 0)  # the stream begins anew
+    check([9, 10, 11, 12, 13], [9, 10, 11, 12, 13])
