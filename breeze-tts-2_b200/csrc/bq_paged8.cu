@@ -86,21 +86,24 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Most positions per CTA of a cluster that the page table may hold, as for 16-bit caches: a cluster costs its longest
 // sequence, so a roomy table, which may hold uneven ones, takes equal shares. Clusters against equal shares, all sequences
-// of the table's length, 128 dims, us:
+// of the table's length, 128 dims (64 dims were not measured apart, and take the same rule), us:
 //   2 of 16 heads   256 / 1024 / 4096 positions    6.2 / 6.8 / 11.3   and    9.0 / 11.2 / 15.3
 //   9 of 8          128 /  512 / 1024 (2 CTAs)     5.8 / 7.7 / 10.6   and    9.5 / 11.0 / 12.8
 //   18 of 8         512 / 1024        (2 CTAs)     8.2 / 11.2         and   13.5 / 16.7
 //   64 of 8         128 /  512        (1 CTA)     10.9 / 19.8         and   14.4 / 24.6   (200 of 8: no difference)
 constexpr int kClusterPositions = 512;
 
-// Rows that share a kv head up to which they go to the kernel for few rows, in tiles of 16, of which all but the first
-// find the codes in L2 mostly. Against the 256-row kernel (as it was then, about 8 % slower than now), 4 kv heads, us:
-//                             24 rows      32          64          96          128
-//   128 dims, 32 x 6000      49 / 134    60 / 134    70 / 136    84 / 136   123 / 138
-//             4 x 20000      32 / 69     35 / 71     42 / 69     48 / 67     93 / 69
-//   64 dims,  32 x 6000      37 / 106    43 / 106    50 / 106    61 / 106    88 / 107
-//             32 x 700       13 / 26     13 / 26     17 / 27     22 / 27     20 / 27
-constexpr int kFewRows = 96;
+// Rows that share a kv head up to which they go to the kernel for few rows, in tiles of 16. Two tiles take less than one
+// of the 256-row kernel; with three, long batches of 64 dims still do, and short or single ones do not. Few / many, us:
+//                                        24 rows      32          48          64          96
+//   128 dims, 8 kv heads, 32 x 6000    160 / 197   146 / 198   211 / 204   278 / 208   409 / 223
+//             4 heads,    4 x 20000     44 / 53     43 / 55     51 / 53     64 / 55     88 / 57
+//             4 heads,    8 x 2000      18 / 22     19 / 23     28 / 23     38 / 24     55 / 25
+//             1 head,     1 x 300       12 / 14     12 / 14     18 / 15     24 / 15     35 / 15
+//   64 dims,  8 heads,    32 x 6000    103 / 173   105 / 173   151 / 174   196 / 176   285 / 179
+//             4 heads,    8 x 2000      15 / 20     15 / 21     22 / 21     30 / 21     44 / 22
+//             1 head,     1 x 300       10 / 12     10 / 12     15 / 13     20 / 13     29 / 13
+constexpr int kFewRows = 32;
 
 // How a call is divided: clusters of `ranks` CTAs per (sequence, kv head), or equal shares of all positions for
 // `grid` CTAs with scratch for the tiles (of `rows` rows) that they share.

@@ -36,9 +36,9 @@ def case_form(c, **kw):
 
 
 @pytest.mark.parametrize("room,new,want", [(0, None, "cluster"), (0, [6, 5], "cluster"), (4096, None, "few"), (4096, [6, 5], "few"),
-                                           (0, [40, 56], "few"), (0, [40, 57], "many"), (4096, [40, 90], "many")])
+                                           (0, [16, 16], "few"), (0, [16, 17], "many"), (4096, [40, 90], "many")])
 def test_the_form_of_a_call(room, new, want):
-    """Two query heads per kv head: 16 rows and less, 96 and less, more; a table's room tells the first two apart."""
+    """Two query heads per kv head: 16 rows and less, 32 and less, more; a table's room tells the first two apart."""
     c = pc.batch([700, 260], new, 4, 2, 128, 32, 16, BF, seed=1)
     c["table"] = torch.nn.functional.pad(c["table"], (0, room), value=-1)
     assert case_form(c) == want
