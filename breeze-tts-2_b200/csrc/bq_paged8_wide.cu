@@ -444,13 +444,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_wide_kernel(const __grid_c
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] *= inv;
-                    if (row < hrows && whole) {
+                    if (row < hrows && whole && !again) {  // (large_row reads the query, which may be where its output goes)
                         uint4* dst = reinterpret_cast<uint4*>(static_cast<E*>(w.out) + orow * w.ldo + head * D + 32 * q);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             dst[i] = make_uint4(pack2<E>(o[8 * i], o[8 * i + 1]), pack2<E>(o[8 * i + 2], o[8 * i + 3]),
                                                 pack2<E>(o[8 * i + 4], o[8 * i + 5]), pack2<E>(o[8 * i + 6], o[8 * i + 7]));
-                    } else if (row < hrows) {
+                    } else if (row < hrows && !whole) {
                         float* dst = w.part_o + at * D + 32 * q;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) store8(dst + 8 * i, o + 8 * i);

@@ -224,3 +224,18 @@ def test_a_rejected_draft_leaves_its_blocks_scale(block, ragged):
     check([0, 1, 2, 3, 4, 5, 7, 8], [6])
     add([9, 10, 11, 12, 13], 0)  # the stream begins anew
     check([9, 10, 11, 12, 13], [9, 10, 11, 12, 13])
+
+
+@pytest.mark.parametrize("lens,new", FORMS + [([130] * 120, [60] * 120)])  # (many tiles: thread blocks have them whole)
+@pytest.mark.parametrize("top", [3.0, 1e9])
+def test_outputs_where_the_queries_are(top, lens, new, table_room):
+    c = table_room(pc.batch(lens, new, 4, 2, 64, 32, 16, BF, seed=3, levels=2))
+    c["q"][:] = 1.0
+    fill(c, lambda b, p: 1.75 if p == 5 else 0.5)
+    scale = top / (1.75 * 64 * LOG2E)
+    out, _ = run(c, scale=scale)
+    d = pc.to({k: c[k] for k in ("q", "k", "v", "ks", "vs", "table", "lens")}, DEV)
+    starts = None if c["starts"] is None else c["starts"].to(DEV)
+    assert _api().paged_attention_fp8(d["q"], *where(d), q_starts=starts, scale=scale, out=d["q"]) is d["q"]
+    torch.cuda.synchronize()
+    assert torch.equal(d["q"].cpu(), out)
