@@ -86,11 +86,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Most positions per CTA of a cluster that the page table may hold, as for 16-bit caches: a cluster costs its longest
 // sequence, so a roomy table, which may hold uneven ones, takes equal shares. Clusters against equal shares, all sequences
-// of the table's length, 128 dims (64 dims were not measured apart, and take the same rule), us:
+// of the table's length, 128 dims, us:
 //   2 of 16 heads   256 / 1024 / 4096 positions    6.2 / 6.8 / 11.3   and    9.0 / 11.2 / 15.3
 //   9 of 8          128 /  512 / 1024 (2 CTAs)     5.8 / 7.7 / 10.6   and    9.5 / 11.0 / 12.8
 //   18 of 8         512 / 1024        (2 CTAs)     8.2 / 11.2         and   13.5 / 16.7
 //   64 of 8         128 /  512        (1 CTA)     10.9 / 19.8         and   14.4 / 24.6   (200 of 8: no difference)
+// and 64 dims:
+//   2 of 16 heads   256 / 1024 / 4096 positions    5.6 / 6.0 /  9.3   and    8.5 / 10.4 / 12.8
+//   9 of 8          128 /  512 / 1024              5.4 / 6.9 /  9.0   and    8.7 /  9.9 / 11.0
+//   64 of 8         128 /  512                     9.8 / 16.3         and   12.8 / 20.4
 constexpr int kClusterPositions = 512;
 
 // Rows that share a kv head up to which they go to the kernel for few rows, in tiles of 16. Two tiles take less than one

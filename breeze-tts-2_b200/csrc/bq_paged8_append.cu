@@ -19,7 +19,10 @@
 // registers between the maximum and the codes; queries go to CTAs of their own.
 //
 // Measured in a graph: 2 rows of 48 heads 2.0 us, 160 rows of 48 heads 3.0 us (both the
-// chain of loads); eight drafted rows of 48 heads 4.8 us; seven prompts of 28 heads of
+// chain of loads) where no scale grows; a block whose scale does is rescaled position by
+// position, each waiting for the one before, and the fullest such block sets the call's
+// time: up to 8.3 us with blocks of 32, 14 with 64, 27 with 128. A few drafted rows of two
+// streams of 48 heads 4.8 us; seven prompts of 28 heads of
 // 64, blocks of 16, 26.9 MB in 11.5 us (2.3 TB/s: waves of short CTAs, each with its search
 // for the sequence, its loads, one barrier and its stores). cos and sin are loaded a row
 // ahead: loaded where they are used, each row waited for its own (prompts 15.0 us).
@@ -265,8 +268,10 @@ __device__ __forceinline__ int find_segments(const PagedKV& kv, int w0, int w1, 
 
 // R: rows of a block that each group of lanes holds: block / R groups take a head's block, GROUPS R / block heads the CTA.
 // As few as give each CTA one head, but for short blocks, of which it takes several heads (blocks of 16 rows of 64 dims:
-// 1 row 13.1 us, 2 rows 11.5, 4 rows 12.9). With two rows three CTAs fit an SM, with more two (three, spilling: 400 rows
-// 11.0 against 7.0 us).
+// 1 row 13.1 us, 2 rows 11.5, 4 rows 12.9). With two rows three CTAs run on an SM (80 registers, up to 88 bytes of them
+// spilled with fp32 tables), with more two (three, spilling: 400 rows of 16 kv heads 11.0 against 7.0 us). Eight rows
+// (blocks of 128 positions of 128 dims) spill 180 to 344 bytes at two, too: 2020 rows of 48 heads take 16.0 us in blocks
+// of 64 and 20.9 in blocks of 128.
 template <typename E, typename C, int D, int R>
 __global__ void __launch_bounds__(kBlockThreads, R == 2 ? 3 : 2) append8_blocks_kernel(const __grid_constant__ Append8Params p) {
     constexpr int LG = D / 8, GROUPS = kBlockThreads / LG;
@@ -494,7 +499,7 @@ extern "C" int32_t bq_paged8_append(const bq_paged8_append_desc* d, void* stream
     p.kv_ctas = (2 * d->kv.HKV + heads - 1) / heads;
     // Queries: a short window's rows do not fill a CTA, which takes several sets of heads then (prompts with blocks of 16:
     // 14.7 -> 11.5 us). A long one's are divided among CTAs until there are three for every SM (400 rows of 16 heads: undivided
-    // 8.0 us, in four 7.0; 16000 of 32: 60 and 74 us).
+    // 8.0 us, in four 7.0; 8000 of 32: 60 and 74 us).
     const DeviceInfo* di = device_info();
     if (!di) return BQ_ERR_CUDA;
     p.q_parts = p.q_sets = 1;

@@ -3,7 +3,8 @@
 // mma.sync m16n8k16 tiles in f16, which holds every e4m3 code exactly.
 //
 // Bound: HBM, at half the bytes per position of a 16-bit cache; so the instructions
-// between the loads and the products count. Four warps per CTA take every fourth
+// between the loads and the products count, and the warps that cover their latencies:
+// two for each scheduler, by the registers of the accumulators. Four warps per CTA take every fourth
 // block of 32 positions of the CTA's share, each through a ring of its own (cp.async,
 // no barrier between warps). The products' inner dimensions may be in any order, so a
 // lane reads codes of neighbouring dims of its position by 16 bytes at a time and
@@ -23,11 +24,13 @@
 // largest loses less than 2^-40 of it). Scores, statistics and outputs are fp32.
 //
 // Measured (bf16, 32 query and 8 kv heads of 128, in a graph, join included): 6 sequences
-// of 40 to 60 thousand positions, 581 MB, 102 us (5.7 TB/s; 115 when run for a second on
-// end, at lower clocks); 64 sequences of 11 to 7000 positions, 168 MB, 44 us (3.9 TB/s:
+// of 40 to 60 thousand positions, 581 MB, 103 us (5.6 TB/s; 114 when run for a second on
+// end, at lower clocks); 64 sequences of 11 to 7000 positions, 168 MB, 44 us (3.8 TB/s:
 // 5 to 7 us of shares and join, and each tile's start and end). The schedulers issue in
-// 46 % of cycles, the ALU pipe (conversion, masks, exponents) is busy in 45 %: between
-// the 16-bit form's balance and HBM. Not kept: a share per warp instead of per CTA (no
+// 41 % of cycles, HBM is busy in 64 %, the ALU pipe (conversion, masks, exponents) in 39 %;
+// a warp waits longest for its own last instruction (1.7 cycles an issue; 0.3 for loads),
+// with eight warps on an SM too few to fill in. The products' 16 rows are half empty or
+// more in a decode step. Not kept: a share per warp instead of per CTA (no
 // sum over warps at a tile's end, but four times the parts to join: 47 us for the
 // 64 sequences), finding the next tile's place and pages ahead (44.3 against 43.7).
 #include "bq_host.h"

@@ -5,8 +5,8 @@
 // Bound: HBM, 1 byte read and 2 (4) written per element. A CTA takes a window of
 // rows and some heads of k or of v; a thread turns 16 codes at a time (32 bytes out),
 // several of them in flight. Measured: 96925 rows of 8 heads of 128 to bf16, 595 MB in
-// 105 us (5.7 TB/s); 410 rows of 16 heads 4.4 us. Two stores
-// of 16 bytes instead of one of 32 cost the long case 5 %.
+// 105 us (5.7 TB/s), to fp32 178 us (991 MB, 5.6 TB/s); 410 rows of 16 heads 4.4 us. Two
+// stores of 16 bytes instead of one of 32 cost the long case 5 %.
 #include <cstring>
 
 #include "bq_host.h"

@@ -18,12 +18,14 @@
 // the ev of a unit lie more than 100 below one of the tile so far, weights that fp32
 // flushes might still count in the sum of exponentials, which is then computed on its own.
 //
-// Measured: a prompt of 6500 tokens, 16 heads over 8 of 128, 173 GFLOP in 246 us (0.70
-// PFLOP/s; tensor cores and exponential units busy in 37 % of cycles each); the 16-bit
-// kernel on the same values takes 254 us. What bounds it is the instructions around the
-// products: softmax, conversion and the roles' loops share the instruction cache, which a
+// Measured: a prompt of 6500 tokens, 16 heads over 8 of 128, 173 GFLOP in 245 us (0.71
+// PFLOP/s; tensor cores and exponential units busy in 37 % of cycles each), 229 us on
+// values without large maxima; the 16-bit kernel takes 214 and 186 us for the same values
+// (64 dims: 213 and 196, 200 and 182), so the smaller cache costs prompts 7 to 23 %. What
+// bounds it is the instructions around the products, codes converted once for each tile of
+// rows among them: softmax, conversion and the roles' loops share the instruction cache, which a
 // conversion unrolled over a tile already overruns (314 us; rolled, one 16-byte piece at a
-// time, 246). Not kept: exponentials against the maximum so far while the new one is found,
+// time, 246 then). Not kept: exponentials against the maximum so far while the new one is found,
 // as the 16-bit kernel has it (257 us on even data, 285 on data whose maxima move; with the
 // maximum first 257 and 267); scores read from tensor memory in pieces of 32, with a
 // buffer for each half (308); two threads per row (253); codes fetched by the converting
