@@ -70,6 +70,7 @@ constexpr int kSpread = 100;
 // the score's distance from the reference first, for all scores, costs prompts 257 us instead of 245, under a condition
 // behind the maximum 255 to 262, before it 269, in an instance of the loop of its own 370 (registers spill).
 constexpr float kLargeScore = 1048576.f;  // 2^20
+constexpr long long kLargeCycles = 60000;  // twice what a position takes a warp there
 
 template <int D>
 struct Wide8Smem {
@@ -807,7 +808,9 @@ int paged8_launch_wide(const PagedWork& w, const Paged8Scales& sc, const bq_page
     const uint32_t type = dtype == BQ_DT_BF16 ? 1u : 0u, common = (1u << 4) | (uint32_t(128 >> 4) << 24);
     p.idesc_qk = common | (type << 7) | (type << 10) | (uint32_t(128 >> 3) << 17);
     p.idesc_pv = common | (1u << 16) | (uint32_t(D >> 3) << 17);
-    p.wait_cycles = kWaitCycles;
+    // (a wait may have to outlast large_row for all positions of a share: 15 us each, and as much again; more than 2^20 of
+    // them, all of rows that need it, end with the error bit of a wait that gave up)
+    p.wait_cycles = kWaitCycles + std::min<int64_t>(int64_t(kv->max_pages) * kv->page_size, 1 << 20) * kLargeCycles;
     const bool bf = dtype == BQ_DT_BF16;
     const void* fn = D == 128 ? (bf ? reinterpret_cast<const void*>(&paged8_wide_kernel<__nv_bfloat16, 128>)
                                     : reinterpret_cast<const void*>(&paged8_wide_kernel<__half, 128>))

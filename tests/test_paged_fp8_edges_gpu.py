@@ -239,3 +239,27 @@ def test_outputs_where_the_queries_are(top, lens, new, table_room):
     assert _api().paged_attention_fp8(d["q"], *where(d), q_starts=starts, scale=scale, out=d["q"]) is d["q"]
     torch.cuda.synchronize()
     assert torch.equal(d["q"].cpu(), out)
+
+
+def test_large_scores_over_a_long_cache():
+    """Tiles of 190 thousand positions whose rows all have large scores take longer than other waits may: they are answered."""
+    from breeze_b200 import _lib
+
+    hkv, dim, page, new, length = 8, 128, 1024, 4800, 190000
+    pages = -(-length // page)
+    k = torch.full((pages, hkv, page, dim), 0.5, device=DEV)
+    k[0, :, 5] = 1.75
+    g = torch.Generator(device=DEV).manual_seed(3)
+    v = torch.randint(0, 256, k.shape, generator=g, device=DEV, dtype=torch.uint8)
+    v[(v & 0x7F) == 0x7F] = 0
+    ks, vs = (torch.full((pages, hkv, page // 128), 127, dtype=torch.uint8, device=DEV) for _ in range(2))
+    q = torch.ones(new, hkv * dim, dtype=BF, device=DEV)
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    lens = torch.tensor([length], dtype=torch.int32, device=DEV)
+    starts = torch.tensor([0, new], dtype=torch.int32, device=DEV)
+    out = _api().paged_attention_fp8(q, k.to(F8), v.view(F8), ks.view(E8), vs.view(E8), table, lens, q_starts=starts,
+                                     scale=1e9 / (1.75 * dim * LOG2E))
+    torch.cuda.synchronize()
+    assert _lib.device_status(0) == 0
+    want = v.view(F8)[0, :, 5].float().to(BF).reshape(-1)
+    assert torch.equal(out, want.expand(new, -1))
